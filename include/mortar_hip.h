@@ -583,6 +583,67 @@ int mortar_sdd_bf16(const int32_t *plan, int32_t n_wg, int32_t blocks_per_wave, 
                     int32_t nnz, const uint16_t *a, int64_t lda, const uint16_t *b, int64_t ldb, int64_t M, float *acc,
                     uint16_t *out, void *stream);
 
+/* ---- dense MLP of a block that is not carved ------------------------------------------------------ */
+
+/* The dense phase of _SwiGLUMortar.forward (morph/model/transformer.py:402-431 over block_sparse.py:590-594) and its
+ * gradients, in bf16 or fp16 (`type`), fp32 sums.  All matrices are row-major with 16-byte aligned rows (leading dimensions in
+ * values, widths and leading dimensions multiples of 8); any number of rows M.
+ *   mortar_dense_gateup_swiglu  h [M, f] = silu(x Wg^T) * (x Wu^T), W = [Wg; Wu] [2 f, d], x [M, d]; with gu [M, 2 f] (or NULL)
+ *                               the two products are stored as well, for the backward
+ *   mortar_dense_linear         y [M, N] = x W^T, x [M, K], W [N, K]
+ *   mortar_dense_swiglu_bwd     dh = dy W for W [d, f] (the down matrix), dy [M, d], and from it and the stored gu: dgu [M, 2 f], the
+ *                               gradient of gu, and (h not NULL) h [M, f] = silu(gate) * up once more
+ *   mortar_dense_linear_dx      dx [M, N] = dy W, dy [M, K], W [K, N]
+ *   mortar_dense_linear_dw      dW [n_out, n_in] = dy^T x, dy [M, n_out], x [M, n_in], M > 0
+ * workspace: mortar_dense_workspace_bytes(rows, columns, length of the sums) bytes of device memory, 16-byte aligned, where that is not 0
+ * (dw: (n_out, n_in, M)): fp32 sums over ranges of K, added in a fixed order. */
+enum { MORTAR_BF16 = 0, MORTAR_FP16 = 1, MORTAR_FP32 = 2 };
+int64_t mortar_dense_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, int64_t ldx, const void *w, int64_t ldw, int32_t f, int32_t type,
+                               void *h, int64_t ldh, void *gu, int64_t ldgu, void *stream);
+int mortar_dense_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const void *w, int64_t ldw, int32_t N, int32_t type, void *y,
+                        int64_t ldy, float *workspace, void *stream);
+int mortar_dense_swiglu_bwd(const void *dy, int64_t M, int32_t d, int64_t lddy, const void *w, int64_t ldw, int32_t f, int32_t type,
+                            const void *gu, int64_t ldgu, void *dgu, int64_t lddgu, void *h, int64_t ldh, void *stream);
+int mortar_dense_linear_dx(const void *dy, int64_t M, int32_t K, int64_t lddy, const void *w, int64_t ldw, int32_t N, int32_t type,
+                           void *dx, int64_t lddx, float *workspace, void *stream);
+int mortar_dense_linear_dw(const void *dy, int64_t M, int32_t n_out, int64_t lddy, const void *x, int64_t ldx, int32_t n_in, int32_t type,
+                           void *dw, int64_t lddw, float *workspace, void *stream);
+
+/* ---- LayerNorm with its gradients --------------------------------------------------------------------- */
+
+/* y = (x - mean) * rstd * w + b per row of x [M, d], the TileRouter's query_norm (morph/model/routing.py:186-191) among others, and
+ * dx, dw, db from dy.  `type` of x, y, dy, dx: bf16, fp16 or fp32; w, b, dw, db in the same type, or fp32 with w_fp32 != 0; w and b may be
+ * NULL (1 and 0).  fp32 arithmetic throughout; any d, strides and alignment (16-byte rows are read in 16-byte words).
+ *   mean, rstd  fp32 [M]: written by the forward (both or neither), read by the backward
+ *   dx, dw, db  NULL: not wanted;  M > 0 in the backward
+ *   workspace   mortar_layernorm_workspace_bytes(M, d) bytes, needed for dw or db: fp32 sums over runs of rows, added in a fixed order */
+int mortar_layernorm(const void *x, int64_t M, int32_t d, int64_t ldx, int32_t type, const void *w, const void *b, int32_t w_fp32, float eps,
+                     void *y, int64_t ldy, float *mean, float *rstd, void *stream);
+int64_t mortar_layernorm_workspace_bytes(int64_t M, int32_t d);
+int mortar_layernorm_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, int64_t M, int32_t d, int32_t type, const void *w,
+                         int32_t w_fp32, const float *mean, const float *rstd, void *dx, int64_t lddx, void *dw, void *db,
+                         float *workspace, void *stream);
+
+/* ---- dense layers in 8 bits --------------------------------------------------------------------------- */
+
+/* e4m3 (OCP FP8) operands with fp32 scales, x one per row and 128 values of K, W one per 128 x 128 block: s = amax / 448 (1 where
+ * amax = 0), q = x / s (fp32 quotient) rounded to nearest even.  K a multiple of 16, N of 8, rows of codes on 16-byte addresses, leading
+ * dimensions in values.  A block with an infinity or NaN gets a scale of the kind and makes the results it enters NaN.
+ *   mortar_fp8_quantize          x bf16 [M, K] -> q [M, K], s(m, kb) at s[m * s_m + kb * s_k]
+ *   mortar_fp8_quantize_weight   w [N, K] in bf16, fp16 or fp32 (`type`) -> q [N, K], s(nb, kb) at s[nb * s_n + kb]
+ *   mortar_fp8_linear            y bf16 [M, N] = sum over kb of sx(m, kb) sw(n / 128, kb) (q_x . q_w of the block).  sx NULL: x is bf16 and is
+ *                                quantised inside, where mortar_fp8_quantizes_inside(M, K) says so (a few rows)
+ *   workspace                    mortar_fp8_workspace_bytes(M, N, K) bytes where that is not 0 */
+int mortar_fp8_quantize(const uint16_t *x, int64_t M, int32_t K, int64_t ldx, uint8_t *q, int64_t ldq, float *s, int64_t s_m, int64_t s_k,
+                        void *stream);
+int mortar_fp8_quantize_weight(const void *w, int32_t N, int32_t K, int64_t ldw, int32_t type, uint8_t *q, int64_t ldq, float *s, int64_t s_n,
+                               void *stream);
+int64_t mortar_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int mortar_fp8_quantizes_inside(int64_t M, int64_t K);
+int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const float *sx, int64_t sx_m, int64_t sx_k, const uint8_t *w, int64_t ldw,
+                      const float *sw, int64_t sw_n, int32_t N, uint16_t *y, int64_t ldy, float *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

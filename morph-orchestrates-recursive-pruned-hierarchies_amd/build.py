@@ -12,7 +12,8 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB = os.path.join(_HERE, "libmortar_hip.so")
 NATIVE = os.path.join(_HERE, "_mortar_native.so")
 SOURCES = ["mortar_host.cpp", "mortar_prefill.hip", "mortar_smallm.hip", "mortar_smallm_chunk.hip", "mortar_mid.hip", "mortar_pipe.hip", "mortar_decode.hip", "mortar_gemv_f32.hip", "mortar_route.hip", "mortar_router_gemm.hip",
-           "mortar_pack.hip", "mortar_sdd.hip", "mortar_swiglu.hip", "mortar_values.hip"]
+           "mortar_pack.hip", "mortar_sdd.hip", "mortar_swiglu.hip", "mortar_values.hip", "mortar_layernorm.hip", "mortar_dense.hip", "mortar_fp8.hip"]
+NATIVE_SOURCES = ["mortar_torch.cpp", "mortar_torch_dense.cpp"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
@@ -43,9 +44,11 @@ def build(verbose: bool = False) -> str:
         procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
         objs.append(obj)
     nflags, nlink = _native_flags(hipcc)
-    nobj = os.path.join(CSRC, "mortar_torch.o")
-    procs.append(("mortar_torch.cpp", subprocess.Popen([hipcc, *nflags, "-c", os.path.join(CSRC, "mortar_torch.cpp"), "-o", nobj],
-                                                       stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    nobjs = []
+    for src in NATIVE_SOURCES:
+        nobjs.append(os.path.join(CSRC, os.path.splitext(src)[0] + ".o"))
+        procs.append((src, subprocess.Popen([hipcc, *nflags, "-c", os.path.join(CSRC, src), "-o", nobjs[-1]],
+                                            stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
     for src, pr in procs:
         out, _ = pr.communicate()
         if pr.returncode != 0:
@@ -53,7 +56,7 @@ def build(verbose: bool = False) -> str:
         if verbose and out.strip():
             print(out)
     subprocess.check_call([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-Wl,-soname,libmortar_hip.so", "-o", LIB, *objs])
-    subprocess.check_call([hipcc, "-shared", "-fPIC", "-o", NATIVE, nobj, LIB, *nlink])
+    subprocess.check_call([hipcc, "-shared", "-fPIC", "-o", NATIVE, *nobjs, LIB, *nlink])
     return LIB
 
 

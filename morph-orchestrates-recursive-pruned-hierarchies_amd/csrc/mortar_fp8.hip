@@ -1,0 +1,305 @@
+// Dense layers served in 8 bits: y = x W^T with both operands in e4m3 (OCP FP8, 448 the largest value), x with one fp32 scale per row and
+// 128 values of K, W with one per 128 x 128 block:
+//   s = amax / 448 (1 for zeros),  q = rne(x / s) with the IEEE fp32 quotient,
+//   y[m, n] = sum over K blocks of sx[m, kb] sw[n / 128, kb] (sum of q_x q_w in the block).
+// The product of a K block is one matrix instruction deep (16x16x128), so that the sums of a block come out of it unscaled and are
+// added to the fp32 result with the product of the two scales: one multiply-add per value and 128 of K.
+#include <hip/hip_runtime.h>
+
+#include "mortar_dense_core.h"
+#include "mortar_internal.h"
+
+namespace {
+
+constexpr float E4M3_MAX = 448.0f;
+constexpr int FEW_ROWS = 64;
+
+__device__ __forceinline__ float scale_of(uint32_t amax_bits) {         // bits of max |x|; NaN and infinity pass through
+    return amax_bits ? __builtin_bit_cast(float, amax_bits) / E4M3_MAX : 1.0f;
+}
+__device__ __forceinline__ uint32_t abs_max8(const float (&v)[8]) {     // as integers: NaN is the largest
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, v[j]) & 0x7fffffffu;
+        m = b > m ? b : m;
+    }
+    return m;
+}
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {               // over the 16 lanes that share a group of 128 values
+    v = umax(v, mortar_row_xor<8>(v));
+    v = umax(v, mortar_row_xor<4>(v));
+    v = umax(v, mortar_row_xor<2>(v));
+    return umax(v, mortar_row_xor<1>(v));
+}
+__device__ __forceinline__ u32x2_t quantise8(const float (&v)[8], float s) {
+    float q[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) q[j] = v[j] / s;
+    int lo = 0, hi = 0;
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
+    return u32x2_t{(uint32_t)lo, (uint32_t)hi};
+}
+template <int TYPE>
+__device__ __forceinline__ void read8(const void *p, int64_t at, float (&v)[8]) {
+    if constexpr (TYPE == MORTAR_FP32) {
+        const f32x4_t a = *reinterpret_cast<const f32x4_t *>(static_cast<const float *>(p) + at), b = *reinterpret_cast<const f32x4_t *>(static_cast<const float *>(p) + at + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = a[j], v[j + 4] = b[j];
+    } else {
+        dense_unpack8<TYPE == MORTAR_FP16 ? DENSE_F16 : DENSE_BF16>(*reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(p) + at), v);
+    }
+}
+
+// Activations: 16 lanes per group, 16 bytes of x per lane.
+__global__ __launch_bounds__(256) void fp8_rows_kernel(const uint16_t *x, int64_t M, int32_t K, int64_t ldx, uint8_t *q, int64_t ldq, float *s, int64_t s_m,
+                                                       int64_t s_k) {
+    const int kb = (K + 127) >> 7;
+    const int64_t grp = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
+    if (grp >= M * kb) return;
+    const int64_t m = grp / kb;
+    const int b = (int)(grp - m * kb), k = b * 128 + (threadIdx.x & 15) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (k < K) read8<MORTAR_BF16>(x, m * ldx + k, v);
+    const float sc = scale_of(row_max(abs_max8(v)));
+    if (k < K) *reinterpret_cast<u32x2_t *>(q + m * ldq + k) = quantise8(v, sc);
+    if ((threadIdx.x & 15) == 0) s[m * s_m + b * s_k] = sc;
+}
+
+// Weights: a workgroup per 128 x 128 block, 8 rows of 8 values per thread.
+template <int TYPE>
+__global__ __launch_bounds__(256) void fp8_blocks_kernel(const void *w, int32_t N, int32_t K, int64_t ldw, uint8_t *q, int64_t ldq, float *s, int64_t s_n) {
+    __shared__ uint32_t part[4];
+    const int n0 = blockIdx.y * 128 + (threadIdx.x >> 4), k = blockIdx.x * 128 + (threadIdx.x & 15) * 8;
+    float v[8][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        if (n0 + i * 16 < N && k < K) read8<TYPE>(w, (n0 + i * 16) * ldw + k, v[i]);
+        m = umax(m, abs_max8(v[i]));
+    }
+    m = mortar_wave_reduce(m, umax);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+    __syncthreads();
+    const float sc = scale_of(umax(umax(part[0], part[1]), umax(part[2], part[3])));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (n0 + i * 16 < N && k < K) *reinterpret_cast<u32x2_t *>(q + (n0 + i * 16) * ldq + k) = quantise8(v[i], sc);
+    if (threadIdx.x == 0) s[blockIdx.y * s_n + blockIdx.x] = sc;
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------
+// As the 16-bit form: 16 rows of W per workgroup, K blocks of 128 dealt to its waves, the weights straight into registers.  QUANT:
+// x is bf16 and every workgroup quantises it into LDS first, while its first weights are on their way (few values: the launch that
+// would do it once takes longer).
+template <bool QUANT, int MT, int NW, int U>
+__global__ __launch_bounds__(NW * 64) void fp8_few_kernel(const DenseArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    f32x4_t *part = reinterpret_cast<f32x4_t *>(smem);                     // [wave][token tile][lane]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
+    const int n0 = blockIdx.x * 16, blocks = (a.K + 127) >> 7;
+    uint8_t *codes = smem + NW * MT * 1024;                                // QUANT: [M][blocks * 128], then the scales [M][blocks]
+    float *scales = reinterpret_cast<float *>(codes + a.M * blocks * 128);
+    const auto whole = [](const void *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, DENSE_OUTSIDE, 0x00020000); };
+    const auto read = [](__amdgpu_buffer_rsrc_t b, uint32_t off) { return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0)); };
+    const __amdgpu_buffer_rsrc_t wb = whole(static_cast<const char *>(a.p) + (int64_t)n0 * a.ldp), xb = whole(a.q);
+    const uint32_t wo = n0 + r < a.N ? (uint32_t)(r * a.ldp) + g * 16 : DENSE_OUTSIDE;
+    const float *sw = a.sw + (n0 >> 7) * a.sw_n;
+    f32x4_t acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = wave; c0 < blocks || (QUANT && c0 == wave); c0 += NW * U) {
+        u32x4_t w[U][2], x[U][MT][2];
+        float f[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kb = (c0 + u * NW) * 128;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[u][h] = read(wb, kb + h * 64 + g * 16 < a.K ? wo + kb + h * 64 : DENSE_OUTSIDE);
+        }
+        if constexpr (QUANT) {
+            if (c0 == wave) {
+                for (int grp = threadIdx.x >> 4; grp < a.M * blocks; grp += NW * 4) {
+                    const int m = grp / blocks, b = grp - m * blocks, k = b * 128 + (threadIdx.x & 15) * 8;
+                    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (k < a.K) read8<MORTAR_BF16>(a.q, m * (a.ldq / 2) + k, v);
+                    const float sc = scale_of(row_max(abs_max8(v)));
+                    *reinterpret_cast<u32x2_t *>(codes + m * blocks * 128 + k) = quantise8(v, sc);
+                    if ((threadIdx.x & 15) == 0) scales[m * blocks + b] = sc;
+                }
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int b = c0 + u * NW, kb = b * 128, bs = min(b, blocks - 1);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const int m = min(t * 16 + r, a.M - 1);
+                if constexpr (QUANT) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) x[u][t][h] = *reinterpret_cast<const u32x4_t *>(codes + m * blocks * 128 + bs * 128 + h * 64 + g * 16);
+                    f[u][t] = scales[m * blocks + bs];
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) x[u][t][h] = read(xb, kb + h * 64 + g * 16 < a.K ? (uint32_t)(m * a.ldq) + kb + h * 64 + g * 16 : DENSE_OUTSIDE);
+                    f[u][t] = a.sx[m * a.sx_m + bs * a.sx_k];
+                }
+                f[u][t] *= sw[bs];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (c0 + u * NW >= blocks) break;
+            const i32x8_t wf = {(int)w[u][0][0], (int)w[u][0][1], (int)w[u][0][2], (int)w[u][0][3], (int)w[u][1][0], (int)w[u][1][1], (int)w[u][1][2], (int)w[u][1][3]};
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const u32x4_t p = x[u][t][0], q = x[u][t][1];
+                const i32x8_t xf = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)q[0], (int)q[1], (int)q[2], (int)q[3]};
+                const f32x4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+#pragma unroll
+                for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(d[v], f[u][t], acc[t][v]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[(wave * MT + t) * 64 + lane] = acc[t];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4_t sum = part[wave * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) sum += part[(w * MT + wave) * 64 + lane];
+    const int64_t m = wave * 16 + r;
+    const int n = n0 + 4 * g;
+    if (m >= a.M || n >= a.N) return;
+    *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(a.c) + m * a.ldc + n) = u32x2_t{bf16_pack2(sum[0], sum[1]), bf16_pack2(sum[2], sum[3])};
+}
+
+int launch_error(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? MORTAR_OK : mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+constexpr int QUANT_GROUPS = 128;        // groups of 128 values that a workgroup quantises for itself
+bool quantises(int64_t M, int64_t K) { return M <= 16 && M * ((K + 127) / 128) <= QUANT_GROUPS; }
+
+template <bool QUANT, int MT, int NW, int U>
+int launch_few(const DenseArgs &a, hipStream_t st, const char *what) {
+    const auto kern = fp8_few_kernel<QUANT, MT, NW, U>;
+    const int smem = NW * MT * 1024 + (QUANT ? a.M * ((a.K + 127) / 128) * 132 : 0);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, NW * MT * 1024 + QUANT_GROUPS * 132);
+    if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    hipLaunchKernelGGL(kern, dim3((unsigned)((a.N + 15) / 16)), dim3(NW * 64), smem, st, a);
+    return launch_error(what);
+}
+
+template <DenseEpilogue E, int B, int WN, int WM>
+int launch_tile(DenseArgs a, hipStream_t st, const char *what) {
+    const auto kern = dense_tile_kernel<DENSE_E4M3, E, false, false, B, B, WN, WM>;
+    constexpr int smem = 4 * B * 128;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    a.tiles_n = (a.N + B - 1) / B;
+    a.tiles_m = (a.M + B - 1) / B;
+    const int64_t wgs = (int64_t)a.tiles_n * a.tiles_m * a.splits;
+    if (wgs > (1 << 30)) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tiles", what);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((wgs + 7) / 8 * 8)), dim3(WN * WM * 64), smem, st, a);
+    return launch_error(what);
+}
+template <DenseEpilogue E>
+int launch_product(const DenseArgs &a, int tile, hipStream_t st, const char *what) {
+    if (tile == 0) return launch_tile<E, 256, 2, 4>(a, st, what);
+    if (tile == 1) return launch_tile<E, 128, 2, 2>(a, st, what);
+    return launch_tile<E, 64, 1, 4>(a, st, what);
+}
+
+int check_codes(const char *what, const char *name, const void *p, int64_t rows, int64_t cols, int64_t ld) {
+    if (!p) return mortar_fail(MORTAR_ERR_ARG, "%s: %s is null", what, name);
+    if (cols % 16 || ld % 16 || ld < cols || (reinterpret_cast<uintptr_t>(p) & 15))
+        return mortar_fail(MORTAR_ERR_ARG, "%s: %s needs rows of a multiple of 16 values on 16-byte addresses", what, name);
+    if (rows >= INT32_MAX / 2 || cols >= INT32_MAX / 4 || 256 * ld >= (int64_t)DENSE_OUTSIDE) return mortar_fail(MORTAR_ERR_LIMIT, "%s: %s is too large", what, name);
+    return MORTAR_OK;
+}
+int check_values(const char *what, const char *name, const void *p, int64_t cols, int64_t ld, int size) {
+    const int unit = 16 / size;
+    if (!p) return mortar_fail(MORTAR_ERR_ARG, "%s: %s is null", what, name);
+    if (cols % 8 || ld % unit || ld < cols || (reinterpret_cast<uintptr_t>(p) & 15))
+        return mortar_fail(MORTAR_ERR_ARG, "%s: %s needs rows of a multiple of 8 values on 16-byte addresses", what, name);
+    return MORTAR_OK;
+}
+#define CHECK(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
+
+}  // namespace
+
+extern "C" int mortar_fp8_quantize(const uint16_t *x, int64_t M, int32_t K, int64_t ldx, uint8_t *q, int64_t ldq, float *s, int64_t s_m, int64_t s_k,
+                                   void *stream) {
+    const char *what = "fp8_quantize";
+    if (M < 0 || K <= 0) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
+    if (M == 0) return MORTAR_OK;
+    CHECK(check_values(what, "x", x, K, ldx, 2));
+    CHECK(check_codes(what, "q", q, M, K, ldq));
+    if (!s) return mortar_fail(MORTAR_ERR_ARG, "%s: s is null", what);
+    const int64_t groups = M * ((K + 127) / 128);
+    if ((groups + 15) / 16 >= INT32_MAX) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
+    hipLaunchKernelGGL(fp8_rows_kernel, dim3((unsigned)((groups + 15) / 16)), dim3(256), 0, static_cast<hipStream_t>(stream), x, M, K, ldx, q, ldq, s, s_m, s_k);
+    return launch_error(what);
+}
+
+extern "C" int mortar_fp8_quantize_weight(const void *w, int32_t N, int32_t K, int64_t ldw, int32_t type, uint8_t *q, int64_t ldq, float *s, int64_t s_n,
+                                          void *stream) {
+    const char *what = "fp8_quantize_weight";
+    if (N <= 0 || K <= 0 || s_n < (K + 127) / 128) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
+    if (type != MORTAR_BF16 && type != MORTAR_FP16 && type != MORTAR_FP32) return mortar_fail(MORTAR_ERR_ARG, "%s: bf16, fp16 or fp32", what);
+    CHECK(check_values(what, "w", w, K, ldw, type == MORTAR_FP32 ? 4 : 2));
+    CHECK(check_codes(what, "q", q, N, K, ldq));
+    if (!s) return mortar_fail(MORTAR_ERR_ARG, "%s: s is null", what);
+    const int64_t nb = ((int64_t)N + 127) / 128;
+    if (nb > 65535) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many rows", what);
+    const dim3 grid((unsigned)((K + 127) / 128), (unsigned)nb);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (type == MORTAR_BF16) hipLaunchKernelGGL(fp8_blocks_kernel<MORTAR_BF16>, grid, dim3(256), 0, st, w, N, K, ldw, q, ldq, s, s_n);
+    else if (type == MORTAR_FP16) hipLaunchKernelGGL(fp8_blocks_kernel<MORTAR_FP16>, grid, dim3(256), 0, st, w, N, K, ldw, q, ldq, s, s_n);
+    else hipLaunchKernelGGL(fp8_blocks_kernel<MORTAR_FP32>, grid, dim3(256), 0, st, w, N, K, ldw, q, ldq, s, s_n);
+    return launch_error(what);
+}
+
+extern "C" int64_t mortar_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) { return M <= FEW_ROWS ? 0 : mortar_dense_workspace_bytes(M, N, (K + 1) / 2); }
+
+extern "C" int mortar_fp8_quantizes_inside(int64_t M, int64_t K) { return quantises(M, K); }
+
+extern "C" int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const float *sx, int64_t sx_m, int64_t sx_k, const uint8_t *w, int64_t ldw,
+                                 const float *sw, int64_t sw_n, int32_t N, uint16_t *y, int64_t ldy, float *workspace, void *stream) {
+    const char *what = "fp8_linear";
+    if (M < 0 || K <= 0 || N <= 0 || sw_n < (K + 127) / 128) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
+    if (M == 0) return MORTAR_OK;
+    if (!sx && !quantises(M, K)) return mortar_fail(MORTAR_ERR_ARG, "%s: this many rows have to be quantised before the call", what);
+    if (sx) CHECK(check_codes(what, "x", x, M, K, ldx));
+    else CHECK(check_values(what, "x", x, K, ldx, 2));
+    CHECK(check_codes(what, "w", w, N, K, ldw));
+    CHECK(check_values(what, "y", y, N, ldy, 2));
+    if (!sw) return mortar_fail(MORTAR_ERR_ARG, "%s: sw is null", what);
+    DenseArgs a{};
+    a.p = w; a.ldp = ldw; a.q = x; a.ldq = sx ? ldx : ldx * 2;
+    a.M = (int32_t)M; a.N = N; a.K = K;
+    a.c = y; a.ldc = ldy;
+    a.sx = sx; a.sx_m = sx_m; a.sx_k = sx_k; a.sw = sw; a.sw_n = sw_n;
+    a.steps = (K + 127) / 128; a.splits = 1;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (!sx) return launch_few<true, 1, 16, 1>(a, st, what);
+    if (M <= 16) return launch_few<false, 1, 16, 2>(a, st, what);
+    if (M <= 32) return launch_few<false, 2, 16, 2>(a, st, what);
+    if (M <= FEW_ROWS) return launch_few<false, 4, 16, 1>(a, st, what);
+    const MortarDensePlan p = mortar_dense_plan(M, N, ((int64_t)K + 1) / 2, 0, 1);
+    a.splits = p.splits;
+    if (p.splits == 1) return launch_product<DENSE_STORE>(a, p.tile, st, what);
+    if (!workspace) return mortar_fail(MORTAR_ERR_ARG, "%s: this shape needs a workspace", what);
+    a.c = workspace;
+    CHECK(launch_product<DENSE_PARTIAL>(a, p.tile, st, what));
+    return mortar_dense_join(workspace, p.splits, M, N, MORTAR_BF16, y, ldy, stream);
+}

@@ -731,9 +731,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_mortar_native", "Native call laye
 
 }  // namespace
 
+int mortar_add_dense_methods(PyObject *module);          // mortar_torch_dense.cpp
+
 PyMODINIT_FUNC PyInit__mortar_native(void) {
     const char *names[N_NAMES] = {"weight", "bias", "sub_keys_a", "sub_keys_b", "group_bias", "iter_embed"};
     for (int i = 0; i < N_NAMES; ++i)
         if (!(g_names[i] = PyUnicode_InternFromString(names[i]))) return nullptr;
-    return PyModule_Create(&module);
+    PyObject *m = PyModule_Create(&module);
+    if (m && mortar_add_dense_methods(m)) Py_CLEAR(m);
+    return m;
 }

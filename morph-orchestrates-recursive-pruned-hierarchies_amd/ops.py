@@ -553,3 +553,38 @@ def rmsnorm(x: Tensor, weight: Tensor | None = None, eps: float = 1e-6) -> Tenso
         _lib.check(_lib.lib().mortar_rmsnorm_bf16(_p(x2), x2.shape[0], shp[-1], x2.stride(0), _p(w), float(eps), _p(y),
                                                   y.stride(0), _stream(x)), "mortar_rmsnorm_bf16")
     return y.reshape(shp)
+
+
+# ----------------------------------------------------------------------------- dense companions
+
+
+def layernorm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = None, eps: float = 1e-5) -> Tensor:
+    """LayerNorm over the last dimension, differentiable: y = (x - mean) / sqrt(var + eps) * weight + bias.  x bf16, fp16 or fp32 of
+    any width and strides; weight / bias [d] in the type of x or fp32, or None.  Statistics, sums and the gradients of weight and
+    bias (added over the rows in a fixed order) are fp32; results are rounded once.  First derivatives only."""
+    return _lib.native().layernorm(x, weight, bias, eps)
+
+
+def dense_mlp(x: Tensor, w_gate_up: Tensor, w_down: Tensor) -> Tensor:
+    """The SwiGLU MLP of a block that is not carved, differentiable: y = (silu(x Wg^T) * (x Wu^T)) Wd^T with w_gate_up = [Wg; Wu]
+    [2 * d_ff, d] and w_down [d_out, d_ff], all bf16 or all fp16, widths multiples of 8.  gate_up, silu and the product are one
+    launch; sums are fp32, the hidden activations rounded to 16 bits between the two launches.  The backward keeps the gate_up
+    output [rows, 2 * d_ff] and forms its gradient in the epilogue of dy Wd.  First derivatives only."""
+    return _lib.native().dense_mlp(x, w_gate_up, w_down)
+
+
+def quantize_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
+    """(codes float8_e4m3fn like x, scales fp32 [..., ceil(K / 128)]) of bf16 activations [..., K], K a multiple of 16: one scale
+    amax / 448 (1 for zeros) per row and 128 values, codes x / scale rounded to nearest even.  The scales are consecutive along the rows."""
+    return _lib.native().quantize_fp8(x)
+
+
+def quantize_fp8_weight(w: Tensor) -> tuple[Tensor, Tensor]:
+    """(codes float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)]) of a weight: as quantize_fp8 with one scale per 128 x 128 block."""
+    return _lib.native().quantize_fp8_weight(w)
+
+
+def linear_fp8(x: Tensor, wq: Tensor, ws: Tensor, x_scale: Tensor | None = None) -> Tensor:
+    """y = x W^T for a weight of quantize_fp8_weight: bf16 x [..., K] is quantised as quantize_fp8 does (a few rows inside the
+    product's launch), float8_e4m3fn x is taken with its ``x_scale`` as it is.  fp32 sums, bf16 result [..., N]; no gradients."""
+    return _lib.native().linear_fp8(x, wq, ws, x_scale)
