@@ -588,11 +588,12 @@ int mortar_sdd_bf16(const int32_t *plan, int32_t n_wg, int32_t blocks_per_wave, 
 /* The dense phase of _SwiGLUMortar.forward (morph/model/transformer.py:402-431 over block_sparse.py:590-594) and its
  * gradients, in bf16 or fp16 (`type`), fp32 sums.  All matrices are row-major with 16-byte aligned rows (leading dimensions in
  * values, widths and leading dimensions multiples of 8); any number of rows M.
- *   mortar_dense_gateup_swiglu  h [M, f] = silu(x Wg^T) * (x Wu^T), W = [Wg; Wu] [2 f, d], x [M, d]; with gu [M, 2 f] (or NULL)
- *                               the two products are stored as well, for the backward
+ *   mortar_dense_gateup_swiglu  h [M, f] = silu(x Wg^T) * (x Wu^T), W = [Wg; Wu] [2 f, d], x [M, d]; with gu (or NULL) the two
+ *                               products are kept for the backward, in the upper 24 bits of their fp32 sums: [M, 2 f] of 16 bits and
+ *                               behind them [M, 2 f] of 8 bits, 6 M f bytes
  *   mortar_dense_linear         y [M, N] = x W^T, x [M, K], W [N, K]
  *   mortar_dense_swiglu_bwd     dh = dy W for W [d, f] (the down matrix), dy [M, d], and from it and the stored gu: dgu [M, 2 f], the
- *                               gradient of gu, and (h not NULL) h [M, f] = silu(gate) * up once more
+ *                               gradient of the two products, and (h not NULL) h [M, f] = silu(gate) * up once more
  *   mortar_dense_linear_dx      dx [M, N] = dy W, dy [M, K], W [K, N]
  *   mortar_dense_linear_dw      dW [n_out, n_in] = dy^T x, dy [M, n_out], x [M, n_in], M > 0
  * workspace: mortar_dense_workspace_bytes(rows, columns, length of the sums) bytes of device memory, 16-byte aligned, where that is not 0
@@ -600,11 +601,11 @@ int mortar_sdd_bf16(const int32_t *plan, int32_t n_wg, int32_t blocks_per_wave, 
 enum { MORTAR_BF16 = 0, MORTAR_FP16 = 1, MORTAR_FP32 = 2 };
 int64_t mortar_dense_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, int64_t ldx, const void *w, int64_t ldw, int32_t f, int32_t type,
-                               void *h, int64_t ldh, void *gu, int64_t ldgu, void *stream);
+                               void *h, int64_t ldh, void *gu, void *stream);
 int mortar_dense_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const void *w, int64_t ldw, int32_t N, int32_t type, void *y,
                         int64_t ldy, float *workspace, void *stream);
 int mortar_dense_swiglu_bwd(const void *dy, int64_t M, int32_t d, int64_t lddy, const void *w, int64_t ldw, int32_t f, int32_t type,
-                            const void *gu, int64_t ldgu, void *dgu, int64_t lddgu, void *h, int64_t ldh, void *stream);
+                            const void *gu, void *dgu, int64_t lddgu, void *h, int64_t ldh, void *stream);
 int mortar_dense_linear_dx(const void *dy, int64_t M, int32_t K, int64_t lddy, const void *w, int64_t ldw, int32_t N, int32_t type,
                            void *dx, int64_t lddx, float *workspace, void *stream);
 int mortar_dense_linear_dw(const void *dy, int64_t M, int32_t n_out, int64_t lddy, const void *x, int64_t ldx, int32_t n_in, int32_t type,

@@ -5,7 +5,8 @@
 //            d_gate = dh u (s + silu(g) (1 - s)), s = sigmoid(g), and h once more, so that only g and u are kept from the
 //            forward;  dx = dgu Wgu,  dWgu = dgu^T x,  dWd = dy^T h.
 // Sums, silu and its derivative are fp32.  Rounded to 16 bits are what goes through memory as an operand of a matrix product
-// (h, g, u, dgu) and the results; h and the derivatives are formed from the unrounded sums of their own kernel.
+// (h, dgu) and the results; h and the derivatives are formed from the unrounded sums of their own kernel, and from g and u as
+// kept, in 24 bits.
 #include <hip/hip_runtime.h>
 
 #include "mortar_dense_core.h"
@@ -21,23 +22,24 @@ int launch_error(const char *what) {
 // ---- tile products ---------------------------------------------------------------------------------------------------
 
 using Plan = MortarDensePlan;
-constexpr int TILE_EDGE[3] = {256, 128, 64};
 
-// Which tile, and in how many K ranges, from the estimated cycles of the slowest CU: workgroups of a CU share its matrix cores
-// (cycles per K step and tile, as measured with the chip full), and a step takes no less than the way of its copies.
-// K ranges cost a pass over their fp32 slabs and a launch.
+// Which tile, and in how many K ranges, from the estimated cycles of the busiest CU: what a step of a tile takes with the chip full (measured,
+// at the 2 GHz that the chip runs under this load; workgroups that share a CU share its matrix cores), and no less than the way of
+// its copies; a tile's start and end; for K ranges a pass over their fp32 slabs and a launch.
 Plan plan_tiles(int64_t M, int64_t N, int64_t K, bool swiglu, bool may_split) {
-    const double step_cycles[3] = {3400, 900, 360}, way = 1400, slab_byte = 0.0005 * 2, launch = 8000;
+    constexpr double step_cycles[DENSE_N_TILES] = {2900, 2230, 1770, 920, 440}, way[DENSE_N_TILES] = {1500, 1500, 1000, 1500, 700};
+    constexpr double ends = 5000, slab_byte = 2 * 0.0005, launch = 8000;
     const int64_t steps = (K + 63) / 64;
     Plan best{0, 1};
     double best_t = 1e300;
-    for (int c = 0; c < 3; ++c) {
-        const int64_t e = TILE_EDGE[c], fe = swiglu ? e / 2 : e;
-        const int64_t tiles = ((N + fe - 1) / fe) * ((M + e - 1) / e);
+    for (int c = 0; c < DENSE_N_TILES; ++c) {
+        const int64_t bn = swiglu ? DENSE_TILES[c].bn / 2 : DENSE_TILES[c].bn, bm = DENSE_TILES[c].bm;
+        const int64_t tiles = ((N + bn - 1) / bn) * ((M + bm - 1) / bm);
         for (int s = 1; s <= 16; s *= 2) {
             if (s > 1 && (!may_split || steps / s < 4)) break;
-            const double wgs = (double)((tiles * s + 255) / 256);
-            double t = (double)((steps + s - 1) / s) * (wgs * step_cycles[c] > way ? wgs * step_cycles[c] : way);
+            const int64_t wgs = (tiles * s + 255) / 256, both = wgs < DENSE_TILES[c].per_cu ? wgs : DENSE_TILES[c].per_cu;
+            const double rounds = (double)wgs / both, per_step = both * step_cycles[c] > way[c] ? both * step_cycles[c] : way[c];
+            double t = rounds * ((double)((steps + s - 1) / s) * per_step + ends);
             if (s > 1) t += launch + slab_byte * s * M * N * 4;
             if (t < best_t) {
                 best_t = t;
@@ -46,27 +48,6 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, bool swiglu, bool may_split) {
         }
     }
     return best;
-}
-
-template <DenseType T, DenseEpilogue E, bool PC, bool QC, int B, int WN, int WM>
-int launch_tile(DenseArgs a, hipStream_t st, const char *what) {
-    const auto kern = dense_tile_kernel<T, E, PC, QC, B, B, WN, WM>;
-    constexpr int smem = 4 * B * 128, F = E == DENSE_SWIGLU ? B / 2 : B;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-    a.tiles_n = (a.N + F - 1) / F;
-    a.tiles_m = (a.M + B - 1) / B;
-    const int64_t wgs = (int64_t)a.tiles_n * a.tiles_m * a.splits;
-    if (wgs > (1 << 30)) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tiles", what);
-    hipLaunchKernelGGL(kern, dim3((unsigned)((wgs + 7) / 8 * 8)), dim3(WN * WM * 64), smem, st, a);
-    return launch_error(what);
-}
-
-template <DenseType T, DenseEpilogue E, bool PC, bool QC>
-int launch_product(const DenseArgs &a, int tile, hipStream_t st, const char *what) {
-    if (tile == 0) return launch_tile<T, E, PC, QC, 256, 2, 4>(a, st, what);
-    if (tile == 1) return launch_tile<T, E, PC, QC, 128, 2, 2>(a, st, what);
-    return launch_tile<T, E, PC, QC, 64, 1, 4>(a, st, what);
 }
 
 // Adds the slabs of the K ranges in their order.
@@ -92,11 +73,11 @@ int run_plain(DenseArgs a, float *ws, hipStream_t st, const char *what) {
     const Plan p = plan_tiles(a.M, a.N, a.K, false, true);
     a.steps = (a.K + 63) / 64;
     a.splits = p.splits;
-    if (p.splits == 1) return launch_product<T, DENSE_STORE, PC, QC>(a, p.tile, st, what);
+    if (p.splits == 1) return dense_launch<T, DENSE_STORE, PC, QC>(a, p.tile, st, what);
     if (!ws) return mortar_fail(MORTAR_ERR_ARG, "%s: this shape needs a workspace", what);
     DenseArgs b = a;
     b.c = ws;
-    const int rc = launch_product<T, DENSE_PARTIAL, PC, QC>(b, p.tile, st, what);
+    const int rc = dense_launch<T, DENSE_PARTIAL, PC, QC>(b, p.tile, st, what);
     if (rc) return rc;
     return mortar_dense_join(ws, p.splits, a.M, a.N, T == DENSE_F16 ? MORTAR_FP16 : MORTAR_BF16, a.c, a.ldc, st);
 }
@@ -179,8 +160,13 @@ __global__ __launch_bounds__(NW * 64) void dense_few_kernel(const DenseArgs a) {
         for (int v = 0; v < 4; ++v) h[v] = sum[0][v] * dense_sigmoid(sum[0][v]) * sum[RS - 1][v];
         put(a.c, m * a.ldc + n, h);
         if (a.gu) {
-            put(a.gu, m * a.ldgu + n, sum[0]);
-            put(a.gu, m * a.ldgu + a.N + n, sum[RS - 1]);
+            const auto keep = [&](int64_t at, f32x4_t v) {
+                const uint32_t b0 = dense_round24(v[0]), b1 = dense_round24(v[1]), b2 = dense_round24(v[2]), b3 = dense_round24(v[3]);
+                *reinterpret_cast<u32x2_t *>(a.gu + at) = u32x2_t{dense_hi2(b0, b1), dense_hi2(b2, b3)};
+                *reinterpret_cast<uint32_t *>(a.gul + at) = dense_lo4(b0, b1, b2, b3);
+            };
+            keep(m * 2 * a.N + n, sum[0]);
+            keep(m * 2 * a.N + a.N + n, sum[RS - 1]);
         }
     } else {
         put(a.c, m * a.ldc + n, sum[0]);
@@ -217,7 +203,7 @@ int check_matrix(const char *what, const char *name, const void *p, int64_t rows
 int check_type(const char *what, int32_t type) {
     return type == MORTAR_BF16 || type == MORTAR_FP16 ? MORTAR_OK : mortar_fail(MORTAR_ERR_ARG, "%s: bf16 or fp16", what);
 }
-#define CHECK(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
+#define CHECK(...) do { const int rc_ = (__VA_ARGS__); if (rc_) return rc_; } while (0)
 
 }  // namespace
 
@@ -239,7 +225,7 @@ extern "C" int64_t mortar_dense_workspace_bytes(int64_t M, int64_t N, int64_t K)
 }
 
 extern "C" int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, int64_t ldx, const void *w, int64_t ldw, int32_t f, int32_t type,
-                                          void *h, int64_t ldh, void *gu, int64_t ldgu, void *stream) {
+                                          void *h, int64_t ldh, void *gu, void *stream) {
     const char *what = "dense_gateup_swiglu";
     if (M < 0 || d <= 0 || f <= 0) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
     CHECK(check_type(what, type));
@@ -247,18 +233,19 @@ extern "C" int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, i
     CHECK(check_matrix(what, "x", x, M, d, ldx));
     CHECK(check_matrix(what, "w", w, 2 * (int64_t)f, d, ldw));
     CHECK(check_matrix(what, "h", h, M, f, ldh));
-    if (gu) CHECK(check_matrix(what, "gu", gu, M, 2 * (int64_t)f, ldgu));
+    if (gu) CHECK(check_matrix(what, "gu", gu, M, 2 * (int64_t)f, 2 * (int64_t)f));
     if ((f + (int64_t)256) * ldw * 2 >= (int64_t)DENSE_OUTSIDE) return mortar_fail(MORTAR_ERR_LIMIT, "%s: w is too large", what);
     DenseArgs a{};
     a.p = w; a.ldp = ldw * 2; a.q = x; a.ldq = ldx * 2;
     a.M = (int32_t)M; a.N = f; a.K = d;
-    a.c = h; a.ldc = ldh; a.gu = gu; a.ldgu = ldgu;
+    a.c = h; a.ldc = ldh;
+    if (gu) a.gu = static_cast<uint16_t *>(gu), a.gul = static_cast<uint8_t *>(gu) + M * 4 * f;
     a.steps = (d + 63) / 64; a.splits = 1;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (M <= FEW_ROWS) return type == MORTAR_BF16 ? launch_few<DENSE_BF16, true>(a, st, what) : launch_few<DENSE_F16, true>(a, st, what);
     const Plan p = plan_tiles(M, f, d, true, false);
-    return type == MORTAR_BF16 ? launch_product<DENSE_BF16, DENSE_SWIGLU, false, false>(a, p.tile, st, what)
-                               : launch_product<DENSE_F16, DENSE_SWIGLU, false, false>(a, p.tile, st, what);
+    return type == MORTAR_BF16 ? dense_launch<DENSE_BF16, DENSE_SWIGLU, false, false>(a, p.tile, st, what)
+                               : dense_launch<DENSE_F16, DENSE_SWIGLU, false, false>(a, p.tile, st, what);
 }
 
 extern "C" int mortar_dense_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const void *w, int64_t ldw, int32_t N, int32_t type, void *y,
@@ -313,23 +300,24 @@ extern "C" int mortar_dense_linear_dw(const void *dy, int64_t M, int32_t n_out, 
 }
 
 extern "C" int mortar_dense_swiglu_bwd(const void *dy, int64_t M, int32_t d, int64_t lddy, const void *w, int64_t ldw, int32_t f, int32_t type,
-                                       const void *gu, int64_t ldgu, void *dgu, int64_t lddgu, void *h, int64_t ldh, void *stream) {
+                                       const void *gu, void *dgu, int64_t lddgu, void *h, int64_t ldh, void *stream) {
     const char *what = "dense_swiglu_bwd";
     if (M < 0 || d <= 0 || f <= 0) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
     CHECK(check_type(what, type));
     if (M == 0) return MORTAR_OK;
     CHECK(check_matrix(what, "dy", dy, M, d, lddy));
     CHECK(check_matrix(what, "w", w, d, f, ldw));
-    CHECK(check_matrix(what, "gu", gu, M, 2 * (int64_t)f, ldgu));
+    CHECK(check_matrix(what, "gu", gu, M, 2 * (int64_t)f, 2 * (int64_t)f));
     CHECK(check_matrix(what, "dgu", dgu, M, 2 * (int64_t)f, lddgu));
     if (h) CHECK(check_matrix(what, "h", h, M, f, ldh));
     DenseArgs a{};
     a.p = w; a.ldp = ldw * 2; a.q = dy; a.ldq = lddy * 2;
     a.M = (int32_t)M; a.N = f; a.K = d;
-    a.c = dgu; a.ldc = lddgu; a.gu = const_cast<void *>(gu); a.ldgu = ldgu; a.h = h; a.ldh = ldh;
+    a.c = dgu; a.ldc = lddgu; a.h = h; a.ldh = ldh;
+    a.gu = static_cast<uint16_t *>(const_cast<void *>(gu)); a.gul = static_cast<uint8_t *>(const_cast<void *>(gu)) + M * 4 * f;
     a.steps = (d + 63) / 64; a.splits = 1;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const Plan p = plan_tiles(M, f, d, false, false);
-    return type == MORTAR_BF16 ? launch_product<DENSE_BF16, DENSE_SWIGLU_BWD, true, false>(a, p.tile, st, what)
-                               : launch_product<DENSE_F16, DENSE_SWIGLU_BWD, true, false>(a, p.tile, st, what);
+    return type == MORTAR_BF16 ? dense_launch<DENSE_BF16, DENSE_SWIGLU_BWD, true, false>(a, p.tile, st, what)
+                               : dense_launch<DENSE_F16, DENSE_SWIGLU_BWD, true, false>(a, p.tile, st, what);
 }

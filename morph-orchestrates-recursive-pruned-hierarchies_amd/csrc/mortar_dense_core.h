@@ -16,6 +16,7 @@
 #define MORTAR_DENSE_CORE_H
 
 #include "mortar_device.h"
+#include "mortar_internal.h"
 
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
@@ -36,12 +37,12 @@ struct DenseArgs {
     int32_t M, N, K;               // N: columns of C (DENSE_SWIGLU: d_ff); K in values
     void *c;                       // C / h (DENSE_SWIGLU) / dgu (DENSE_SWIGLU_BWD) / slabs (DENSE_PARTIAL), leading dimension in values
     int64_t ldc;
-    void *gu;                      // DENSE_SWIGLU: gate_up output to store or null; DENSE_SWIGLU_BWD: the stored one
-    int64_t ldgu;
+    uint16_t *gu;                  // DENSE_SWIGLU: gate_up output to store or null; DENSE_SWIGLU_BWD: the stored one.  The upper 24 bits of
+    uint8_t *gul;                  // the fp32 values: 16 bits [M, 2 N] in gu, 8 bits [M, 2 N] in gul
     void *h;                       // DENSE_SWIGLU_BWD: h to store or null
     int64_t ldh;
     const float *sx, *sw;          // e4m3: scales of Q per (m, K block) with strides, of P per (128 n, K block)
-    int64_t sx_m, sx_k, sw_n;
+    int64_t sx_m, sx_k, sw_n;      // (4 M sx_m is below 2^31)
     int32_t tiles_n, tiles_m;
     int32_t steps, splits;         // K steps in all, and how many ranges they are cut into
 };
@@ -87,18 +88,20 @@ struct DenseSlice {
     static constexpr int BYTES = ROWS * 128, L = BYTES / 1024 / NW;
     static_assert(L * 1024 * NW == BYTES, "whole instructions per wave");
     static constexpr int UPR = COLS ? ROWS / 8 : 8;          // 16-byte units per LDS row
-    static constexpr int RPI = 64 / UPR;                     // LDS rows per instruction
+    static constexpr bool EVEN = 64 % UPR == 0;              // an instruction fills whole LDS rows
     const char *base;
-    uint32_t off[L];       // of this lane's unit in the first K step
-    uint32_t kpos[L];      // and where in K it lies: bytes (rows) or values (columns)
-    int64_t step;          // bytes from one K step to the next
+    uint32_t off[L];              // of this lane's unit in the first K step
+    int kpos[COLS && !EVEN ? L : 1];      // where in a K step it lies: bytes (rows: the same in all copies) or values (columns)
+    int64_t step;                 // bytes from one K step to the next
 
     // Permutation of a K-strided slice: 32-byte pieces (16 n, one fragment's width) of the rows that one transposing read
     // touches, 4 rows per 16 lanes at distances of 8, fall into different pieces of the 256-byte bank window.
+    // (Of 192 columns the last four pieces only change places among themselves: two rows of the eight meet there.)
     static __device__ __forceinline__ int piece_swz(int k) {
         if constexpr (ROWS == 64) return ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
         else return (k & 3) | ((k >> 3) & 1) << 2;
     }
+    static __device__ __forceinline__ int piece(int c, int k) { return c ^ (ROWS == 192 && c >= 8 ? piece_swz(k) & 3 : piece_swz(k)); }
 
     // row_of(r): row of the matrix that LDS row r of a K-contiguous slice holds, relative to `base`, or -1;
     // n_left: columns from `base` on of a K-strided one.
@@ -108,25 +111,27 @@ struct DenseSlice {
         step = COLS ? 64 * ld : 128;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int r = (wave * L + i) * RPI + lane / UPR, u = lane % UPR;
+            const int t = (wave * L + i) * 64 + lane, r = t / UPR, u = t % UPR;
             if constexpr (COLS) {
-                const int src = ((u >> 1) ^ piece_swz(r)) << 1 | (u & 1);
-                kpos[i] = r;
+                const int src = piece(u >> 1, r) << 1 | (u & 1);
+                if (i < (int)(sizeof kpos / 4)) kpos[i] = r;
                 off[i] = src * 8 < n_left ? (uint32_t)(r * ld) + src * 16 : DENSE_OUTSIDE;
             } else {
                 const int src = u ^ (r & 7), row = row_of(r);
-                kpos[i] = src * 16;
+                if (i == 0) kpos[0] = src * 16;         // (r & 7 is the lane's alone)
                 off[i] = row >= 0 ? (uint32_t)(row * ld) + src * 16 : DENSE_OUTSIDE;
             }
         }
     }
-    // Copies K step s (K values in all) to LDS address `lds` (the wave's first kilobyte is wave * L).
-    __device__ __forceinline__ void copy(int s, int K, uint32_t lds) const {
-        const u32x4_t buf = dense_buffer(base + s * step);
-        const int left = COLS ? K - s * 64 : K * ESIZE - s * 128;
-        const bool whole = left >= (COLS ? 64 : 128);
-#pragma unroll
-        for (int i = 0; i < L; ++i) dense_copy(buf, whole || (int)kpos[i] < left ? off[i] : DENSE_OUTSIDE, lds + i * 1024);
+    // What is left of K from step s on, in the units of kpos.
+    static __device__ __forceinline__ int left(int s, int K) { return COLS ? K - s * 64 : K * ESIZE - s * 128; }
+    __device__ __forceinline__ u32x4_t buffer(int s) const { return dense_buffer(base + s * step); }
+    // Copy i of a whole K step.
+    __device__ __forceinline__ void copy(int i, u32x4_t buf, uint32_t lds) const { dense_copy(buf, off[i], lds + i * 1024); }
+    // Copy i of a K step with `left` to go, to LDS address `lds` (the wave's first kilobyte is wave * L).
+    __device__ __forceinline__ void copy(int i, u32x4_t buf, int left, uint32_t lds) const {
+        const int k = COLS ? (EVEN ? kpos[0] + i * (64 / UPR) : kpos[EVEN ? 0 : i]) : kpos[0];
+        dense_copy(buf, k < left ? off[i] : DENSE_OUTSIDE, lds + i * 1024);
     }
 };
 
@@ -137,11 +142,12 @@ __device__ __forceinline__ uint32_t dense_row_addr(int row, int lane) {
 __device__ __forceinline__ u32x4_t dense_read(uint32_t addr) {
     return *(const MORTAR_LDS u32x4_t *)(uintptr_t)addr;
 }
-// The same of a K-strided slice: K values 32 s + 8 g + 4 t + {0..3} of column (lane & 15) in half t.
+// The same of a K-strided slice: K values 32 s + 8 g + 4 t + {0..3} of column (lane & 15) in half t.  Address of fragment `first`
+// (a multiple of the power of two that is the number of the wave's fragments); fragment first + i lies at ^ (32 i).
 template <int ROWS>
-__device__ __forceinline__ uint32_t dense_col_addr(int frag, int lane) {
+__device__ __forceinline__ uint32_t dense_col_addr(int first, int lane) {
     const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
-    return (uint32_t)(k * ROWS * 2 + (frag ^ DenseSlice<ROWS, true, 1, 2>::piece_swz(k)) * 32 + (lane & 3) * 8);
+    return (uint32_t)(k * ROWS * 2 + DenseSlice<ROWS, true, 1, 2>::piece(first, k) * 32 + (lane & 3) * 8);
 }
 template <int ROWS>
 __device__ __forceinline__ u32x4_t dense_read_t(uint32_t addr) {
@@ -183,40 +189,94 @@ __device__ __forceinline__ void dense_unpack8(u32x4_t w, float (&v)[8]) {
     }
 }
 
+// The gate and up values that the backward needs are kept in the upper 24 bits of their fp32 sums, 16 bits in one array and 8 in
+// another: rounded to 16 alone, they were the largest part of the gradients' error (root mean square 3.5e-3 of the bf16 gradients
+// instead of 2.4e-3, of which 1.7e-3 is their own rounding).  One byte more per value is 2 % of a training step.
+__device__ __forceinline__ uint32_t dense_round24(float f) { return __builtin_bit_cast(uint32_t, f) + 0x80u; }       // (a NaN of the matrix cores has zeros there)
+__device__ __forceinline__ uint32_t dense_hi2(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+__device__ __forceinline__ uint32_t dense_lo4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0501u), __builtin_amdgcn_perm(b, a, 0x0c0c0501u), 0x05040100u);
+}
+__device__ __forceinline__ void dense_store24(uint16_t *hi, uint8_t *lo, int64_t at, const float (&v)[8]) {
+    uint32_t u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = dense_round24(v[j]);
+    *reinterpret_cast<u32x4_t *>(hi + at) = u32x4_t{dense_hi2(u[0], u[1]), dense_hi2(u[2], u[3]), dense_hi2(u[4], u[5]), dense_hi2(u[6], u[7])};
+    *reinterpret_cast<u32x2_t *>(lo + at) = u32x2_t{dense_lo4(u[0], u[1], u[2], u[3]), dense_lo4(u[4], u[5], u[6], u[7])};
+}
+__device__ __forceinline__ void dense_load24(const uint16_t *hi, const uint8_t *lo, int64_t at, float (&v)[8]) {
+    const u32x4_t h = *reinterpret_cast<const u32x4_t *>(hi + at);
+    const u32x2_t l = *reinterpret_cast<const u32x2_t *>(lo + at);
+    constexpr uint32_t pick[4] = {0x0504000cu, 0x0706010cu, 0x0504020cu, 0x0706030cu};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t hw = h[j >> 1], lw = l[j >> 2];
+        v[j] = __builtin_bit_cast(float, __builtin_amdgcn_perm(hw, lw, pick[j & 3]));
+    }
+}
+
 __device__ __forceinline__ float dense_sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
-template <DenseType T, DenseEpilogue E, bool PC, bool QC, int BN, int BM, int WN, int WM>
-__global__ __launch_bounds__(WN *WM * 64, WN *WM >= 8 ? 2 : 2) void dense_tile_kernel(const DenseArgs a) {
+template <int V>
+struct Const {
+    static constexpr int value = V;
+};
+
+template <DenseType T, DenseEpilogue E, bool PC, bool QC, int BN, int BM, int WN, int WM, int NS>
+__global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseArgs a) {
     constexpr int NW = WN * WM, FN = BN / WN / 16, FM = BM / WM / 16, ES = T == DENSE_E4M3 ? 1 : 2;
     static_assert(T != DENSE_E4M3 || (!PC && !QC), "e4m3 operands are K-contiguous");
     static_assert(FN % (E == DENSE_SWIGLU ? 4 : 2) == 0, "fragments are joined in pairs");
+    static_assert((FN & (FN - 1)) == 0, "K-strided fragments of P are found by xor");
     constexpr int PB = BN * 128, STAGE = PB + BM * 128;
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wn = wave % WN, wm = wave / WN, g = lane >> 4;
+    const int wn = wave % WN, wm = wave / WN;
+    const int fp = wn * FN, fq = wm * FM;            // first fragments of the wave
+    using SliceP = DenseSlice<BN, PC, NW, ES>;
+    using SliceQ = DenseSlice<BM, QC, NW, ES>;
+    const uint32_t l0 = mortar_lds_addr(lds), lp = l0 + wave * SliceP::L * 1024, lq = l0 + PB + wave * SliceQ::L * 1024;
+    const uint32_t ap = l0 + (PC ? dense_col_addr<BN>(fp, lane) : dense_row_addr(fp * 16, lane));
+    constexpr bool XQ = (FM & (FM - 1)) == 0;        // so are those of Q, if their number is a power of two
+    uint32_t aq[QC && !XQ ? FM : 1];
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof aq / 4); ++j) aq[j] = l0 + PB + (QC ? dense_col_addr<BM>(fq + j, lane) : dense_row_addr(fq * 16, lane));
+    const auto read_p = [&](int i, int h, uint32_t stage) {
+        if constexpr (PC) return dense_read_t<BN>(((ap + stage) ^ (i * 32)) + h * 32 * BN * 2);
+        else return dense_read(((ap + stage) ^ (h * 64)) + i * 2048);
+    };
+    const auto read_q = [&](int j, int h, uint32_t stage) {
+        if constexpr (QC) return dense_read_t<BM>((XQ ? (aq[0] + stage) ^ (j * 32) : aq[XQ ? 0 : j] + stage) + h * 32 * BM * 2);
+        else return dense_read(((aq[0] + stage) ^ (h * 64)) + j * 2048);
+    };
 
-    // Workgroups of one XCD (blockIdx % 8) take a contiguous run of tiles, in bands of 8 tiles along m, so that the operands
+    // Workgroups of one XCD (blockIdx % 8) walk over a contiguous run of tiles, in bands of 8 tiles along m, so that the operands
     // which the 32 of them share at a time stay in their L2.
-    const int tiles = a.tiles_n * a.tiles_m;
-    const int per_xcd = (tiles * a.splits + 7) >> 3;
-    const int t0 = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if (t0 >= tiles * a.splits) return;
-    const int split = t0 / tiles, t = t0 - split * tiles;
-    const int band = t / (8 * a.tiles_n), rest = t - band * 8 * a.tiles_n;
-    const int bh = min(8, a.tiles_m - band * 8);
-    const int tn = rest / bh, tm = band * 8 + rest - tn * bh;
-    const int first = (int)((int64_t)a.steps * split / a.splits), last = (int)((int64_t)a.steps * (split + 1) / a.splits);
-
-    // DENSE_SWIGLU: LDS rows of a wave's half are BN / WN / 2 gate features, then the same up features
+    const int tiles = a.tiles_n * a.tiles_m, total = tiles * a.splits;
+    const int xcd = blockIdx.x & 7, stride = gridDim.x >> 3, per_xcd = (total + 7) >> 3;
+    const int end = min(total, (xcd + 1) * per_xcd);
     constexpr int FEAT = E == DENSE_SWIGLU ? BN / 2 : BN;
-    const int n0 = tn * FEAT, m0 = tm * BM;
-    DenseSlice<BN, PC, NW, ES> P;
-    DenseSlice<BM, QC, NW, ES> Q;
-    {
-        const char *pb = static_cast<const char *>(a.p) + (PC ? (int64_t)n0 * ES : (int64_t)n0 * a.ldp);
-        const int n_left = a.N - n0;
+    struct Tile {
+        int n0, m0, split, first, last;
+    };
+    const auto tile_of = [&](int id) {
+        Tile r;
+        r.split = id / tiles;
+        const int t = id - r.split * tiles, band = t / (8 * a.tiles_n), rest = t - band * 8 * a.tiles_n;
+        const int bh = min(8, a.tiles_m - band * 8), tn = rest / bh;
+        r.n0 = tn * FEAT;
+        r.m0 = (band * 8 + rest - tn * bh) * BM;
+        r.first = a.steps * r.split / a.splits;
+        r.last = a.steps * (r.split + 1) / a.splits;
+        return r;
+    };
+    SliceP P;
+    SliceQ Q;
+    const auto aim = [&](const Tile &t) {
+        const char *pb = static_cast<const char *>(a.p) + (PC ? (int64_t)t.n0 * ES : (int64_t)t.n0 * a.ldp);
+        const int n_left = a.N - t.n0;
         P.init(pb, a.ldp, wave, lane, [&](int r) {
-            if constexpr (E == DENSE_SWIGLU) {
+            if constexpr (E == DENSE_SWIGLU) {       // LDS rows of a wave's half are BN / WN / 2 gate features, then the same up features
                 constexpr int H = BN / WN / 2;
                 const int f = r / (2 * H) * H + r % H;
                 return f < n_left ? f + (r / H & 1) * a.N : -1;
@@ -224,106 +284,226 @@ __global__ __launch_bounds__(WN *WM * 64, WN *WM >= 8 ? 2 : 2) void dense_tile_k
                 return r < n_left ? r : -1;
             }
         }, n_left);
-        const char *qb = static_cast<const char *>(a.q) + (QC ? (int64_t)m0 * ES : (int64_t)m0 * a.ldq);
-        const int m_left = a.M - m0;
+        const char *qb = static_cast<const char *>(a.q) + (QC ? (int64_t)t.m0 * ES : (int64_t)t.m0 * a.ldq);
+        const int m_left = a.M - t.m0;
         Q.init(qb, a.ldq, wave, lane, [&](int r) { return r < m_left ? r : -1; }, m_left);
-    }
-    const uint32_t l0 = mortar_lds_addr(lds), lp = l0 + wave * P.L * 1024, lq = l0 + PB + wave * Q.L * 1024;
-    const auto copy = [&](int s, int stage) {
-        P.copy(s, a.K, lp + stage * STAGE);
-        Q.copy(s, a.K, lq + stage * STAGE);
     };
-
-    // this lane's read addresses in stage 0
-    const int fp = wn * FN, fq = wm * FM;            // first fragment of the wave
-    uint32_t ap[PC ? FN : 1], aq[QC ? FM : 1];
-    if constexpr (PC) {
+    // Copies run ahead of the products over the steps of this workgroup's tiles, one behind the other: step `ahead` of tile `aim_id` is
+    // the next to be copied.
+    constexpr int COPIES = SliceP::L + SliceQ::L, RING = NS * STAGE, FIRST = NS;
+    const auto behind = [](uint32_t st) { return st + STAGE == RING ? 0u : st + STAGE; };
+    int id = xcd * per_xcd + (int)(blockIdx.x >> 3);
+    if (id >= end) return;
+    int aim_id = id, ahead, ahead_last;
+    const auto aim_at = [&](int which) {
+        const Tile t = tile_of(which);
+        aim(t);
+        ahead = t.first;
+        ahead_last = t.last;
+    };
+    const auto advance = [&] {
+        if (++ahead == ahead_last && (aim_id += stride) < end) aim_at(aim_id);
+    };
+    const auto copying = [&] { return aim_id < end; };
+    const auto copy_all = [&](uint32_t st) {
+        const u32x4_t pb = P.buffer(ahead), qb = Q.buffer(ahead);
 #pragma unroll
-        for (int i = 0; i < FN; ++i) ap[i] = l0 + dense_col_addr<BN>(fp + i, lane);
-    } else {
-        ap[0] = l0 + dense_row_addr(fp * 16, lane);
-    }
-    if constexpr (QC) {
+        for (int i = 0; i < SliceP::L; ++i) P.copy(i, pb, P.left(ahead, a.K), lp + st);
 #pragma unroll
-        for (int j = 0; j < FM; ++j) aq[j] = l0 + PB + dense_col_addr<BM>(fq + j, lane);
-    } else {
-        aq[0] = l0 + PB + dense_row_addr(fq * 16, lane);
-    }
-    const auto read_p = [&](int i, int s, uint32_t stage) {
-        if constexpr (PC) return dense_read_t<BN>(ap[i] + stage + s * 32 * BN * 2);
-        else return dense_read(((ap[0] + stage) ^ (s * 64)) + i * 2048);
+        for (int i = 0; i < SliceQ::L; ++i) Q.copy(i, qb, Q.left(ahead, a.K), lq + st);
     };
-    const auto read_q = [&](int j, int s, uint32_t stage) {
-        if constexpr (QC) return dense_read_t<BM>(aq[j] + stage + s * 32 * BM * 2);
-        else return dense_read(((aq[0] + stage) ^ (s * 64)) + j * 2048);
+    aim_at(id);
+    uint32_t stage = 0;                              // of the step that is multiplied next
+#pragma unroll
+    for (int i = 0; i < FIRST; ++i)
+        if (copying()) {
+            copy_all(i * STAGE);
+            advance();
+        }
+    // Waits until this wave's copies of a step have landed and every wave is here, all its LDS reads done.  `newer` steps were copied
+    // behind that step if there still is one to be copied: then their copies may be on their way.
+    const auto meet = [&](auto newer) {
+        if (newer.value > 0 && copying()) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(newer.value * COPIES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
-
+    meet(Const<FIRST - 1>{});
+    for (;;) {
     f32x4_t acc[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const Tile cur = tile_of(id);
+    const int n0 = cur.n0, m0 = cur.m0;
+    id += stride;
+    const bool more = id < end;
 
-    // e4m3: the scales of the next step's blocks
-    float sx[FM], sw = 0.f;
-    const float *sxp[FM];
-    const float *swp = nullptr;
-    const auto load_scales = [&](int s) {
-        sw = swp[s];
-#pragma unroll
-        for (int j = 0; j < FM; ++j) sx[j] = sxp[j][s * a.sx_k];
-    };
+    int s = cur.first;
+    const bool long_run = s + NS + 1 < cur.last;      // the copies are NS steps ahead in this tile
     if constexpr (T == DENSE_E4M3) {
+        // One matrix instruction is a step deep: FN groups of FM products, scaled and added a group later.  Fragments of P are read two groups
+        // ahead, those of Q behind their last use; all waves meet two groups before the end, when the step is in registers.
         const int nb = min(n0 + fp * 16, a.N - 1) >> 7;
-        swp = a.sw + nb * a.sw_n;
+        const float *swp = a.sw + nb * a.sw_n;
+        uint32_t sxo[FM];                             // bytes
+        float sx[FM], sw;                             // the scales of the next step
 #pragma unroll
-        for (int j = 0; j < FM; ++j) sxp[j] = a.sx + min(m0 + (fq + j) * 16 + (lane & 15), a.M - 1) * a.sx_m;
-        if (first < last) load_scales(first);
-    }
-
-    if (first < last) copy(first, 0);
-    for (int s = first; s < last; ++s) {
-        // this step's slices have landed for every wave, and every wave has read the other stage into registers
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int cur = (s - first) & 1;
-        if (s + 1 < last) copy(s + 1, cur ^ 1);
-        const uint32_t stage = cur * STAGE;
-        if constexpr (T == DENSE_E4M3) {
+        for (int j = 0; j < FM; ++j) sxo[j] = (uint32_t)(min(m0 + (fq + j) * 16 + (lane & 15), a.M - 1) * (int)a.sx_m) * 4;
+        const auto load_scales = [&](int k) {
+            sw = swp[k];
+            const char *row = reinterpret_cast<const char *>(a.sx + k * a.sx_k);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) sx[j] = *reinterpret_cast<const float *>(row + sxo[j]);
+        };
+        float sum[FN][FM][4];                         // (single floats: as vectors they are copied about)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) sum[i][j][v] = 0.f;
+        const auto whole = [](u32x4_t x, u32x4_t y) { return i32x8_t{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]}; };
+        i32x8_t pf[FN], qf[FM];
+        load_scales(s);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) qf[j] = whole(read_q(j, 0, stage), read_q(j, 1, stage));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) pf[i] = whole(read_p(i, 0, stage), read_p(i, 1, stage));
+        constexpr int MEET = FN - 2, EACH = (COPIES + 1) / 2;
+        const auto step = [&](auto on, auto plain, int k, int scales) {          // as below; scales: the step whose scales are loaded
             float f[FM];
 #pragma unroll
             for (int j = 0; j < FM; ++j) f[j] = sx[j] * sw;
-            if (s + 1 < last) load_scales(s + 1);
-            i32x8_t qf[FM];
+            if constexpr (on.value) load_scales(scales);
+            f32x4_t d[2][FM];
+            const auto add = [&](int i) {
 #pragma unroll
-            for (int j = 0; j < FM; ++j) {
-                const u32x4_t x = read_q(j, 0, stage), y = read_q(j, 1, stage);
-                qf[j] = i32x8_t{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-            }
+                for (int j = 0; j < FM; ++j)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) sum[i][j][v] = __builtin_fmaf(d[i & 1][j][v], f[j], sum[i][j][v]);
+            };
+            const uint32_t next = behind(stage);
+            bool go = true;
+            u32x4_t pb{}, qb{};
 #pragma unroll
             for (int i = 0; i < FN; ++i) {
-                const u32x4_t x = read_p(i, 0, stage), y = read_p(i, 1, stage);
-                const i32x8_t pf = {(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
-#pragma unroll
-                for (int j = 0; j < FM; ++j) {
-                    const f32x4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pf, qf[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[i][j][v] = __builtin_fmaf(d[v], f[j], acc[i][j][v]);
+                if (i == MEET) {
+                    if constexpr (plain.value) {
+                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * COPIES) : "memory");
+                    } else {
+                        meet(Const<NS - 2>{});
+                        k = ahead;
+                        go = copying();
+                    }
+                    pb = P.buffer(k), qb = Q.buffer(k);
                 }
-            }
-        } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x4_t qf[FM];
+                for (int j = 0; j < FM; ++j)
+                    d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pf[i], qf[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+                if (i + 2 < FN) pf[i + 2] = whole(read_p(i + 2, 0, stage), read_p(i + 2, 1, stage));
+                else if constexpr (on.value) pf[i + 2 - FN] = whole(read_p(i + 2 - FN, 0, next), read_p(i + 2 - FN, 1, next));
+                if (i >= MEET && go) {
 #pragma unroll
-                for (int j = 0; j < FM; ++j) qf[j] = read_q(j, h, stage);
-#pragma unroll
-                for (int i = 0; i < FN; ++i) {
-                    const u32x4_t pf = read_p(i, h, stage);
-#pragma unroll
-                    for (int j = 0; j < FM; ++j) acc[i][j] = dense_mfma<T>(pf, qf[j], acc[i][j]);
+                    for (int q = (i - MEET) * EACH; q < (i - MEET + 1) * EACH && q < COPIES; ++q) {
+                        if constexpr (plain.value) {
+                            if (q < SliceP::L) P.copy(q, pb, lp + stage);
+                            else Q.copy(q - SliceP::L, qb, lq + stage);
+                        } else {
+                            if (q < SliceP::L) P.copy(q, pb, P.left(k, a.K), lp + stage);
+                            else Q.copy(q - SliceP::L, qb, Q.left(k, a.K), lq + stage);
+                        }
+                    }
                 }
+                if (i) add(i - 1);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            if constexpr (on.value) {
+#pragma unroll
+                for (int j = 0; j < FM; ++j) qf[j] = whole(read_q(j, 0, next), read_q(j, 1, next));
+            }
+            add(FN - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!plain.value && go) advance();
+            stage = next;
+        };
+        if (long_run) {
+            for (; s + NS + 1 < cur.last; ++s) step(Const<1>{}, Const<1>{}, s + NS, s + 1);
+            ahead = s + NS;
         }
+        for (; s + 1 < cur.last; ++s) step(Const<1>{}, Const<0>{}, 0, s + 1);
+        step(Const<0>{}, Const<0>{}, 0, 0);
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+#pragma unroll
+            for (int j = 0; j < FM; ++j) acc[i][j] = f32x4_t{sum[i][j][0], sum[i][j][1], sum[i][j][2], sum[i][j][3]};
+    } else {
+        // A step is two halves of K.  While the matrix cores work on one half its successor is read from LDS into the other set of
+        // registers; between the halves of a step all waves meet: the step is then in registers everywhere and its stage free for
+        // the copies, and the next step has landed.
+        u32x4_t pf[2][FN], qf[2][FM];
+        // Per group of FM products: the fragments of Q first, then those of P, each behind the products that free a register for it.
+        constexpr int EACH = (COPIES + FN - 1) / FN;
+        constexpr auto reads = [](int groups) { return groups == 0 ? 0 : groups == FN ? FM + FN : FM + (3 * (groups - 1) / 2 < FN ? 3 * (groups - 1) / 2 : FN); };
+#pragma unroll
+        for (int j = 0; j < FM; ++j) qf[0][j] = read_q(j, 0, stage);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) pf[0][i] = read_p(i, 0, stage);
+        // on: the tile goes on behind this step; plain: and so does the run of whole steps that are copied, `k` the one due
+        const auto step = [&](auto on, auto plain, int k) {
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+#pragma unroll
+                for (int q = reads(i); q < reads(i + 1); ++q) {
+                    if (q < FM) qf[1][q] = read_q(q, 1, stage);
+                    else pf[1][q - FM] = read_p(q - FM, 1, stage);
+                }
+#pragma unroll
+                for (int j = 0; j < FM; ++j) acc[i][j] = dense_mfma<T>(pf[0][i], qf[0][j], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if constexpr (plain.value) {
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * COPIES) : "memory");
+            } else {
+                meet(Const<NS - 2>{});
+                k = ahead;
+            }
+            const uint32_t next = behind(stage);
+            const bool go = plain.value || copying();
+            const u32x4_t pb = P.buffer(k), qb = Q.buffer(k);
+#pragma unroll
+            for (int i = 0; i < FN; ++i) {
+                if constexpr (on.value) {
+#pragma unroll
+                    for (int q = reads(i); q < reads(i + 1); ++q) {
+                        if (q < FM) qf[0][q] = read_q(q, 0, next);
+                        else pf[0][q - FM] = read_p(q - FM, 0, next);
+                    }
+                }
+                if (go) {
+#pragma unroll
+                    for (int q = i * EACH; q < (i + 1) * EACH && q < COPIES; ++q) {
+                        if constexpr (plain.value) {
+                            if (q < SliceP::L) P.copy(q, pb, lp + stage);
+                            else Q.copy(q - SliceP::L, qb, lq + stage);
+                        } else {
+                            if (q < SliceP::L) P.copy(q, pb, P.left(k, a.K), lp + stage);
+                            else Q.copy(q - SliceP::L, qb, Q.left(k, a.K), lq + stage);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < FM; ++j) acc[i][j] = dense_mfma<T>(pf[1][i], qf[1][j], acc[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (!plain.value && go) advance();
+            stage = next;
+        };
+        if (long_run) {
+            for (; s + NS + 1 < cur.last; ++s) step(Const<1>{}, Const<1>{}, s + NS);
+            ahead = s + NS;
+        }
+        for (; s + 1 < cur.last; ++s) step(Const<1>{}, Const<0>{}, 0);
+        step(Const<0>{}, Const<0>{}, 0);
     }
 
     // ---- epilogue: pairs of fragments joined to eight consecutive n per lane, 16-byte stores
@@ -345,9 +525,9 @@ __global__ __launch_bounds__(WN *WM * 64, WN *WM >= 8 ? 2 : 2) void dense_tile_k
                 if (n < a.N) {
                     *reinterpret_cast<u32x4_t *>(static_cast<uint16_t *>(a.c) + m * a.ldc + n) = dense_pack8<O>(hv);
                     if (a.gu) {
-                        uint16_t *o = static_cast<uint16_t *>(a.gu) + m * a.ldgu + n;
-                        *reinterpret_cast<u32x4_t *>(o) = dense_pack8<O>(gt);
-                        *reinterpret_cast<u32x4_t *>(o + a.N) = dense_pack8<O>(up);
+                        const int64_t at = m * 2 * a.N + n;
+                        dense_store24(a.gu, a.gul, at, gt);
+                        dense_store24(a.gu, a.gul, at + a.N, up);
                     }
                 }
             }
@@ -361,14 +541,14 @@ __global__ __launch_bounds__(WN *WM * 64, WN *WM >= 8 ? 2 : 2) void dense_tile_k
                 if constexpr (E == DENSE_STORE) {
                     *reinterpret_cast<u32x4_t *>(static_cast<uint16_t *>(a.c) + m * a.ldc + n) = dense_pack8<O>(d);
                 } else if constexpr (E == DENSE_PARTIAL) {
-                    float *o = static_cast<float *>(a.c) + ((int64_t)split * a.M + m) * a.N + n;
+                    float *o = static_cast<float *>(a.c) + ((int64_t)cur.split * a.M + m) * a.N + n;
                     *reinterpret_cast<f32x4_t *>(o) = f32x4_t{d[0], d[1], d[2], d[3]};
                     *reinterpret_cast<f32x4_t *>(o + 4) = f32x4_t{d[4], d[5], d[6], d[7]};
                 } else {
-                    const uint16_t *gu = static_cast<const uint16_t *>(a.gu) + m * a.ldgu + n;
+                    const int64_t at = m * 2 * a.N + n;
                     float gt[8], up[8], dg[8], du[8], hv[8];
-                    dense_unpack8<O>(*reinterpret_cast<const u32x4_t *>(gu), gt);
-                    dense_unpack8<O>(*reinterpret_cast<const u32x4_t *>(gu + a.N), up);
+                    dense_load24(a.gu, a.gul, at, gt);
+                    dense_load24(a.gu, a.gul, at + a.N, up);
 #pragma unroll
                     for (int v = 0; v < 8; ++v) {
                         const float sg = dense_sigmoid(gt[v]), si = gt[v] * sg;
@@ -384,6 +564,39 @@ __global__ __launch_bounds__(WN *WM * 64, WN *WM >= 8 ? 2 : 2) void dense_tile_k
             }
         }
     }
+    if (!more) return;
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+
+// The tiles: BN x BM of C by WN x WM waves, NS stages of LDS, workgroups per CU.  The larger the tile the fewer bytes go through the L1 for a
+// product (64 per cycle and CU is what it takes: 256 x 256 keeps it half busy, 256 x 128 three quarters); the smaller ones
+// are for matrices that do not fill the chip with large ones.
+struct DenseTile {
+    int bn, bm, wn, wm, stages, per_cu;
+};
+constexpr DenseTile DENSE_TILES[] = {{256, 256, 2, 4, 2, 1}, {256, 192, 2, 4, 2, 1}, {256, 128, 4, 2, 3, 1}, {128, 128, 2, 2, 2, 2}, {64, 64, 1, 4, 4, 2}};
+constexpr int DENSE_N_TILES = sizeof DENSE_TILES / sizeof DENSE_TILES[0];
+
+template <DenseType T, DenseEpilogue E, bool PC, bool QC, int I = 0>
+int dense_launch(DenseArgs a, int tile, hipStream_t st, const char *what) {
+    if constexpr (I + 1 < DENSE_N_TILES)
+        if (tile != I) return dense_launch<T, E, PC, QC, I + 1>(a, tile, st, what);
+    constexpr DenseTile D = DENSE_TILES[I];
+    const auto kern = dense_tile_kernel<T, E, PC, QC, D.bn, D.bm, D.wn, D.wm, D.stages>;
+    constexpr int smem = D.stages * (D.bn + D.bm) * 128, feat = E == DENSE_SWIGLU ? D.bn / 2 : D.bn;
+    static_assert(smem * D.per_cu <= 160 * 1024, "LDS");
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    const int64_t tn = ((int64_t)a.N + feat - 1) / feat, tm = ((int64_t)a.M + D.bm - 1) / D.bm, total = tn * tm * a.splits;
+    if (total > (1 << 30)) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tiles", what);
+    a.tiles_n = (int)tn;
+    a.tiles_m = (int)tm;
+    const int64_t per_xcd = (total + 7) / 8, slots = 32 * D.per_cu;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(8 * (per_xcd < slots ? per_xcd : slots))), dim3(D.wn * D.wm * 64), smem, st, a);
+    const hipError_t l = hipGetLastError();
+    return l == hipSuccess ? MORTAR_OK : mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(l));
 }
 
 #endif

@@ -25,7 +25,7 @@ __attribute__((visibility("hidden"))) int mortar_router_project_skinny(const uin
                                                                        int32_t d_out, const float *bias, float *qv, int64_t ldq, void *stream,
                                                                        const uint16_t *norm_w = nullptr, float eps = 0.f, uint16_t *xn = nullptr);
 
-// Tile edge (0: 256, 1: 128, 2: 64) and number of K ranges of a dense product C [M, N] with sums over K 16-bit values (e4m3: half their number).
+// Tile (index into DENSE_TILES) and number of K ranges of a dense product C [M, N] with sums over K 16-bit values (e4m3: half their number).
 struct MortarDensePlan {
     int tile, splits;
 };

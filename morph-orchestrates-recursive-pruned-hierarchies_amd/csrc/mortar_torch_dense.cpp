@@ -201,8 +201,8 @@ at::Tensor mlp_forward(const at::Tensor &x, const at::Tensor &wgu, const at::Ten
     void *st = stream_of(x);
     r.x = rows_of(x, d, 8);
     const at::Tensor h = empty_like_rows(x, {M, f});
-    if (keep) r.gu = empty_like_rows(x, {M, 2 * f});
-    check_rc(mortar_dense_gateup_swiglu(data(r.x), M, (int32_t)d, ld_of(r.x), data(r.wgu), ld_of(r.wgu), (int32_t)f, type, mut(h), f, mut(r.gu), 2 * f, st),
+    if (keep) r.gu = empty_bytes(x, 6 * M * f);
+    check_rc(mortar_dense_gateup_swiglu(data(r.x), M, (int32_t)d, ld_of(r.x), data(r.wgu), ld_of(r.wgu), (int32_t)f, type, mut(h), f, mut(r.gu), st),
              "mortar_dense_gateup_swiglu");
     const at::Tensor ws = M > 64 ? workspace(x, M, n, f) : at::Tensor();
     check_rc(mortar_dense_linear(data(h), M, (int32_t)f, f, data(r.wd), ld_of(r.wd), (int32_t)n, type, mut(y), n, floats(ws), st), "mortar_dense_linear");
@@ -239,7 +239,7 @@ struct DenseMlpFn : public torch::autograd::Function<DenseMlpFn> {
             void *st = stream_of(dy);
             const at::Tensor g = rows_of(dy, n, 8);
             const at::Tensor dgu = empty_like_rows(dy, {M, 2 * f}), h = need_dn ? empty_like_rows(dy, {M, f}) : at::Tensor();
-            check_rc(mortar_dense_swiglu_bwd(data(g), M, (int32_t)n, ld_of(g), data(wd), ld_of(wd), (int32_t)f, type, data(gu), 2 * f, mut(dgu), 2 * f, mut(h), f, st),
+            check_rc(mortar_dense_swiglu_bwd(data(g), M, (int32_t)n, ld_of(g), data(wd), ld_of(wd), (int32_t)f, type, data(gu), mut(dgu), 2 * f, mut(h), f, st),
                      "mortar_dense_swiglu_bwd");
             if (need_dn) {
                 ddw = empty_like_rows(dy, {n, f});

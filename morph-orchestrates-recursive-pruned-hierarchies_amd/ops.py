@@ -568,8 +568,8 @@ def layernorm(x: Tensor, weight: Tensor | None = None, bias: Tensor | None = Non
 def dense_mlp(x: Tensor, w_gate_up: Tensor, w_down: Tensor) -> Tensor:
     """The SwiGLU MLP of a block that is not carved, differentiable: y = (silu(x Wg^T) * (x Wu^T)) Wd^T with w_gate_up = [Wg; Wu]
     [2 * d_ff, d] and w_down [d_out, d_ff], all bf16 or all fp16, widths multiples of 8.  gate_up, silu and the product are one
-    launch; sums are fp32, the hidden activations rounded to 16 bits between the two launches.  The backward keeps the gate_up
-    output [rows, 2 * d_ff] and forms its gradient in the epilogue of dy Wd.  First derivatives only."""
+    launch; sums are fp32, the hidden activations rounded to 16 bits between the two launches.  For the backward the
+    gate_up output [rows, 2 * d_ff] is kept in 24 bits per value; its gradient is formed in the epilogue of dy Wd.  First derivatives only."""
     return _lib.native().dense_mlp(x, w_gate_up, w_down)
 
 
