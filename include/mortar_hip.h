@@ -599,6 +599,7 @@ int mortar_sdd_bf16(const int32_t *plan, int32_t n_wg, int32_t blocks_per_wave, 
  * workspace: mortar_dense_workspace_bytes(rows, columns, length of the sums) bytes of device memory, 16-byte aligned, where that is not 0
  * (dw: (n_out, n_in, M)): fp32 sums over ranges of K, added in a fixed order. */
 enum { MORTAR_BF16 = 0, MORTAR_FP16 = 1, MORTAR_FP32 = 2 };
+#define MORTAR_DENSE_FEW_ROWS 8        /* rows up to which forward products stream the weights past the rows */
 int64_t mortar_dense_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, int64_t ldx, const void *w, int64_t ldw, int32_t f, int32_t type,
                                void *h, int64_t ldh, void *gu, void *stream);

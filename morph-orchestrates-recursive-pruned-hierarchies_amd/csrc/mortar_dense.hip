@@ -23,24 +23,34 @@ int launch_error(const char *what) {
 
 using Plan = MortarDensePlan;
 
-// Which tile, and in how many K ranges, from the estimated cycles of the busiest CU: what a step of a tile takes with the chip full (measured,
-// at the 2 GHz that the chip runs under this load; workgroups that share a CU share its matrix cores), and no less than the way of
-// its copies; a tile's start and end; for K ranges a pass over their fp32 slabs and a launch.
-Plan plan_tiles(int64_t M, int64_t N, int64_t K, bool swiglu, bool may_split) {
-    constexpr double step_cycles[DENSE_N_TILES] = {2900, 2230, 1770, 920, 440}, way[DENSE_N_TILES] = {1500, 1500, 1000, 1500, 700};
-    constexpr double ends = 5000, slab_byte = 2 * 0.0005, launch = 8000;
-    const int64_t steps = (K + 63) / 64;
+// Which tile, and in how many K ranges: the smallest estimate of
+//   launch + rounds of workgroups * (steps * time of a step + end of a tile + its output bytes at a CU's share of the memory)
+// with, for K ranges, a second launch and the slabs' way out and back.  The times are those of the kernels as they are, fitted to 3200
+// measurements of the 16-bit products (80 to 16384 rows, widths 88 to 13000, all five tiles, up to 16 ranges, error 12 %); over these
+// the choice is 2 % slower than the best one on average (the best number of ranges of the fourth tile alone: 18 %, of the first: 80 %).
+struct TileTimes {
+    double step, step_alone, end;      // us; a step of one of several workgroups on a CU, of a workgroup alone there
+};
+constexpr TileTimes TIMES_16[DENSE_N_TILES] = {{1.23, 1.23, 2.1}, {0.94, 0.94, 1.2}, {0.75, 0.75, 1.3}, {0.91, 0.58, 0.7}, {0.43, 0.23, 1.2}};
+constexpr TileTimes TIMES_8[DENSE_N_TILES] = {{2.3, 2.3, 24}, {1.5, 1.5, 13}, {1.25, 1.25, 2.6}, {1.3, 0.8, 0.5}, {0.6, 0.33, 1.2}};
+
+Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int form) {
+    constexpr double byte = 2.5e-5, launch = 2.5, join = 2.1, slab_byte = 2.8e-7;
+    constexpr int ranges[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
+    const TileTimes *times = form == MORTAR_PLAN_E4M3 ? TIMES_8 : TIMES_16;
+    const bool swiglu = form == MORTAR_PLAN_SWIGLU || form == MORTAR_PLAN_SWIGLU_KEEP, plain = form == MORTAR_PLAN_PLAIN || form == MORTAR_PLAN_E4M3;
+    const int out = form == MORTAR_PLAN_SWIGLU_BWD ? 12 : form == MORTAR_PLAN_SWIGLU_KEEP ? 8 : 2;
     Plan best{0, 1};
     double best_t = 1e300;
     for (int c = 0; c < DENSE_N_TILES; ++c) {
         const int64_t bn = swiglu ? DENSE_TILES[c].bn / 2 : DENSE_TILES[c].bn, bm = DENSE_TILES[c].bm;
         const int64_t tiles = ((N + bn - 1) / bn) * ((M + bm - 1) / bm);
-        for (int s = 1; s <= 16; s *= 2) {
-            if (s > 1 && (!may_split || steps / s < 4)) break;
+        for (const int s : ranges) {
+            if (s > 1 && (!plain || steps / s < 4)) break;
             const int64_t wgs = (tiles * s + 255) / 256, both = wgs < DENSE_TILES[c].per_cu ? wgs : DENSE_TILES[c].per_cu;
-            const double rounds = (double)wgs / both, per_step = both * step_cycles[c] > way[c] ? both * step_cycles[c] : way[c];
-            double t = rounds * ((double)((steps + s - 1) / s) * per_step + ends);
-            if (s > 1) t += launch + slab_byte * s * M * N * 4;
+            const double step = both == DENSE_TILES[c].per_cu ? times[c].step : times[c].step_alone;
+            double t = launch + (double)wgs / both * ((double)((steps + s - 1) / s) * step + times[c].end + both * byte * bn * bm * (s > 1 ? 4 : out));
+            if (s > 1) t += join + slab_byte * s * M * N * 4;
             if (t < best_t) {
                 best_t = t;
                 best = Plan{c, s};
@@ -50,28 +60,30 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t K, bool swiglu, bool may_split) {
     return best;
 }
 
-// Adds the slabs of the K ranges in their order.
+// Adds the slabs of the K ranges in their order, up to eight loads in flight.
 template <DenseType T>
 __global__ __launch_bounds__(256) void dense_join_kernel(const float *slabs, int splits, int64_t M, int64_t N, uint16_t *c, int64_t ldc) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = N >> 3;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = N >> 2;
     if (i >= M * per) return;
-    const int64_t m = i / per, n = (i - m * per) * 8;
+    const int64_t m = i / per, n = (i - m * per) * 4, slab = M * N / 4;
     const f32x4_t *p = reinterpret_cast<const f32x4_t *>(slabs + m * N + n);
-    f32x4_t lo = p[0], hi = p[1];
-    for (int s = 1; s < splits; ++s) {
-        p += M * N / 4;
-        lo += p[0];
-        hi += p[1];
+    f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; s += 8) {
+        f32x4_t v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = p[(s + k < splits ? s + k : s) * slab];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (s + k < splits) sum += v[k];
     }
-    const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    *reinterpret_cast<u32x4_t *>(c + m * ldc + n) = dense_pack8<T>(v);
+    *reinterpret_cast<u32x2_t *>(c + m * ldc + n) = u32x2_t{dense_pack2<T>(sum[0], sum[1]), dense_pack2<T>(sum[2], sum[3])};
 }
 
 // One plain product into 16-bit C, over K ranges where the plan has them.
 template <DenseType T, bool PC, bool QC>
 int run_plain(DenseArgs a, float *ws, hipStream_t st, const char *what) {
-    const Plan p = plan_tiles(a.M, a.N, a.K, false, true);
     a.steps = (a.K + 63) / 64;
+    const Plan p = plan_tiles(a.M, a.N, a.steps, MORTAR_PLAN_PLAIN);
     a.splits = p.splits;
     if (p.splits == 1) return dense_launch<T, DENSE_STORE, PC, QC>(a, p.tile, st, what);
     if (!ws) return mortar_fail(MORTAR_ERR_ARG, "%s: this shape needs a workspace", what);
@@ -83,74 +95,82 @@ int run_plain(DenseArgs a, float *ws, hipStream_t st, const char *what) {
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// Up to 64 rows the weights are the traffic: a workgroup owns 16 rows of W (with SWIGLU the 16 gate rows and their up rows),
-// its waves take K in turns of 64 values and read W straight into the matrix cores' operand registers, U turns (2 U loads per
-// row set) in flight; the waves' sums meet in LDS.
-constexpr int FEW_ROWS = 64;
+// Up to 8 rows the weights are the traffic, and the launch.  A workgroup owns 8 rows of W (with SWIGLU 8 gate rows and their up rows); the
+// matrix instruction's 16 rows and 16 columns hold two halves of K side by side, so that two of the four quarters of its result
+// are sums and the others are not used (with 16 rows per workgroup instead, `down` of 2048 rows keeps half of the chip).  W goes
+// straight into the operand registers, U turns of 64 values per half and wave in flight, while x is staged in LDS (read as
+// operands from memory it costs as many load cycles as W); the waves' and halves' sums meet there.  2048 / 5632, weights in no cache:
+// gate_up 10.2 us at one row and 11.7 at eight, down 5.9 and 7.7, where plain reads of the weights take 9.3 and 4.8 and the 64 x 64
+// tile 13.1 and 9.6 (its rows are then free up to 64).
+constexpr int FEW_ROWS = MORTAR_DENSE_FEW_ROWS, FEW_LDS = 96 * 1024;
 
-__device__ __forceinline__ u32x4_t buffer_read(__amdgpu_buffer_rsrc_t buf, uint32_t off) {
-    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(buf, off, 0, 0));
-}
+// x rows in LDS: two halves of whole turns, and 16 bytes so that the rows start on different banks.
+constexpr int64_t few_pitch(int64_t K) { return ((K + 63) / 64 + 1) / 2 * 256 + 16; }
 
-template <DenseType T, bool SWIGLU, int MT, int NW, int U>
+template <DenseType T, bool SWIGLU, int NW, int U>
 __global__ __launch_bounds__(NW * 64) void dense_few_kernel(const DenseArgs a) {
     constexpr int RS = SWIGLU ? 2 : 1;
-    extern __shared__ __attribute__((aligned(16))) f32x4_t part[];          // [wave][row set][token tile][lane]
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    f32x4_t *part = reinterpret_cast<f32x4_t *>(smem);                      // [wave][row set][lane]
+    unsigned char *xs = smem + NW * RS * 1024;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
-    const int n0 = blockIdx.x * 16;
-    const auto whole = [](const void *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, DENSE_OUTSIDE, 0x00020000); };
-    __amdgpu_buffer_rsrc_t wb[RS], xb = whole(a.q);
-    uint32_t wo, xo[MT];
-#pragma unroll
-    for (int s = 0; s < RS; ++s) wb[s] = whole(static_cast<const char *>(a.p) + ((int64_t)n0 + (int64_t)s * a.N) * a.ldp);
-    wo = n0 + r < a.N ? (uint32_t)(r * a.ldp) + g * 16 : DENSE_OUTSIDE;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) xo[t] = t * 16 + r < a.M ? (uint32_t)((t * 16 + r) * a.ldq) + g * 16 : DENSE_OUTSIDE;
-
-    f32x4_t acc[RS][MT];
+    const int n0 = blockIdx.x * 8, turns = (((a.K + 63) >> 6) + 1) >> 1, half = (r >> 3) * turns * 128;       // (half: bytes in front of it)
+    const int pitch = turns * 256 + 16;
+    __amdgpu_buffer_rsrc_t wb[RS];
 #pragma unroll
     for (int s = 0; s < RS; ++s)
+        wb[s] = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(static_cast<const char *>(a.p) + ((int64_t)n0 + (int64_t)s * a.N) * a.ldp), 0, DENSE_OUTSIDE, 0x00020000);
+    const uint32_t wo = (uint32_t)((r & 7) * a.ldp) + half + g * 16;
+    const int left = a.K * 2 - half - g * 16;                               // bytes of the row behind this lane's first unit
+    const unsigned char *xl = xs + min(r & 7, a.M - 1) * pitch + half + g * 16;
+
+    f32x4_t acc[RS];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[s][t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    const int turns = (a.K + 63) / 64;
-    for (int c0 = wave; c0 < turns; c0 += NW * U) {
-        u32x4_t w[U][2][RS], x[U][2][MT];
+    for (int s = 0; s < RS; ++s) acc[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = wave; c0 < turns || c0 == wave; c0 += NW * U) {
+        u32x4_t w[U][2][RS];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int kb = (c0 + u * NW) * 128 + h * 64;               // bytes into the rows
-                const bool in = kb + g * 16 < a.K * 2;
-#pragma unroll
-                for (int s = 0; s < RS; ++s) w[u][h][s] = buffer_read(wb[s], in ? wo + kb : DENSE_OUTSIDE);
-#pragma unroll
-                for (int t = 0; t < MT; ++t) x[u][h][t] = buffer_read(xb, in ? xo[t] + kb : DENSE_OUTSIDE);
-            }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * NW < turns ? c0 + u * NW : 0;            // (beyond the end: not used)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int s = 0; s < RS; ++s)
+                    w[u][h][s] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(wb[s], c * 128 + h * 64 < left ? wo : DENSE_OUTSIDE, c * 128 + h * 64, 0));
+        }
+        if (c0 == wave) {                                                   // every wave once
+            const int units = turns * 16;
+            for (int i = threadIdx.x; i < a.M * units; i += NW * 64) {
+                const int m = i / units, u = i - m * units;
+                u32x4_t v = {0, 0, 0, 0};
+                if (u * 8 < a.K) v = *reinterpret_cast<const u32x4_t *>(static_cast<const char *>(a.q) + m * a.ldq + u * 16);
+                *reinterpret_cast<u32x4_t *>(xs + m * pitch + u * 16) = v;
+            }
+            __syncthreads();
+        }
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) acc[s][t] = dense_mfma<T>(w[u][h][s], x[u][h][t], acc[s][t]);
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * NW < turns)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4_t x = *reinterpret_cast<const u32x4_t *>(xl + (c0 + u * NW) * 128 + h * 64);
+#pragma unroll
+                    for (int s = 0; s < RS; ++s) acc[s] = dense_mfma<T>(w[u][h][s], x, acc[s]);
+                }
     }
 #pragma unroll
-    for (int s = 0; s < RS; ++s)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) part[((wave * RS + s) * MT + t) * 64 + lane] = acc[s][t];
+    for (int s = 0; s < RS; ++s) part[(wave * RS + s) * 64 + lane] = acc[s];
     __syncthreads();
-    if (wave >= MT) return;
+    if (wave || g > 1 || r >= a.M) return;                                  // lane: token r, features 4 g .. 4 g + 3
     f32x4_t sum[RS];
 #pragma unroll
     for (int s = 0; s < RS; ++s) {
-        sum[s] = part[(s * MT + wave) * 64 + lane];
+        sum[s] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 1; w < NW; ++w) sum[s] += part[((w * RS + s) * MT + wave) * 64 + lane];
+        for (int w = 0; w < NW; ++w) sum[s] += part[(w * RS + s) * 64 + lane] + part[(w * RS + s) * 64 + lane + 40];       // + 40: the other half of K
     }
-    const int64_t m = wave * 16 + r;
+    const int64_t m = r;
     const int n = n0 + 4 * g;
-    if (m >= a.M || n >= a.N) return;
     const auto put = [&](void *c, int64_t at, f32x4_t v) {
         *reinterpret_cast<u32x2_t *>(static_cast<uint16_t *>(c) + at) = u32x2_t{dense_pack2<T>(v[0], v[1]), dense_pack2<T>(v[2], v[3])};
     };
@@ -173,20 +193,21 @@ __global__ __launch_bounds__(NW * 64) void dense_few_kernel(const DenseArgs a) {
     }
 }
 
-template <DenseType T, bool SWIGLU, int MT, int NW, int U>
+bool few_rows(int64_t M, int64_t K) { return M <= FEW_ROWS && M * few_pitch(K) <= FEW_LDS; }
+
+template <DenseType T, bool SWIGLU, int NW, int U>
 int launch_few_form(const DenseArgs &a, hipStream_t st, const char *what) {
-    const auto kern = dense_few_kernel<T, SWIGLU, MT, NW, U>;
-    constexpr int smem = NW * (SWIGLU ? 2 : 1) * MT * 1024;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const auto kern = dense_few_kernel<T, SWIGLU, NW, U>;
+    constexpr int sums = NW * (SWIGLU ? 2 : 1) * 1024;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, sums + FEW_LDS);
     if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-    hipLaunchKernelGGL(kern, dim3((unsigned)((a.N + 15) / 16)), dim3(NW * 64), smem, st, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.N / 8)), dim3(NW * 64), sums + a.M * few_pitch(a.K), st, a);
     return launch_error(what);
 }
 template <DenseType T, bool SWIGLU>
 int launch_few(const DenseArgs &a, hipStream_t st, const char *what) {
-    if (a.M <= 16) return launch_few_form<T, SWIGLU, 1, 16, 2>(a, st, what);
-    if (a.M <= 32) return launch_few_form<T, SWIGLU, 2, 16, 2>(a, st, what);
-    return launch_few_form<T, SWIGLU, 4, 16, 1>(a, st, what);
+    if constexpr (SWIGLU) return launch_few_form<T, true, 8, 2>(a, st, what);
+    else return launch_few_form<T, false, 16, 3>(a, st, what);
 }
 
 // ---- checks ----------------------------------------------------------------------------------------------------------
@@ -207,10 +228,10 @@ int check_type(const char *what, int32_t type) {
 
 }  // namespace
 
-MortarDensePlan mortar_dense_plan(int64_t M, int64_t N, int64_t K, int swiglu, int may_split) { return plan_tiles(M, N, K, swiglu, may_split); }
+MortarDensePlan mortar_dense_plan(int64_t M, int64_t N, int64_t steps, int form) { return plan_tiles(M, N, steps, form); }
 
 int mortar_dense_join(const float *slabs, int splits, int64_t M, int64_t N, int32_t type, void *c, int64_t ldc, void *stream) {
-    const int64_t n = M * (N / 8);
+    const int64_t n = M * (N / 4);
     if ((n + 255) / 256 >= INT32_MAX) return mortar_fail(MORTAR_ERR_LIMIT, "dense: too many results");
     const auto kern = type == MORTAR_FP16 ? dense_join_kernel<DENSE_F16> : dense_join_kernel<DENSE_BF16>;
     hipLaunchKernelGGL(kern, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), slabs, splits, M, N,
@@ -220,7 +241,7 @@ int mortar_dense_join(const float *slabs, int splits, int64_t M, int64_t N, int3
 
 extern "C" int64_t mortar_dense_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const Plan p = plan_tiles(M, N, K, false, true);
+    const Plan p = plan_tiles(M, N, (K + 63) / 64, MORTAR_PLAN_PLAIN);
     return p.splits > 1 ? p.splits * M * N * 4 : 0;
 }
 
@@ -242,8 +263,8 @@ extern "C" int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, i
     if (gu) a.gu = static_cast<uint16_t *>(gu), a.gul = static_cast<uint8_t *>(gu) + M * 4 * f;
     a.steps = (d + 63) / 64; a.splits = 1;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (M <= FEW_ROWS) return type == MORTAR_BF16 ? launch_few<DENSE_BF16, true>(a, st, what) : launch_few<DENSE_F16, true>(a, st, what);
-    const Plan p = plan_tiles(M, f, d, true, false);
+    if (few_rows(M, a.K)) return type == MORTAR_BF16 ? launch_few<DENSE_BF16, true>(a, st, what) : launch_few<DENSE_F16, true>(a, st, what);
+    const Plan p = plan_tiles(M, f, a.steps, gu ? MORTAR_PLAN_SWIGLU_KEEP : MORTAR_PLAN_SWIGLU);
     return type == MORTAR_BF16 ? dense_launch<DENSE_BF16, DENSE_SWIGLU, false, false>(a, p.tile, st, what)
                                : dense_launch<DENSE_F16, DENSE_SWIGLU, false, false>(a, p.tile, st, what);
 }
@@ -262,7 +283,7 @@ extern "C" int mortar_dense_linear(const void *x, int64_t M, int32_t K, int64_t 
     a.M = (int32_t)M; a.N = N; a.K = K;
     a.c = y; a.ldc = ldy;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (M <= FEW_ROWS) return type == MORTAR_BF16 ? launch_few<DENSE_BF16, false>(a, st, what) : launch_few<DENSE_F16, false>(a, st, what);
+    if (few_rows(M, a.K)) return type == MORTAR_BF16 ? launch_few<DENSE_BF16, false>(a, st, what) : launch_few<DENSE_F16, false>(a, st, what);
     return type == MORTAR_BF16 ? run_plain<DENSE_BF16, false, false>(a, workspace, st, what) : run_plain<DENSE_F16, false, false>(a, workspace, st, what);
 }
 
@@ -317,7 +338,7 @@ extern "C" int mortar_dense_swiglu_bwd(const void *dy, int64_t M, int32_t d, int
     a.gu = static_cast<uint16_t *>(const_cast<void *>(gu)); a.gul = static_cast<uint8_t *>(const_cast<void *>(gu)) + M * 4 * f;
     a.steps = (d + 63) / 64; a.splits = 1;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const Plan p = plan_tiles(M, f, d, false, false);
+    const Plan p = plan_tiles(M, f, a.steps, MORTAR_PLAN_SWIGLU_BWD);
     return type == MORTAR_BF16 ? dense_launch<DENSE_BF16, DENSE_SWIGLU_BWD, true, false>(a, p.tile, st, what)
                                : dense_launch<DENSE_F16, DENSE_SWIGLU_BWD, true, false>(a, p.tile, st, what);
 }

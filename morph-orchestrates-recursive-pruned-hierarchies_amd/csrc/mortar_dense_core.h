@@ -376,11 +376,9 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
             for (int j = 0; j < FM; ++j) f[j] = sx[j] * sw;
             if constexpr (on.value) load_scales(scales);
             f32x4_t d[2][FM];
-            const auto add = [&](int i) {
+            const auto add = [&](int i, int j) {
 #pragma unroll
-                for (int j = 0; j < FM; ++j)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) sum[i][j][v] = __builtin_fmaf(d[i & 1][j][v], f[j], sum[i][j][v]);
+                for (int v = 0; v < 4; ++v) sum[i][j][v] = __builtin_fmaf(d[i & 1][j][v], f[j], sum[i][j][v]);
             };
             const uint32_t next = behind(stage);
             bool go = true;
@@ -397,11 +395,14 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
                     }
                     pb = P.buffer(k), qb = Q.buffer(k);
                 }
-#pragma unroll
-                for (int j = 0; j < FM; ++j)
-                    d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pf[i], qf[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
                 if (i + 2 < FN) pf[i + 2] = whole(read_p(i + 2, 0, stage), read_p(i + 2, 1, stage));
                 else if constexpr (on.value) pf[i + 2 - FN] = whole(read_p(i + 2 - FN, 0, next), read_p(i + 2 - FN, 1, next));
+#pragma unroll
+                for (int j = 0; j < FM; ++j) {
+                    d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pf[i], qf[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                    if (i) add(i - 1, j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 if (i >= MEET && go) {
 #pragma unroll
                     for (int q = (i - MEET) * EACH; q < (i - MEET + 1) * EACH && q < COPIES; ++q) {
@@ -414,14 +415,14 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
                         }
                     }
                 }
-                if (i) add(i - 1);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if constexpr (on.value) {
 #pragma unroll
                 for (int j = 0; j < FM; ++j) qf[j] = whole(read_q(j, 0, next), read_q(j, 1, next));
             }
-            add(FN - 1);
+#pragma unroll
+            for (int j = 0; j < FM; ++j) add(FN - 1, j);
             __builtin_amdgcn_sched_barrier(0);
             if (!plain.value && go) advance();
             stage = next;

@@ -269,7 +269,11 @@ extern "C" int mortar_fp8_quantize_weight(const void *w, int32_t N, int32_t K, i
     return launch_error(what);
 }
 
-extern "C" int64_t mortar_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) { return M <= FEW_ROWS ? 0 : mortar_dense_workspace_bytes(M, N, (K + 1) / 2); }
+extern "C" int64_t mortar_fp8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (M <= FEW_ROWS || N <= 0 || K <= 0) return 0;
+    const MortarDensePlan p = mortar_dense_plan(M, N, (K + 127) / 128, MORTAR_PLAN_E4M3);
+    return p.splits > 1 ? p.splits * M * N * 4 : 0;
+}
 
 extern "C" int mortar_fp8_quantizes_inside(int64_t M, int64_t K) { return quantises(M, K); }
 
@@ -296,7 +300,7 @@ extern "C" int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ld
     if (M <= 16) return launch_few<false, 1, 16, 2>(a, st, what);
     if (M <= 32) return launch_few<false, 2, 16, 2>(a, st, what);
     if (M <= FEW_ROWS) return launch_few<false, 4, 16, 1>(a, st, what);
-    const MortarDensePlan p = mortar_dense_plan(M, N, ((int64_t)K + 1) / 2, 0, 1);
+    const MortarDensePlan p = mortar_dense_plan(M, N, a.steps, MORTAR_PLAN_E4M3);
     a.splits = p.splits;
     if (p.splits == 1) return dense_launch<DENSE_E4M3, DENSE_STORE, false, false>(a, p.tile, st, what);
     if (!workspace) return mortar_fail(MORTAR_ERR_ARG, "%s: this shape needs a workspace", what);

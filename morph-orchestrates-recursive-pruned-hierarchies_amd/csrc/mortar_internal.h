@@ -25,11 +25,12 @@ __attribute__((visibility("hidden"))) int mortar_router_project_skinny(const uin
                                                                        int32_t d_out, const float *bias, float *qv, int64_t ldq, void *stream,
                                                                        const uint16_t *norm_w = nullptr, float eps = 0.f, uint16_t *xn = nullptr);
 
-// Tile (index into DENSE_TILES) and number of K ranges of a dense product C [M, N] with sums over K 16-bit values (e4m3: half their number).
+// Tile (index into DENSE_TILES) and number of K ranges of a dense product C [M, N] of `steps` K steps (64 16-bit values, 128 e4m3 values).
 struct MortarDensePlan {
     int tile, splits;
 };
-__attribute__((visibility("hidden"))) MortarDensePlan mortar_dense_plan(int64_t M, int64_t N, int64_t K, int swiglu, int may_split);
+enum { MORTAR_PLAN_PLAIN, MORTAR_PLAN_SWIGLU, MORTAR_PLAN_SWIGLU_KEEP, MORTAR_PLAN_SWIGLU_BWD, MORTAR_PLAN_E4M3 };
+__attribute__((visibility("hidden"))) MortarDensePlan mortar_dense_plan(int64_t M, int64_t N, int64_t steps, int form);
 // c = the sum of the fp32 slabs [M, N] of the K ranges, in their order, rounded to `type` (bf16, fp16).
 __attribute__((visibility("hidden"))) int mortar_dense_join(const float *slabs, int splits, int64_t M, int64_t N, int32_t type, void *c, int64_t ldc, void *stream);
 
