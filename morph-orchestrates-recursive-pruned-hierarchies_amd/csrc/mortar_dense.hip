@@ -25,17 +25,20 @@ using Plan = MortarDensePlan;
 
 // Which tile, and in how many K ranges: the smallest estimate of
 //   launch + rounds of workgroups * (steps * time of a step + end of a tile + its output bytes at a CU's share of the memory)
-// with, for K ranges, a second launch and the slabs' way out and back.  The times are those of the kernels as they are, fitted to 3200
-// measurements of the 16-bit products (80 to 16384 rows, widths 88 to 13000, all five tiles, up to 16 ranges, error 12 %); over these
-// the choice is 2 % slower than the best one on average (the best number of ranges of the fourth tile alone: 18 %, of the first: 80 %).
+// with, for K ranges, a second launch and the slabs' way out and back.  The times are those of the kernels as they are, fitted to 1100
+// measurements of 70 16-bit products (100 to 16384 rows, widths 88 to 11264, all five tiles, up to 16 ranges; the operands in the caches
+// and in none of them, geometric mean of the two; error 9 %).  Over these the choice is 0.7 % slower than the best one on average (the best
+// number of ranges of the fourth tile alone: 15 %, of the first: 57 %).
 struct TileTimes {
     double step, step_alone, end;      // us; a step of one of several workgroups on a CU, of a workgroup alone there
 };
-constexpr TileTimes TIMES_16[DENSE_N_TILES] = {{1.23, 1.23, 2.1}, {0.94, 0.94, 1.2}, {0.75, 0.75, 1.3}, {0.91, 0.58, 0.7}, {0.43, 0.23, 1.2}};
-constexpr TileTimes TIMES_8[DENSE_N_TILES] = {{2.3, 2.3, 24}, {1.5, 1.5, 13}, {1.25, 1.25, 2.6}, {1.3, 0.8, 0.5}, {0.6, 0.33, 1.2}};
+constexpr TileTimes TIMES_16[DENSE_N_TILES] = {{1.31, 1.31, 0.1}, {1.10, 1.10, 0.1}, {0.84, 0.84, 0.65}, {1.06, 0.68, 0.44}, {0.46, 0.26, 1.0}};
+// e4m3: from 4096 x 2048 x 11264, 4096 x 8192 x 4096 and 8192^3.  256 x 256 does not fit the registers beside the unscaled sums: 320 us for
+// the first, where 256 x 192, 256 x 128 and 128 x 128 take 138, 137 and 121.
+constexpr TileTimes TIMES_8[DENSE_N_TILES] = {{25, 25, 50}, {1.48, 1.48, 10.8}, {1.19, 1.19, 3.8}, {1.28, 0.75, 0.3}, {0.6, 0.33, 1.2}};
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int form) {
-    constexpr double byte = 2.5e-5, launch = 2.5, join = 2.1, slab_byte = 2.8e-7;
+    constexpr double byte = 3.7e-5, launch = 4.8, join = 2.0, slab_byte = 2.4e-7;
     constexpr int ranges[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16};
     const TileTimes *times = form == MORTAR_PLAN_E4M3 ? TIMES_8 : TIMES_16;
     const bool swiglu = form == MORTAR_PLAN_SWIGLU || form == MORTAR_PLAN_SWIGLU_KEEP, plain = form == MORTAR_PLAN_PLAIN || form == MORTAR_PLAN_E4M3;

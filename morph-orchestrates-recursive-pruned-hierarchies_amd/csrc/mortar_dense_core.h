@@ -7,11 +7,14 @@
 //   dx = dy W     P = W  columns,  Q = dy rows
 //   dW = dy^T x   P = x  columns,  Q = dy columns
 //
-// A workgroup computes BN x BM of C in steps of 128 bytes of K (64 16-bit values, 128 e4m3 values).  Both operands' slices go
-// from global memory into LDS by asynchronous 16-byte copies (buffer loads: rows, columns and K values outside the matrix are
-// given an offset beyond the record count and arrive as zeros, so no tail is treated apart), one stage ahead of the stage that
-// is multiplied.  In LDS the 16-byte units are permuted within their rows so that the operand reads are free of bank conflicts;
-// the permutation is applied to the copies' source addresses, their destination being linear by construction.
+// A workgroup computes BN x BM of C in steps of 128 bytes of K (64 16-bit values, 128 e4m3 values), multiplied in halves.  Both operands
+// go from global memory into a ring of LDS slots by asynchronous 16-byte copies (buffer loads: rows, columns and K values outside the
+// matrix are given an offset beyond the record count and arrive as zeros, so no tail is treated apart), ahead of the products.  A
+// slot is a whole step where an operand is K-contiguous, since its rows then are whole 128-byte lines (in halves of lines the
+// products of 4096 x 2048 x 11264 take 10 to 25 % longer), and half a step where both are K-strided: the copies are then four halves
+// ahead instead of one to two (dW of 2048 x 5632 from 4096 rows in no cache: 139 -> 96 us in 256 x 256 tiles).  In LDS the 16-byte
+// units are permuted within their rows so that the operand reads are free of bank conflicts; the permutation is applied to the
+// copies' source addresses, their destination being linear by construction.
 #ifndef MORTAR_DENSE_CORE_H
 #define MORTAR_DENSE_CORE_H
 
@@ -82,20 +85,22 @@ __device__ __forceinline__ void dense_copy(u32x4_t buf, uint32_t off, uint32_t l
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(buf) : "memory", "m0");
 }
 
-// One operand's slice of ROWS (n or m) x 128 bytes of K, copied by NW waves, L instructions each.
-template <int ROWS, bool COLS, int NW, int ESIZE>
+// One operand's slot: ROWS (n or m) x KB bytes of K, copied by NW waves in turns of one kilobyte.
+template <int ROWS, bool COLS, int NW, int ESIZE, int KB>
 struct DenseSlice {
-    static constexpr int BYTES = ROWS * 128, L = BYTES / 1024 / NW;
-    static_assert(L * 1024 * NW == BYTES, "whole instructions per wave");
-    static constexpr int UPR = COLS ? ROWS / 8 : 8;          // 16-byte units per LDS row
-    static constexpr bool EVEN = 64 % UPR == 0;              // an instruction fills whole LDS rows
+    static constexpr int BYTES = ROWS * KB, COPIES = BYTES / 1024, L = (COPIES + NW - 1) / NW, LEAST = COPIES / NW;
+    static constexpr int UPR = COLS ? ROWS / 8 : KB / 16;          // 16-byte units per LDS row
+    static_assert(COLS || KB == 128, "rows are whole lines");
+    static constexpr bool EVEN = 64 % UPR == 0;              // a copy fills whole LDS rows
     const char *base;
-    uint32_t off[L];              // of this lane's unit in the first K step
-    int kpos[COLS && !EVEN ? L : 1];      // where in a K step it lies: bytes (rows: the same in all copies) or values (columns)
-    int64_t step;                 // bytes from one K step to the next
+    uint32_t off[L];              // of this lane's unit in the first slot
+    int kpos[COLS && !EVEN ? L : 1];      // where in a slot it lies: bytes (rows: the same in all copies) or values (columns)
+    int64_t step;                 // bytes from one slot to the next
 
-    // Permutation of a K-strided slice: 32-byte pieces (16 n, one fragment's width) of the rows that one transposing read
-    // touches, 4 rows per 16 lanes at distances of 8, fall into different pieces of the 256-byte bank window.
+    // Permutation of K-contiguous rows of eight units.
+    static __device__ __forceinline__ int unit(int u, int r) { return u ^ (r & 7); }
+    // Permutation of K-strided rows: 32-byte pieces (16 n, one fragment's width) of the rows that one transposing read touches, 4 rows
+    // per 16 lanes at distances of 8, fall into different pieces of the 256-byte bank window.
     // (Of 192 columns the last four pieces only change places among themselves: two rows of the eight meet there.)
     static __device__ __forceinline__ int piece_swz(int k) {
         if constexpr (ROWS == 64) return ((k >> 1) & 1) | ((k >> 3) & 1) << 1;
@@ -108,46 +113,49 @@ struct DenseSlice {
     template <typename RowOf>
     __device__ __forceinline__ void init(const char *b, int64_t ld, int wave, int lane, RowOf row_of, int n_left) {
         base = b;
-        step = COLS ? 64 * ld : 128;
+        step = COLS ? KB / 2 * ld : KB;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-            const int t = (wave * L + i) * 64 + lane, r = t / UPR, u = t % UPR;
+            const int t = (i * NW + wave) * 64 + lane, r = t / UPR, u = t % UPR;
             if constexpr (COLS) {
                 const int src = piece(u >> 1, r) << 1 | (u & 1);
                 if (i < (int)(sizeof kpos / 4)) kpos[i] = r;
                 off[i] = src * 8 < n_left ? (uint32_t)(r * ld) + src * 16 : DENSE_OUTSIDE;
             } else {
-                const int src = u ^ (r & 7), row = row_of(r);
+                const int src = unit(u, r), row = row_of(r);
                 if (i == 0) kpos[0] = src * 16;         // (r & 7 is the lane's alone)
                 off[i] = row >= 0 ? (uint32_t)(row * ld) + src * 16 : DENSE_OUTSIDE;
             }
         }
     }
-    // What is left of K from step s on, in the units of kpos.
-    static __device__ __forceinline__ int left(int s, int K) { return COLS ? K - s * 64 : K * ESIZE - s * 128; }
-    __device__ __forceinline__ u32x4_t buffer(int s) const { return dense_buffer(base + s * step); }
-    // Copy i of a whole K step.
-    __device__ __forceinline__ void copy(int i, u32x4_t buf, uint32_t lds) const { dense_copy(buf, off[i], lds + i * 1024); }
-    // Copy i of a K step with `left` to go, to LDS address `lds` (the wave's first kilobyte is wave * L).
-    __device__ __forceinline__ void copy(int i, u32x4_t buf, int left, uint32_t lds) const {
-        const int k = COLS ? (EVEN ? kpos[0] + i * (64 / UPR) : kpos[EVEN ? 0 : i]) : kpos[0];
-        dense_copy(buf, k < left ? off[i] : DENSE_OUTSIDE, lds + i * 1024);
+    // What is left of K from slot k on, in the units of kpos.
+    static __device__ __forceinline__ int left(int k, int K) { return COLS ? K - k * (KB / 2) : K * ESIZE - k * KB; }
+    __device__ __forceinline__ u32x4_t buffer(int k) const { return dense_buffer(base + k * step); }
+    // Copy i of a slot, all of it inside K or `left` to go, to LDS address `lds` (that of the wave's first one).
+    static __device__ __forceinline__ bool has(int i, int wave) { return COPIES % NW == 0 || i * NW + wave < COPIES; }
+    __device__ __forceinline__ void copy(int i, int wave, u32x4_t buf, uint32_t lds) const {
+        if (has(i, wave)) dense_copy(buf, off[i], lds + i * NW * 1024);
+    }
+    __device__ __forceinline__ void copy(int i, int wave, u32x4_t buf, int left, uint32_t lds) const {
+        const int k = COLS ? (EVEN ? kpos[0] + i * NW * (64 / UPR) : kpos[EVEN ? 0 : i]) : kpos[0];
+        if (has(i, wave)) dense_copy(buf, k < left ? off[i] : DENSE_OUTSIDE, lds + i * NW * 1024);
     }
 };
 
-// Fragment (16 rows x half a K step) of a K-contiguous slice: address of K half 0; the other half lies at ^ 64.
+// Fragment (16 rows x half a K step) of a K-contiguous slice: a lane holds unit (lane >> 4) of row (lane & 15).  Address of half 0; the other
+// half lies at ^ 64.
 __device__ __forceinline__ uint32_t dense_row_addr(int row, int lane) {
     return (uint32_t)((row + (lane & 15)) * 128 + (((lane >> 4) ^ (lane & 7)) * 16));
 }
 __device__ __forceinline__ u32x4_t dense_read(uint32_t addr) {
     return *(const MORTAR_LDS u32x4_t *)(uintptr_t)addr;
 }
-// The same of a K-strided slice: K values 32 s + 8 g + 4 t + {0..3} of column (lane & 15) in half t.  Address of fragment `first`
-// (a multiple of the power of two that is the number of the wave's fragments); fragment first + i lies at ^ (32 i).
+// The same of a K-strided slice: K values 32 h + 8 g + 4 t + {0..3} of column (lane & 15) in part t of half h.  Address of fragment `first` (a multiple of the
+// power of two that is the number of the wave's fragments); fragment first + i lies at ^ (32 i).
 template <int ROWS>
 __device__ __forceinline__ uint32_t dense_col_addr(int first, int lane) {
     const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
-    return (uint32_t)(k * ROWS * 2 + DenseSlice<ROWS, true, 1, 2>::piece(first, k) * 32 + (lane & 3) * 8);
+    return (uint32_t)(k * ROWS * 2 + DenseSlice<ROWS, true, 1, 2, 64>::piece(first, k) * 32 + (lane & 3) * 8);
 }
 template <int ROWS>
 __device__ __forceinline__ u32x4_t dense_read_t(uint32_t addr) {
@@ -222,32 +230,35 @@ struct Const {
     static constexpr int value = V;
 };
 
+constexpr int dense_slot_bytes(bool pc, bool qc) { return pc && qc ? 64 : 128; }
+
 template <DenseType T, DenseEpilogue E, bool PC, bool QC, int BN, int BM, int WN, int WM, int NS>
 __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseArgs a) {
     constexpr int NW = WN * WM, FN = BN / WN / 16, FM = BM / WM / 16, ES = T == DENSE_E4M3 ? 1 : 2;
     static_assert(T != DENSE_E4M3 || (!PC && !QC), "e4m3 operands are K-contiguous");
     static_assert(FN % (E == DENSE_SWIGLU ? 4 : 2) == 0, "fragments are joined in pairs");
     static_assert((FN & (FN - 1)) == 0, "K-strided fragments of P are found by xor");
-    constexpr int PB = BN * 128, STAGE = PB + BM * 128;
+    constexpr int KB = dense_slot_bytes(PC, QC), PER_STEP = 128 / KB;       // slots per step
+    using SliceP = DenseSlice<BN, PC, NW, ES, KB>;
+    using SliceQ = DenseSlice<BM, QC, NW, ES, KB>;
+    constexpr int SLOT = SliceP::BYTES + SliceQ::BYTES, RING = NS * SLOT, LEAST = SliceP::LEAST + SliceQ::LEAST;
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int wn = wave % WN, wm = wave / WN;
     const int fp = wn * FN, fq = wm * FM;            // first fragments of the wave
-    using SliceP = DenseSlice<BN, PC, NW, ES>;
-    using SliceQ = DenseSlice<BM, QC, NW, ES>;
-    const uint32_t l0 = mortar_lds_addr(lds), lp = l0 + wave * SliceP::L * 1024, lq = l0 + PB + wave * SliceQ::L * 1024;
+    const uint32_t l0 = mortar_lds_addr(lds), lp = l0 + wave * 1024, lq = l0 + SliceP::BYTES + wave * 1024;
     const uint32_t ap = l0 + (PC ? dense_col_addr<BN>(fp, lane) : dense_row_addr(fp * 16, lane));
-    constexpr bool XQ = (FM & (FM - 1)) == 0;        // so are those of Q, if their number is a power of two
+    constexpr bool XQ = (FM & (FM - 1)) == 0;        // K-strided fragments of Q are found by xor, too, if their number is a power of two
     uint32_t aq[QC && !XQ ? FM : 1];
 #pragma unroll
-    for (int j = 0; j < (int)(sizeof aq / 4); ++j) aq[j] = l0 + PB + (QC ? dense_col_addr<BM>(fq + j, lane) : dense_row_addr(fq * 16, lane));
-    const auto read_p = [&](int i, int h, uint32_t stage) {
-        if constexpr (PC) return dense_read_t<BN>(((ap + stage) ^ (i * 32)) + h * 32 * BN * 2);
-        else return dense_read(((ap + stage) ^ (h * 64)) + i * 2048);
+    for (int j = 0; j < (int)(sizeof aq / 4); ++j) aq[j] = l0 + SliceP::BYTES + (QC ? dense_col_addr<BM>(fq + j, lane) : dense_row_addr(fq * 16, lane));
+    const auto read_p = [&](int i, int h, uint32_t slot) {
+        if constexpr (PC) return dense_read_t<BN>(((ap + slot) ^ (i * 32)) + h * 32 * BN * 2);
+        else return dense_read(((ap + slot) ^ (h * 64)) + i * 2048);
     };
-    const auto read_q = [&](int j, int h, uint32_t stage) {
-        if constexpr (QC) return dense_read_t<BM>((XQ ? (aq[0] + stage) ^ (j * 32) : aq[XQ ? 0 : j] + stage) + h * 32 * BM * 2);
-        else return dense_read(((aq[0] + stage) ^ (h * 64)) + j * 2048);
+    const auto read_q = [&](int j, int h, uint32_t slot) {
+        if constexpr (QC) return dense_read_t<BM>((XQ ? (aq[0] + slot) ^ (j * 32) : aq[XQ ? 0 : j] + slot) + h * 32 * BM * 2);
+        else return dense_read(((aq[0] + slot) ^ (h * 64)) + j * 2048);
     };
 
     // Workgroups of one XCD (blockIdx % 8) walk over a contiguous run of tiles, in bands of 8 tiles along m, so that the operands
@@ -288,45 +299,58 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
         const int m_left = a.M - t.m0;
         Q.init(qb, a.ldq, wave, lane, [&](int r) { return r < m_left ? r : -1; }, m_left);
     };
-    // Copies run ahead of the products over the steps of this workgroup's tiles, one behind the other: step `ahead` of tile `aim_id` is
-    // the next to be copied.
-    constexpr int COPIES = SliceP::L + SliceQ::L, RING = NS * STAGE, FIRST = NS;
-    const auto behind = [](uint32_t st) { return st + STAGE == RING ? 0u : st + STAGE; };
+    // Copies run NS slots ahead of the products over the slots of this workgroup's tiles, one behind the other: slot `ahead` of the
+    // tile `aim_id` is the next to be copied.
+    const auto behind = [](uint32_t slot) { return slot + SLOT == RING ? 0u : slot + SLOT; };
     int id = xcd * per_xcd + (int)(blockIdx.x >> 3);
     if (id >= end) return;
     int aim_id = id, ahead, ahead_last;
     const auto aim_at = [&](int which) {
         const Tile t = tile_of(which);
         aim(t);
-        ahead = t.first;
-        ahead_last = t.last;
+        ahead = PER_STEP * t.first;
+        ahead_last = PER_STEP * t.last;
     };
     const auto advance = [&] {
         if (++ahead == ahead_last && (aim_id += stride) < end) aim_at(aim_id);
     };
     const auto copying = [&] { return aim_id < end; };
-    const auto copy_all = [&](uint32_t st) {
-        const u32x4_t pb = P.buffer(ahead), qb = Q.buffer(ahead);
-#pragma unroll
-        for (int i = 0; i < SliceP::L; ++i) P.copy(i, pb, P.left(ahead, a.K), lp + st);
-#pragma unroll
-        for (int i = 0; i < SliceQ::L; ++i) Q.copy(i, qb, Q.left(ahead, a.K), lq + st);
-    };
-    aim_at(id);
-    uint32_t stage = 0;                              // of the step that is multiplied next
-#pragma unroll
-    for (int i = 0; i < FIRST; ++i)
-        if (copying()) {
-            copy_all(i * STAGE);
-            advance();
+    // Copy q of the wave's for slot k, all of it inside K (plain) or with the tails looked after.
+    const auto copy = [&](auto plain, int q, int k, u32x4_t pb, u32x4_t qb, uint32_t slot) {
+        if constexpr (plain.value) {
+            if (q < SliceP::L) P.copy(q, wave, pb, lp + slot);
+            else Q.copy(q - SliceP::L, wave, qb, lq + slot);
+        } else {
+            if (q < SliceP::L) P.copy(q, wave, pb, P.left(k, a.K), lp + slot);
+            else Q.copy(q - SliceP::L, wave, qb, Q.left(k, a.K), lq + slot);
         }
-    // Waits until this wave's copies of a step have landed and every wave is here, all its LDS reads done.  `newer` steps were copied
-    // behind that step if there still is one to be copied: then their copies may be on their way.
-    const auto meet = [&](auto newer) {
-        if (newer.value > 0 && copying()) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(newer.value * COPIES) : "memory");
+    };
+    constexpr int COPIES = SliceP::L + SliceQ::L;
+    // Waits until this wave's copies of a slot have landed and every wave is here, all its LDS reads done.  `newer` slots were copied
+    // behind that one if there still is one to be copied: then their copies may be on their way.
+    const auto meet = [&](auto newer, auto plain) {
+        if (plain.value || (newer.value > 0 && copying())) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(newer.value * LEAST) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
-    meet(Const<FIRST - 1>{});
+    aim_at(id);
+    uint32_t slot = 0;                               // of the values that are multiplied next
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+        if (copying()) {
+            const u32x4_t pb = P.buffer(ahead), qb = Q.buffer(ahead);
+#pragma unroll
+            for (int q = 0; q < COPIES; ++q) copy(Const<0>{}, q, ahead, pb, qb, i * SLOT);
+            advance();
+        }
+    [[maybe_unused]] u32x4_t pf[T == DENSE_E4M3 ? 1 : 2][FN], qf[T == DENSE_E4M3 ? 1 : 2][FM];
+    meet(Const<NS - 1>{}, Const<0>{});
+    if constexpr (T != DENSE_E4M3) {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) qf[0][j] = read_q(j, 0, slot);
+#pragma unroll
+        for (int i = 0; i < FN; ++i) pf[0][i] = read_p(i, 0, slot);
+        if constexpr (PER_STEP == 2) meet(Const<NS - 2>{}, Const<0>{});
+    }
     for (;;) {
     f32x4_t acc[FN][FM];
 #pragma unroll
@@ -339,7 +363,8 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
     const bool more = id < end;
 
     int s = cur.first;
-    const bool long_run = s + NS + 1 < cur.last;      // the copies are NS steps ahead in this tile
+    const int plain_end = cur.last - 1 - (NS + PER_STEP - 1) / PER_STEP;     // up to here a step's copies are of whole slots of this tile
+
     if constexpr (T == DENSE_E4M3) {
         // One matrix instruction is a step deep: FN groups of FM products, scaled and added a group later.  Fragments of P are read two groups
         // ahead, those of Q behind their last use; all waves meet two groups before the end, when the step is in registers.
@@ -363,13 +388,13 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
 #pragma unroll
                 for (int v = 0; v < 4; ++v) sum[i][j][v] = 0.f;
         const auto whole = [](u32x4_t x, u32x4_t y) { return i32x8_t{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]}; };
-        i32x8_t pf[FN], qf[FM];
+        i32x8_t p8[FN], q8[FM];
         load_scales(s);
 #pragma unroll
-        for (int j = 0; j < FM; ++j) qf[j] = whole(read_q(j, 0, stage), read_q(j, 1, stage));
+        for (int j = 0; j < FM; ++j) q8[j] = whole(read_q(j, 0, slot), read_q(j, 1, slot));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) pf[i] = whole(read_p(i, 0, stage), read_p(i, 1, stage));
-        constexpr int MEET = FN - 2, EACH = (COPIES + 1) / 2;
+        for (int i = 0; i < 2; ++i) p8[i] = whole(read_p(i, 0, slot), read_p(i, 1, slot));
+        constexpr int MEET = FN - 2;
         const auto step = [&](auto on, auto plain, int k, int scales) {          // as below; scales: the step whose scales are loaded
             float f[FM];
 #pragma unroll
@@ -380,55 +405,41 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
 #pragma unroll
                 for (int v = 0; v < 4; ++v) sum[i][j][v] = __builtin_fmaf(d[i & 1][j][v], f[j], sum[i][j][v]);
             };
-            const uint32_t next = behind(stage);
+            const uint32_t next = behind(slot);
+            constexpr int EACH = (COPIES + FN - MEET - 1) / (FN - MEET);
             bool go = true;
             u32x4_t pb{}, qb{};
 #pragma unroll
             for (int i = 0; i < FN; ++i) {
-                if (i == MEET) {
-                    if constexpr (plain.value) {
-                        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * COPIES) : "memory");
-                    } else {
-                        meet(Const<NS - 2>{});
-                        k = ahead;
-                        go = copying();
-                    }
+                if (i == MEET) {                      // the step is in registers, or will be without its slot
+                    meet(Const<NS - 2>{}, plain);
+                    if constexpr (!plain.value) k = ahead, go = copying();
                     pb = P.buffer(k), qb = Q.buffer(k);
                 }
-                if (i + 2 < FN) pf[i + 2] = whole(read_p(i + 2, 0, stage), read_p(i + 2, 1, stage));
-                else if constexpr (on.value) pf[i + 2 - FN] = whole(read_p(i + 2 - FN, 0, next), read_p(i + 2 - FN, 1, next));
-#pragma unroll
-                for (int j = 0; j < FM; ++j) {
-                    d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(pf[i], qf[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-                    if (i) add(i - 1, j);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                if (i + 2 < FN) p8[i + 2] = whole(read_p(i + 2, 0, slot), read_p(i + 2, 1, slot));
+                else if constexpr (on.value) p8[i + 2 - FN] = whole(read_p(i + 2 - FN, 0, next), read_p(i + 2 - FN, 1, next));
                 if (i >= MEET && go) {
 #pragma unroll
-                    for (int q = (i - MEET) * EACH; q < (i - MEET + 1) * EACH && q < COPIES; ++q) {
-                        if constexpr (plain.value) {
-                            if (q < SliceP::L) P.copy(q, pb, lp + stage);
-                            else Q.copy(q - SliceP::L, qb, lq + stage);
-                        } else {
-                            if (q < SliceP::L) P.copy(q, pb, P.left(k, a.K), lp + stage);
-                            else Q.copy(q - SliceP::L, qb, Q.left(k, a.K), lq + stage);
-                        }
-                    }
+                    for (int q = (i - MEET) * EACH; q < (i - MEET + 1) * EACH && q < COPIES; ++q) copy(plain, q, k, pb, qb, slot);
+                }
+#pragma unroll
+                for (int j = 0; j < FM; ++j) {
+                    d[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(p8[i], q8[j], f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+                    if (i) add(i - 1, j);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (on.value)
+                        if (i == FN - 1) q8[j] = whole(read_q(j, 0, next), read_q(j, 1, next));
                 }
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            if constexpr (on.value) {
-#pragma unroll
-                for (int j = 0; j < FM; ++j) qf[j] = whole(read_q(j, 0, next), read_q(j, 1, next));
             }
 #pragma unroll
             for (int j = 0; j < FM; ++j) add(FN - 1, j);
             __builtin_amdgcn_sched_barrier(0);
             if (!plain.value && go) advance();
-            stage = next;
+            slot = next;
         };
-        if (long_run) {
-            for (; s + NS + 1 < cur.last; ++s) step(Const<1>{}, Const<1>{}, s + NS, s + 1);
+        if (s < plain_end) {
+            for (; s < plain_end; ++s) step(Const<1>{}, Const<1>{}, s + NS, s + 1);
             ahead = s + NS;
         }
         for (; s + 1 < cur.last; ++s) step(Const<1>{}, Const<0>{}, 0, s + 1);
@@ -438,73 +449,52 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
 #pragma unroll
             for (int j = 0; j < FM; ++j) acc[i][j] = f32x4_t{sum[i][j][0], sum[i][j][1], sum[i][j][2], sum[i][j][3]};
     } else {
-        // A step is two halves of K.  While the matrix cores work on one half its successor is read from LDS into the other set of
-        // registers; between the halves of a step all waves meet: the step is then in registers everywhere and its stage free for
-        // the copies, and the next step has landed.
-        u32x4_t pf[2][FN], qf[2][FM];
-        // Per group of FM products: the fragments of Q first, then those of P, each behind the products that free a register for it.
+        // While the matrix cores work on one half the next one is read from LDS into the other set of registers.  Behind the half that read the
+        // last of a slot all waves meet: that slot is then in registers everywhere and copied over next, and the slot behind it has landed.
+        // The reads of a group of FM products: the fragments of Q first, then those of P, each behind the products that free a register for it.
         constexpr int EACH = (COPIES + FN - 1) / FN;
         constexpr auto reads = [](int groups) { return groups == 0 ? 0 : groups == FN ? FM + FN : FM + (3 * (groups - 1) / 2 < FN ? 3 * (groups - 1) / 2 : FN); };
-#pragma unroll
-        for (int j = 0; j < FM; ++j) qf[0][j] = read_q(j, 0, stage);
-#pragma unroll
-        for (int i = 0; i < FN; ++i) pf[0][i] = read_p(i, 0, stage);
-        // on: the tile goes on behind this step; plain: and so does the run of whole steps that are copied, `k` the one due
-        const auto step = [&](auto on, auto plain, int k) {
-#pragma unroll
-            for (int i = 0; i < FN; ++i) {
-#pragma unroll
-                for (int q = reads(i); q < reads(i + 1); ++q) {
-                    if (q < FM) qf[1][q] = read_q(q, 1, stage);
-                    else pf[1][q - FM] = read_p(q - FM, 1, stage);
-                }
-#pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = dense_mfma<T>(pf[0][i], qf[0][j], acc[i][j]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if constexpr (plain.value) {
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * COPIES) : "memory");
-            } else {
-                meet(Const<NS - 2>{});
-                k = ahead;
-            }
-            const uint32_t next = behind(stage);
-            const bool go = plain.value || copying();
+        // set: of the registers that are multiplied, the half of the step; on: there is a next half; plain: the copies are of a whole slot of
+        // this tile, k the one due
+        const auto half = [&](auto set, bool on, auto plain, int k) {
+            constexpr bool LAST = PER_STEP == 2 || set.value == 1;        // of its slot: that is free, the next half is in the next one
+            const uint32_t next = LAST ? behind(slot) : slot;
+            constexpr int h = PER_STEP == 2 ? 0 : 1 - set.value;
+            if constexpr (!plain.value) k = ahead;
+            const bool go = LAST && (plain.value || copying());
             const u32x4_t pb = P.buffer(k), qb = Q.buffer(k);
 #pragma unroll
             for (int i = 0; i < FN; ++i) {
-                if constexpr (on.value) {
+                if (on) {
 #pragma unroll
                     for (int q = reads(i); q < reads(i + 1); ++q) {
-                        if (q < FM) qf[0][q] = read_q(q, 0, next);
-                        else pf[0][q - FM] = read_p(q - FM, 0, next);
+                        if (q < FM) qf[1 - set.value][q] = read_q(q, h, next);
+                        else pf[1 - set.value][q - FM] = read_p(q - FM, h, next);
                     }
                 }
                 if (go) {
 #pragma unroll
-                    for (int q = i * EACH; q < (i + 1) * EACH && q < COPIES; ++q) {
-                        if constexpr (plain.value) {
-                            if (q < SliceP::L) P.copy(q, pb, lp + stage);
-                            else Q.copy(q - SliceP::L, qb, lq + stage);
-                        } else {
-                            if (q < SliceP::L) P.copy(q, pb, P.left(k, a.K), lp + stage);
-                            else Q.copy(q - SliceP::L, qb, Q.left(k, a.K), lq + stage);
-                        }
-                    }
+                    for (int q = i * EACH; q < (i + 1) * EACH && q < COPIES; ++q) copy(plain, q, k, pb, qb, slot);
                 }
 #pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = dense_mfma<T>(pf[1][i], qf[1][j], acc[i][j]);
+                for (int j = 0; j < FM; ++j) acc[i][j] = dense_mfma<T>(pf[set.value][i], qf[set.value][j], acc[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (!plain.value && go) advance();
-            stage = next;
+            if constexpr (PER_STEP == 2 || set.value == 0) meet(Const<NS - 2>{}, plain);
+            slot = next;
         };
-        if (long_run) {
-            for (; s + NS + 1 < cur.last; ++s) step(Const<1>{}, Const<1>{}, s + NS);
-            ahead = s + NS;
+        if (s < plain_end) {
+            for (; s < plain_end; ++s) {
+                half(Const<0>{}, true, Const<1>{}, PER_STEP * s + NS);
+                half(Const<1>{}, true, Const<1>{}, PER_STEP * (s + 1) - 1 + NS);
+            }
+            ahead = PER_STEP * s + NS;
         }
-        for (; s + 1 < cur.last; ++s) step(Const<1>{}, Const<0>{}, 0);
-        step(Const<0>{}, Const<0>{}, 0);
+        for (; s < cur.last; ++s) {
+            half(Const<0>{}, true, Const<0>{}, 0);
+            half(Const<1>{}, more || s + 1 < cur.last, Const<0>{}, 0);
+        }
     }
 
     // ---- epilogue: pairs of fragments joined to eight consecutive n per lane, 16-byte stores
@@ -571,13 +561,13 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
 
 // ---- host side -------------------------------------------------------------------------------------------------------
 
-// The tiles: BN x BM of C by WN x WM waves, NS stages of LDS, workgroups per CU.  The larger the tile the fewer bytes go through the L1 for a
+// The tiles: BN x BM of C by WN x WM waves, LDS steps (slots: twice as many halves, and one more where they fit), workgroups per CU.  The larger the tile the fewer bytes go through the L1 for a
 // product (64 per cycle and CU is what it takes: 256 x 256 keeps it half busy, 256 x 128 three quarters); the smaller ones
 // are for matrices that do not fill the chip with large ones.
 struct DenseTile {
-    int bn, bm, wn, wm, stages, per_cu;
+    int bn, bm, wn, wm, steps, halves, per_cu;
 };
-constexpr DenseTile DENSE_TILES[] = {{256, 256, 2, 4, 2, 1}, {256, 192, 2, 4, 2, 1}, {256, 128, 4, 2, 3, 1}, {128, 128, 2, 2, 2, 2}, {64, 64, 1, 4, 4, 2}};
+constexpr DenseTile DENSE_TILES[] = {{256, 256, 2, 4, 2, 5, 1}, {256, 192, 2, 4, 2, 5, 1}, {256, 128, 4, 2, 3, 6, 1}, {128, 128, 2, 2, 2, 5, 2}, {64, 64, 1, 4, 4, 10, 2}};
 constexpr int DENSE_N_TILES = sizeof DENSE_TILES / sizeof DENSE_TILES[0];
 
 template <DenseType T, DenseEpilogue E, bool PC, bool QC, int I = 0>
@@ -585,8 +575,9 @@ int dense_launch(DenseArgs a, int tile, hipStream_t st, const char *what) {
     if constexpr (I + 1 < DENSE_N_TILES)
         if (tile != I) return dense_launch<T, E, PC, QC, I + 1>(a, tile, st, what);
     constexpr DenseTile D = DENSE_TILES[I];
-    const auto kern = dense_tile_kernel<T, E, PC, QC, D.bn, D.bm, D.wn, D.wm, D.stages>;
-    constexpr int smem = D.stages * (D.bn + D.bm) * 128, feat = E == DENSE_SWIGLU ? D.bn / 2 : D.bn;
+    constexpr int kb = dense_slot_bytes(PC, QC), slots = kb == 64 ? D.halves : D.steps;
+    const auto kern = dense_tile_kernel<T, E, PC, QC, D.bn, D.bm, D.wn, D.wm, slots>;
+    constexpr int smem = slots * (D.bn + D.bm) * kb, feat = E == DENSE_SWIGLU ? D.bn / 2 : D.bn;
     static_assert(smem * D.per_cu <= 160 * 1024, "LDS");
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
@@ -594,8 +585,8 @@ int dense_launch(DenseArgs a, int tile, hipStream_t st, const char *what) {
     if (total > (1 << 30)) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tiles", what);
     a.tiles_n = (int)tn;
     a.tiles_m = (int)tm;
-    const int64_t per_xcd = (total + 7) / 8, slots = 32 * D.per_cu;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(8 * (per_xcd < slots ? per_xcd : slots))), dim3(D.wn * D.wm * 64), smem, st, a);
+    const int64_t per_xcd = (total + 7) / 8, room = 32 * D.per_cu;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(8 * (per_xcd < room ? per_xcd : room))), dim3(D.wn * D.wm * 64), smem, st, a);
     const hipError_t l = hipGetLastError();
     return l == hipSuccess ? MORTAR_OK : mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(l));
 }
