@@ -36,10 +36,24 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {               // over 
     v = umax(v, mortar_row_xor<2>(v));
     return umax(v, mortar_row_xor<1>(v));
 }
+// Eight values over their scale, rounded to e4m3.  BF16: the values have 8 significant bits; the quotient is then formed from the rounded
+// reciprocal of the scale with one correction, x r + r (x - (x r) s), which gives the bits of the division for every such value and every
+// fp32 significand of the scale (all 2^31 pairs were compared; x r alone is off for a quarter of them).  Scales near the ends of the
+// range, where the correction would leave it, take the division itself: it is a dozen instructions per value, more time than the memory takes.
+template <bool BF16>
 __device__ __forceinline__ u32x2_t quantise8(const float (&v)[8], float s) {
     float q[8];
+    if (BF16 && s > 0x1p-90f && s < 0x1p100f) {
+        const float r = 1.0f / s;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j] = v[j] / s;
+        for (int j = 0; j < 8; ++j) {
+            const float q0 = v[j] * r;
+            q[j] = __builtin_fmaf(__builtin_fmaf(-q0, s, v[j]), r, q0);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = v[j] / s;
+    }
     int lo = 0, hi = 0;
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
@@ -58,19 +72,26 @@ __device__ __forceinline__ void read8(const void *p, int64_t at, float (&v)[8]) 
     }
 }
 
-// Activations: 16 lanes per group, 16 bytes of x per lane.
+// Activations: 16 lanes per group of 128 values, 16 bytes of x per lane; a workgroup takes one group of each of 64 rows, so that the scales
+// of a K block, which lie along the rows, are written together.
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint16_t *x, int64_t M, int32_t K, int64_t ldx, uint8_t *q, int64_t ldq, float *s, int64_t s_m,
                                                        int64_t s_k) {
-    const int kb = (K + 127) >> 7;
-    const int64_t grp = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4;
-    if (grp >= M * kb) return;
-    const int64_t m = grp / kb;
-    const int b = (int)(grp - m * kb), k = b * 128 + (threadIdx.x & 15) * 8;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (k < K) read8<MORTAR_BF16>(x, m * ldx + k, v);
-    const float sc = scale_of(row_max(abs_max8(v)));
-    if (k < K) *reinterpret_cast<u32x2_t *>(q + m * ldq + k) = quantise8(v, sc);
-    if ((threadIdx.x & 15) == 0) s[m * s_m + b * s_k] = sc;
+    const int b = blockIdx.y, k = b * 128 + (threadIdx.x & 15) * 8;
+    const int64_t m0 = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 4);
+    float v[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        if (m0 + i * 16 < M && k < K) read8<MORTAR_BF16>(x, (m0 + i * 16) * ldx + k, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t m = m0 + i * 16;
+        const float sc = scale_of(row_max(abs_max8(v[i])));
+        if (m < M && k < K) *reinterpret_cast<u32x2_t *>(q + m * ldq + k) = quantise8<true>(v[i], sc);
+        if (m < M && (threadIdx.x & 15) == 0) s[m * s_m + b * s_k] = sc;
+    }
 }
 
 // Weights: a workgroup per 128 x 128 block, 8 rows of 8 values per thread.
@@ -93,7 +114,7 @@ __global__ __launch_bounds__(256) void fp8_blocks_kernel(const void *w, int32_t 
     const float sc = scale_of(umax(umax(part[0], part[1]), umax(part[2], part[3])));
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        if (n0 + i * 16 < N && k < K) *reinterpret_cast<u32x2_t *>(q + (n0 + i * 16) * ldq + k) = quantise8(v[i], sc);
+        if (n0 + i * 16 < N && k < K) *reinterpret_cast<u32x2_t *>(q + (n0 + i * 16) * ldq + k) = quantise8<TYPE == MORTAR_BF16>(v[i], sc);
     if (threadIdx.x == 0) s[blockIdx.y * s_n + blockIdx.x] = sc;
 }
 
@@ -141,7 +162,7 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(const DenseArgs a) {
                     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                     if (k < a.K) read8<MORTAR_BF16>(a.q, m * (a.ldq / 2) + k, v);
                     const float sc = scale_of(row_max(abs_max8(v)));
-                    const u32x2_t q = quantise8(v, sc);
+                    const u32x2_t q = quantise8<true>(v, sc);
                     *reinterpret_cast<u32x4_t *>(values + m * blocks * 128 + k) = codes_bf16(q[0], q[1]);
                     if ((threadIdx.x & 15) == 0) scales[m * blocks + b] = sc;
                 }
@@ -245,9 +266,9 @@ extern "C" int mortar_fp8_quantize(const uint16_t *x, int64_t M, int32_t K, int6
     CHECK(check_values(what, "x", x, K, ldx, 2));
     CHECK(check_codes(what, "q", q, M, K, ldq));
     if (!s) return mortar_fail(MORTAR_ERR_ARG, "%s: s is null", what);
-    const int64_t groups = M * ((K + 127) / 128);
-    if ((groups + 15) / 16 >= INT32_MAX) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
-    hipLaunchKernelGGL(fp8_rows_kernel, dim3((unsigned)((groups + 15) / 16)), dim3(256), 0, static_cast<hipStream_t>(stream), x, M, K, ldx, q, ldq, s, s_m, s_k);
+    const int64_t rows = (M + 63) / 64, blocks = ((int64_t)K + 127) / 128;
+    if (rows >= INT32_MAX / 256 || blocks > 65535) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
+    hipLaunchKernelGGL(fp8_rows_kernel, dim3((unsigned)rows, (unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream), x, M, K, ldx, q, ldq, s, s_m, s_k);
     return launch_error(what);
 }
 

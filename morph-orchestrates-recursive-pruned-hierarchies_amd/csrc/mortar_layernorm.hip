@@ -36,21 +36,43 @@ __device__ __forceinline__ typename Elem<T>::type from_float(float v) {
     else if constexpr (T == LN_F16) return __builtin_bit_cast(uint16_t, (_Float16)v);
     else return (uint16_t)bf16_bits_rne(v);
 }
-// VEC consecutive values at p: 16 bytes, 32 bytes (eight floats) or one value.
+// VEC consecutive values as they lie in memory: 16 bytes or one value.
+template <int T, int VEC>
+struct Raw {
+    u32x4_t w;
+    __device__ __forceinline__ void read(const typename Elem<T>::type *p) { w = *reinterpret_cast<const u32x4_t *>(p); }
+    __device__ __forceinline__ void clear() { w = u32x4_t{0, 0, 0, 0}; }
+    __device__ __forceinline__ void values(float (&v)[VEC]) const {
+        if constexpr (T == LN_F32) {
+            const f32x4_t f = __builtin_bit_cast(f32x4_t, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = f[j];
+        } else {
+            dense_unpack8<T == LN_F16 ? DENSE_F16 : DENSE_BF16>(w, v);
+        }
+    }
+};
+template <int T>
+struct Raw<T, 1> {
+    typename Elem<T>::type e;
+    __device__ __forceinline__ void read(const typename Elem<T>::type *p) { e = *p; }
+    __device__ __forceinline__ void clear() { e = 0; }
+    __device__ __forceinline__ void values(float (&v)[1]) const { v[0] = to_float<T>(e); }
+};
+// Weights beside VEC values of the rows: fp32 ones may be two words.
 template <int T, int VEC>
 __device__ __forceinline__ void load(const typename Elem<T>::type *p, float (&v)[VEC]) {
-    if constexpr (VEC == 1) {
-        v[0] = to_float<T>(*p);
-    } else if constexpr (T == LN_F32) {
+    if constexpr (T == LN_F32 && VEC == 8) {
+        Raw<T, 4> a, b;
+        a.read(p), b.read(p + 4);
+        float lo[4], hi[4];
+        a.values(lo), b.values(hi);
 #pragma unroll
-        for (int i = 0; i < VEC; i += 4) {
-            const f32x4_t w = *reinterpret_cast<const f32x4_t *>(p + i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[i + j] = w[j];
-        }
+        for (int j = 0; j < 4; ++j) v[j] = lo[j], v[j + 4] = hi[j];
     } else {
-        static_assert(VEC == 8, "16 bytes");
-        dense_unpack8<T == LN_F16 ? DENSE_F16 : DENSE_BF16>(*reinterpret_cast<const u32x4_t *>(p), v);
+        Raw<T, VEC> r;
+        r.read(p);
+        r.values(v);
     }
 }
 template <int T, int VEC>
@@ -107,16 +129,23 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LnArgs a) {
     }
     constexpr int RPW = 256 / TPR;
     const float inv_d = 1.0f / (float)d;
-    for (int64_t m = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR; m < a.M; m += (int64_t)gridDim.x * RPW) {
+    Raw<T, VEC> raw[PER];                         // the row after the one that is worked on is on its way
+    const auto fetch = [&](int64_t m) {
         const E *x = static_cast<const E *>(a.x) + m * a.ldx;
-        float v[PER][VEC], s = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (i * TPR + t) * VEC;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
-            if (c < d) load<T, VEC>(x + c, v[i]);
+            raw[i].clear();
+            if (c < d) raw[i].read(x + c);
         }
+    };
+    const int64_t first = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR, step = (int64_t)gridDim.x * RPW;
+    if (first < a.M) fetch(first);
+    for (int64_t m = first; m < a.M; m += step) {
+        float v[PER][VEC], s = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) raw[i].values(v[i]);
+        if (m + step < a.M) fetch(m + step);
 #pragma unroll
         for (int i = 0; i < PER; ++i)
 #pragma unroll
@@ -165,20 +194,26 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LnArgs a) {
     }
     constexpr int RPW = 256 / TPR;
     const float inv_d = 1.0f / (float)d;
-    for (int64_t m = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR; m < a.M; m += (int64_t)gridDim.x * RPW) {
+    Raw<T, VEC> rx[PER], rdy[PER];                // the row after the one that is worked on is on its way
+    float mu_next = 0.f, r_next = 0.f;
+    const auto fetch = [&](int64_t m) {
         const E *x = static_cast<const E *>(a.x) + m * a.ldx, *dy = static_cast<const E *>(a.dy) + m * a.lddy;
-        float z[PER][VEC], g[PER][VEC];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int c = (i * TPR + t) * VEC;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) z[i][j] = 0.f, g[i][j] = 0.f;
-            if (c < d) {
-                load<T, VEC>(x + c, z[i]);
-                load<T, VEC>(dy + c, g[i]);
-            }
+            rx[i].clear(), rdy[i].clear();
+            if (c < d) rx[i].read(x + c), rdy[i].read(dy + c);
         }
-        const float mu = a.mean[m], r = a.rstd[m];
+        mu_next = a.mean[m], r_next = a.rstd[m];
+    };
+    const int64_t first = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR, step = (int64_t)gridDim.x * RPW;
+    if (first < a.M) fetch(first);
+    for (int64_t m = first; m < a.M; m += step) {
+        float z[PER][VEC], g[PER][VEC];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) rx[i].values(z[i]), rdy[i].values(g[i]);
+        const float mu = mu_next, r = r_next;
+        if (m + step < a.M) fetch(m + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < PER; ++i)
@@ -295,21 +330,26 @@ __global__ __launch_bounds__(256) void ln_columns_long_kernel(const LnArgs a, in
     out[a.d + c] = db;
 }
 
-// dw, db from the slabs: 64 columns per workgroup, 16 runs of slabs side by side, added in a fixed order.
+// dw, db from the slabs: 32 columns per workgroup, 32 runs of slabs side by side, added in a fixed order.
 template <int WT>
 __global__ __launch_bounds__(1024) void ln_join_kernel(const float *slabs, int n, int d, void *dw, void *db) {
     using W = typename Elem<WT>::type;
-    __shared__ float part[16][64];
-    const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
-    const int64_t col = (int64_t)blockIdx.y * d + c;
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x & 31, run = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    const float *p = slabs + (int64_t)blockIdx.y * d + min(c, d - 1);
     float s = 0.f;
-    if (c < d)
-        for (int i = run; i < n; i += 16) s += slabs[(int64_t)i * 2 * d + col];
+    for (int i = run; i < n; i += 32 * 8) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = p[(int64_t)min(i + k * 32, n - 1) * 2 * d];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += i + k * 32 < n ? v[k] : 0.f;
+    }
     part[run][lane] = s;
     __syncthreads();
     if (run || c >= d) return;
 #pragma unroll
-    for (int i = 1; i < 16; ++i) s += part[i][lane];
+    for (int i = 1; i < 32; ++i) s += part[i][lane];
     W *out = static_cast<W *>(blockIdx.y ? db : dw);
     if (out) out[c] = from_float<WT>(s);
 }
@@ -436,7 +476,7 @@ extern "C" int mortar_layernorm_bwd(const void *dy, int64_t lddy, const void *x,
     const hipStream_t st = static_cast<hipStream_t>(stream);
     launch_typed(a, type, w_fp32, true, vectors, st);
     if (params) {
-        const dim3 grid((unsigned)((d + 63) / 64), 2);
+        const dim3 grid((unsigned)((d + 31) / 32), 2);
         const int n = (int)slabs_of(M);
         if (type == LN_F32 || w_fp32) hipLaunchKernelGGL((ln_join_kernel<LN_F32>), grid, dim3(1024), 0, st, workspace, n, d, dw, db);
         else if (type == LN_BF16) hipLaunchKernelGGL((ln_join_kernel<LN_BF16>), grid, dim3(1024), 0, st, workspace, n, d, dw, db);
