@@ -164,16 +164,6 @@ def test_errors_are_those_of_rounding(dev):
         assert float((g.double() - r).norm() / r.norm()) <= one * n ** 0.5
 
 
-def test_formulas_against_differences():
-    """The 64-bit gradients that the kernels are compared with, against central differences of the 64-bit forward (CPU)."""
-    x, wgu, wd, dy = (v.double() for v in _case(5, 16, 24, torch.float32, "cpu", 3))
-    _, *grads = mlp_reference(x, wgu, wd, dy)
-    for i, grad in enumerate(grads):
-        v, e = normals(grad.shape, 50 + i, torch.float64, "cpu"), 1e-4
-        at = lambda s: float((dy * mlp_reference(*[p + s * v if j == i else p for j, p in enumerate((x, wgu, wd))])).sum())
-        assert abs((at(e) - at(-e)) / (2 * e) - float((grad * v).sum())) <= 1e-5 * float(grad.abs().sum())
-
-
 def test_gradient_against_differences(dev):
     """fp16 MLP along a direction: the loss <dy, y> at x +- e v against dx; each y is off by its bound at most, the quotient by e^2 times a third derivative."""
     x, wgu, wd, dy = _case(9, 64, 96, torch.float16, dev, 13)
