@@ -2,7 +2,7 @@
 MortarLinear / _SwiGLUMortar / stk_dds / mortar_gemv interfaces, served by hand-written HIP kernels."""
 from . import _lib, ops, pack, synth                                   # noqa: F401
 from .block_sparse import CMSBlockLinear                              # noqa: F401
-from .deploy_quant import (pack_mortar_ternary, pack_ternary_codes, shrink_mlp_to_mortar_ternary,  # noqa: F401
+from .deploy_quant import (pack_dense_fp8, pack_mortar_ternary, pack_ternary_codes, shrink_mlp_to_mortar_ternary,  # noqa: F401
                            unpack_ternary)
 from .engine import MortarDecodeMLP, looped_core_forward, mortar_gemv, mortar_pack_strips  # noqa: F401
 from .mlp import _KwargSequential, _make_swiglu, _SwiGLUMortar        # noqa: F401
@@ -13,5 +13,5 @@ from .stk import stk_dds, stk_sdd_at_b                                # noqa: F4
 
 __all__ = ["CMSBlockLinear", "MortarLinear", "_SwiGLUMortar", "_KwargSequential", "_make_swiglu", "TileRouter",
            "MortarPack", "MortarDecodeMLP", "stk_dds", "stk_sdd_at_b", "mortar_gemv", "mortar_pack_strips", "looped_core_forward",
-           "pack_mortar_ternary", "pack_ternary_codes", "unpack_ternary", "shrink_mlp_to_mortar_ternary",
+           "pack_dense_fp8", "pack_mortar_ternary", "pack_ternary_codes", "unpack_ternary", "shrink_mlp_to_mortar_ternary",
            "ops", "pack", "synth"]

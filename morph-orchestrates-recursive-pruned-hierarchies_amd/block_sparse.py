@@ -101,6 +101,7 @@ class CMSBlockLinear(nn.Module):
         W[row_j*blk+lr, col_j*blk+c], plus the transposed-topology metadata."""
         assert self._dense_mode, "carve() requires dense mode (pre-carve)"
         assert not self._mortar, "carve() already applied"
+        assert "dense_fp8" not in self._buffers, "carve() needs the weight, not its 8-bit codes"
         if self.out_features % blocking or self.in_features % blocking:
             raise ValueError(f"carve: [{self.out_features},{self.in_features}] not divisible by blocking {blocking}")
         B = self.tile_size
@@ -358,14 +359,29 @@ class CMSBlockLinear(nn.Module):
             y = y + self.bias
         return y.reshape(*lead, self.out_features)
 
+    def dense_weight(self) -> Tensor | None:
+        """The weight of a layer that is not carved, its pruned tiles zeroed; None for a layer that holds it in another form."""
+        w = self._parameters.get("weight")
+        if w is not None and self._prune_mask is not None:
+            B = self.tile_size
+            w = w * self._prune_mask.to(w.device).repeat_interleave(B, 0).repeat_interleave(B, 1).to(w.dtype)
+        return w
+
+    def _forward_fp8(self, x: Tensor) -> Tensor:
+        """A dense layer in 8 bits (deploy_quant.pack_dense_fp8): bf16 activations, output in the activation dtype, no backward."""
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("autograd through a layer of 8-bit codes: it serves inference only")
+        y = ops.linear_fp8(x if x.dtype == torch.bfloat16 else x.to(torch.bfloat16), self.dense_fp8.view(torch.float8_e4m3fn), self.dense_fp8_scale)
+        if self.bias is not None:
+            y = y + self.bias
+        return y if y.dtype == x.dtype else y.to(x.dtype)
+
     def forward(self, x: Tensor) -> Tensor:
         if self._mortar:
             return self._forward_mortar(x)
-        w = self.weight
-        if self._prune_mask is not None:
-            B = self.tile_size
-            w = w * self._prune_mask.to(w.device).repeat_interleave(B, 0).repeat_interleave(B, 1).to(w.dtype)
-        return F.linear(x, w, self.bias)
+        if "dense_fp8" in self._buffers:
+            return self._forward_fp8(x)
+        return F.linear(x, self.dense_weight(), self.bias)
 
     def _apply(self, fn, *a, **k):
         self._pack = None       # device may change
@@ -375,8 +391,14 @@ class CMSBlockLinear(nn.Module):
 
     def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
         """Accepts the reference's carved key set (block_sparse.py:983-1036): mortar_data + six index buffers
-        + mortar_ternary, or the packed variant mortar_packed + mortar_scale in place of mortar_data."""
-        dk, pk = prefix + "mortar_data", prefix + "mortar_packed"
+        + mortar_ternary, or the packed variant mortar_packed + mortar_scale in place of mortar_data; and dense_fp8 +
+        dense_fp8_scale in place of the weight of a layer that pack_dense_fp8 was applied to."""
+        dk, pk, fk = prefix + "mortar_data", prefix + "mortar_packed", prefix + "dense_fp8"
+        if fk in state_dict and "dense_fp8" not in self._buffers and not self._mortar:
+            dev = self.weight.device
+            del self._parameters["weight"]
+            for k in ("dense_fp8", "dense_fp8_scale"):
+                self.register_buffer(k, torch.empty_like(state_dict[prefix + k], device=dev))
         if (dk in state_dict or pk in state_dict) and not self._mortar:
             dev = self.weight.device
             idx = {k: torch.empty_like(state_dict[prefix + k], device=dev) for k in (

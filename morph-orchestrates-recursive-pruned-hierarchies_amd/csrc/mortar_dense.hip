@@ -215,7 +215,7 @@ int launch_few(const DenseArgs &a, hipStream_t st, const char *what) {
 
 // ---- checks ----------------------------------------------------------------------------------------------------------
 
-// A [rows, cols] matrix of 16-bit values as the kernels read it: 16-byte rows, and 512 rows or 2 * rows2 of them within 2 GiB of each other.
+// A [rows, cols] matrix of 16-bit values as the kernels read it: 16-byte rows, 256 of which lie within 2 GiB (DENSE_OUTSIDE: a tile is addressed in 32 bits).
 int check_matrix(const char *what, const char *name, const void *p, int64_t rows, int64_t cols, int64_t ld) {
     if (!p) return mortar_fail(MORTAR_ERR_ARG, "%s: %s is null", what, name);
     if (cols % 8 || ld % 8 || ld < cols || (reinterpret_cast<uintptr_t>(p) & 15))

@@ -6,7 +6,7 @@ import torch
 from torch import Tensor, nn
 
 __all__ = ["pack_ternary_codes", "unpack_ternary", "_ternary_quantize", "_ternary_quantize_per_block",
-           "pack_mortar_ternary", "shrink_mlp_to_mortar_ternary"]
+           "pack_mortar_ternary", "shrink_mlp_to_mortar_ternary", "pack_dense_fp8"]
 
 _CODES_PER_BYTE = 4
 _PLACE = (1, 4, 16, 64)          # value of a code in slot 0..3 of its byte (2 bits each, slot 0 lowest)
@@ -93,3 +93,23 @@ def shrink_mlp_to_mortar_ternary(bel, target_density: float = 0.25, blocking: in
     info = pack_mortar_ternary(cms, threshold, per_block=per_block)
     info.update(block_density=nnz / (Rb * Cb), nnz=nnz)
     return info
+
+
+def pack_dense_fp8(cms: nn.Module) -> dict:
+    """The weight of a CMSBlockLinear that stays dense in deployment, IN PLACE as e4m3 codes with one fp32 scale per 128 x 128 block
+    (ops.quantize_fp8_weight; its pruned tiles zeroed first): registers ``dense_fp8`` (the codes' bytes, so that casting the module
+    leaves them alone) and ``dense_fp8_scale`` and drops the parameter.  The layer then runs ops.linear_fp8."""
+    from . import ops
+    assert not getattr(cms, "_mortar", False) and "weight" in cms._parameters, "pack_dense_fp8 requires a layer that is not carved"
+    if cms.in_features % 16 or cms.out_features % 8:
+        raise ValueError(f"pack_dense_fp8: [{cms.out_features},{cms.in_features}] is not a multiple of [8, 16]")
+    with torch.no_grad():
+        w = cms.dense_weight()
+        q, scale = ops.quantize_fp8_weight(w)
+        error = float((q.float() * scale.repeat_interleave(128, 0)[:w.shape[0]].repeat_interleave(128, 1)[:, :w.shape[1]] - w.float()).norm()
+                      / w.float().norm().clamp(min=1e-30))
+    del cms._parameters["weight"]
+    cms.register_buffer("dense_fp8", q.view(torch.uint8))
+    cms.register_buffer("dense_fp8_scale", scale)
+    cms._prune_mask = None
+    return {"packed_bytes": q.numel() + 4 * scale.numel(), "relative_error": error}

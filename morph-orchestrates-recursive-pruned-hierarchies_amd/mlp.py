@@ -146,6 +146,10 @@ class _SwiGLUMortarFn(torch.autograd.Function):
 
 
 class _SwiGLUMortar(nn.Module):
+    # Before the carve: the whole MLP through ops.dense_mlp (bf16 or fp16 on the GPU, no router) instead of torch's linear layers and
+    # their backward.  Off by default: the results agree to rounding, not bit for bit.
+    dense_fused = False
+
     def __init__(self, d_model: int, d_ff: int):
         super().__init__()
         self.gate_up = MortarLinear(d_model, d_ff * 2, bias=False, initial_density=1.0)
@@ -224,6 +228,22 @@ class _SwiGLUMortar(nn.Module):
         y = _SwiGLUMortarFn.apply(x2, dg, dd, self)
         return y if x.dim() == 2 else y.reshape(*x.shape[:-1], self.d_model)
 
+    def _dense_step(self, x: Tensor) -> Tensor | None:
+        """The uncarved MLP in ops.dense_mlp, or None where that does not cover the layers or would pass by what hangs on them."""
+        if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or torch.is_autocast_enabled("cuda"):
+            return None
+        weights = []
+        for m in (self.gate_up, self.down):
+            cms = getattr(m, "_cms", None)
+            if (type(m) is not MortarLinear or type(cms) is not CMSBlockLinear or not call_is_forward(m, MortarLinear.forward)
+                    or not call_is_forward(cms, CMSBlockLinear.forward)):
+                return None
+            w = cms.dense_weight()
+            if w is None or cms.bias is not None or w.dtype != x.dtype or w.device != x.device or any(n % 8 for n in w.shape):
+                return None
+            weights.append(w)
+        return ops.dense_mlp(x, *weights)
+
     def _routed(self, x: Tensor, iter_idx: int):
         """(gates, auxiliary loss) of the module's router: one native call where calling it is nothing but its forward."""
         rt = self.router
@@ -274,6 +294,8 @@ class _SwiGLUMortar(nn.Module):
             xb = x2 if x2.dtype == torch.bfloat16 else x2.to(torch.bfloat16)
             y = _SwiGLUMortarFn.apply(xb, self.gate_up._cms.mortar_data, self.down._cms.mortar_data, self)
             return (y if y.dtype == x.dtype else y.to(x.dtype)).reshape(*lead, self.d_model)
+        if self.dense_fused and gates is None and self.router is None and not self._carved() and (y := self._dense_step(x)) is not None:
+            return y
         if not self._carved() or train:
             gu = self.gate_up(x)
             gate, up = gu.chunk(2, dim=-1)
