@@ -58,7 +58,7 @@ def test_codes_of_weights(dev, N, K, t):
 
 
 SIZES = [(1, 8, 16), (2, 24, 128), (7, 136, 272), (16, 264, 1360), (16, 128, 2048), (17, 136, 400), (33, 256, 144), (64, 520, 1040), (65, 8, 16), (130, 264, 400), (300, 136, 2736), (520, 1032, 272),
-         (2100, 2056, 400), (70, 64, 8192)]
+         (2100, 2056, 400), (70, 64, 8192), (20, 2056, 4112)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)
