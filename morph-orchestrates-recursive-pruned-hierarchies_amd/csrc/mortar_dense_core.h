@@ -31,7 +31,8 @@ enum DenseEpilogue {
     DENSE_STORE,        // C in the 16-bit type (e4m3 operands: bf16)
     DENSE_PARTIAL,      // fp32 sums of one K range into a slab of the workspace
     DENSE_SWIGLU,       // P rows are gate and up features: h = silu(g) u, and g, u themselves where asked for
-    DENSE_SWIGLU_BWD    // C is dh: the derivatives of the stored g, u, and h once more
+    DENSE_SWIGLU_BWD,   // C is dh: the derivatives of the stored g, u, and h once more
+    DENSE_STREAM        // as DENSE_STORE, past the caches
 };
 
 struct DenseArgs {
@@ -531,6 +532,8 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
                 if (n >= a.N) continue;
                 if constexpr (E == DENSE_STORE) {
                     *reinterpret_cast<u32x4_t *>(static_cast<uint16_t *>(a.c) + m * a.ldc + n) = dense_pack8<O>(d);
+                } else if constexpr (E == DENSE_STREAM) {
+                    __builtin_nontemporal_store(dense_pack8<O>(d), reinterpret_cast<u32x4_t *>(static_cast<uint16_t *>(a.c) + m * a.ldc + n));
                 } else if constexpr (E == DENSE_PARTIAL) {
                     float *o = static_cast<float *>(a.c) + ((int64_t)cur.split * a.M + m) * a.N + n;
                     *reinterpret_cast<f32x4_t *>(o) = f32x4_t{d[0], d[1], d[2], d[3]};
