@@ -361,7 +361,7 @@ class CMSBlockLinear(nn.Module):
 
     def dense_weight(self) -> Tensor | None:
         """The weight of a layer that is not carved, its pruned tiles zeroed; None for a layer that holds it in another form."""
-        w = self._parameters.get("weight")
+        w = getattr(self, "weight", None)            # (a parametrisation or a replica has it as an attribute)
         if w is not None and self._prune_mask is not None:
             B = self.tile_size
             w = w * self._prune_mask.to(w.device).repeat_interleave(B, 0).repeat_interleave(B, 1).to(w.dtype)

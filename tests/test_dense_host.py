@@ -4,9 +4,11 @@ import ctypes as C
 
 import pytest
 import torch
+import torch.nn.utils.parametrize
 
 from dense_util import mlp_reference, norm_reference, normals
 from mortar_amd import _lib, ops
+from mortar_amd.block_sparse import CMSBlockLinear
 
 A = 1 << 20                                   # an aligned address that is never read: every call here is refused
 
@@ -110,3 +112,18 @@ def test_formulas_against_autograd_and_differences():
         v, e = normals(grad.shape, 50 + i, torch.float64, "cpu"), 1e-4
         at = lambda s: float((dy * mlp_reference(*[p + s * v if j == i else p for j, p in enumerate((x, g, d))])).sum())
         assert abs((at(e) - at(-e)) / (2 * e) - float((grad * v).sum())) <= 1e-5 * float(grad.abs().sum())
+
+
+def test_a_parametrised_weight_is_the_layers_weight():
+    """The uncarved layer reads its weight as an attribute: under a parametrisation it is no parameter of the module."""
+    lin = CMSBlockLinear(32, 48)
+    w, x = lin.weight.detach().clone(), normals((3, 32), 1, torch.float32, "cpu")
+    torch.nn.utils.parametrize.register_parametrization(lin, "weight", Doubled())
+    assert "weight" not in lin._parameters
+    assert torch.equal(lin(x), torch.nn.functional.linear(x, 2 * w, lin.bias))
+    assert torch.equal(lin.dense_weight(), 2 * w)
+
+
+class Doubled(torch.nn.Module):
+    def forward(self, w):
+        return 2 * w
