@@ -575,7 +575,7 @@ def dense_mlp(x: Tensor, w_gate_up: Tensor, w_down: Tensor) -> Tensor:
 
 def quantize_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
     """(codes float8_e4m3fn like x, scales fp32 [..., ceil(K / 128)]) of bf16 activations [..., K], K a multiple of 16: one scale
-    amax / 448 (1 for zeros) per row and 128 values, codes x / scale rounded to nearest even.  The scales are consecutive along the rows."""
+    amax * (1 / 448) (1 for zeros) per row and 128 values, codes x / scale rounded to nearest even.  The scales are consecutive along the rows."""
     return _lib.native().quantize_fp8(x)
 
 

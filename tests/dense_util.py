@@ -153,7 +153,7 @@ def fp8_rows(x):
     p[:, :k] = x.float()
     p = p.view(m, kb, 128)
     a = p.abs().amax(2)
-    s = torch.where(a > 0, a / 448.0, torch.ones_like(a))
+    s = torch.where(a > 0, a * torch.tensor(1.0 / 448.0, dtype=torch.float32, device=a.device), torch.ones_like(a))
     q = (p / s[:, :, None]).to(torch.float8_e4m3fn).view(torch.uint8).view(m, kb * 128)[:, :k].contiguous()
     return q.view(torch.float8_e4m3fn), s
 
@@ -165,7 +165,7 @@ def fp8_weight(w):
     p[:n, :k] = w.float()
     p = p.view(nb, 128, kb, 128)
     a = p.abs().amax((1, 3))
-    s = torch.where(a > 0, a / 448.0, torch.ones_like(a))
+    s = torch.where(a > 0, a * torch.tensor(1.0 / 448.0, dtype=torch.float32, device=a.device), torch.ones_like(a))
     q = (p / s[:, None, :, None]).to(torch.float8_e4m3fn).view(torch.uint8).view(nb * 128, kb * 128)[:n, :k].contiguous()
     return q.view(torch.float8_e4m3fn), s
 
