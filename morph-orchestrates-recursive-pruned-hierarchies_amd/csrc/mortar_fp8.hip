@@ -118,24 +118,16 @@ __global__ __launch_bounds__(256) void fp8_blocks_kernel(const void *w, int32_t 
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// As the 16-bit form: 16 rows of W per workgroup, K blocks of 128 dealt to its waves, the weights straight into registers.  The weights'
-// traffic is what bounds these calls, so the codes are turned into bf16 (exactly) and multiplied there, with fp32 sums: the e4m3
-// instructions align the products of a group to the largest and cut them 13 bits below it.  QUANT: x is bf16 and every workgroup
-// quantises it into LDS first, while its first weights are on their way (few values: the launch that would do it once takes longer).
-__device__ __forceinline__ u32x4_t codes_bf16(uint32_t lo, uint32_t hi) {      // eight codes
-    return u32x4_t{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
-}
-
+// As the 16-bit form: 16 rows of W per workgroup, K blocks of 128 dealt to its waves, the weights straight into registers: their
+// traffic is what bounds these calls.  QUANT: x is bf16 and every workgroup quantises it into LDS first, while its first weights are
+// on their way (few values: the launch that would do it once takes longer).
 template <bool QUANT, int MT, int NW, int U>
 __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(const DenseArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     f32x4_t *part = reinterpret_cast<f32x4_t *>(smem);                     // [wave][token tile][lane]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4, r = lane & 15;
     const int n0 = blockIdx.x * 16, blocks = (a.K + 127) >> 7;
-    uint16_t *values = reinterpret_cast<uint16_t *>(smem + NW * MT * 1024);        // QUANT: the codes as bf16 [M][blocks * 128], then the scales [M][blocks]
+    unsigned char *values = smem + NW * MT * 1024;                         // QUANT: the codes [M][blocks * 128], then the scales [M][blocks]
     float *scales = reinterpret_cast<float *>(values + a.M * blocks * 128);
     const auto whole = [](const void *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, DENSE_OUTSIDE, 0x00020000); };
     const auto read = [](__amdgpu_buffer_rsrc_t b, uint32_t off) { return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0)); };
@@ -146,7 +138,7 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(const DenseArgs a) {
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     for (int c0 = wave; c0 < blocks || (QUANT && c0 == wave); c0 += NW * U) {
-        u32x4_t w[U][2], x[U][MT][QUANT ? 4 : 2];
+        u32x4_t w[U][2], x[U][MT][2];
         float f[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -162,7 +154,7 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(const DenseArgs a) {
                     if (k < a.K) read8<MORTAR_BF16>(a.q, m * (a.ldq / 2) + k, v);
                     const float sc = scale_of(row_max(abs_max8(v)));
                     const u32x2_t q = quantise8<true>(v, sc);
-                    *reinterpret_cast<u32x4_t *>(values + m * blocks * 128 + k) = codes_bf16(q[0], q[1]);
+                    *reinterpret_cast<u32x2_t *>(values + m * blocks * 128 + k) = q;
                     if ((threadIdx.x & 15) == 0) scales[m * blocks + b] = sc;
                 }
                 __syncthreads();
@@ -176,7 +168,7 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(const DenseArgs a) {
                 const int m = min(t * 16 + r, a.M - 1);
                 if constexpr (QUANT) {
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) x[u][t][h] = *reinterpret_cast<const u32x4_t *>(values + m * blocks * 128 + bs * 128 + (h >> 1) * 64 + g * 16 + (h & 1) * 8);
+                    for (int h = 0; h < 2; ++h) x[u][t][h] = *reinterpret_cast<const u32x4_t *>(values + m * blocks * 128 + bs * 128 + h * 64 + g * 16);
                     f[u][t] = scales[m * blocks + bs];
                 } else {
 #pragma unroll
@@ -189,19 +181,10 @@ __global__ __launch_bounds__(NW * 64) void fp8_few_kernel(const DenseArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (c0 + u * NW >= blocks) break;
-            u32x4_t wv[4];                       // values 16 g .. 16 g + 15 of the block's halves, eight at a time
-#pragma unroll
-            for (int h = 0; h < 4; ++h) wv[h] = codes_bf16(w[u][h >> 1][(h & 1) * 2], w[u][h >> 1][(h & 1) * 2 + 1]);
+            const auto both = [](const u32x4_t (&v)[2]) { return i32x8_t{(int)v[0][0], (int)v[0][1], (int)v[0][2], (int)v[0][3], (int)v[1][0], (int)v[1][1], (int)v[1][2], (int)v[1][3]}; };
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    u32x4_t xv;
-                    if constexpr (QUANT) xv = x[u][t][h];
-                    else xv = codes_bf16(x[u][t][h >> 1][(h & 1) * 2], x[u][t][h >> 1][(h & 1) * 2 + 1]);
-                    d = mortar_mfma(wv[h], xv, d);
-                }
+                const f32x4_t d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(both(w[u]), both(x[u][t]), f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
 #pragma unroll
                 for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(d[v], f[u][t], acc[t][v]);
             }
@@ -226,7 +209,7 @@ int launch_error(const char *what) {
 }
 
 constexpr int QUANT_GROUPS = 128;        // groups of 128 values that a workgroup quantises for itself
-constexpr int GROUP_BYTES = 256 + 4;     // and what one takes in LDS
+constexpr int GROUP_BYTES = 128 + 4;     // and what one takes in LDS
 // Rows that the weights' traffic bounds.  In us, 16 / 17 / 32 rows here and 33 in tiles: 2048 -> 2048 4.2 / 4.6 / 5.3 and 7.1 (a short ring
 // of tiles that cannot hide its start), 2048 -> 11264 8.0 / 9.2 / 11.0 and 8.0 (23 MB of weights, 4.8 to read), 5632 -> 2048 7.3 / 8.2 /
 // 10.0 and 8.0, 8192 -> 8192 17 / 20 / 25 and 23: above 16 rows the second fragment of x per wave pays for small weights only.
