@@ -84,6 +84,7 @@ def test_fp8():
                 dict(ldy=60), dict(sx=None), dict(x=A + 8)):
         _refused(y(**bad))
     _refused(y(s_m=1 << 40), -4)
+    _refused(y(N=1 << 26, ldy=1 << 26), -4)
     assert q(M=0) == 0 and y(M=0) == 0
     assert L.mortar_fp8_quantizes_inside(1, 2048) == 1 and L.mortar_fp8_quantizes_inside(17, 128) == 0 and L.mortar_fp8_quantizes_inside(16, 2048) == 0
 
