@@ -62,22 +62,18 @@ struct Raw<T, 1> {
     __device__ __forceinline__ void clear() { e = 0; }
     __device__ __forceinline__ void values(float (&v)[1]) const { v[0] = to_float<T>(e); }
 };
-// Weights beside VEC values of the rows: fp32 ones may be two words.
-template <int T, int VEC>
-__device__ __forceinline__ void load(const typename Elem<T>::type *p, float (&v)[VEC]) {
-    if constexpr (T == LN_F32 && VEC == 8) {
-        Raw<T, 4> a, b;
-        a.read(p), b.read(p + 4);
+template <>
+struct Raw<LN_F32, 8> {                           // fp32 weights beside eight 16-bit values
+    Raw<LN_F32, 4> a, b;
+    __device__ __forceinline__ void read(const float *p) { a.read(p), b.read(p + 4); }
+    __device__ __forceinline__ void clear() { a.clear(), b.clear(); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
         float lo[4], hi[4];
         a.values(lo), b.values(hi);
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = lo[j], v[j + 4] = hi[j];
-    } else {
-        Raw<T, VEC> r;
-        r.read(p);
-        r.values(v);
     }
-}
+};
 template <int T, int VEC>
 __device__ __forceinline__ void store(typename Elem<T>::type *p, const float (&v)[VEC]) {
     if constexpr (VEC == 1) {
@@ -121,15 +117,6 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LnArgs a) {
     __shared__ float sm[2][4];
     int turn = 0;
     const int t = threadIdx.x % TPR, d = a.d;
-    float w[PER][VEC], b[PER][VEC];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int c = (i * TPR + t) * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) w[i][j] = 1.f, b[i][j] = 0.f;
-        if (c < d && a.w) load<WT, VEC>(static_cast<const W *>(a.w) + c, w[i]);
-        if (c < d && a.b) load<WT, VEC>(static_cast<const W *>(a.b) + c, b[i]);
-    }
     constexpr int RPW = 256 / TPR;
     const float inv_d = 1.0f / (float)d;
     Raw<T, VEC> raw[PER];                         // the row after the one that is worked on is on its way
@@ -144,6 +131,24 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const LnArgs a) {
     };
     const int64_t first = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR, step = (int64_t)gridDim.x * RPW;
     if (first < a.M) fetch(first);
+    float w[PER][VEC], b[PER][VEC];
+    {
+        Raw<WT, VEC> rw[PER], rb[PER];            // all of them on their way at once
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (i * TPR + t) * VEC;
+            rw[i].clear(), rb[i].clear();
+            if (c < d && a.w) rw[i].read(static_cast<const W *>(a.w) + c);
+            if (c < d && a.b) rb[i].read(static_cast<const W *>(a.b) + c);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            rw[i].values(w[i]), rb[i].values(b[i]);
+            if (!a.w)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) w[i][j] = 1.f;
+        }
+    }
     for (int64_t m = first; m < a.M; m += step) {
         float v[PER][VEC], s = 0.f;
 #pragma unroll
@@ -184,17 +189,6 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LnArgs a) {
     __shared__ float sm[2][2][4];
     int turn = 0, turn2 = 0;
     const int t = threadIdx.x % TPR, d = a.d;
-    float w[PER][VEC], dw[PARAMS ? PER : 1][VEC], db[PARAMS ? PER : 1][VEC];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int c = (i * TPR + t) * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            w[i][j] = 1.f;
-            if constexpr (PARAMS) dw[i][j] = 0.f, db[i][j] = 0.f;
-        }
-        if (c < d && a.w) load<WT, VEC>(static_cast<const W *>(a.w) + c, w[i]);
-    }
     constexpr int RPW = 256 / TPR;
     const float inv_d = 1.0f / (float)d;
     Raw<T, VEC> rx[PER], rdy[PER];                // the row after the one that is worked on is on its way
@@ -211,6 +205,25 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LnArgs a) {
     };
     const int64_t first = (int64_t)blockIdx.x * RPW + threadIdx.x / TPR, step = (int64_t)gridDim.x * RPW;
     if (first < a.M) fetch(first);
+    float w[PER][VEC], dw[PARAMS ? PER : 1][VEC], db[PARAMS ? PER : 1][VEC];
+    {
+        Raw<WT, VEC> rw[PER];
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int c = (i * TPR + t) * VEC;
+            rw[i].clear();
+            if (c < d && a.w) rw[i].read(static_cast<const W *>(a.w) + c);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            rw[i].values(w[i]);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                if (!a.w) w[i][j] = 1.f;
+                if constexpr (PARAMS) dw[i][j] = 0.f, db[i][j] = 0.f;
+            }
+        }
+    }
     for (int64_t m = first; m < a.M; m += step) {
         float z[PER][VEC], g[PER][VEC];
 #pragma unroll
