@@ -7,9 +7,10 @@
 // and its result.  A row belongs to one wavefront (up to 2 KB x 4 of it) or to the four of a workgroup; workgroups walk over rows, w
 // and b in registers, and the backward adds dw and db of its rows there: one fp32 slab per workgroup, added in order by a second
 // kernel, so that results do not depend on timing.
-// Measured, forward / backward / join of the slabs: 16384 x 2048 bf16 26 / 36 / 4 us (134 and 201 MB: 5.1 and 5.5 TB/s, where a large copy
-// reaches 5.0), 16384 x 768 fp32 17 / 25 / 4, 1021 x 1999 fp16 (no row is aligned: single values) 6 / 9 / 4.  The next row is loaded
-// before the sums of the present one (without that the backward of the first took 43), the slabs by 32 threads per column (9).
+// Measured, forward / backward / join of the slabs: 16384 x 2048 bf16 23 / 35 / 4 us (134 and 201 MB: 5.8 TB/s, where a large copy reaches
+// 5.0), 16384 x 768 fp32 17 / 25 / 4, 1021 x 1999 fp16 (no row is aligned: single values) 6 / 10 / 4.  The next row is loaded before the
+// sums of the present one (without that the backward of the first took 43), the weights behind the first row and all at once (one by
+// one its forward took 26), the slabs by 32 threads per column (9).
 #include <hip/hip_runtime.h>
 
 #include "mortar_dense_core.h"
