@@ -128,3 +128,21 @@ def test_a_parametrised_weight_is_the_layers_weight():
 class Doubled(torch.nn.Module):
     def forward(self, w):
         return 2 * w
+
+
+def test_layers_that_cannot_be_packed():
+    """Widths that the 8-bit product does not take are refused before the layer is touched, carved and packed layers likewise."""
+    from mortar_amd.deploy_quant import pack_dense_fp8
+    for shape in ((20, 32), (32, 12)):
+        lin = CMSBlockLinear(*shape, tile_size=4)
+        with pytest.raises(ValueError, match="not a multiple"):
+            pack_dense_fp8(lin)
+        assert "weight" in lin._parameters
+    lin = CMSBlockLinear(32, 32)
+    lin.carve()
+    with pytest.raises(AssertionError):
+        pack_dense_fp8(lin)
+    lin = CMSBlockLinear(32, 32)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        pack_dense_fp8(lin)
+    assert "weight" in lin._parameters and not lin._buffers.keys() & {"dense_fp8"}
