@@ -23,10 +23,12 @@ _router_forward = TileRouter.forward
 
 def call_is_forward(m, forward) -> bool:
     """True if calling ``m`` is the module method ``forward`` and nothing else: not another kind of object, not overridden by a
-    subclass or on the instance, no hooks of its own or global ones.  Whoever does a module's work without calling it has to
-    ask first."""
+    subclass or on the instance, no hooks of its own or global ones, of the forward or of the backward.  Whoever does a
+    module's work without calling it has to ask first."""
     return (getattr(type(m), "forward", None) is forward and type(m).__call__ is nn.Module.__call__ and "forward" not in m.__dict__
-            and not (m._forward_hooks or m._forward_pre_hooks or _module._global_forward_hooks or _module._global_forward_pre_hooks))
+            and not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                     or _module._global_forward_hooks or _module._global_forward_pre_hooks
+                     or _module._global_backward_hooks or _module._global_backward_pre_hooks))
 
 
 class _KwargSequential(nn.Sequential):
