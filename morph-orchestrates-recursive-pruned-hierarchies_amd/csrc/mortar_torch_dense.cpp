@@ -54,11 +54,13 @@ void same_device(const at::Tensor &a, const at::Tensor &b, const char *what, con
 
 int type_code(at::ScalarType t) { return t == at::kBFloat16 ? MORTAR_BF16 : t == at::kHalf ? MORTAR_FP16 : t == at::kFloat ? MORTAR_FP32 : -1; }
 
-// t [..., d] as rows [M, d] that the kernels can read: `unit` values per 16 bytes; copied where strides or address do not allow it.
-at::Tensor rows_of(const at::Tensor &t, int64_t d, int64_t unit) {
+// t [..., d] as rows [M, d] that the kernels can read: `unit` values per 16 bytes, tiles: 256 rows within 2 GiB; copied where strides or
+// address do not allow it.
+at::Tensor rows_of(const at::Tensor &t, int64_t d, int64_t unit, bool tiles = true) {
     at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, d});
     const bool one = r.size(0) <= 1;
-    if ((d > 1 && r.stride(1) != 1) || (!one && (r.stride(0) % unit || r.stride(0) < d)) || !aligned16(r.const_data_ptr()))
+    if ((d > 1 && r.stride(1) != 1) || (!one && (r.stride(0) % unit || r.stride(0) < d || (tiles && r.stride(0) * 256 * r.element_size() >= INT64_C(1) << 31))) ||
+        !aligned16(r.const_data_ptr()))
         r = r.clone(at::MemoryFormat::Contiguous);
     return r;
 }
@@ -312,7 +314,7 @@ PyObject *py_quantize_fp8(PyObject *, PyObject *const *a, Py_ssize_t na) {
     at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn).requires_grad(false));
     at::Tensor s = at::empty({kb, M}, x.options().dtype(at::kFloat).requires_grad(false));
     if (M) {
-        const at::Tensor r = rows_of(x, K, 8);
+        const at::Tensor r = rows_of(x, K, 8, false);
         check_rc(mortar_fp8_quantize(static_cast<const uint16_t *>(data(r)), M, (int32_t)K, ld_of(r), static_cast<uint8_t *>(mut(q)), K, floats(s), 1, M, stream_of(x)),
                  "mortar_fp8_quantize");
     }
@@ -335,7 +337,7 @@ PyObject *py_quantize_fp8_weight(PyObject *, PyObject *const *a, Py_ssize_t na) 
     check_k(K, what);
     TORCH_CHECK_VALUE(N < (1 << 23), what, ": too many rows");
     const c10::DeviceGuard guard(w.device());
-    const at::Tensor r = rows_of(w, K, w.scalar_type() == at::kFloat ? 4 : 8);
+    const at::Tensor r = rows_of(w, K, w.scalar_type() == at::kFloat ? 4 : 8, false);
     at::Tensor q = at::empty({N, K}, w.options().dtype(at::kFloat8_e4m3fn).requires_grad(false));
     at::Tensor s = at::empty({(N + 127) / 128, (K + 127) / 128}, w.options().dtype(at::kFloat).requires_grad(false));
     check_rc(mortar_fp8_quantize_weight(data(r), (int32_t)N, (int32_t)K, ld_of(r), type_code(w.scalar_type()), static_cast<uint8_t *>(mut(q)), K, floats(s),
@@ -389,7 +391,7 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *a, Py_ssize_t na) {
             xp = data(xr), ldx = ld_of(xr);
             sx = static_cast<const float *>(xs.const_data_ptr()), s_m = xs.stride(0), s_k = xs.stride(1);
         } else {
-            xr = rows_of(x, K, 8);
+            xr = rows_of(x, K, 8, false);
             xp = data(xr), ldx = ld_of(xr);
             if (!mortar_fp8_quantizes_inside(M, K)) {
                 buf = empty_bytes(x, M * K + M * kb * 4);        // codes, then scales (M K is a multiple of 16)
