@@ -4,6 +4,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
+
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
@@ -36,12 +38,15 @@ c10::DispatchKeySet riders() {
                                 K::FuncTorchDynamicLayerBackMode, K::Batched, K::Functionalize, K::Conjugate, K::Negative, K::ZeroTensor, K::Tracer});
 }
 
+bool plain(const at::Tensor &t) {
+    return !c10::impl::tls_local_dispatch_key_set().included_.has_any(riders()) && !t.key_set().has_any(riders()) && t.layout() == at::kStrided;
+}
+
 // Argument `name` as a plain tensor on the GPU.
 const at::Tensor &tensor_arg(PyObject *o, const char *what, const char *name) {
     TORCH_CHECK_TYPE(THPVariable_CheckExact(o) || THPVariable_Check(o), what, ": ", name, " must be a tensor");
     const at::Tensor &t = THPVariable_Unpack(o);
-    TORCH_CHECK(!c10::impl::tls_local_dispatch_key_set().included_.has_any(riders()) && !t.key_set().has_any(riders()) && t.layout() == at::kStrided,
-                what, ": ", name, " must be a plain strided tensor, outside functional transforms and tracing");
+    TORCH_CHECK(plain(t), what, ": ", name, " must be a plain strided tensor, outside functional transforms and tracing");
     TORCH_CHECK(t.is_cuda(), what, ": tensor must live on a ROCm device (the MORTAR runtime has no CPU path)");
     TORCH_CHECK(!t._fw_grad(0).defined(), what, ": no forward-mode gradients");
     return t;
@@ -292,6 +297,20 @@ PyObject *py_dense_mlp(PyObject *, PyObject *const *a, Py_ssize_t na) {
     return THPVariable_Wrap(std::move(y));
 }
 
+// dense_mlp_covers(x, w_gate_up, w_down) -> whether dense_mlp takes these tensors, of fitting sizes and types, as they are and where the call
+// stands: no subclass, transform, tracing, mode or forward-mode gradient that it would refuse, and matrices that the kernels can address.
+PyObject *py_dense_mlp_covers(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    TORCH_CHECK_TYPE(na == 3, "dense_mlp_covers: 3 arguments");
+    for (Py_ssize_t i = 0; i < 3; ++i) {
+        if (!THPVariable_CheckExact(a[i])) Py_RETURN_FALSE;
+        const at::Tensor &t = THPVariable_Unpack(a[i]);
+        if (!plain(t) || !t.is_cuda() || t._fw_grad(0).defined()) Py_RETURN_FALSE;
+    }
+    const at::Tensor &x = THPVariable_Unpack(a[0]), &wgu = THPVariable_Unpack(a[1]), &wd = THPVariable_Unpack(a[2]);
+    const int64_t d = wgu.size(1), f = wd.size(1), n = wd.size(0), span = INT64_C(1) << 30;        // (values of 16 bits in 2 GiB)
+    return PyBool_FromLong(x.numel() < d * span && 256 * std::max({d, 2 * f, n}) < span && (f + 256) * d < span);
+}
+
 // ---- 8 bits ----------------------------------------------------------------------------------------------------------
 
 void no_gradients(const at::Tensor &t, const char *what) {
@@ -420,6 +439,7 @@ PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t na) {
 #define MORTAR_METHOD(name, f, doc) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<f>)), METH_FASTCALL, doc}
 PyMethodDef methods[] = {MORTAR_METHOD("layernorm", py_layernorm, "LayerNorm of the rows of x, with its autograd node."),
                          MORTAR_METHOD("dense_mlp", py_dense_mlp, "The dense SwiGLU MLP of the rows of x, with its autograd node."),
+                         MORTAR_METHOD("dense_mlp_covers", py_dense_mlp_covers, "Whether dense_mlp takes these tensors."),
                          MORTAR_METHOD("quantize_fp8", py_quantize_fp8, "e4m3 codes and scales of activations."),
                          MORTAR_METHOD("quantize_fp8_weight", py_quantize_fp8_weight, "e4m3 codes and block scales of a weight."),
                          MORTAR_METHOD("linear_fp8", py_linear_fp8, "x W^T in e4m3."),

@@ -149,7 +149,8 @@ class _SwiGLUMortarFn(torch.autograd.Function):
 
 class _SwiGLUMortar(nn.Module):
     # Before the carve: the whole MLP through ops.dense_mlp (bf16 or fp16 on the GPU, no router) instead of torch's linear layers and
-    # their backward.  Off by default: the results agree to rounding, not bit for bit.
+    # their backward.  Off by default: the results agree to rounding, not bit for bit, and its gradients cannot be differentiated
+    # again (a backward with create_graph=True raises).  Calls that dense_mlp does not cover run the layers.
     dense_fused = False
 
     def __init__(self, d_model: int, d_ff: int):
@@ -232,7 +233,8 @@ class _SwiGLUMortar(nn.Module):
 
     def _dense_step(self, x: Tensor) -> Tensor | None:
         """The uncarved MLP in ops.dense_mlp, or None where that does not cover the layers or would pass by what hangs on them."""
-        if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or torch.is_autocast_enabled("cuda"):
+        if (torch.compiler.is_compiling() or not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16)
+                or torch.is_autocast_enabled("cuda")):
             return None
         weights = []
         for m in (self.gate_up, self.down):
@@ -244,7 +246,7 @@ class _SwiGLUMortar(nn.Module):
             if w is None or cms.bias is not None or w.dtype != x.dtype or w.device != x.device or any(n % 8 for n in w.shape):
                 return None
             weights.append(w)
-        return ops.dense_mlp(x, *weights)
+        return ops.dense_mlp(x, *weights) if _lib.native().dense_mlp_covers(x, *weights) else None
 
     def _routed(self, x: Tensor, iter_idx: int):
         """(gates, auxiliary loss) of the module's router: one native call where calling it is nothing but its forward."""

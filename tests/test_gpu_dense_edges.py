@@ -87,3 +87,76 @@ def test_codes_of_rows_far_apart(dev, M):
     assert torch.equal(ops.linear_fp8(_apart(q, 1 << 23), wq, ws, s), want)
     far = _apart(x, 1 << 22)
     assert torch.equal(ops.linear_fp8(far, wq, ws), want) and torch.equal(ops.quantize_fp8(far)[0].view(torch.uint8), q.view(torch.uint8))
+
+
+class _Sub(torch.Tensor):
+    seen = 0
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        if func is torch.nn.functional.linear:
+            cls.seen += 1
+        return super().__torch_function__(func, types, args, kwargs or {})
+
+
+class _Watch(TorchDispatchMode):
+    def __init__(self):
+        super().__init__()
+        self.names = []
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        self.names.append(str(func))
+        return func(*args, **(kwargs or {}))
+
+
+def test_calls_that_only_torchs_layers_cover(dev):
+    """Functional transforms, tracing, forward mode, subclasses, modes: the results of the layers, not an exception."""
+    mlp = _mlp(dev)
+    x, t = normals((3, 64), 1, BF16, dev), normals((3, 64), 2, BF16, dev)
+    plain = _mlp(dev)
+    plain.dense_fused = False
+
+    def equal(f):
+        a, b = f(mlp), f(plain)
+        assert all(torch.equal(p, q) for p, q in zip(a, b)) if isinstance(a, tuple) else torch.equal(a, b)
+    equal(lambda m: torch.func.vmap(m)(x.view(3, 1, 64)))
+    equal(lambda m: torch.func.jvp(m, (x,), (t,)))
+    equal(lambda m: torch.func.grad(lambda v: m(v).float().sum())(x))
+    equal(lambda m: torch.jit.trace(m, x, check_trace=False)(x))
+    equal(lambda m: torch.compile(m, backend="eager", fullgraph=True)(x))
+
+    def forward_mode(m):
+        with torch.autograd.forward_ad.dual_level():
+            y = torch.autograd.forward_ad.unpack_dual(m(torch.autograd.forward_ad.make_dual(x, t)))
+            return y.primal, y.tangent
+    equal(forward_mode)
+
+    def weights_tangent(m):
+        w = m.down._cms.weight
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(w.detach(), torch.ones_like(w))
+            y = torch.autograd.forward_ad.unpack_dual(torch.func.functional_call(m, {"down._cms.weight": dual}, (x,)))
+            return y.primal, y.tangent
+    equal(weights_tangent)
+    with _Watch() as watch:
+        y = mlp(x)
+    assert torch.equal(y, plain(x)) and sum("mm" in n or "linear" in n for n in watch.names) == 2
+    y = mlp(x.as_subclass(_Sub))
+    assert type(y) is _Sub and _Sub.seen == 2 and torch.equal(y.as_subclass(torch.Tensor), plain(x))
+
+
+def test_the_second_derivative_is_refused(dev):
+    x = normals((3, 64), 1, BF16, dev).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(_mlp(dev)(x).sum(), [x], create_graph=True)
+
+
+def test_weights_that_one_launch_cannot_address(dev):
+    """gate_up of 2 GiB for the gate rows alone (one value, repeated): torch's layers run."""
+    n = 1 << 15
+    mlp = _mlp(dev)
+    one = lambda *s: torch.nn.Parameter(torch.full((), 2.0 ** -15, dtype=BF16, device=dev).expand(s), requires_grad=False)
+    mlp.gate_up._cms.weight, mlp.down._cms.weight = one(2 * n, n), one(n, n)
+    y = mlp(torch.ones((1, n), dtype=BF16, device=dev))
+    h = torch.nn.functional.silu(torch.ones((), dtype=BF16, device=dev))           # gate = up = 1 exactly, y the mean of n values of h
+    assert torch.equal(y, h.expand(1, n))
