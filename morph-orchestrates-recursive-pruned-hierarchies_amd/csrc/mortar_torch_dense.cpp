@@ -201,6 +201,7 @@ at::Tensor mlp_forward(const at::Tensor &x, const at::Tensor &wgu, const at::Ten
     shape.back() = n;
     at::Tensor y = empty_like_rows(x, shape);
     r.wgu = rows_of(wgu, d, 8);
+    if ((f + 256) * ld_of(r.wgu) >= INT64_C(1) << 30) r.wgu = r.wgu.contiguous();        // a gate row and its up row are addressed together: 2 GiB
     r.wd = rows_of(wd, f, 8);
     if (x.numel() == 0) return y;
     const int64_t M = x.numel() / d;

@@ -160,3 +160,10 @@ def test_weights_that_one_launch_cannot_address(dev):
     y = mlp(torch.ones((1, n), dtype=BF16, device=dev))
     h = torch.nn.functional.silu(torch.ones((), dtype=BF16, device=dev))           # gate = up = 1 exactly, y the mean of n values of h
     assert torch.equal(y, h.expand(1, n))
+
+
+@pytest.mark.parametrize("M", [3, 70])
+def test_gate_and_up_rows_far_apart(dev, M):
+    """A gate row and its up row 2 GiB apart, in rows that are not."""
+    x, wgu, wd = normals((M, 64), 1, BF16, dev), normals((2048, 64), 2, BF16, dev, 0.1), normals((16, 1024), 3, BF16, dev, 0.03)
+    assert torch.equal(ops.dense_mlp(x, _apart(wgu, 1 << 20), wd), ops.dense_mlp(x, wgu, wd))
