@@ -389,11 +389,18 @@ class CMSBlockLinear(nn.Module):
 
     # ------------------------------------------------------------------ checkpoints
 
-    def _load_from_state_dict(self, state_dict, prefix, *args, **kwargs):
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
         """Accepts the reference's carved key set (block_sparse.py:983-1036): mortar_data + six index buffers
         + mortar_ternary, or the packed variant mortar_packed + mortar_scale in place of mortar_data; and dense_fp8 +
         dense_fp8_scale in place of the weight of a layer that pack_dense_fp8 was applied to."""
         dk, pk, fk = prefix + "mortar_data", prefix + "mortar_packed", prefix + "dense_fp8"
+        if fk in state_dict and not self._mortar:
+            expected = {"dense_fp8": (self.out_features, self.in_features), "dense_fp8_scale": (-(-self.out_features // 128), -(-self.in_features // 128))}
+            errors = [f"size mismatch for {prefix + k}: {tuple(state_dict[prefix + k].shape)} in the checkpoint, {size} in this layer"
+                      for k, size in expected.items() if state_dict[prefix + k].shape != size]
+            if errors:                           # (an error of strict and other loads, as for every parameter; the layer stays as it was)
+                error_msgs.extend(errors)
+                return
         if fk in state_dict and "dense_fp8" not in self._buffers and not self._mortar:
             dev = self.weight.device
             del self._parameters["weight"]
@@ -428,7 +435,7 @@ class CMSBlockLinear(nn.Module):
             Rb, Cb = self.out_features // blocking, self.in_features // blocking
             self.density = nnz / (Rb * Cb)
         self._pack = None
-        super()._load_from_state_dict(state_dict, prefix, *args, **kwargs)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, tile_size={self.tile_size}, "

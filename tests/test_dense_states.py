@@ -25,3 +25,43 @@ def test_a_layer_with_hooks_is_called(register):
     finally:
         handle.remove()
     assert call_is_forward(lin, CMSBlockLinear.forward)
+
+
+def _codes(n=N, k=K, seed=0):
+    """The two buffers of a packed layer, as pack_dense_fp8 makes them."""
+    g = torch.Generator().manual_seed(seed)
+    codes = torch.randn((n, k), generator=g).to(torch.float8_e4m3fn).view(torch.uint8)
+    return codes, torch.rand((-(-n // 128), -(-k // 128)), generator=g) / 7
+
+
+def _packed(seed=0, bias=False):
+    lin = CMSBlockLinear(K, N, bias=bias)
+    state = {"dense_fp8": _codes(seed=seed)[0], "dense_fp8_scale": _codes(seed=seed)[1]}
+    if bias:
+        state["bias"] = torch.arange(N, dtype=torch.float32)
+    lin.load_state_dict(state)
+    return lin, state
+
+
+def _holds(lin, state):
+    return all(torch.equal(lin.state_dict()[k], v) and lin.state_dict()[k].dtype == v.dtype for k, v in state.items()) and lin.state_dict().keys() == state.keys()
+
+
+def test_packed_state_loads():
+    for bias in (False, True):
+        lin, state = _packed(bias=bias)
+        assert "weight" not in lin._parameters and _holds(lin, state)
+        lin.load_state_dict({**state, "dense_fp8_scale": state["dense_fp8_scale"] * 2})            # and once more, into a packed layer
+        assert torch.equal(lin.dense_fp8_scale, state["dense_fp8_scale"] * 2)
+
+
+@pytest.mark.parametrize("strict", [True, False])
+@pytest.mark.parametrize("into_packed", [False, True])
+@pytest.mark.parametrize("n,k,rows,cols", [(N + 16, K, 3, 2), (N, K + 16, 3, 2), (N, K, 4, 2), (N, K, 3, 3), (16, K, 1, 2)])
+def test_packed_state_of_another_size_is_an_error(n, k, rows, cols, into_packed, strict):
+    """As for every other parameter, in strict and other loads: the layer keeps its features."""
+    lin = _packed(seed=3)[0] if into_packed else CMSBlockLinear(K, N, bias=False)
+    before = {k: v.clone() for k, v in lin.state_dict().items()}
+    with pytest.raises(RuntimeError, match="size mismatch"):
+        lin.load_state_dict({"dense_fp8": _codes(n, k)[0], "dense_fp8_scale": torch.ones(rows, cols)}, strict=strict)
+    assert _holds(lin, before)
