@@ -394,14 +394,15 @@ class CMSBlockLinear(nn.Module):
         + mortar_ternary, or the packed variant mortar_packed + mortar_scale in place of mortar_data; and dense_fp8 +
         dense_fp8_scale in place of the weight of a layer that pack_dense_fp8 was applied to."""
         dk, pk, fk = prefix + "mortar_data", prefix + "mortar_packed", prefix + "dense_fp8"
-        if fk in state_dict and not self._mortar:
+        packed = fk in state_dict and fk + "_scale" in state_dict and not self._mortar          # (half of it: missing keys, the layer as it was)
+        if packed:
             expected = {"dense_fp8": (self.out_features, self.in_features), "dense_fp8_scale": (-(-self.out_features // 128), -(-self.in_features // 128))}
             errors = [f"size mismatch for {prefix + k}: {tuple(state_dict[prefix + k].shape)} in the checkpoint, {size} in this layer"
                       for k, size in expected.items() if state_dict[prefix + k].shape != size]
             if errors:                           # (an error of strict and other loads, as for every parameter; the layer stays as it was)
                 error_msgs.extend(errors)
                 return
-        if fk in state_dict and "dense_fp8" not in self._buffers and not self._mortar:
+        if packed and "dense_fp8" not in self._buffers:
             dev = self.weight.device
             del self._parameters["weight"]
             for k in ("dense_fp8", "dense_fp8_scale"):

@@ -65,3 +65,17 @@ def test_packed_state_of_another_size_is_an_error(n, k, rows, cols, into_packed,
     with pytest.raises(RuntimeError, match="size mismatch"):
         lin.load_state_dict({"dense_fp8": _codes(n, k)[0], "dense_fp8_scale": torch.ones(rows, cols)}, strict=strict)
     assert _holds(lin, before)
+
+
+@pytest.mark.parametrize("missing", ["dense_fp8", "dense_fp8_scale"])
+def test_half_a_packed_state_leaves_the_layer_alone(missing):
+    """Codes without scales (or the other way round) are missing keys, reported as such; the layer still has its weight."""
+    lin = CMSBlockLinear(K, N, bias=False)
+    weight = lin.weight.detach().clone()
+    _, state = _packed()
+    del state[missing]
+    with pytest.raises(RuntimeError, match="[Mm]issing key"):
+        lin.load_state_dict(state)
+    assert torch.equal(lin.weight, weight) and "dense_fp8" not in lin._buffers and "dense_fp8_scale" not in lin._buffers
+    result = lin.load_state_dict(state, strict=False)
+    assert result.missing_keys == ["weight"] and torch.equal(lin.weight, weight)
