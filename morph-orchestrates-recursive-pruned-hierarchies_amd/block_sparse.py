@@ -408,7 +408,9 @@ class CMSBlockLinear(nn.Module):
             for k in ("dense_fp8", "dense_fp8_scale"):
                 self.register_buffer(k, torch.empty_like(state_dict[prefix + k], device=dev))
         if (dk in state_dict or pk in state_dict) and not self._mortar:
-            dev = self.weight.device
+            dev = self.weight.device if "dense_fp8" not in self._buffers else self.dense_fp8.device
+            for k in ("dense_fp8", "dense_fp8_scale"):
+                self._buffers.pop(k, None)
             idx = {k: torch.empty_like(state_dict[prefix + k], device=dev) for k in (
                 "mortar_row_indices", "mortar_column_indices", "mortar_offsets", "mortar_column_indices_t",
                 "mortar_offsets_t", "mortar_block_offsets_t")}

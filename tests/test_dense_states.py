@@ -79,3 +79,13 @@ def test_half_a_packed_state_leaves_the_layer_alone(missing):
     assert torch.equal(lin.weight, weight) and "dense_fp8" not in lin._buffers and "dense_fp8_scale" not in lin._buffers
     result = lin.load_state_dict(state, strict=False)
     assert result.missing_keys == ["weight"] and torch.equal(lin.weight, weight)
+
+
+def test_a_carved_state_loads_into_a_packed_layer():
+    torch.manual_seed(0)
+    carved = CMSBlockLinear(K, N, bias=False)
+    carved.carve()
+    lin, _ = _packed()
+    lin.load_state_dict(carved.state_dict())
+    assert lin._mortar and not lin._dense_mode and "dense_fp8" not in lin._buffers and "dense_fp8_scale" not in lin._buffers and "weight" not in lin._parameters
+    assert _holds(lin, carved.state_dict())
