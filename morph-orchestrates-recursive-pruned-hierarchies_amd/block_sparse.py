@@ -84,6 +84,7 @@ class CMSBlockLinear(nn.Module):
 
     def set_block_mask(self, block_mask: Tensor, blocking: int = 16) -> None:
         """Install a block-aligned prune mask ([out/blocking, in/blocking] bool) as the [R, C] tile mask."""
+        assert "dense_fp8" not in self._buffers, "set_block_mask() needs the weight, not its 8-bit codes"
         tpb = blocking // self.tile_size
         if blocking % self.tile_size:
             raise ValueError(f"blocking ({blocking}) not divisible by tile_size ({self.tile_size})")

@@ -89,3 +89,10 @@ def test_a_carved_state_loads_into_a_packed_layer():
     lin.load_state_dict(carved.state_dict())
     assert lin._mortar and not lin._dense_mode and "dense_fp8" not in lin._buffers and "dense_fp8_scale" not in lin._buffers and "weight" not in lin._parameters
     assert _holds(lin, carved.state_dict())
+
+
+def test_a_mask_on_a_packed_layer_is_refused():
+    lin, state = _packed()
+    with pytest.raises(AssertionError, match="8-bit codes"):
+        lin.set_block_mask(torch.ones(N // 16, K // 16, dtype=torch.bool))
+    assert lin._prune_mask is None and _holds(lin, state)
