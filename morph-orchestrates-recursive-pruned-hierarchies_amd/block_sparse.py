@@ -400,6 +400,8 @@ class CMSBlockLinear(nn.Module):
             expected = {"dense_fp8": (self.out_features, self.in_features), "dense_fp8_scale": (-(-self.out_features // 128), -(-self.in_features // 128))}
             errors = [f"size mismatch for {prefix + k}: {tuple(state_dict[prefix + k].shape)} in the checkpoint, {size} in this layer"
                       for k, size in expected.items() if state_dict[prefix + k].shape != size]
+            errors += [f"{prefix + k} must be {t} in the checkpoint, it is {state_dict[prefix + k].dtype}"          # (a copy would round them)
+                       for k, t in (("dense_fp8", torch.uint8), ("dense_fp8_scale", torch.float32)) if state_dict[prefix + k].dtype != t]
             if errors:                           # (an error of strict and other loads, as for every parameter; the layer stays as it was)
                 error_msgs.extend(errors)
                 return

@@ -96,3 +96,12 @@ def test_a_mask_on_a_packed_layer_is_refused():
     with pytest.raises(AssertionError, match="8-bit codes"):
         lin.set_block_mask(torch.ones(N // 16, K // 16, dtype=torch.bool))
     assert lin._prune_mask is None and _holds(lin, state)
+
+
+def test_codes_and_scales_of_other_types_are_an_error():
+    """They are no numbers that a copy may round: scales in 16 bits, codes as floats."""
+    codes, scale = _codes()
+    for into in (CMSBlockLinear(K, N, bias=False), _packed(seed=3)[0]):
+        for state in ({"dense_fp8": codes, "dense_fp8_scale": scale.bfloat16()}, {"dense_fp8": codes.float(), "dense_fp8_scale": scale}):
+            with pytest.raises(RuntimeError, match="must be"):
+                into.load_state_dict(state)
