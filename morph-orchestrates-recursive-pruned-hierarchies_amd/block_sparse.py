@@ -59,6 +59,7 @@ class _MortarLinearFn(torch.autograd.Function):
 
 
 class CMSBlockLinear(nn.Module):
+    _fp8_scale = None         # the fp32 scales of a layer of 8-bit codes whose buffer was cast to another type
     _step_key = None          # of the values that a native step under way is encoding (step_pack); modules saved before it have none
 
     def __init__(self, in_features: int, out_features: int, tile_size: int = 16, density: float = 1.0,
@@ -386,9 +387,22 @@ class CMSBlockLinear(nn.Module):
 
     def _apply(self, fn, *a, **k):
         self._pack = None       # device may change
-        return super()._apply(fn, *a, **k)
+        was = self._buffers.get("dense_fp8_scale")
+        super()._apply(fn, *a, **k)
+        if was is not None:     # scales in 16 bits are refused by the product; cast back they are those that the layer was packed with
+            now = self._buffers["dense_fp8_scale"]
+            if now.dtype != torch.float32 and was.dtype == torch.float32:
+                self._fp8_scale = was
+            elif now.dtype == torch.float32 and self._fp8_scale is not None:
+                self._buffers["dense_fp8_scale"], self._fp8_scale = self._fp8_scale.to(now.device), None
+        return self
 
     # ------------------------------------------------------------------ checkpoints
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        if self._fp8_scale is not None:
+            destination[prefix + "dense_fp8_scale"] = self._fp8_scale.to(self.dense_fp8.device)
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
         """Accepts the reference's carved key set (block_sparse.py:983-1036): mortar_data + six index buffers
@@ -402,6 +416,8 @@ class CMSBlockLinear(nn.Module):
                       for k, size in expected.items() if state_dict[prefix + k].shape != size]
             errors += [f"{prefix + k} must be {t} in the checkpoint, it is {state_dict[prefix + k].dtype}"          # (a copy would round them)
                        for k, t in (("dense_fp8", torch.uint8), ("dense_fp8_scale", torch.float32)) if state_dict[prefix + k].dtype != t]
+            if self._fp8_scale is not None:
+                errors.append(f"{prefix}dense_fp8_scale is held in {self.dense_fp8_scale.dtype} since a cast of the module: cast it to float32 first")
             if errors:                           # (an error of strict and other loads, as for every parameter; the layer stays as it was)
                 error_msgs.extend(errors)
                 return
@@ -414,6 +430,7 @@ class CMSBlockLinear(nn.Module):
             dev = self.weight.device if "dense_fp8" not in self._buffers else self.dense_fp8.device
             for k in ("dense_fp8", "dense_fp8_scale"):
                 self._buffers.pop(k, None)
+            self._fp8_scale = None
             idx = {k: torch.empty_like(state_dict[prefix + k], device=dev) for k in (
                 "mortar_row_indices", "mortar_column_indices", "mortar_offsets", "mortar_column_indices_t",
                 "mortar_offsets_t", "mortar_block_offsets_t")}

@@ -97,8 +97,10 @@ def shrink_mlp_to_mortar_ternary(bel, target_density: float = 0.25, blocking: in
 
 def pack_dense_fp8(cms: nn.Module) -> dict:
     """The weight of a CMSBlockLinear that stays dense in deployment, IN PLACE as e4m3 codes with one fp32 scale per 128 x 128 block
-    (ops.quantize_fp8_weight; its pruned tiles zeroed first): registers ``dense_fp8`` (the codes' bytes, so that casting the module
-    leaves them alone) and ``dense_fp8_scale`` and drops the parameter.  The layer then runs ops.linear_fp8."""
+    (ops.quantize_fp8_weight; its pruned tiles zeroed first): registers ``dense_fp8`` (the codes' bytes, which a cast of the module
+    leaves alone) and ``dense_fp8_scale`` and drops the parameter.  The layer then runs ops.linear_fp8.  Cast a module before its
+    layers are packed: with the scales in another type than fp32 a call raises TypeError, until the module is cast back (nothing
+    is lost by that; a checkpoint holds the fp32 scales throughout).  Activations may have any floating type."""
     from . import ops
     assert not getattr(cms, "_mortar", False) and "weight" in cms._parameters, "pack_dense_fp8 requires a layer that is not carved"
     if cms.in_features % 16 or cms.out_features % 8:

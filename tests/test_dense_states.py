@@ -105,3 +105,20 @@ def test_codes_and_scales_of_other_types_are_an_error():
         for state in ({"dense_fp8": codes, "dense_fp8_scale": scale.bfloat16()}, {"dense_fp8": codes.float(), "dense_fp8_scale": scale}):
             with pytest.raises(RuntimeError, match="must be"):
                 into.load_state_dict(state)
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16])
+def test_scales_are_whole_again_behind_a_cast(t):
+    """A module that was cast to 16 bits and back holds the scales that it was packed with, not rounded ones."""
+    lin, state = _packed(bias=True)
+    assert not torch.equal(state["dense_fp8_scale"].to(t).float(), state["dense_fp8_scale"])
+    cast = lin.to(t)
+    assert cast.dense_fp8.dtype == torch.uint8 and torch.equal(cast.dense_fp8, state["dense_fp8"])
+    for back in (copy.deepcopy(cast).float(), copy.deepcopy(cast).to(torch.float16).bfloat16().float(), copy.deepcopy(cast).double().float(), cast.float()):
+        assert back.dense_fp8_scale.dtype == torch.float32 and torch.equal(back.dense_fp8_scale, state["dense_fp8_scale"])
+    cast, new = lin.to(t), _codes(seed=9)
+    assert _holds(cast, {**state, "bias": state["bias"].to(t)})                       # a checkpoint of it is whole, too
+    with pytest.raises(RuntimeError, match="float32"):
+        cast.load_state_dict({"dense_fp8": new[0], "dense_fp8_scale": new[1], "bias": state["bias"]})
+    lin, state = _packed(seed=2)
+    assert torch.equal(lin.double().dense_fp8_scale.float(), state["dense_fp8_scale"])
