@@ -393,7 +393,8 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *a, Py_ssize_t na) {
     if (codes) {
         same_device(x, xs, what, "x_scale");
         TORCH_CHECK_TYPE(xs.scalar_type() == at::kFloat, what, ": x_scale must be float32");
-        TORCH_CHECK_VALUE(xs.dim() == x.dim() && xs.numel() == M * kb && xs.size(-1) == kb, what, ": x_scale must be [..., ", kb, "], got ", xs.sizes());
+        TORCH_CHECK_VALUE(xs.dim() == x.dim() && xs.size(-1) == kb && xs.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1), what,
+                          ": x_scale must be [..., ", kb, "] with the rows of x, got ", xs.sizes(), " for ", x.sizes());
     }
     at::DimVector shape(x.sizes());
     shape.back() = N;

@@ -167,3 +167,12 @@ def test_gate_and_up_rows_far_apart(dev, M):
     """A gate row and its up row 2 GiB apart, in rows that are not."""
     x, wgu, wd = normals((M, 64), 1, BF16, dev), normals((2048, 64), 2, BF16, dev, 0.1), normals((16, 1024), 3, BF16, dev, 0.03)
     assert torch.equal(ops.dense_mlp(x, _apart(wgu, 1 << 20), wd), ops.dense_mlp(x, wgu, wd))
+
+
+def test_scales_of_other_rows_are_refused(dev):
+    wq, ws = ops.quantize_fp8_weight(normals((72, 160), 1, torch.float32, dev, 0.1))
+    q, s = ops.quantize_fp8(normals((2, 3, 160), 2, BF16, dev))
+    assert ops.linear_fp8(q, wq, ws, s).shape == (2, 3, 72)
+    for other in (s.transpose(0, 1), s.reshape(3, 2, 2), s.reshape(6, 1, 2)):
+        with pytest.raises(ValueError, match="x_scale must be"):
+            ops.linear_fp8(q, wq, ws, other)
