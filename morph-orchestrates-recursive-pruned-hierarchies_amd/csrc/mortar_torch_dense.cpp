@@ -401,7 +401,7 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *a, Py_ssize_t na) {
     at::Tensor y = at::empty(shape, x.options().dtype(at::kBFloat16).requires_grad(false));
     if (M) {
         void *st = stream_of(x);
-        const at::Tensor wsc = ws.stride(1) == 1 ? ws : ws.contiguous();
+        const at::Tensor wsc = ws.stride(1) == 1 && ws.stride(0) >= kb ? ws : ws.clone(at::MemoryFormat::Contiguous);
         at::Tensor xr, buf;
         const void *xp;
         const float *sx = nullptr;

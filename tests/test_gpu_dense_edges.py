@@ -176,3 +176,11 @@ def test_scales_of_other_rows_are_refused(dev):
     for other in (s.transpose(0, 1), s.reshape(3, 2, 2), s.reshape(6, 1, 2)):
         with pytest.raises(ValueError, match="x_scale must be"):
             ops.linear_fp8(q, wq, ws, other)
+
+
+def test_scales_of_a_weight_that_are_repeated(dev):
+    wq, ws = ops.quantize_fp8_weight(normals((264, 272), 1, torch.float32, dev, 0.1))
+    x = normals((4, 272), 2, BF16, dev)
+    for rows in (x, x.repeat(20, 1)):
+        for view in (ws[:1].expand(3, 3), ws[:, :1].expand(3, 3), ws[0, 0].expand(3, 3)):
+            assert torch.equal(ops.linear_fp8(rows, wq, view), ops.linear_fp8(rows, wq, view.clone()))
