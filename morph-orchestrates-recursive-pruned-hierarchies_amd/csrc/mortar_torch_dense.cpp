@@ -38,9 +38,8 @@ c10::DispatchKeySet riders() {
                                 K::FuncTorchDynamicLayerBackMode, K::Batched, K::Functionalize, K::Conjugate, K::Negative, K::ZeroTensor, K::Tracer});
 }
 
-bool plain(const at::Tensor &t) {
-    return !c10::impl::tls_local_dispatch_key_set().included_.has_any(riders()) && !t.key_set().has_any(riders()) && t.layout() == at::kStrided;
-}
+bool plain_values(const at::Tensor &t) { return !t.key_set().has_any(riders()) && t.layout() == at::kStrided; }
+bool plain(const at::Tensor &t) { return !c10::impl::tls_local_dispatch_key_set().included_.has_any(riders()) && plain_values(t); }
 
 // Argument `name` as a plain tensor on the GPU.
 const at::Tensor &tensor_arg(PyObject *o, const char *what, const char *name) {
@@ -77,8 +76,13 @@ float *floats(const at::Tensor &t) { return t.defined() ? static_cast<float *>(t
 const void *data(const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void *mut(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-void check_once(const char *what) {
+// The gradient of a result as the backward reads it: values as they lie in memory, once.
+at::Tensor plain_gradient(const at::Tensor &dy, const char *what) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), what, ": its gradients cannot be differentiated again (create_graph=True)");
+    if (!dy.defined()) return dy;
+    const at::Tensor g = dy.resolve_neg();                 // (the imaginary part of a conjugate is negated lazily)
+    TORCH_CHECK(plain_values(g), what, ": its gradient must be a plain strided tensor");
+    return g;
 }
 
 // ---- LayerNorm -------------------------------------------------------------------------------------------------------
@@ -111,13 +115,12 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        check_once("layernorm");
         variable_list out(4);
-        if (!grads[0].defined()) return out;
+        const at::Tensor dy = plain_gradient(grads[0], "layernorm");
+        if (!dy.defined()) return out;
         const auto v = ctx->get_saved_variables();
         const at::Tensor &rows = v[0], &w = v[1], &stats = v[2];
         const auto shape = ctx->saved_data["shape"].toIntVector();
-        const at::Tensor &dy = grads[0];
         const int64_t d = shape.back();
         // (edges are counted over the tensors that are there)
         const bool has_b = !ctx->saved_data["bias"].isNone();
@@ -226,15 +229,14 @@ struct DenseMlpFn : public torch::autograd::Function<DenseMlpFn> {
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        check_once("dense_mlp");
         variable_list out(3);
-        if (!grads[0].defined()) return out;
+        const at::Tensor dy = plain_gradient(grads[0], "dense_mlp");
+        if (!dy.defined()) return out;
         const auto v = ctx->get_saved_variables();
         const at::Tensor &x = v[0], &wgu = v[1], &wd = v[2], &gu = v[3];
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const int64_t d = shape.back(), f = wd.size(1), n = wd.size(0);
         const bool need_x = ctx->needs_input_grad(0), need_gu = ctx->needs_input_grad(1), need_dn = ctx->needs_input_grad(2);
-        const at::Tensor &dy = grads[0];
         const c10::DeviceGuard guard(dy.device());
         at::Tensor dx, dgw, ddw;
         if (need_x) dx = at::empty(shape, dy.options().requires_grad(false));

@@ -184,3 +184,36 @@ def test_scales_of_a_weight_that_are_repeated(dev):
     for rows in (x, x.repeat(20, 1)):
         for view in (ws[:1].expand(3, 3), ws[:, :1].expand(3, 3), ws[0, 0].expand(3, 3)):
             assert torch.equal(ops.linear_fp8(rows, wq, view), ops.linear_fp8(rows, wq, view.clone()))
+
+
+# ---- gradients and scales in unusual forms
+
+
+def test_gradients_that_are_negated_lazily(dev):
+    """A gradient with the negative bit, as the imaginary part of a conjugate has it."""
+    x, w, b = normals((6, 64), 1, BF16, dev).requires_grad_(True), normals((64,), 2, BF16, dev).requires_grad_(True), normals((64,), 3, BF16, dev).requires_grad_(True)
+    wgu, wd, dy = normals((48, 64), 4, BF16, dev, 0.1).requires_grad_(True), normals((64, 24), 5, BF16, dev, 0.2).requires_grad_(True), normals((6, 64), 6, BF16, dev)
+    for leaves, f in (((x, w, b), ops.layernorm), ((x, wgu, wd), ops.dense_mlp)):
+        want = torch.autograd.grad(f(*leaves), leaves, -dy)
+        got = torch.autograd.grad(f(*leaves), leaves, torch._neg_view(dy))
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_batched_gradients_are_refused(dev):
+    x, w = normals((6, 64), 1, BF16, dev).requires_grad_(True), normals((64,), 2, BF16, dev)
+    wgu, wd, dy = normals((48, 64), 4, BF16, dev, 0.1), normals((64, 24), 5, BF16, dev, 0.2), normals((2, 6, 64), 6, BF16, dev)
+    for y in (ops.layernorm(x, w), ops.dense_mlp(x, wgu, wd)):
+        with pytest.raises(RuntimeError, match="plain strided tensor"):
+            torch.autograd.grad(y, [x], dy, is_grads_batched=True)
+
+
+def test_a_mode_that_watches_the_backward(dev):
+    """Forward calls inside a dispatch mode are left to torch; a backward inside one has plain gradients and runs."""
+    x = normals((6, 64), 1, BF16, dev).requires_grad_(True)
+    wgu, wd, dy = normals((48, 64), 4, BF16, dev, 0.1), normals((64, 24), 5, BF16, dev, 0.2), normals((6, 64), 6, BF16, dev)
+    for f in (lambda: ops.layernorm(x), lambda: ops.dense_mlp(x, wgu, wd)):
+        (want,) = torch.autograd.grad(f(), [x], dy)
+        y = f()
+        with _Watch():
+            (got,) = torch.autograd.grad(y, [x], dy)
+        assert torch.equal(got, want)
