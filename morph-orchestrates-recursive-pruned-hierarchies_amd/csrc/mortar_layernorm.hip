@@ -233,10 +233,11 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LnArgs a) {
         if (m + step < a.M) fetch(m + step);
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
+        for (int i = 0; i < PER; ++i) {
+            const float mean = (i * TPR + t) * VEC < d ? mu : 0.f;        // beyond the row z = 0, also where mu r is not finite
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                z[i][j] = (z[i][j] - mu) * r;             // beyond the row: multiplied by g = 0 everywhere
+                z[i][j] = (z[i][j] - mean) * r;
                 if constexpr (PARAMS) {
                     dw[i][j] = __builtin_fmaf(g[i][j], z[i][j], dw[i][j]);
                     db[i][j] += g[i][j];
@@ -245,6 +246,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const LnArgs a) {
                 s1 += g[i][j];
                 s2 = __builtin_fmaf(g[i][j], z[i][j], s2);
             }
+        }
         if (!a.y) continue;
         s1 = row_sum<TPR>(s1, sm[0], turn) * inv_d;
         s2 = row_sum<TPR>(s2, sm[1], turn2) * inv_d;

@@ -217,3 +217,33 @@ def test_a_mode_that_watches_the_backward(dev):
         with _Watch():
             (got,) = torch.autograd.grad(y, [x], dy)
         assert torch.equal(got, want)
+
+
+# ---- values at the ends of the range
+
+
+@pytest.mark.parametrize("t", [torch.float32, BF16], ids=str)
+@pytest.mark.parametrize("d", [16, 40, 1000, 1544, 5000])
+@pytest.mark.parametrize("params", [True, False])
+def test_rows_around_a_large_mean_have_a_gradient(dev, params, d, t):
+    """x = mean = 2^120 and 1 / deviation = 2^9: what lies beyond the row in registers, (0 - mean) / deviation there, is not finite.
+    z = 0, so dx = r (g - mean(g)), dw = 0 and db = sum of dy; d fills neither a vector's, a wave's nor a workgroup's last lanes."""
+    M, r = 5, 2.0 ** 9
+    w, dy = normals((d,), 1, torch.float32, dev).to(t), normals((M, d), 2, torch.float32, dev).to(t)
+    mean, rstd = torch.full((M,), 2.0 ** 120, device=dev), torch.full((M,), r, device=dev)
+    L = _lib.lib()
+    ws = torch.full((L.mortar_layernorm_workspace_bytes(M, d) // 4,), float("nan"), device=dev)
+    for off in (0, 1):
+        x = torch.full((M, d + off), 2.0 ** 120, dtype=t, device=dev)[:, off:]
+        dx, dw, db = torch.full((M, d), float("nan"), dtype=t, device=dev), torch.full((d,), float("nan"), dtype=t, device=dev), torch.full((d,), float("nan"), dtype=t, device=dev)
+        ptr = lambda v: v.data_ptr() if params else None
+        _lib.check(L.mortar_layernorm_bwd(dy.data_ptr(), d, x.data_ptr(), x.stride(0), M, d, {torch.float32: 2, BF16: 0}[t], w.data_ptr(), 0, mean.data_ptr(), rstd.data_ptr(),
+                                          dx.data_ptr(), d, ptr(dw), ptr(db), ptr(ws), torch.cuda.current_stream().cuda_stream), "layernorm_bwd")
+        g = dy.double() * w.double()
+        ref = r * (g - g.mean(1, keepdim=True))
+        chain = 2.0 ** -24 * (72 + d // 256 + 10)                   # as dense_util.norm_bounds: the products, their sum, the difference
+        assert_within(dx, ref, 2 * r * (2.0 ** -23 * g.abs() + chain * g.abs().mean(1, keepdim=True)) + rounding(t, ref), "dx")
+        if params:
+            assert not dw.any()
+            ref = dy.double().sum(0)
+            assert_within(db, ref, 2.0 ** -24 * M * dy.double().abs().sum(0) + rounding(t, ref), "db")
