@@ -630,7 +630,7 @@ int mortar_layernorm_bwd(const void *dy, int64_t lddy, const void *x, int64_t ld
 /* ---- dense layers in 8 bits --------------------------------------------------------------------------- */
 
 /* e4m3 (OCP FP8) operands with fp32 scales, x one per row and 128 values of K, W one per 128 x 128 block: s = amax * (1 / 448) in fp32 (1 where
- * amax = 0), q = x / s (fp32 quotient) rounded to nearest even.  K a multiple of 16, N of 8, rows of codes on 16-byte addresses, leading
+ * that is below 2^-145, zeros above all), q = x / s (fp32 quotient) rounded to nearest even.  K a multiple of 16, N of 8, rows of codes on 16-byte addresses, leading
  * dimensions in values.  A block with an infinity or NaN gets a scale of the kind and makes the results it enters NaN.
  *   mortar_fp8_quantize          x bf16 [M, K] -> q [M, K], s(m, kb) at s[m * s_m + kb * s_k]
  *   mortar_fp8_quantize_weight   w [N, K] in bf16, fp16 or fp32 (`type`) -> q [N, K], s(nb, kb) at s[nb * s_n + kb]

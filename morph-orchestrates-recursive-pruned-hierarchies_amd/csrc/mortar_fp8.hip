@@ -1,6 +1,6 @@
 // Dense layers served in 8 bits: y = x W^T with both operands in e4m3 (OCP FP8, 448 the largest value), x with one fp32 scale per row and
 // 128 values of K, W with one per 128 x 128 block:
-//   s = amax * (1 / 448), fp32 factors and product (1 for zeros),  q = rne(x / s) with the IEEE fp32 quotient,
+//   s = amax * (1 / 448), fp32 factors and product (1 where that is below 2^-145),  q = rne(x / s) with the IEEE fp32 quotient,
 //   y[m, n] = sum over K blocks of sx[m, kb] sw[n / 128, kb] (sum of q_x q_w in the block).
 // The product of a K block is one matrix instruction deep (16x16x128), so that the sums of a block come out of it unscaled and are
 // added to the fp32 result with the product of the two scales: one multiply-add per value and 128 of K.  Inside the instruction the
@@ -18,8 +18,11 @@ namespace {
 
 constexpr float PER_MAX = 1.0f / 448.0f;
 
-__device__ __forceinline__ float scale_of(uint32_t amax_bits) {         // bits of max |x|; NaN and infinity pass through
-    return amax_bits ? __builtin_bit_cast(float, amax_bits) * PER_MAX : 1.0f;
+// From the bits of max |x|; NaN and infinity pass through.  Below 2^-145 a scale has four bits or fewer or is 0, and amax / s could pass 464, beyond
+// which e4m3 has only NaN: such a block (fp32 weights around 2^-137; bf16 and fp16 hold none) has the scale 1, like one of zeros, and codes of 0.
+__device__ __forceinline__ float scale_of(uint32_t amax_bits) {
+    const float s = __builtin_bit_cast(float, amax_bits) * PER_MAX;
+    return s < 0x1p-145f ? 1.0f : s;
 }
 __device__ __forceinline__ uint32_t abs_max8(const float (&v)[8]) {     // as integers: NaN is the largest
     uint32_t m = 0;

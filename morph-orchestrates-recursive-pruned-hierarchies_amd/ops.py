@@ -580,7 +580,8 @@ def quantize_fp8(x: Tensor) -> tuple[Tensor, Tensor]:
 
 
 def quantize_fp8_weight(w: Tensor) -> tuple[Tensor, Tensor]:
-    """(codes float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)]) of a weight: as quantize_fp8 with one scale per 128 x 128 block."""
+    """(codes float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)]) of a weight: as quantize_fp8 with one scale per 128 x 128 block.
+    A block of fp32 weights that are too small for a scale (amax / 448 below 2^-145) is one of zeros."""
     return _lib.native().quantize_fp8_weight(w)
 
 

@@ -247,3 +247,26 @@ def test_rows_around_a_large_mean_have_a_gradient(dev, params, d, t):
             assert not dw.any()
             ref = dy.double().sum(0)
             assert_within(db, ref, 2.0 ** -24 * M * dy.double().abs().sum(0) + rounding(t, ref), "db")
+
+
+@pytest.mark.parametrize("exponent", [-149, -147, -145, -142, -141, -140, -139, -138, -137, -136, -135, -130, -120])
+def test_weights_of_hardly_any_size(dev, exponent):
+    """Blocks whose scale fp32 can hold only in a few bits or not at all: finite codes, the block's values or zeros, and finite results."""
+    w = torch.zeros((136, 272))
+    w[:128, :128] = normals((128, 128), 1, torch.float32, "cpu", 0.1)
+    w[:128, 128:256] = (torch.linspace(1.0, 1.99, 128).double() * 2.0 ** exponent).float()
+    w[128:, :128] = 2.0 ** exponent
+    q, s = ops.quantize_fp8_weight(w.to(dev))
+    codes, sizes = q.cpu().float().double(), s.cpu().double()
+    v = codes * sizes.repeat_interleave(128, 0)[:136].repeat_interleave(128, 1)[:, :272]
+    assert not v.isnan().any() and bool((sizes > 0).all())
+    for block in ((slice(0, 128), slice(128, 256)), (slice(128, 136), slice(0, 128))):
+        a, r, sc = w[block].double(), v[block], float(sizes[block[0].start // 128, block[1].start // 128])
+        if exponent <= -138:                             # amax / 448 below 2^-145: nothing that 8 bits could hold beside a scale
+            assert sc == 1.0 and not r.any()
+        elif exponent >= -135:                           # a step of e4m3 at most from it: half of 2^-3, and the scale's own rounding, 1/32 at most, at the top
+            assert sc < 1e-30 and bool(((r - a).abs() <= a.abs() * 2.0 ** -3).all())
+    x = normals((5, 272), 2, BF16, dev)
+    for rows in (x, x.repeat(20, 1)):
+        y = ops.linear_fp8(rows, q, s)
+        assert bool(y.isfinite().all())
