@@ -601,6 +601,11 @@ int mortar_sdd_bf16(const int32_t *plan, int32_t n_wg, int32_t blocks_per_wave, 
 enum { MORTAR_BF16 = 0, MORTAR_FP16 = 1, MORTAR_FP32 = 2 };
 #define MORTAR_DENSE_FEW_ROWS 8        /* rows up to which forward products stream the weights past the rows */
 int64_t mortar_dense_workspace_bytes(int64_t M, int64_t N, int64_t K);
+/* Form that a product C [M, N] over K takes (host only, nothing is launched): *tile_n x *tile_m of C per workgroup, 0 x 0 for the kernels of
+ * few rows; *ranges that the sums are cut into.  A product of `few rows` or of one range takes no workspace.
+ * kind 0: dense_linear, 1: dense_linear_dx and (M: n_out, K: rows) dense_linear_dw, 2: dense_gateup_swiglu (N: f) without gu, 3: with it,
+ * 4: dense_swiglu_bwd (N: f), 5: fp8_linear of given codes. */
+int mortar_dense_form_host(int32_t kind, int64_t M, int64_t N, int64_t K, int32_t *tile_n, int32_t *tile_m, int32_t *ranges);
 int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, int64_t ldx, const void *w, int64_t ldw, int32_t f, int32_t type,
                                void *h, int64_t ldh, void *gu, void *stream);
 int mortar_dense_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const void *w, int64_t ldw, int32_t N, int32_t type, void *y,

@@ -103,6 +103,7 @@ _SIGS = {
     "mortar_gemv_bf16_noalloc": (C.c_int, [c_vp, c_vp, c_i64, c_i32, c_vp, c_i32, c_i32, c_vp, c_i32, c_i64, c_vp, c_i64,
                                            c_vp, c_i32, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp]),
     "mortar_dense_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
+    "mortar_dense_form_host": (C.c_int, [c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "mortar_dense_gateup_swiglu": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_vp]),
     "mortar_dense_linear": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_vp]),
     "mortar_dense_swiglu_bwd": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_i64, c_vp, c_i64, c_vp]),

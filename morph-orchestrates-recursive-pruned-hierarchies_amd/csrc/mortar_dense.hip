@@ -255,6 +255,17 @@ extern "C" int64_t mortar_dense_workspace_bytes(int64_t M, int64_t N, int64_t K)
     return p.splits > 1 ? p.splits * M * N * 4 : 0;
 }
 
+extern "C" int mortar_dense_form_host(int32_t kind, int64_t M, int64_t N, int64_t K, int32_t *tile_n, int32_t *tile_m, int32_t *ranges) {
+    if (kind < 0 || kind > 5 || M <= 0 || N <= 0 || K <= 0 || !tile_n || !tile_m || !ranges) return mortar_fail(MORTAR_ERR_ARG, "dense_form: bad argument");
+    constexpr int forms[] = {MORTAR_PLAN_PLAIN, MORTAR_PLAN_PLAIN, MORTAR_PLAN_SWIGLU, MORTAR_PLAN_SWIGLU_KEEP, MORTAR_PLAN_SWIGLU_BWD, MORTAR_PLAN_E4M3};
+    const bool few = kind == 5 ? mortar_fp8_few_rows(M, N, K) : kind != 1 && kind != 4 && few_rows(M, N, K);
+    const Plan p = few ? Plan{0, 1} : plan_tiles(M, N, kind == 5 ? (K + 127) / 128 : (K + 63) / 64, forms[kind]);
+    *tile_n = few ? 0 : DENSE_TILES[p.tile].bn;
+    *tile_m = few ? 0 : DENSE_TILES[p.tile].bm;
+    *ranges = p.splits;
+    return MORTAR_OK;
+}
+
 extern "C" int mortar_dense_gateup_swiglu(const void *x, int64_t M, int32_t d, int64_t ldx, const void *w, int64_t ldw, int32_t f, int32_t type,
                                           void *h, int64_t ldh, void *gu, void *stream) {
     const char *what = "dense_gateup_swiglu";

@@ -249,6 +249,8 @@ int check_values(const char *what, const char *name, const void *p, int64_t cols
 
 }  // namespace
 
+bool mortar_fp8_few_rows(int64_t M, int64_t N, int64_t K) { return few_rows(M, N, K); }
+
 extern "C" int mortar_fp8_quantize(const uint16_t *x, int64_t M, int32_t K, int64_t ldx, uint8_t *q, int64_t ldq, float *s, int64_t s_m, int64_t s_k,
                                    void *stream) {
     const char *what = "fp8_quantize";

@@ -31,6 +31,8 @@ struct MortarDensePlan {
 };
 enum { MORTAR_PLAN_PLAIN, MORTAR_PLAN_SWIGLU, MORTAR_PLAN_SWIGLU_KEEP, MORTAR_PLAN_SWIGLU_BWD, MORTAR_PLAN_E4M3 };
 __attribute__((visibility("hidden"))) MortarDensePlan mortar_dense_plan(int64_t M, int64_t N, int64_t steps, int form);
+// Whether an e4m3 product is the few-rows kernel's.
+__attribute__((visibility("hidden"))) bool mortar_fp8_few_rows(int64_t M, int64_t N, int64_t K);
 // c = the sum of the fp32 slabs [M, N] of the K ranges, in their order, rounded to `type` (bf16, fp16).
 __attribute__((visibility("hidden"))) int mortar_dense_join(const float *slabs, int splits, int64_t M, int64_t N, int32_t type, void *c, int64_t ldc, void *stream);
 

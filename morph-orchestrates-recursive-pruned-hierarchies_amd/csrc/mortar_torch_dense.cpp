@@ -215,7 +215,9 @@ at::Tensor mlp_forward(const at::Tensor &x, const at::Tensor &wgu, const at::Ten
     if (keep) r.gu = empty_bytes(x, 6 * M * f);
     check_rc(mortar_dense_gateup_swiglu(data(r.x), M, (int32_t)d, ld_of(r.x), data(r.wgu), ld_of(r.wgu), (int32_t)f, type, mut(h), f, mut(r.gu), st),
              "mortar_dense_gateup_swiglu");
-    const at::Tensor ws = workspace(x, M, n, f);          // (up to 8 rows it is not needed, unless they are very long)
+    int32_t tile_n, tile_m, ranges;
+    check_rc(mortar_dense_form_host(0, M, n, f, &tile_n, &tile_m, &ranges), "mortar_dense_form_host");
+    const at::Tensor ws = ranges > 1 ? empty_bytes(x, ranges * M * n * 4) : at::Tensor();          // (few rows take none)
     check_rc(mortar_dense_linear(data(h), M, (int32_t)f, f, data(r.wd), ld_of(r.wd), (int32_t)n, type, mut(y), n, floats(ws), st), "mortar_dense_linear");
     return y;
 }

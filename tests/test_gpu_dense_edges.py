@@ -270,3 +270,15 @@ def test_weights_of_hardly_any_size(dev, exponent):
     for rows in (x, x.repeat(20, 1)):
         y = ops.linear_fp8(rows, q, s)
         assert bool(y.isfinite().all())
+
+
+def test_few_rows_take_no_scratch(dev):
+    """Up to 8 rows a forward call allocates its result and the hidden activations, and nothing else."""
+    wgu, wd = normals((11264, 256), 1, BF16, dev, 0.06), normals((264, 5632), 2, BF16, dev, 0.02)
+    for M in (1, 8):
+        x = normals((M, 256), 3, BF16, dev)
+        ops.dense_mlp(x, wgu, wd)
+        count = lambda: torch.cuda.memory_stats()["allocation.all.allocated"]
+        before = count()
+        y = ops.dense_mlp(x, wgu, wd)
+        assert count() - before == 2 and y.shape == (M, 264)
