@@ -39,9 +39,8 @@ struct TileTimes {
     double step, step_alone, end;      // us; a step of one of several workgroups on a CU, of a workgroup alone there
 };
 constexpr TileTimes TIMES_16[DENSE_N_TILES] = {{1.31, 1.31, 0.1}, {1.10, 1.10, 0.1}, {0.84, 0.84, 0.65}, {1.06, 0.68, 0.44}, {0.46, 0.26, 1.0}};
-// e4m3: from 4096 x 2048 x 11264, 4096 x 8192 x 4096 and 8192^3.  256 x 256 does not fit the registers beside the unscaled sums: 320 us for
-// the first, where 256 x 192, 256 x 128 and 128 x 128 take 138, 137 and 121.
-constexpr TileTimes TIMES_8[DENSE_N_TILES] = {{25, 25, 50}, {1.48, 1.48, 10.8}, {1.19, 1.19, 3.8}, {1.28, 0.75, 0.3}, {0.6, 0.33, 1.2}};
+// e4m3 (from DENSE_E4M3_FIRST on): from 4096 x 2048 x 11264, 4096 x 8192 x 4096 and 8192^3.
+constexpr TileTimes TIMES_8[DENSE_N_TILES] = {{}, {1.48, 1.48, 10.8}, {1.19, 1.19, 3.8}, {1.28, 0.75, 0.3}, {0.6, 0.33, 1.2}};
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int form) {
     constexpr double byte = 3.7e-5, launch = 4.8, join = 2.0, slab_byte = 2.4e-7;
@@ -51,7 +50,7 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int form) {
     const int out = form == MORTAR_PLAN_SWIGLU_BWD ? 12 : form == MORTAR_PLAN_SWIGLU_KEEP ? 8 : 2;
     Plan best{0, 1};
     double best_t = 1e300;
-    for (int c = 0; c < DENSE_N_TILES; ++c) {
+    for (int c = form == MORTAR_PLAN_E4M3 ? DENSE_E4M3_FIRST : 0; c < DENSE_N_TILES; ++c) {
         const int64_t bn = swiglu ? DENSE_TILES[c].bn / 2 : DENSE_TILES[c].bn, bm = DENSE_TILES[c].bm;
         const int64_t tiles = ((N + bn - 1) / bn) * ((M + bm - 1) / bm);
         for (const int s : ranges) {

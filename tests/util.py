@@ -40,3 +40,11 @@ def prefill_form(kind, M, n_units, Cb, tiled=False):
     L, upw, span = _lib.lib(), C.c_int32(), C.c_int32()
     _lib.check(L.mortar_prefill_form_host(kind, M, n_units, Cb, L.mortar_prefill_max_seg_cb(), int(tiled), C.byref(upw), C.byref(span)), "prefill_form")
     return upw.value, span.value
+
+
+def dense_form(kind, M, N, K):
+    """((columns, rows) of the tiles, (0, 0): the kernels of few rows; number of K ranges) of a dense product: kind 0 y, 1 dx or dW, 2 gate_up, 3 gate_up with its
+    values kept, 4 the SwiGLU gradient, 5 e4m3."""
+    out = [C.c_int32() for _ in range(3)]
+    _lib.check(_lib.lib().mortar_dense_form_host(kind, M, N, K, *map(C.byref, out)), "dense_form")
+    return (out[0].value, out[1].value), out[2].value
