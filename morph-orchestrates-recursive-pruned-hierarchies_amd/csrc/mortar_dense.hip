@@ -32,15 +32,19 @@ using Plan = MortarDensePlan;
 // with, for K ranges, a second launch and the slabs' way out and back.  The times are those of the kernels as they are, fitted to 1100
 // measurements of 70 16-bit products (100 to 16384 rows, widths 88 to 11264, all five tiles, up to 16 ranges; the operands in the caches
 // and in none of them, geometric mean of the two; error 9 %).  Over these the choice is 0.7 % slower than the best one on average (the best
-// number of ranges of the fourth tile alone: 15 %, of the first: 57 %).  The backward of SwiGLU reads as much as it writes: above 100 MB a
-// byte is 1.6 times as dear, and 2.1 times in the first tile, where the values on their way do not fit the registers (16384 rows, 768 and
-// 2048 wide: 161, 153, 140 and 146 us in the first four tiles; 4096 rows, 2048 and 5632: 192, 152, 149 and 158).
+// number of ranges of the fourth tile alone: 15 %, of the first: 57 %).  The backward of SwiGLU reads as much as it writes: above 6 M values a
+// byte is dearer by TIMES_BWD, most in the large tiles, where the values on their way do not fit the registers.  Of 494 such products (1 to
+// 20000 rows, widths 64 to 11264) the choice is then 0.3 % slower than the best tile on average, of the 139 above the line 0.4 % and 11 % at
+// worst; with one price it is 2.6 %, 8.8 % and 31 %.  (16384 rows, 768 and 2048 wide: 161, 153, 140 and 146 us in the first four tiles; 4096 rows,
+// 2048 and 5632: 192, 152, 149 and 158.)
 struct TileTimes {
     double step, step_alone, end;      // us; a step of one of several workgroups on a CU, of a workgroup alone there
 };
 constexpr TileTimes TIMES_16[DENSE_N_TILES] = {{1.31, 1.31, 0.1}, {1.10, 1.10, 0.1}, {0.84, 0.84, 0.65}, {1.06, 0.68, 0.44}, {0.46, 0.26, 1.0}};
 // e4m3 (from DENSE_E4M3_FIRST on): from 4096 x 2048 x 11264, 4096 x 8192 x 4096 and 8192^3.
 constexpr TileTimes TIMES_8[DENSE_N_TILES] = {{}, {1.48, 1.48, 10.8}, {1.19, 1.19, 3.8}, {1.28, 0.75, 0.3}, {0.6, 0.33, 1.2}};
+
+constexpr double TIMES_BWD[DENSE_N_TILES] = {2.1, 1.8, 1.2, 1.2, 1.2};
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int form) {
     constexpr double byte = 3.7e-5, launch = 4.8, join = 2.0, slab_byte = 2.4e-7;
@@ -56,7 +60,7 @@ Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int form) {
         for (const int s : ranges) {
             if (s > 1 && (!plain || steps / s < 4)) break;
             const int64_t wgs = (tiles * s + 255) / 256, both = wgs < DENSE_TILES[c].per_cu ? wgs : DENSE_TILES[c].per_cu;
-            const double each = byte * (form != MORTAR_PLAN_SWIGLU_BWD || M * N <= 8 << 20 ? 1 : c == 0 ? 2.1 : 1.6);
+            const double each = byte * (form == MORTAR_PLAN_SWIGLU_BWD && M * N > 6 << 20 ? TIMES_BWD[c] : 1);
             const double step = both == DENSE_TILES[c].per_cu ? times[c].step : times[c].step_alone;
             double t = launch + (double)wgs / both * ((double)((steps + s - 1) / s) * step + times[c].end + both * each * bn * bm * (s > 1 ? 4 : out));
             if (s > 1) t += join + slab_byte * s * M * N * 4;
