@@ -8,9 +8,9 @@
 // (h, dgu) and the results; h and the derivatives are formed from the unrounded sums of their own kernel, and from g and u as
 // kept, in 24 bits.
 //
-// Measured at 4096 rows, 2048 and 5632 wide, bf16: g, u, h 146 us (1.3 PFLOP/s), with g and u kept 183 (the 138 MB are written between
-// products, at 5 TB/s), y 84 (1.12), the derivative 151 alone and 174 behind the forward (138 MB read, 138 written), dWd 96, dWgu 184, dx
-// 160 + 16 for the join of its K ranges (1.0 to 1.1).  The library's product of 4096 x 2048 x 11264 takes 163 (1.16).
+// Measured at 4096 rows, 2048 and 5632 wide, bf16: g, u, h 146 to 150 us (1.3 PFLOP/s), with g and u kept 184 (the 138 MB are written between
+// products, at 5 TB/s), y 83 to 91 (1.1), the derivative 151 alone and 167 behind the forward (138 MB read, 138 written), dWd 97, dWgu 185, dx
+// 162 + 16 for the join of its K ranges (1.0 to 1.1).  The library's product of 4096 x 2048 x 11264 takes 163 (1.16).
 #include <hip/hip_runtime.h>
 
 #include "mortar_dense_core.h"
@@ -29,21 +29,20 @@ using Plan = MortarDensePlan;
 
 // Which tile, and in how many K ranges: the smallest estimate of
 //   launch + rounds of workgroups * (steps * time of a step + end of a tile + its output bytes at a CU's share of the memory)
-// with, for K ranges, a second launch and the slabs' way out and back.  The times are those of the kernels as they are, fitted to 1100
-// measurements of 70 16-bit products (100 to 16384 rows, widths 88 to 11264, all five tiles, up to 16 ranges; the operands in the caches
-// and in none of them, geometric mean of the two; error 9 %).  Over these the choice is 0.7 % slower than the best one on average (the best
-// number of ranges of the fourth tile alone: 15 %, of the first: 57 %).  The backward of SwiGLU reads as much as it writes: above 6 M values a
-// byte is dearer by TIMES_BWD, most in the large tiles, where the values on their way do not fit the registers.  Of 494 such products (1 to
-// 20000 rows, widths 64 to 11264) the choice is then 0.3 % slower than the best tile on average, of the 139 above the line 0.4 % and 11 % at
-// worst; with one price it is 2.6 %, 8.8 % and 31 %.  (16384 rows, 768 and 2048 wide: 161, 153, 140 and 146 us in the first four tiles; 4096 rows,
-// 2048 and 5632: 192, 152, 149 and 158.)
+// with, for K ranges, a second launch and the slabs' way out and back.  The times are those of the kernels as they are, fitted to 16-bit
+// products of 100 to 16384 rows and widths of 88 to 11264, the operands in the caches and in none of them (geometric mean of the two).  Over 396 others
+// the choice is 0.8 % slower than the best tile and number of ranges on average, 15 % at worst; the best number of ranges of the fourth tile
+// alone 12 %, of the first 45 % on average.  The backward of SwiGLU reads as much as it writes: above 6 M values a byte is dearer by
+// TIMES_BWD, most in the large tiles, where the values on their way do not fit the registers.  Of 494 such products (1 to 20000 rows, widths 64 to 11264)
+// the choice is 0.3 % slower than the best tile on average, of the 139 above the line 0.4 % and 11 % at worst; with one price it is 2.6 %, 8.8 %
+// and 31 %.  (16384 rows, 768 and 2048 wide: 161, 153, 140 and 146 us in the first four tiles; 4096 rows, 2048 and 5632: 192, 152, 149 and 158.)
 struct TileTimes {
     double step, step_alone, end;      // us; a step of one of several workgroups on a CU, of a workgroup alone there
 };
 constexpr TileTimes TIMES_16[DENSE_N_TILES] = {{1.31, 1.31, 0.1}, {1.10, 1.10, 0.1}, {0.84, 0.84, 0.65}, {1.06, 0.68, 0.44}, {0.46, 0.26, 1.0}};
-// e4m3 (from DENSE_E4M3_FIRST on): from 4096 x 2048 x 11264, 4096 x 8192 x 4096 and 8192^3.
+// e4m3 (from DENSE_E4M3_FIRST on): from 4096 x 2048 x 11264, 4096 x 8192 x 4096 and 8192^3.  Over 470 products of 33 to 9000 rows the choice is 2.3 % slower
+// than the best tile and number of ranges on average (33 to 128 rows 1.5, 129 to 2399 3.2, above 0.9), 41 % at worst.
 constexpr TileTimes TIMES_8[DENSE_N_TILES] = {{}, {1.48, 1.48, 10.8}, {1.19, 1.19, 3.8}, {1.28, 0.75, 0.3}, {0.6, 0.33, 1.2}};
-
 constexpr double TIMES_BWD[DENSE_N_TILES] = {2.1, 1.8, 1.2, 1.2, 1.2};
 
 Plan plan_tiles(int64_t M, int64_t N, int64_t steps, int form) {

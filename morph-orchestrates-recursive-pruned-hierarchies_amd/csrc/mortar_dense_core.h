@@ -597,7 +597,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void dense_tile_kernel(const DenseA
 // ---- host side -------------------------------------------------------------------------------------------------------
 
 // The tiles: BN x BM of C by WN x WM waves, LDS steps (slots: twice as many halves, and one more where they fit), workgroups per CU.  The larger the tile the fewer bytes go through the L1 for a
-// product (64 per cycle and CU is what it takes: 256 x 256 keeps it half busy, 256 x 128 three quarters); the smaller ones
+// product (64 per cycle and CU is what it takes: at the full matrix rate 256 x 256 would keep it half busy, 256 x 128 three quarters); the smaller ones
 // are for matrices that do not fill the chip with large ones.
 struct DenseTile {
     int bn, bm, wn, wm, steps, halves, per_cu;
