@@ -85,17 +85,31 @@ at::Tensor plain_gradient(const at::Tensor &dy, const char *what) {
     return g;
 }
 
+// A tensor kept from the forward, as it comes back: saved-tensor hooks may have brought it to another place and other strides, and no further.
+const at::Tensor &kept(const at::Tensor &t, const at::Tensor &dy, at::IntArrayRef sizes, at::ScalarType type, const char *what) {
+    TORCH_CHECK(t.defined() && plain_values(t) && t.device() == dy.device() && t.scalar_type() == type && t.sizes() == sizes, what,
+                ": a tensor that was saved for the backward came back with another shape, type or device");
+    return t;
+}
+
 // ---- LayerNorm -------------------------------------------------------------------------------------------------------
+
+// x as rows [M, d] of consecutive values; 16-byte units where d is whole ones.
+at::Tensor norm_rows(const at::Tensor &x, int64_t d) {
+    const int64_t unit = x.scalar_type() == at::kFloat ? 4 : 8;
+    const at::Tensor rows = x.dim() == 2 ? x : x.reshape({-1, d});
+    const int64_t M = rows.size(0);
+    return (d > 1 && rows.stride(1) != 1) || (M > 1 && rows.stride(0) < d) || (d % unit == 0 && M > 1 && rows.stride(0) % unit) ? rows.contiguous() : rows;
+}
 
 // y, and for the backward (stats) the rows and their mean and 1 / deviation.
 at::Tensor norm_forward(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, double eps, bool keep, at::Tensor &rows, at::Tensor &stats) {
-    const int64_t d = x.size(-1), unit = x.scalar_type() == at::kFloat ? 4 : 8;
+    const int64_t d = x.size(-1);
     const c10::DeviceGuard guard(x.device());
     at::Tensor y = empty_like_rows(x, x.sizes());
     if (x.numel() == 0) return y;
     const int64_t M = x.numel() / d;
-    rows = x.dim() == 2 ? x : x.reshape({-1, d});
-    if ((d > 1 && rows.stride(1) != 1) || (M > 1 && rows.stride(0) < d) || (d % unit == 0 && M > 1 && rows.stride(0) % unit)) rows = rows.contiguous();
+    rows = norm_rows(x, d);
     if (keep) stats = at::empty({2, M}, x.options().dtype(at::kFloat).requires_grad(false));
     const bool w32 = x.scalar_type() != at::kFloat && ((w.defined() && w.scalar_type() == at::kFloat) || (b.defined() && b.scalar_type() == at::kFloat));
     check_rc(mortar_layernorm(data(rows), M, (int32_t)d, M > 1 ? rows.stride(0) : d, type_code(x.scalar_type()), data(w), data(b), w32, (float)eps, mut(y), d,
@@ -119,7 +133,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
         const at::Tensor dy = plain_gradient(grads[0], "layernorm");
         if (!dy.defined()) return out;
         const auto v = ctx->get_saved_variables();
-        const at::Tensor &rows = v[0], &w = v[1], &stats = v[2];
+        const at::Tensor &w = v[1];
         const auto shape = ctx->saved_data["shape"].toIntVector();
         const int64_t d = shape.back();
         // (edges are counted over the tensors that are there)
@@ -136,13 +150,16 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
             return out;
         }
         const int64_t M = dy.numel() / d;
+        const char *what = "layernorm";
+        const at::Tensor rows = norm_rows(kept(v[0], dy, {M, d}, dy.scalar_type(), what), d), stats = kept(v[2], dy, {2, M}, at::kFloat, what).contiguous();
+        const at::Tensor wc = w.defined() ? kept(w, dy, {d}, pt, what).contiguous() : w;
         const at::Tensor g = dy.dim() == 2 ? dy.contiguous() : dy.reshape({-1, d}).contiguous();
         at::Tensor dx, dw, db, ws;
         if (need_x) dx = at::empty(shape, dy.options().requires_grad(false));
         if (need_w) dw = at::empty({d}, params);
         if (need_b) db = at::empty({d}, params);
         if (need_w || need_b) ws = empty_bytes(dy, mortar_layernorm_workspace_bytes(M, (int32_t)d));
-        check_rc(mortar_layernorm_bwd(data(g), d, data(rows), M > 1 ? rows.stride(0) : d, M, (int32_t)d, type_code(dy.scalar_type()), data(w),
+        check_rc(mortar_layernorm_bwd(data(g), d, data(rows), M > 1 ? rows.stride(0) : d, M, (int32_t)d, type_code(dy.scalar_type()), data(wc),
                                       dy.scalar_type() != at::kFloat && pt == at::kFloat, floats(stats), floats(stats) + M, mut(dx), d, mut(dw), mut(db),
                                       floats(ws), stream_of(dy)),
                  "mortar_layernorm_bwd");
@@ -228,6 +245,7 @@ struct DenseMlpFn : public torch::autograd::Function<DenseMlpFn> {
         at::Tensor y = mlp_forward(x, wgu, wd, true, r);
         ctx->save_for_backward({r.x, r.wgu, r.wd, r.gu});
         ctx->saved_data["shape"] = x.sizes();
+        ctx->saved_data["d_ff"] = wd.size(1);
         return y;
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -235,9 +253,8 @@ struct DenseMlpFn : public torch::autograd::Function<DenseMlpFn> {
         const at::Tensor dy = plain_gradient(grads[0], "dense_mlp");
         if (!dy.defined()) return out;
         const auto v = ctx->get_saved_variables();
-        const at::Tensor &x = v[0], &wgu = v[1], &wd = v[2], &gu = v[3];
         const auto shape = ctx->saved_data["shape"].toIntVector();
-        const int64_t d = shape.back(), f = wd.size(1), n = wd.size(0);
+        const int64_t d = shape.back(), f = ctx->saved_data["d_ff"].toInt(), n = dy.size(-1);
         const bool need_x = ctx->needs_input_grad(0), need_gu = ctx->needs_input_grad(1), need_dn = ctx->needs_input_grad(2);
         const c10::DeviceGuard guard(dy.device());
         at::Tensor dx, dgw, ddw;
@@ -249,6 +266,8 @@ struct DenseMlpFn : public torch::autograd::Function<DenseMlpFn> {
             const int64_t M = dy.numel() / n;
             const int type = type_code(dy.scalar_type());
             void *st = stream_of(dy);
+            const auto matrix = [&](int i, int64_t rows, int64_t cols) { return rows_of(kept(v[i], dy, {rows, cols}, dy.scalar_type(), "dense_mlp"), cols, 8); };
+            const at::Tensor x = matrix(0, M, d), wgu = matrix(1, 2 * f, d), wd = matrix(2, n, f), gu = kept(v[3], dy, {6 * M * f}, at::kByte, "dense_mlp").contiguous();
             const at::Tensor g = rows_of(dy, n, 8);
             const at::Tensor dgu = empty_like_rows(dy, {M, 2 * f}), h = need_dn ? empty_like_rows(dy, {M, f}) : at::Tensor();
             check_rc(mortar_dense_swiglu_bwd(data(g), M, (int32_t)n, ld_of(g), data(wd), ld_of(wd), (int32_t)f, type, data(gu), mut(dgu), 2 * f, mut(h), f, st),

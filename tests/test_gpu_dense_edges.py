@@ -282,3 +282,29 @@ def test_few_rows_take_no_scratch(dev):
         before = count()
         y = ops.dense_mlp(x, wgu, wd)
         assert count() - before == 2 and y.shape == (M, 264)
+
+
+def test_saved_tensors_that_come_back_in_other_strides(dev):
+    """Saved-tensor hooks hand back the same values: elsewhere, transposed, or by way of the host."""
+    x, w, b = normals((6, 64), 1, BF16, dev).requires_grad_(True), normals((64,), 2, BF16, dev).requires_grad_(True), normals((64,), 3, BF16, dev).requires_grad_(True)
+    wgu, wd, dy = normals((48, 64), 4, BF16, dev, 0.1).requires_grad_(True), normals((64, 24), 5, BF16, dev, 0.2).requires_grad_(True), normals((6, 64), 6, BF16, dev)
+    turned = (lambda t: t.detach().t().contiguous(), lambda t: t.t())
+    spread = (lambda t: t.detach().repeat_interleave(2, 0), lambda t: t[::2])
+    host = (lambda t: t.detach().cpu(), lambda t: t.to(dev))
+    for leaves, f in (((x, w, b), ops.layernorm), ((x, wgu, wd), ops.dense_mlp)):
+        want = torch.autograd.grad(f(*leaves), leaves, dy)
+        for pack, unpack in (turned, spread, host):
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                y = f(*leaves)
+            assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, dy), want))
+
+
+@pytest.mark.parametrize("unpack", [lambda t: t.cpu(), lambda t: t[:1], lambda t: t.float() if t.is_floating_point() else t.int(), lambda t: t.unsqueeze(0)], ids=["host", "shape", "type", "dims"])
+def test_saved_tensors_that_come_back_as_others_are_refused(dev, unpack):
+    x, w = normals((6, 64), 1, BF16, dev).requires_grad_(True), normals((64,), 2, BF16, dev)
+    wgu, wd, dy = normals((48, 64), 4, BF16, dev, 0.1), normals((64, 24), 5, BF16, dev, 0.2), normals((6, 64), 6, BF16, dev)
+    for f in (lambda: ops.layernorm(x, w), lambda: ops.dense_mlp(x, wgu, wd)):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+            y = f()
+        with pytest.raises(RuntimeError, match="came back"):
+            torch.autograd.grad(y, [x], dy)
