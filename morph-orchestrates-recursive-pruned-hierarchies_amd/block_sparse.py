@@ -394,14 +394,16 @@ class CMSBlockLinear(nn.Module):
             if now.dtype != torch.float32 and was.dtype == torch.float32:
                 self._fp8_scale = was
             elif now.dtype == torch.float32 and self._fp8_scale is not None:
-                self._buffers["dense_fp8_scale"], self._fp8_scale = self._fp8_scale.to(now.device), None
+                if was.dtype != torch.float32:
+                    self._buffers["dense_fp8_scale"] = self._fp8_scale.to(now.device)
+                self._fp8_scale = None
         return self
 
     # ------------------------------------------------------------------ checkpoints
 
     def _save_to_state_dict(self, destination, prefix, keep_vars):
         super()._save_to_state_dict(destination, prefix, keep_vars)
-        if self._fp8_scale is not None:
+        if self._fp8_scale is not None and self.dense_fp8_scale.dtype != torch.float32:
             destination[prefix + "dense_fp8_scale"] = self._fp8_scale.to(self.dense_fp8.device)
 
     def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
@@ -416,7 +418,7 @@ class CMSBlockLinear(nn.Module):
                       for k, size in expected.items() if state_dict[prefix + k].shape != size]
             errors += [f"{prefix + k} must be {t} in the checkpoint, it is {state_dict[prefix + k].dtype}"          # (a copy would round them)
                        for k, t in (("dense_fp8", torch.uint8), ("dense_fp8_scale", torch.float32)) if state_dict[prefix + k].dtype != t]
-            if self._fp8_scale is not None:
+            if "dense_fp8" in self._buffers and self.dense_fp8_scale.dtype != torch.float32:
                 errors.append(f"{prefix}dense_fp8_scale is held in {self.dense_fp8_scale.dtype} since a cast of the module: cast it to float32 first")
             if errors:                           # (an error of strict and other loads, as for every parameter; the layer stays as it was)
                 error_msgs.extend(errors)

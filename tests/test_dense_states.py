@@ -122,3 +122,13 @@ def test_scales_are_whole_again_behind_a_cast(t):
         cast.load_state_dict({"dense_fp8": new[0], "dense_fp8_scale": new[1], "bias": state["bias"]})
     lin, state = _packed(seed=2)
     assert torch.equal(lin.double().dense_fp8_scale.float(), state["dense_fp8_scale"])
+
+
+def test_scales_that_are_set_anew_behind_a_cast():
+    """The layer's own buffer counts, whatever was kept through a cast."""
+    lin, state = _packed()
+    new = state["dense_fp8_scale"] * 2
+    lin.bfloat16().dense_fp8_scale = new.clone()
+    assert torch.equal(lin.state_dict()["dense_fp8_scale"], new) and torch.equal(copy.deepcopy(lin).float().dense_fp8_scale, new)
+    lin.load_state_dict(state)
+    assert _holds(lin, state) and torch.equal(lin.bfloat16().float().dense_fp8_scale, state["dense_fp8_scale"])
