@@ -432,6 +432,7 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *a, Py_ssize_t na) {
         if (codes) {
             xr = rows_of(x, K, 16);
             xs = xs.dim() == 2 ? xs : xs.reshape({-1, kb});
+            if (xs.stride(0) >= (INT64_C(1) << 29) / M) xs = xs.t().clone(at::MemoryFormat::Contiguous).t();        // (rows within 2 GiB)
             xp = data(xr), ldx = ld_of(xr);
             sx = static_cast<const float *>(xs.const_data_ptr()), s_m = xs.stride(0), s_k = xs.stride(1);
         } else {

@@ -308,3 +308,15 @@ def test_saved_tensors_that_come_back_as_others_are_refused(dev, unpack):
             y = f()
         with pytest.raises(RuntimeError, match="came back"):
             torch.autograd.grad(y, [x], dy)
+
+
+@pytest.mark.parametrize("M", [1, 20, 70])
+def test_scales_of_rows_far_apart(dev, M):
+    """x_scale whose rows span 2 GiB, in one matrix or as the last of every sequence's."""
+    wq, ws = ops.quantize_fp8_weight(normals((72, 160), 1, torch.float32, dev, 0.1))
+    q, s = ops.quantize_fp8(normals((M, 160), 2, BF16, dev))
+    wide = torch.zeros((M, (1 << 29) // M + 8), device=dev)
+    wide[:, -2:] = s
+    want = ops.linear_fp8(q, wq, ws, s)
+    assert torch.equal(ops.linear_fp8(q, wq, ws, wide[:, -2:]), want)
+    assert torch.equal(ops.linear_fp8(q[:, None], wq, ws, wide[:, None, -2:]), want[:, None])
