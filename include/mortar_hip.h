@@ -651,6 +651,66 @@ int mortar_fp8_quantizes_inside(int64_t M, int64_t K);
 int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const float *sx, int64_t sx_m, int64_t sx_k, const uint8_t *w, int64_t ldw,
                       const float *sw, int64_t sw_n, int32_t N, uint16_t *y, int64_t ldy, float *workspace, void *stream);
 
+/* ---- dense layers in 4 bits --------------------------------------------------------------------------- */
+
+/* W [N, K] as 4-bit codes c with one scale s and zero point z per row and group of `group` (32, 64 or 128) consecutive K: W = (c - z) s.
+ * Codes: 32-bit words of eight consecutive K, value j of them in bits 4 p .. 4 p + 3 with p = 0 4 1 5 2 6 3 7 for j = 0 .. 7, rows of whole 32
+ * values (4 ceil(K / 32) words; what lies behind K is not used), on 16-byte addresses, ldc in words.  s(n, g) at s[n * s_n + g * s_g] in bf16, fp16 or
+ * fp32, z(n, g) at z[n * z_n + g * z_g] in 8 bits, or NULL for 8 throughout.
+ *   mortar_int4_quantize   w [N, K] in bf16, fp16 or fp32 (`type`) -> c, s and (not NULL) z.  With z: s = (max - min) / 15 and
+ *                          z = rne(-min / s) over the group and 0; without: s = max(max / 7, -min / 8); s rounded to its type (1 where that is 0),
+ *                          c = rne(w / s) + z, 0 at least and 15 at most, quotients in fp32.  What lies behind K gets the code 8.
+ *   mortar_int4_linear     y [M, N] = x W^T, x [M, K] and y in bf16 or fp16 (`type`), fp32 sums.  K a multiple of 8, rows of x on 16-byte addresses.
+ *                          Sums are formed over x (16 + c) and x, both exact in the matrix cores, and joined per group in fp32: a row of x whose group
+ *                          holds an infinity or NaN is NaN in every column.
+ *   workspace              mortar_int4_workspace_bytes(M, N, K, group) bytes, 16-byte aligned, where that is not 0 */
+int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t ldw, int32_t type, int32_t group, uint32_t *c, int64_t ldc, void *s, int32_t s_type,
+                         int64_t s_n, int64_t s_g, uint8_t *z, int64_t z_n, int64_t z_g, void *stream);
+int64_t mortar_int4_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t group);
+int mortar_int4_linear(const void *x, int64_t M, int32_t K, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group, const void *s,
+                       int32_t s_type, int64_t s_n, int64_t s_g, const uint8_t *z, int64_t z_n, int64_t z_g, void *y, int64_t ldy, void *workspace,
+                       void *stream);
+
+/* ---- norm of many gradients, and clipping -------------------------------------------------------------- */
+
+/* One gradient of a list in host memory (read during the call): n consecutive values of `type` on an address of that type, and for the clipping where the
+ * result goes: the same type or fp32; dst = src is in place.  No two results may overlap. */
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t n;
+    int32_t type, out_type;
+} mortar_grad_t;
+/* *norm (device) = (sum of all g^2)^(1/2), or with `largest` max |g| (NaN if there is one); squares and sums in 64 bits, in a fixed order.
+ * mortar_grad_clip: dst = g min(1, max_norm / (*norm + 1e-6)) besides, the factor formed in 64 bits and rounded to fp32, the product rounded once; in
+ * place nothing is written where the factor is 1.  workspace: mortar_grad_workspace_bytes of the list, 8-byte aligned device memory. */
+int64_t mortar_grad_workspace_bytes(const mortar_grad_t *grads, int64_t count);
+int mortar_grad_norm(const mortar_grad_t *grads, int64_t count, int32_t largest, float *norm, void *workspace, void *stream);
+int mortar_grad_clip(const mortar_grad_t *grads, int64_t count, int32_t largest, double max_norm, float *norm, void *workspace, void *stream);
+
+/* ---- tokens to experts and back ------------------------------------------------------------------------ */
+
+/* N tokens with k slots each, ids [N, k] (int32, or int64 with ids_64): the expert of each slot, 0 .. n_experts - 1 (at most 1024), anything else an empty one.
+ *   mortar_expert_sort         position [N, k]: the row of each slot when all are sorted by expert, those of one expert in the order of the slots,
+ *                              empty ones behind all others; token [N k]: the token of each row; offsets [n_experts + 1]: first row of each expert, then the
+ *                              number of full rows.  workspace: mortar_expert_sort_workspace_bytes(N k, n_experts) bytes where that is not 0
+ *   mortar_expert_dispatch     xs [N k, d]: row position[n, j] = x[n], zeros for empty slots;  x [N, d], ldx >= 0 in values
+ *   mortar_expert_combine      y [N, d] = sum over the full slots j of weights[n, j] ys[position[n, j]], in order, fp32 sums; weights [N, k] in w_type or
+ *                              NULL for 1; rows of empty slots are not read
+ *   mortar_expert_combine_bwd  dys [N k, d]: row position[n, j] = weights[n, j] dy[n], zeros for empty slots; dw [N, k] in w_type = <dy[n], ys[position[n, j]]>,
+ *                              0 for empty slots; either may be NULL
+ * full: device, the number of full rows (offsets + n_experts).  x, ys, xs, y, dy, dys in `type` (bf16, fp16 or fp32) of any width and on any address of the type.
+ * N k below 2^26. */
+int64_t mortar_expert_sort_workspace_bytes(int64_t slots, int32_t n_experts);
+int mortar_expert_sort(const void *ids, int32_t ids_64, int64_t N, int32_t k, int32_t n_experts, int32_t *position, int32_t *token, int32_t *offsets,
+                       void *workspace, void *stream);
+int mortar_expert_dispatch(const void *x, int64_t N, int32_t d, int64_t ldx, int32_t type, int32_t k, const int32_t *position, const int32_t *full, void *xs,
+                           void *stream);
+int mortar_expert_combine(const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position, const int32_t *full, const void *weights,
+                          int32_t w_type, void *y, void *stream);
+int mortar_expert_combine_bwd(const void *dy, int64_t lddy, const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position,
+                              const int32_t *full, const void *weights, int32_t w_type, void *dys, void *dw, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -117,7 +117,24 @@ _SIGS = {
     "mortar_fp8_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64]),
     "mortar_fp8_quantizes_inside": (C.c_int, [c_i64, c_i64]),
     "mortar_fp8_linear": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_i64, c_vp, c_vp]),
+    "mortar_int4_quantize": (C.c_int, [c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp]),
+    "mortar_int4_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
+    "mortar_int4_linear": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64,
+                                     c_vp, c_vp]),
+    "mortar_grad_workspace_bytes": (c_i64, [c_vp, c_i64]),
+    "mortar_grad_norm": (C.c_int, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp]),
+    "mortar_grad_clip": (C.c_int, [c_vp, c_i64, c_i32, C.c_double, c_vp, c_vp, c_vp]),
+    "mortar_expert_sort_workspace_bytes": (c_i64, [c_i64, c_i32]),
+    "mortar_expert_sort": (C.c_int, [c_vp, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "mortar_expert_dispatch": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp]),
+    "mortar_expert_combine": (C.c_int, [c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "mortar_expert_combine_bwd": (C.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
 }
+
+class GradStruct(C.Structure):
+    """mortar_grad_t"""
+    _fields_ = [("src", c_vp), ("dst", c_vp), ("n", c_i64), ("type", c_i32), ("out_type", c_i32)]
+
 
 class PackHandle(C.Structure):
     """One packed matrix for the native call layer: its mortar_bcsr_t, the schedules built so far and, once it has been re-packed,

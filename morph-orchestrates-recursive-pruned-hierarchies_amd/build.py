@@ -12,8 +12,8 @@ CSRC = os.path.join(_HERE, "csrc")
 LIB = os.path.join(_HERE, "libmortar_hip.so")
 NATIVE = os.path.join(_HERE, "_mortar_native.so")
 SOURCES = ["mortar_host.cpp", "mortar_prefill.hip", "mortar_smallm.hip", "mortar_smallm_chunk.hip", "mortar_mid.hip", "mortar_pipe.hip", "mortar_decode.hip", "mortar_gemv_f32.hip", "mortar_route.hip", "mortar_router_gemm.hip",
-           "mortar_pack.hip", "mortar_sdd.hip", "mortar_swiglu.hip", "mortar_values.hip", "mortar_layernorm.hip", "mortar_dense.hip", "mortar_fp8.hip"]
-NATIVE_SOURCES = ["mortar_torch.cpp", "mortar_torch_dense.cpp"]
+           "mortar_pack.hip", "mortar_sdd.hip", "mortar_swiglu.hip", "mortar_values.hip", "mortar_layernorm.hip", "mortar_dense.hip", "mortar_fp8.hip", "mortar_int4.hip", "mortar_clip.hip", "mortar_experts.hip"]
+NATIVE_SOURCES = ["mortar_torch.cpp", "mortar_torch_dense.cpp", "mortar_torch_train.cpp"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

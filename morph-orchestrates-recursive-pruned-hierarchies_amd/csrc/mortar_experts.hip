@@ -1,0 +1,465 @@
+// Tokens sorted by expert and back.  A token n has k slots, each with the number of an expert or empty (any number outside 0 .. E - 1):
+//   sort       position[n, j] = row of slot (n, j) when all N k slots are sorted by expert, in the order of the slots within one (a stable counting
+//              sort), the empty ones behind all others; token[row] = n; offsets[e] = the first row of expert e, offsets[E] = the full rows
+//   dispatch   xs[position[n, j]] = x[n], zeros in the rows of empty slots;     backward: dx[n] = sum_j dxs[position[n, j]] over full slots
+//   combine    y[n] = sum_j w[n, j] ys[position[n, j]] over full slots
+//              backward: dys[position[n, j]] = w[n, j] dy[n] (zeros for empty slots),  dw[n, j] = <dy[n], ys[position[n, j]]> (0 for empty ones)
+// Positions are a permutation of the rows, so every row is written by exactly one wave and no atomics are needed: sums run over a token's slots in
+// their order, in fp32, and are rounded once.  Rows of empty slots are not read.  What bounds all but the sort is the memory.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "mortar_device.h"
+#include "mortar_internal.h"
+
+namespace {
+
+constexpr int MOST_EXPERTS = 1024, MOST_SLOTS = 1 << 26;        // (a wave per slot: a grid has 2^32 threads at most)
+
+int launch_error(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? MORTAR_OK : mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+// ---- sort ------------------------------------------------------------------------------------------------------------
+// Up to SORT_BLOCKS workgroups of 16 waves, each with a run of slots: first they count the slots per expert, then each of them adds up what lies in
+// front of its own (the experts in front, the runs in front) and places its slots.  The counts of a run are kept per wave; within a wave's 64 slots
+// the order is found with one ballot per bit of the expert's number.  Few slots are one workgroup's, in one launch.
+constexpr int SORT_WAVES = 16, SORT_BLOCKS = 64, SORT_ALONE = 4096;
+
+template <typename ID>
+struct Slots {
+    const ID *ids;
+    int64_t n;
+    int experts;
+    __device__ __forceinline__ int key(int64_t i) const {
+        const ID v = ids[i];
+        return v >= 0 && v < experts ? (int)v : experts;
+    }
+};
+
+// counts[e] of the slots [first, last) of each wave: one row of `counts` per wave, in LDS and zeroed here.
+template <typename ID>
+__device__ __forceinline__ void count_run(const Slots<ID> &s, int64_t first, int64_t last, int *counts) {
+    const int keys = s.experts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i = threadIdx.x; i < keys * SORT_WAVES; i += SORT_WAVES * 64) counts[i] = 0;
+    __syncthreads();
+    const int64_t per = (last - first + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) * 64, begin = first + wave * per;
+    for (int64_t i = begin + lane; i < min(begin + per, last); i += 64) atomicAdd(&counts[wave * keys + s.key(i)], 1);
+    __syncthreads();
+}
+
+template <typename ID>
+__global__ __launch_bounds__(SORT_WAVES * 64) void expert_count_kernel(const Slots<ID> s, int64_t run, int32_t *totals) {
+    extern __shared__ int counts[];
+    const int keys = s.experts + 1;
+    const int64_t first = blockIdx.x * run, last = min(first + run, s.n);
+    count_run(s, first, last, counts);
+    for (int e = threadIdx.x; e < keys; e += SORT_WAVES * 64) {
+        int sum = 0;
+#pragma unroll
+        for (int w = 0; w < SORT_WAVES; ++w) sum += counts[w * keys + e];
+        totals[(int64_t)blockIdx.x * keys + e] = sum;
+    }
+}
+
+// Exclusive sums of v over the workgroup's threads.
+__device__ __forceinline__ int scan_workgroup(int v, int *part) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int up = __shfl_up(sum, d);
+        if (lane >= d) sum += up;
+    }
+    if (lane == 63) part[wave] = sum;
+    __syncthreads();
+    int base = 0;
+    for (int w = 0; w < wave; ++w) base += part[w];
+    __syncthreads();
+    return base + sum - v;
+}
+
+// ALONE: one workgroup has all slots and no totals of others.
+template <typename ID, bool ALONE>
+__global__ __launch_bounds__(SORT_WAVES * 64) void expert_place_kernel(const Slots<ID> s, int64_t run, int slots_per_token, const int32_t *totals, int32_t *position,
+                                                                       int32_t *token, int32_t *offsets) {
+    extern __shared__ int counts[];
+    __shared__ int part[SORT_WAVES];
+    const int keys = s.experts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = blockIdx.x * run, last = min(first + run, s.n);
+    count_run(s, first, last, counts);
+    // Rows in front of this workgroup's slots of an expert, and from them those of each wave: in place of the counts.
+    for (int e0 = 0, before = 0; e0 < keys; e0 += SORT_WAVES * 64) {
+        const int e = e0 + threadIdx.x;
+        int all = 0, mine = 0;
+        if (e < keys) {
+            if constexpr (ALONE) {
+                for (int w = 0; w < SORT_WAVES; ++w) all += counts[w * keys + e];
+            } else {
+                for (int b = 0; b < (int)gridDim.x; ++b) {
+                    const int c = totals[(int64_t)b * keys + e];
+                    if (b < (int)blockIdx.x) mine += c;
+                    all += c;
+                }
+            }
+        }
+        const int front = before + scan_workgroup(all, part);
+        if (e < keys) {
+            int at = front + mine;
+#pragma unroll
+            for (int w = 0; w < SORT_WAVES; ++w) {
+                const int c = counts[w * keys + e];
+                counts[w * keys + e] = at;
+                at += c;
+            }
+            if (blockIdx.x == 0) offsets[e] = front;
+        }
+        if (e0 + SORT_WAVES * 64 < keys) {               // (more keys than threads: 1025)
+            if (threadIdx.x == SORT_WAVES * 64 - 1) part[0] = front + all;
+            __syncthreads();
+            before = part[0];
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+    const int bits = 32 - __builtin_clz(s.experts);
+    int *next = counts + wave * keys;
+    const int64_t per = (last - first + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) * 64, begin = first + wave * per, end = min(begin + per, last);
+    for (int64_t i0 = begin; i0 < end; i0 += 64) {
+        const int64_t i = i0 + lane;
+        const bool on = i < end;
+        const int key = on ? s.key(i) : 0;
+        uint64_t same = __ballot(on);
+        for (int b = 0; b < bits; ++b) {
+            const uint64_t set = __ballot(key >> b & 1);
+            same &= key >> b & 1 ? set : ~set;
+        }
+        const int rank = __popcll(same & ((UINT64_C(1) << lane) - 1));
+        int at = 0;
+        if (on) at = __hip_atomic_load(next + key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) + rank;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (on && (same >> lane) == 1) __hip_atomic_store(next + key, at + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);      // the last lane of its expert
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (on) {
+            position[i] = at;
+            token[at] = (int32_t)(i / slots_per_token);
+        }
+    }
+}
+
+template <typename ID>
+int sort(const Slots<ID> &s, int slots_per_token, int32_t *position, int32_t *token, int32_t *offsets, int32_t *totals, hipStream_t st, const char *what) {
+    const int smem = (s.experts + 1) * SORT_WAVES * 4;
+    const auto room = [&](const void *kern) { return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (MOST_EXPERTS + 1) * SORT_WAVES * 4); };
+    if (s.n <= SORT_ALONE) {
+        const auto kern = expert_place_kernel<ID, true>;
+        if (const hipError_t e = room(reinterpret_cast<const void *>(kern)); e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+        hipLaunchKernelGGL(kern, dim3(1), dim3(SORT_WAVES * 64), smem, st, s, s.n, slots_per_token, nullptr, position, token, offsets);
+        return launch_error(what);
+    }
+    const int64_t run = std::max<int64_t>(2048, ((s.n + SORT_BLOCKS - 1) / SORT_BLOCKS + 63) / 64 * 64);
+    const unsigned blocks = (unsigned)((s.n + run - 1) / run);
+    const auto count = expert_count_kernel<ID>;
+    const auto place = expert_place_kernel<ID, false>;
+    for (const void *kern : {reinterpret_cast<const void *>(count), reinterpret_cast<const void *>(place)})
+        if (const hipError_t e = room(kern); e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    hipLaunchKernelGGL(count, dim3(blocks), dim3(SORT_WAVES * 64), smem, st, s, run, totals);
+    if (const int rc = launch_error(what)) return rc;
+    hipLaunchKernelGGL(place, dim3(blocks), dim3(SORT_WAVES * 64), smem, st, s, run, slots_per_token, totals, position, token, offsets);
+    return launch_error(what);
+}
+
+// ---- rows ------------------------------------------------------------------------------------------------------------
+// Rows are read and written in 16-byte units on whatever addresses they lie (odd widths: multiples of 2 bytes), what is left behind the last whole one
+// value by value.
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+
+template <int TYPE>
+struct Row {
+    static constexpr int UNIT = TYPE == MORTAR_FP32 ? 4 : 8, SIZE = 16 / UNIT;
+    static __device__ __forceinline__ u32x4_t load(const char *p) { return *reinterpret_cast<const u32x4_any_t *>(p); }
+    static __device__ __forceinline__ void store(char *p, u32x4_t w) { *reinterpret_cast<u32x4_any_t *>(p) = w; }
+    static __device__ __forceinline__ void unpack(u32x4_t w, float (&v)[UNIT]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t d = w[j];
+            if constexpr (TYPE == MORTAR_FP32) {
+                v[j] = __builtin_bit_cast(float, d);
+            } else if constexpr (TYPE == MORTAR_FP16) {
+                const f32x2_t f = __builtin_convertvector(__builtin_bit_cast(f16x2_t, d), f32x2_t);
+                v[2 * j] = f[0], v[2 * j + 1] = f[1];
+            } else {
+                v[2 * j] = __builtin_bit_cast(float, d << 16);
+                v[2 * j + 1] = __builtin_bit_cast(float, d & 0xffff0000u);
+            }
+        }
+    }
+    static __device__ __forceinline__ u32x4_t pack(const float (&v)[UNIT]) {
+        u32x4_t w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (TYPE == MORTAR_FP32) w[j] = __builtin_bit_cast(uint32_t, v[j]);
+            else if constexpr (TYPE == MORTAR_FP16) w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{v[2 * j], v[2 * j + 1]}, f16x2_t));
+            else w[j] = bf16_pack2(v[2 * j], v[2 * j + 1]);
+        }
+        return w;
+    }
+    static __device__ __forceinline__ float one(const char *p) {
+        if constexpr (TYPE == MORTAR_FP32) return *reinterpret_cast<const float *>(p);
+        else if constexpr (TYPE == MORTAR_FP16) return (float)*reinterpret_cast<const _Float16 *>(p);
+        else return bf16_to_f32(*reinterpret_cast<const uint16_t *>(p));
+    }
+    static __device__ __forceinline__ void put(char *p, float v) {
+        if constexpr (TYPE == MORTAR_FP32) *reinterpret_cast<float *>(p) = v;
+        else if constexpr (TYPE == MORTAR_FP16) *reinterpret_cast<_Float16 *>(p) = (_Float16)v;
+        else *reinterpret_cast<uint16_t *>(p) = (uint16_t)bf16_bits_rne(v);
+    }
+};
+
+struct RowArgs {
+    const char *x;               // rows per token (dispatch: x, combine backward: dy), ldx bytes apart
+    const char *ys;              // rows per slot, d values apart
+    char *out;                   // dispatch: xs, combine: y, combine backward: dys or null
+    char *dw;                    // combine backward: gradients of the weights or null
+    const char *w;               // weights [N, k], or null for 1
+    const int32_t *position, *full;
+    int64_t ldx, slots;          // slots: N k
+    int32_t k, d, w_type;
+};
+
+__device__ __forceinline__ float read_weight(const RowArgs &a, int64_t i) {
+    if (!a.w) return 1.0f;
+    return a.w_type == MORTAR_FP32 ? Row<MORTAR_FP32>::one(a.w + i * 4) : a.w_type == MORTAR_FP16 ? Row<MORTAR_FP16>::one(a.w + i * 2) : Row<MORTAR_BF16>::one(a.w + i * 2);
+}
+
+// A wave per slot; the rows of a token are read by neighbouring waves and come out of the caches but once.
+template <int SIZE>
+__global__ __launch_bounds__(256) void expert_dispatch_kernel(const RowArgs a) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t i = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (i >= a.slots) return;
+    const int row = a.position[i];
+    if ((uint32_t)row >= (uint32_t)a.slots) return;        // (no order of this many slots)
+    const char *src = a.x + i / (uint32_t)a.k * a.ldx;
+    char *dst = a.out + (int64_t)row * a.d * SIZE;
+    const int bytes = a.d * SIZE, units = bytes / 16;
+    const bool live = row < *a.full;
+    int u = lane;
+    for (; u + 192 < units; u += 256) {
+        u32x4_t v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = live ? *reinterpret_cast<const u32x4_any_t *>(src + (u + q * 64) * 16) : u32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<u32x4_any_t *>(dst + (u + q * 64) * 16) = v[q];
+    }
+    for (; u < units; u += 64) *reinterpret_cast<u32x4_any_t *>(dst + u * 16) = live ? *reinterpret_cast<const u32x4_any_t *>(src + u * 16) : u32x4_t{0, 0, 0, 0};
+    const int at = units * 16 + lane * SIZE;
+    if (at < bytes) {
+        if constexpr (SIZE == 4) *reinterpret_cast<uint32_t *>(dst + at) = live ? *reinterpret_cast<const uint32_t *>(src + at) : 0u;
+        else *reinterpret_cast<uint16_t *>(dst + at) = live ? *reinterpret_cast<const uint16_t *>(src + at) : (uint16_t)0;
+    }
+}
+
+// A wave per token and 64 units of the row; the rows of eight slots are on their way at a time.
+template <int TYPE>
+__global__ __launch_bounds__(256) void expert_combine_kernel(const RowArgs a, int parts) {
+    using R = Row<TYPE>;
+    const int lane = threadIdx.x & 63;
+    const uint32_t task = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int64_t n = task / (uint32_t)parts;
+    if (n * a.k >= a.slots) return;
+    const int unit = (int)(task - (uint32_t)n * parts) * 64 + lane, left = a.d - unit * R::UNIT;
+    const int64_t pitch = (int64_t)a.d * R::SIZE, in = (int64_t)unit * 16;
+    const uint32_t full = min((uint32_t)*a.full, (uint32_t)a.slots);
+    float sum[R::UNIT];
+#pragma unroll
+    for (int v = 0; v < R::UNIT; ++v) sum[v] = 0.f;
+    for (int j0 = 0; j0 < a.k; j0 += 8) {
+        u32x4_t v[8];
+        float w[8];
+        uint32_t row[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            row[q] = j0 + q < a.k ? (uint32_t)a.position[n * a.k + j0 + q] : UINT32_MAX;
+            w[q] = row[q] < full ? read_weight(a, n * a.k + j0 + q) : 0.f;
+        }
+        if (left >= R::UNIT) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (row[q] < full) v[q] = R::load(a.ys + row[q] * pitch + in);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (row[q] < full) {
+                    float f[R::UNIT];
+                    R::unpack(v[q], f);
+#pragma unroll
+                    for (int t = 0; t < R::UNIT; ++t) sum[t] = __builtin_fmaf(w[q], f[t], sum[t]);
+                }
+        } else {
+            for (int q = 0; q < 8; ++q)
+                if (row[q] < full) {
+#pragma unroll
+                    for (int t = 0; t < R::UNIT; ++t)
+                        if (t < left) sum[t] = __builtin_fmaf(w[q], R::one(a.ys + row[q] * pitch + in + t * R::SIZE), sum[t]);
+                }
+        }
+    }
+    char *dst = a.out + n * pitch + in;
+    if (left >= R::UNIT) {
+        R::store(dst, R::pack(sum));
+    } else {
+#pragma unroll
+        for (int t = 0; t < R::UNIT; ++t)
+            if (t < left) R::put(dst + t * R::SIZE, sum[t]);
+    }
+}
+
+// A wave per slot: its row of dys, and the dot product over the row.
+template <int TYPE>
+__global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a) {
+    using R = Row<TYPE>;
+    const int lane = threadIdx.x & 63;
+    const uint32_t i = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (i >= a.slots) return;
+    const int row = a.position[i];
+    if ((uint32_t)row >= (uint32_t)a.slots) return;
+    const bool live = row < *a.full;
+    const float w = live ? read_weight(a, i) : 0.f;
+    const char *dy = a.x + i / (uint32_t)a.k * a.ldx;
+    const int64_t at_row = (int64_t)row * a.d * R::SIZE;
+    const int units = a.d / R::UNIT;
+    float dot = 0.f;
+    for (int u = lane; u < units; u += 64) {
+        float g[R::UNIT], f[R::UNIT];
+#pragma unroll
+        for (int t = 0; t < R::UNIT; ++t) g[t] = f[t] = 0.f;
+        if (live) {
+            const u32x4_t gw = R::load(dy + (int64_t)u * 16);
+            if (a.dw) R::unpack(R::load(a.ys + at_row + (int64_t)u * 16), f);
+            R::unpack(gw, g);
+#pragma unroll
+            for (int t = 0; t < R::UNIT; ++t) dot = __builtin_fmaf(g[t], f[t], dot);
+        }
+        if (a.out) {
+#pragma unroll
+            for (int t = 0; t < R::UNIT; ++t) g[t] = live ? g[t] * w : 0.f;
+            R::store(a.out + at_row + (int64_t)u * 16, R::pack(g));
+        }
+    }
+    const int last = units * R::UNIT + lane;
+    if (last < a.d) {
+        const float g = live ? R::one(dy + (int64_t)last * R::SIZE) : 0.f;
+        if (live && a.dw) dot = __builtin_fmaf(g, R::one(a.ys + at_row + (int64_t)last * R::SIZE), dot);
+        if (a.out) R::put(a.out + at_row + (int64_t)last * R::SIZE, live ? g * w : 0.f);
+    }
+    if (!a.dw) return;
+    dot = mortar_wave_sum(dot);
+    if (lane) return;
+    if (a.w_type == MORTAR_FP32) Row<MORTAR_FP32>::put(a.dw + i * 4, dot);
+    else if (a.w_type == MORTAR_FP16) Row<MORTAR_FP16>::put(a.dw + i * 2, dot);
+    else Row<MORTAR_BF16>::put(a.dw + i * 2, dot);
+}
+
+bool known(int32_t type) { return type == MORTAR_BF16 || type == MORTAR_FP16 || type == MORTAR_FP32; }
+
+int check_rows(const char *what, int64_t N, int32_t k, int32_t d, int32_t type) {
+    if (N < 0 || k <= 0 || d <= 0 || !known(type)) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape or type", what);
+    if (d >= 1 << 28 || N >= MOST_SLOTS || N * k >= MOST_SLOTS) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many slots or values", what);
+    return MORTAR_OK;
+}
+int check_pointer(const char *what, const char *name, const void *p, int32_t type) {
+    if (!p) return mortar_fail(MORTAR_ERR_ARG, "%s: %s is null", what, name);
+    return reinterpret_cast<uintptr_t>(p) % (type == MORTAR_FP32 ? 4 : 2) ? mortar_fail(MORTAR_ERR_ARG, "%s: %s is not on an address of its type", what, name) : MORTAR_OK;
+}
+#define CHECK(...) do { const int rc_ = (__VA_ARGS__); if (rc_) return rc_; } while (0)
+
+}  // namespace
+
+extern "C" int64_t mortar_expert_sort_workspace_bytes(int64_t slots, int32_t n_experts) {
+    return slots <= SORT_ALONE || n_experts <= 0 ? 0 : INT64_C(4) * SORT_BLOCKS * (n_experts + 1);
+}
+
+extern "C" int mortar_expert_sort(const void *ids, int32_t ids_64, int64_t N, int32_t k, int32_t n_experts, int32_t *position, int32_t *token, int32_t *offsets,
+                                  void *workspace, void *stream) {
+    const char *what = "expert_sort";
+    CHECK(check_rows(what, N, k, 1, MORTAR_FP32));
+    if (n_experts <= 0) return mortar_fail(MORTAR_ERR_ARG, "%s: no experts", what);
+    if (n_experts > MOST_EXPERTS) return mortar_fail(MORTAR_ERR_LIMIT, "%s: more than %d experts", what, MOST_EXPERTS);
+    const int64_t n = N * k;
+    if (!offsets || (n && (!ids || !position || !token)) || (mortar_expert_sort_workspace_bytes(n, n_experts) && !workspace))
+        return mortar_fail(MORTAR_ERR_ARG, "%s: a pointer is null", what);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    int32_t *totals = static_cast<int32_t *>(workspace);
+    if (ids_64) return sort(Slots<int64_t>{static_cast<const int64_t *>(ids), n, n_experts}, k, position, token, offsets, totals, st, what);
+    return sort(Slots<int32_t>{static_cast<const int32_t *>(ids), n, n_experts}, k, position, token, offsets, totals, st, what);
+}
+
+extern "C" int mortar_expert_dispatch(const void *x, int64_t N, int32_t d, int64_t ldx, int32_t type, int32_t k, const int32_t *position, const int32_t *full, void *xs,
+                                      void *stream) {
+    const char *what = "expert_dispatch";
+    CHECK(check_rows(what, N, k, d, type));
+    if (N == 0) return MORTAR_OK;
+    CHECK(check_pointer(what, "x", x, type));
+    CHECK(check_pointer(what, "xs", xs, type));
+    CHECK(check_pointer(what, "position", position, MORTAR_FP32));
+    CHECK(check_pointer(what, "full", full, MORTAR_FP32));
+    RowArgs a{};
+    a.x = static_cast<const char *>(x); a.ldx = ldx * (type == MORTAR_FP32 ? 4 : 2);
+    a.out = static_cast<char *>(xs); a.position = position; a.full = full;
+    a.slots = N * k; a.k = k; a.d = d;
+    const dim3 grid((unsigned)((a.slots + 3) / 4));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (type == MORTAR_FP32) hipLaunchKernelGGL(expert_dispatch_kernel<4>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(expert_dispatch_kernel<2>, grid, dim3(256), 0, st, a);
+    return launch_error(what);
+}
+
+extern "C" int mortar_expert_combine(const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position, const int32_t *full, const void *weights,
+                                     int32_t w_type, void *y, void *stream) {
+    const char *what = "expert_combine";
+    CHECK(check_rows(what, N, k, d, type));
+    if (N == 0) return MORTAR_OK;
+    CHECK(check_pointer(what, "ys", ys, type));
+    CHECK(check_pointer(what, "y", y, type));
+    CHECK(check_pointer(what, "position", position, MORTAR_FP32));
+    CHECK(check_pointer(what, "full", full, MORTAR_FP32));
+    if (weights && !known(w_type)) return mortar_fail(MORTAR_ERR_ARG, "%s: bad type of the weights", what);
+    if (weights) CHECK(check_pointer(what, "weights", weights, w_type));
+    RowArgs a{};
+    a.ys = static_cast<const char *>(ys); a.out = static_cast<char *>(y); a.w = static_cast<const char *>(weights); a.w_type = w_type;
+    a.position = position; a.full = full; a.slots = N * k; a.k = k; a.d = d;
+    const int per = 64 * (type == MORTAR_FP32 ? 4 : 8), parts = (d + per - 1) / per;
+    const int64_t groups = (N * parts + 3) / 4;
+    if (groups >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const auto kern = type == MORTAR_FP32 ? expert_combine_kernel<MORTAR_FP32> : type == MORTAR_FP16 ? expert_combine_kernel<MORTAR_FP16> : expert_combine_kernel<MORTAR_BF16>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, st, a, parts);
+    return launch_error(what);
+}
+
+extern "C" int mortar_expert_combine_bwd(const void *dy, int64_t lddy, const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position,
+                                         const int32_t *full, const void *weights, int32_t w_type, void *dys, void *dw, void *stream) {
+    const char *what = "expert_combine_bwd";
+    CHECK(check_rows(what, N, k, d, type));
+    if (N == 0 || (!dys && !dw)) return MORTAR_OK;
+    CHECK(check_pointer(what, "dy", dy, type));
+    CHECK(check_pointer(what, "position", position, MORTAR_FP32));
+    CHECK(check_pointer(what, "full", full, MORTAR_FP32));
+    if (dys) CHECK(check_pointer(what, "dys", dys, type));
+    if ((weights || dw) && !known(w_type)) return mortar_fail(MORTAR_ERR_ARG, "%s: bad type of the weights", what);
+    if (weights) CHECK(check_pointer(what, "weights", weights, w_type));
+    if (dw) CHECK(check_pointer(what, "dw", dw, w_type));
+    if (dw) CHECK(check_pointer(what, "ys", ys, type));
+    RowArgs a{};
+    a.x = static_cast<const char *>(dy); a.ldx = lddy * (type == MORTAR_FP32 ? 4 : 2);
+    a.ys = static_cast<const char *>(ys); a.out = static_cast<char *>(dys); a.dw = static_cast<char *>(dw);
+    a.w = static_cast<const char *>(weights); a.w_type = w_type;
+    a.position = position; a.full = full; a.slots = N * k; a.k = k; a.d = d;
+    const dim3 grid((unsigned)((a.slots + 3) / 4));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const auto kern = type == MORTAR_FP32 ? expert_combine_bwd_kernel<MORTAR_FP32> : type == MORTAR_FP16 ? expert_combine_bwd_kernel<MORTAR_FP16> : expert_combine_bwd_kernel<MORTAR_BF16>;
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a);
+    return launch_error(what);
+}

@@ -1,0 +1,508 @@
+// Dense layers served in 4 bits: y = x W^T, W = (c - z) s with 4-bit codes c, one scale s and zero point z per row and group of 32, 64 or 128 K.
+//   y[m, n] = sum_g s[n, g] ( sum_{k in g} x[m, k] (16 + c[n, k]) - (16 + z[n, g]) sum_{k in g} x[m, k] )
+// 16 + c is exact in bf16 and in fp16: a code's four bits are the upper mantissa bits behind the exponent of 16, so that two weights are made
+// by one shift and one and-or, and go into the matrix cores beside x as it is.  The sums of a group come out of them unscaled and enter the fp32 result with one
+// multiply-add: W is never rounded.  (W in 16 bits instead would cost as much again as the rounding of y.)  What the 16 adds is a few times the
+// codes' own size in sums of 24 bits, and is taken off exactly.
+// The codes of a word lie so that one shift brings a pair of neighbours into its two halves.
+#include <hip/hip_runtime.h>
+
+#include "mortar_dense_core.h"
+#include "mortar_internal.h"
+
+namespace {
+
+struct Int4Args {
+    const void *x;
+    int64_t ldx;                         // bytes
+    const uint32_t *c;
+    int64_t ldc;                         // bytes
+    const void *s;
+    int64_t s_n, s_g;                    // values
+    const uint8_t *z;
+    int64_t z_n, z_g;
+    uint16_t *y;
+    int64_t ldy;
+    int32_t M, N, K, groups;
+    const float *xs, *st, *zt;           // tiles: sums of x [groups][Mp], scales and 16 + z [groups][Np]
+    int32_t Mp, Np, tiles_n, tiles_m;
+};
+
+// Eight weights 16 + c of a word, in the order of K.
+template <DenseType T>
+__device__ __forceinline__ u32x4_t int4_unpack(uint32_t w) {
+    if constexpr (T == DENSE_F16) {
+        constexpr uint32_t mask = 0x03C003C0u, one = 0x4C004C00u;
+        return u32x4_t{(w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one, (w >> 6 & mask) | one};
+    } else {
+        constexpr uint32_t mask = 0x00780078u, one = 0x41804180u;
+        return u32x4_t{(w << 3 & mask) | one, (w >> 1 & mask) | one, (w >> 5 & mask) | one, (w >> 9 & mask) | one};
+    }
+}
+template <DenseType T, int S>
+__device__ __forceinline__ float int4_scale(const void *s, int64_t i) {
+    if constexpr (S == 4) return static_cast<const float *>(s)[i];
+    else if constexpr (T == DENSE_F16) return (float)static_cast<const _Float16 *>(s)[i];
+    else return bf16_to_f32(static_cast<const uint16_t *>(s)[i]);
+}
+
+// ---- few rows --------------------------------------------------------------------------------------------------------
+// 16 rows of W per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what bounds
+// these calls.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per lane and
+// group.  The sums of x come from one more product, with ones.
+// Groups of 128: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product:
+// the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7}.
+template <DenseType T, int G, int S, bool Z, int MT, int NW, int U>
+__global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
+    constexpr int GPC = 128 / G, PER = 4 / GPC;                 // groups of a chunk, products of a group
+    __shared__ f32x4_t part[NW][MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane >> 4, r = lane & 15;
+    const int n0 = blockIdx.x * 16, chunks = (a.K + 127) >> 7, words = (a.K + 31) >> 5 << 4;        // (bytes of a row of codes)
+    const auto whole = [](const void *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, DENSE_OUTSIDE, 0x00020000); };
+    const auto read = [](__amdgpu_buffer_rsrc_t b, uint32_t off) { return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0)); };
+    const __amdgpu_buffer_rsrc_t cb = whole(reinterpret_cast<const char *>(a.c) + (int64_t)n0 * a.ldc), xb = whole(a.x);
+    const uint32_t co = n0 + r < a.N ? (uint32_t)(r * a.ldc) + q * 16 : DENSE_OUTSIDE;
+    const int64_t n = min(n0 + r, a.N - 1);
+    uint32_t xo[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xo[t] = t * 16 + r < a.M ? (uint32_t)((t * 16 + r) * a.ldx) : DENSE_OUTSIDE;
+    const uint32_t one2 = T == DENSE_F16 ? 0x3C003C00u : 0x3F803F80u;
+    const u32x4_t ones = {one2, one2, one2, one2};
+    f32x4_t acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c0 = wave; c0 < chunks; c0 += NW * U) {
+        u32x4_t w[U], x[U][MT][4];
+        float s[U][GPC], z[U][GPC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * NW;
+            w[u] = read(cb, c * 64 + q * 16 < words ? co + c * 64 : DENSE_OUTSIDE);
+#pragma unroll
+            for (int i = 0; i < GPC; ++i) {
+                const int g = min(c * GPC + i, a.groups - 1);
+                s[u][i] = int4_scale<T, S>(a.s, n * a.s_n + g * a.s_g);
+                z[u][i] = Z ? -16.0f - (float)a.z[n * a.z_n + g * a.z_g] : -24.0f;
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    const int k = c * 128 + (G == 128 ? q * 32 + p * 8 : p * 32 + q * 8);
+                    x[u][t][p] = read(xb, k < a.K ? xo[t] + 2 * k : DENSE_OUTSIDE);
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * NW;
+            if (c >= chunks) break;
+            if constexpr (G != 128) {                            // word p of lane q <-> word q of lane p
+                const auto l0 = __builtin_amdgcn_permlane16_swap(w[u][0], w[u][1], false, false), l1 = __builtin_amdgcn_permlane16_swap(w[u][2], w[u][3], false, false);
+                const auto h0 = __builtin_amdgcn_permlane32_swap(l0[0], l1[0], false, false), h1 = __builtin_amdgcn_permlane32_swap(l0[1], l1[1], false, false);
+                w[u] = u32x4_t{h0[0], h1[0], h0[1], h1[1]};
+            }
+#pragma unroll
+            for (int i = 0; i < GPC; ++i) {
+                if (c * GPC + i >= a.groups) break;
+                f32x4_t d[MT], e[MT];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) d[t] = e[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int p = i * PER; p < (i + 1) * PER; ++p) {
+                    const uint32_t word = w[u][p];
+                    const u32x4_t f = int4_unpack<T>(word);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        d[t] = dense_mfma<T>(x[u][t][p], f, d[t]);
+                        e[t] = dense_mfma<T>(x[u][t][p], ones, e[t]);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(s[u][i], __builtin_fmaf(z[u][i], e[t][v], d[t][v]), acc[t][v]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    __syncthreads();
+    if (wave >= MT) return;
+    f32x4_t sum = part[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) sum += part[w][wave][lane];
+    if (n0 + r >= a.N) return;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        const int m = wave * 16 + 4 * q + v;
+        if (m < a.M) a.y[m * a.ldy + n0 + r] = (uint16_t)dense_pack2<T>(sum[v], 0.f);
+    }
+}
+
+// ---- many rows -------------------------------------------------------------------------------------------------------
+// What a tile needs of the groups, laid out so that its pieces are whole 16-byte units: sums of x [groups][Mp], scales and 16 + z [groups][Np], zeros beyond M,
+// N and the last group.
+template <DenseType T, int S>
+__global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int group, int groups, float *xs, float *st, float *zt, unsigned x_blocks) {
+    if (blockIdx.x < x_blocks) {                                 // 8 values per thread, the lanes of a group side by side
+        const int per = group / 8;
+        const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / per, m = i / groups;
+        const int g = (int)(i - m * groups), lane = threadIdx.x & (per - 1), k = g * group + lane * 8;
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (m < a.M && k < a.K) dense_unpack8<T>(*reinterpret_cast<const u32x4_t *>(static_cast<const char *>(a.x) + m * a.ldx + (int64_t)k * 2), v);
+        float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+        const auto add = [&](uint32_t other) { sum += __builtin_bit_cast(float, other); };
+        if (per > 8) add(mortar_row_xor<8>(__builtin_bit_cast(uint32_t, sum)));
+        if (per > 4) add(mortar_row_xor<4>(__builtin_bit_cast(uint32_t, sum)));
+        add(mortar_row_xor<2>(__builtin_bit_cast(uint32_t, sum)));
+        add(mortar_row_xor<1>(__builtin_bit_cast(uint32_t, sum)));
+        if (lane == 0 && m < a.Mp) xs[(int64_t)g * a.Mp + m] = sum;
+        return;
+    }
+    const int64_t i = (int64_t)(blockIdx.x - x_blocks) * 256 + threadIdx.x;
+    const int g = (int)(i / a.Np), n = (int)(i - (int64_t)g * a.Np);
+    if (g >= groups) return;
+    const bool on = g < a.groups && n < a.N;
+    st[i] = on ? int4_scale<T, S>(a.s, n * a.s_n + g * a.s_g) : 0.f;
+    if (a.z) zt[i] = on ? 16.0f + (float)a.z[n * a.z_n + g * a.z_g] : 0.f;
+}
+
+// BN features x BM tokens by WN x WM waves, steps of 64 K through a ring of NS slots in LDS filled by asynchronous copies: x in rows of 128 bytes with their
+// units permuted, codes in rows of 32 bytes, and the step's groups: scales, sums of x, 16 + z.  One barrier per step.  A wave makes its weights from
+// the codes in registers.  The first product of a group starts at -(16 + z) sum x instead of 0.
+template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS>
+__global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Args a) {
+    constexpr int NW = WN * WM, FN = BN / WN / 16, FM = BM / WM / 16, GPS = G == 32 ? 2 : 1;
+    constexpr int X = BM * 128, C = BN * 32, GB = (BN + BM + (Z ? BN : 0)) * 4, GC = (GB + 1023) / 1024, SLOT = X + C + GPS * GC * 1024;
+    constexpr int LX = X / 1024 / NW, CC = C / 1024, EXTRA = CC + GPS * GC, LE = (EXTRA + NW - 1) / NW, LEAST = LX + EXTRA / NW;
+    static_assert(X % (1024 * NW) == 0 && C % 1024 == 0, "whole copies");
+    static_assert(FN % 2 == 0, "fragments are joined in pairs");
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane >> 4, r = lane & 15;
+    const int wn = wave % WN, wm = wave / WN;
+    const uint32_t l0 = mortar_lds_addr(lds);
+    // As in the 16-bit products: workgroups of one XCD take a contiguous run of tiles, in bands of 8 along m.
+    const int total = a.tiles_n * a.tiles_m, per_xcd = (total + 7) >> 3, id = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (id >= min(total, (int)((blockIdx.x & 7) + 1) * per_xcd)) return;
+    const int band = id / (8 * a.tiles_n), rest = id - band * 8 * a.tiles_n, bh = min(8, a.tiles_m - band * 8), tn = rest / bh;
+    const int n0 = tn * BN, m0 = (band * 8 + rest - tn * bh) * BM;
+    const int steps = (a.K + 63) >> 6, row_bytes = (a.K + 31) >> 5 << 4;
+
+    // Sources of this lane's copies: offsets that move on with the steps, and where K ends for them.
+    const u32x4_t xbuf = dense_buffer(static_cast<const char *>(a.x) + (int64_t)m0 * a.ldx), cbuf = dense_buffer(reinterpret_cast<const char *>(a.c) + (int64_t)n0 * a.ldc);
+    uint32_t xoff[LX], coff[LE];
+    int kx;
+    {
+        const int u = lane & 7;
+#pragma unroll
+        for (int i = 0; i < LX; ++i) {
+            const int row = (i * NW + wave) * 8 + (lane >> 3);
+            xoff[i] = m0 + row < a.M ? (uint32_t)(row * a.ldx) + (u ^ (row & 7)) * 16 : DENSE_OUTSIDE;
+        }
+        kx = (u ^ ((lane >> 3) & 7)) * 16;                       // (the same in all copies: their rows are 8 apart)
+#pragma unroll
+        for (int i = 0; i < LE; ++i) {
+            const int e = i * NW + wave;                         // copies of codes, then those of the groups
+            const int row = e * 32 + (lane >> 1);
+            coff[i] = e < CC && n0 + row < a.N ? (uint32_t)(row * a.ldc) + (lane & 1) * 16 : DENSE_OUTSIDE;
+        }
+    }
+    const auto copy_step = [&](int k, uint32_t slot) {           // k: the step; beyond the last one it copies zeros
+        const uint32_t base = l0 + slot;
+#pragma unroll
+        for (int i = 0; i < LX; ++i) dense_copy(xbuf, kx + k * 128 < a.K * 2 ? xoff[i] + k * 128 : DENSE_OUTSIDE, base + (i * NW + wave) * 1024);
+#pragma unroll
+        for (int i = 0; i < LE; ++i) {
+            const int e = i * NW + wave;
+            if (e < CC) {
+                dense_copy(cbuf, (lane & 1) * 16 + k * 32 < row_bytes ? coff[i] + k * 32 : DENSE_OUTSIDE, base + X + e * 1024);
+            } else if (e < EXTRA) {
+                const int gc = e - CC, gi = gc / GC, at = (gc - gi * GC) * 256 + lane * 4;      // float of the group's piece: scales, sums, zero points
+                const int64_t g = k < steps ? (G == 128 ? k >> 1 : G == 64 ? k : 2 * k + gi) : 0;
+                const float *src = at < BN ? a.st + g * a.Np + n0 + at : at < BN + BM || !Z ? a.xs + g * a.Mp + m0 + min(at - BN, BM - 4) : a.zt + g * a.Np + n0 + min(at - BN - BM, BN - 4);
+                mortar_load_to_lds(reinterpret_cast<const MORTAR_GLOBAL char *>(reinterpret_cast<uintptr_t>(src)), base + X + C + gc * 1024);
+            }
+        }
+    };
+    const uint32_t ax = l0 + dense_row_addr(wm * FM * 16, lane), ac = l0 + X + (wn * FN * 16 + r) * 32 + q * 4, ag = l0 + X + C;
+
+    f32x4_t acc[FN][FM], part[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = part[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) copy_step(i, i * SLOT);
+    uint32_t slot = 0, free_slot = (NS - 1) * SLOT;
+    // first / last: the step begins / ends a group (groups of 128: two steps)
+    const auto step = [&](int k, auto first, auto last) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * LEAST) : "memory");
+        copy_step(k + NS - 1, free_slot);
+        const uint32_t ga = ag + slot;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t gt = ga + (GPS == 2 ? t * GC * 1024 : 0);
+            u32x4_t xf[FM], wf[FN];
+#pragma unroll
+            for (int i = 0; i < FN; ++i) wf[i] = int4_unpack<T>(*(const MORTAR_LDS uint32_t *)(uintptr_t)(ac + slot + i * 512 + t * 16));
+#pragma unroll
+            for (int j = 0; j < FM; ++j) xf[j] = dense_read(((ax + slot) ^ (t * 64)) + j * 2048);
+            const bool begin = GPS == 2 || (first.value && t == 0), end = GPS == 2 || (last.value && t == 1);
+            if (begin) {
+                float sx[FM];
+#pragma unroll
+                for (int j = 0; j < FM; ++j) sx[j] = *(const MORTAR_LDS float *)(uintptr_t)(gt + (BN + (wm * FM + j) * 16 + r) * 4);
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    f32x4_t zv = {24.f, 24.f, 24.f, 24.f};
+                    if constexpr (Z) zv = *(const MORTAR_LDS f32x4_t *)(uintptr_t)(gt + (BN + BM + (wn * FN + i) * 16 + 4 * q) * 4);
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) {
+                        f32x4_t c;
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) c[v] = -zv[v] * sx[j];
+                        part[i][j] = dense_mfma<T>(wf[i], xf[j], c);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < FN; ++i)
+#pragma unroll
+                    for (int j = 0; j < FM; ++j) part[i][j] = dense_mfma<T>(wf[i], xf[j], part[i][j]);
+            }
+            if (end) {
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    const f32x4_t sv = *(const MORTAR_LDS f32x4_t *)(uintptr_t)(gt + ((wn * FN + i) * 16 + 4 * q) * 4);
+#pragma unroll
+                    for (int j = 0; j < FM; ++j)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) acc[i][j][v] = __builtin_fmaf(sv[v], part[i][j][v], acc[i][j][v]);
+                }
+            }
+        }
+        free_slot = slot;
+        slot = slot + SLOT == NS * SLOT ? 0u : slot + SLOT;
+    };
+    if constexpr (G == 128) {
+        int k = 0;
+        for (; k + 1 < steps; k += 2) {
+            step(k, Const<1>{}, Const<0>{});
+            step(k + 1, Const<0>{}, Const<1>{});
+        }
+        if (k < steps) step(k, Const<1>{}, Const<1>{});
+    } else {
+        for (int k = 0; k < steps; ++k) step(k, Const<1>{}, Const<1>{});
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (the copies of the steps behind the last)
+
+    const bool vector = a.ldy % 8 == 0 && a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
+#pragma unroll
+    for (int j = 0; j < FM; ++j) {
+        const int64_t m = m0 + (wm * FM + j) * 16 + r;
+        if (m >= a.M) continue;
+#pragma unroll
+        for (int i = 0; i < FN; i += 2) {
+            float d[8];
+            dense_join8(acc[i][j], acc[i + 1][j], d);
+            const int n = n0 + (wn * FN + i) * 16 + dense_lane_n(lane);
+            if (n >= a.N) continue;
+            uint16_t *o = a.y + m * a.ldy + n;
+            if (vector) {
+                *reinterpret_cast<u32x4_t *>(o) = dense_pack8<T>(d);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 8; ++v)
+                    if (n + v < a.N) o[v] = (uint16_t)dense_pack2<T>(d[v], 0.f);
+            }
+        }
+    }
+}
+
+// ---- quantising ------------------------------------------------------------------------------------------------------
+template <int TYPE>
+__device__ __forceinline__ float int4_read(const void *p, int64_t i) {
+    if constexpr (TYPE == MORTAR_FP32) return static_cast<const float *>(p)[i];
+    else if constexpr (TYPE == MORTAR_FP16) return (float)static_cast<const _Float16 *>(p)[i];
+    else return bf16_to_f32(static_cast<const uint16_t *>(p)[i]);
+}
+// 8 values per thread, the lanes of a group side by side (16 of them at most: within a row of lanes).
+template <int TYPE, int STYPE>
+__global__ __launch_bounds__(256) void int4_quantize_kernel(const void *w, int32_t N, int32_t K, int64_t ldw, int group, uint32_t *c, int64_t ldc, void *s, int64_t s_n,
+                                                            int64_t s_g, uint8_t *z, int64_t z_n, int64_t z_g) {
+    const int per = group / 8, groups = (K + group - 1) / group, words = (K + 31) / 32 * 4;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / per, n = i / groups;
+    if (n >= N) return;                                          // (whole groups of lanes)
+    const int g = (int)(i - n * groups), lane = threadIdx.x & (per - 1), k = g * group + lane * 8;
+    float v[8], lo = 0.f, hi = 0.f;
+    uint32_t bad = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] = k + j < K ? int4_read<TYPE>(w, n * ldw + k + j) : 0.f;
+        lo = fminf(lo, v[j]);
+        hi = fmaxf(hi, v[j]);
+        bad |= !(__builtin_fabsf(v[j]) < __builtin_inff());
+    }
+    const auto join = [&](auto x) {
+        constexpr int X = decltype(x)::value;
+        lo = fminf(lo, __builtin_bit_cast(float, mortar_row_xor<X>(__builtin_bit_cast(uint32_t, lo))));
+        hi = fmaxf(hi, __builtin_bit_cast(float, mortar_row_xor<X>(__builtin_bit_cast(uint32_t, hi))));
+        bad |= mortar_row_xor<X>(bad);            // (with every lane: no shortcut)
+    };
+    if (per > 8) join(Const<8>{});
+    if (per > 4) join(Const<4>{});
+    join(Const<2>{});
+    join(Const<1>{});
+    float sc = z ? (hi - lo) / 15.0f : fmaxf(hi / 7.0f, lo / -8.0f);
+    if (bad) sc = __builtin_nanf("");
+    if constexpr (STYPE == MORTAR_FP16) sc = (float)(_Float16)sc;
+    else if constexpr (STYPE == MORTAR_BF16) sc = bf16r(sc);
+    if (sc == 0.f) sc = 1.0f;
+    const float zero = z ? fminf(fmaxf(rintf(-lo / sc), 0.f), 15.f) : 8.0f;
+    uint32_t word = 0;
+    constexpr int place[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float code = k + j < K ? fminf(fmaxf(rintf(v[j] / sc) + zero, 0.f), 15.f) : 8.0f;
+        word |= (uint32_t)code << 4 * place[j];
+    }
+    if (k / 8 < words) c[n * ldc + k / 8] = word;
+    if (lane) return;
+    if constexpr (STYPE == MORTAR_FP32) static_cast<float *>(s)[n * s_n + g * s_g] = sc;
+    else if constexpr (STYPE == MORTAR_FP16) static_cast<_Float16 *>(s)[n * s_n + g * s_g] = (_Float16)sc;
+    else static_cast<uint16_t *>(s)[n * s_n + g * s_g] = (uint16_t)bf16_bits_rne(sc);
+    if (z) z[n * z_n + g * z_g] = (uint8_t)zero;
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+
+int launch_error(const char *what) {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? MORTAR_OK : mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+constexpr int FEW_ROWS = 32;
+bool few_rows(int64_t M) { return M <= FEW_ROWS; }
+int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
+int64_t groups_padded(int64_t K, int group) { return group == 32 ? (K + 63) / 64 * 2 : (K + group - 1) / group; }
+
+template <DenseType T, int G, int S, bool Z>
+int launch_few(const Int4Args &a, hipStream_t st, const char *what) {
+    const dim3 grid((unsigned)((a.N + 15) / 16));
+    if (a.M <= 16) hipLaunchKernelGGL((int4_few_kernel<T, G, S, Z, 1, 16, 2>), grid, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((int4_few_kernel<T, G, S, Z, 2, 16, 1>), grid, dim3(1024), 0, st, a);
+    return launch_error(what);
+}
+
+template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS>
+int launch_tile_form(Int4Args a, hipStream_t st, const char *what) {
+    const auto kern = int4_tile_kernel<T, G, Z, BN, BM, WN, WM, NS>;
+    constexpr int smem = NS * (BM * 128 + BN * 32 + (G == 32 ? 2 : 1) * (((BN + BM + (Z ? BN : 0)) * 4 + 1023) / 1024) * 1024);
+    static_assert(smem * 2 <= 160 * 1024, "two workgroups per CU");
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    const int64_t tn = ((int64_t)a.N + BN - 1) / BN, tm = ((int64_t)a.M + BM - 1) / BM;
+    if (tn * tm > 1 << 22) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tiles", what);
+    a.tiles_n = (int)tn;
+    a.tiles_m = (int)tm;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(8 * ((tn * tm + 7) / 8))), dim3(WN * WM * 64), smem, st, a);
+    return launch_error(what);
+}
+
+template <DenseType T, int G, int S, bool Z>
+int launch_many(Int4Args a, float *ws, hipStream_t st, const char *what) {
+    const int64_t groups = groups_padded(a.K, G);
+    a.Mp = (int32_t)up128(a.M);
+    a.Np = (int32_t)up128(a.N);
+    float *xs = ws, *s = xs + groups * a.Mp, *zt = Z ? s + groups * a.Np : nullptr;
+    a.xs = xs; a.st = s; a.zt = zt;
+    const int64_t x_blocks = (groups * a.Mp * (G / 8) + 255) / 256, n_blocks = (groups * a.Np + 255) / 256;
+    if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
+    hipLaunchKernelGGL((int4_prepare_kernel<T, S>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, G, (int)groups, xs, s, zt, (unsigned)x_blocks);
+    if (const int rc = launch_error(what)) return rc;
+    return launch_tile_form<T, G, Z, 128, 128, 2, 2, 3>(a, st, what);
+}
+
+template <DenseType T, int G, int S, bool Z>
+int launch_last(const Int4Args &a, float *ws, hipStream_t st, const char *what) {
+    return few_rows(a.M) ? launch_few<T, G, S, Z>(a, st, what) : launch_many<T, G, S, Z>(a, ws, st, what);
+}
+template <DenseType T, int G, int S>
+int launch_zeros(const Int4Args &a, float *ws, hipStream_t st, const char *what) {
+    return a.z ? launch_last<T, G, S, true>(a, ws, st, what) : launch_last<T, G, S, false>(a, ws, st, what);
+}
+template <DenseType T, int G>
+int launch_scales(const Int4Args &a, bool s32, float *ws, hipStream_t st, const char *what) {
+    return s32 ? launch_zeros<T, G, 4>(a, ws, st, what) : launch_zeros<T, G, 2>(a, ws, st, what);
+}
+template <DenseType T>
+int launch_group(const Int4Args &a, int group, bool s32, float *ws, hipStream_t st, const char *what) {
+    return group == 32 ? launch_scales<T, 32>(a, s32, ws, st, what) : group == 64 ? launch_scales<T, 64>(a, s32, ws, st, what) : launch_scales<T, 128>(a, s32, ws, st, what);
+}
+
+int check_group(const char *what, int group) {
+    return group == 32 || group == 64 || group == 128 ? MORTAR_OK : mortar_fail(MORTAR_ERR_ARG, "%s: groups of 32, 64 or 128 values", what);
+}
+bool known(int32_t type) { return type == MORTAR_BF16 || type == MORTAR_FP16 || type == MORTAR_FP32; }
+int check_codes(const char *what, const void *c, int64_t K, int64_t ldc) {
+    if (!c) return mortar_fail(MORTAR_ERR_ARG, "%s: the codes are null", what);
+    if (ldc % 4 || ldc < (K + 31) / 32 * 4 || (reinterpret_cast<uintptr_t>(c) & 15)) return mortar_fail(MORTAR_ERR_ARG, "%s: the codes need whole rows of 32 values on 16-byte addresses", what);
+    if (128 * ldc * 4 >= (int64_t)DENSE_OUTSIDE) return mortar_fail(MORTAR_ERR_LIMIT, "%s: the rows of codes are too far apart", what);
+    return MORTAR_OK;
+}
+#define CHECK(...) do { const int rc_ = (__VA_ARGS__); if (rc_) return rc_; } while (0)
+
+}  // namespace
+
+extern "C" int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t ldw, int32_t type, int32_t group, uint32_t *c, int64_t ldc, void *s, int32_t s_type,
+                                    int64_t s_n, int64_t s_g, uint8_t *z, int64_t z_n, int64_t z_g, void *stream) {
+    const char *what = "int4_quantize";
+    if (N <= 0 || K <= 0 || !known(type) || !known(s_type)) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape or type", what);
+    CHECK(check_group(what, group));
+    CHECK(check_codes(what, c, K, ldc));
+    if (!w || !s || ldw < K) return mortar_fail(MORTAR_ERR_ARG, "%s: w or s is null, or rows overlap", what);
+    const int64_t threads = (int64_t)N * ((K + group - 1) / group) * (group / 8);
+    if (threads >= INT64_C(1) << 32) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const auto launch = [&](auto t, auto u) {
+        hipLaunchKernelGGL((int4_quantize_kernel<decltype(t)::value, decltype(u)::value>), grid, dim3(256), 0, st, w, N, K, ldw, group, c, ldc, s, s_n, s_g, z, z_n, z_g);
+        return launch_error(what);
+    };
+    const auto scales = [&](auto t) {
+        return s_type == MORTAR_FP32 ? launch(t, Const<MORTAR_FP32>{}) : s_type == MORTAR_FP16 ? launch(t, Const<MORTAR_FP16>{}) : launch(t, Const<MORTAR_BF16>{});
+    };
+    return type == MORTAR_FP32 ? scales(Const<MORTAR_FP32>{}) : type == MORTAR_FP16 ? scales(Const<MORTAR_FP16>{}) : scales(Const<MORTAR_BF16>{});
+}
+
+extern "C" int64_t mortar_int4_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t group) {
+    if (M <= 0 || N <= 0 || K <= 0 || group < 32 || few_rows(M)) return 0;
+    return 4 * groups_padded(K, group) * (up128(M) + 2 * up128(N));
+}
+
+extern "C" int mortar_int4_linear(const void *x, int64_t M, int32_t K, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group, const void *s,
+                                  int32_t s_type, int64_t s_n, int64_t s_g, const uint8_t *z, int64_t z_n, int64_t z_g, void *y, int64_t ldy, void *workspace,
+                                  void *stream) {
+    const char *what = "int4_linear";
+    if (M < 0 || K <= 0 || N <= 0) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
+    if (type != MORTAR_BF16 && type != MORTAR_FP16) return mortar_fail(MORTAR_ERR_ARG, "%s: bf16 or fp16", what);
+    if (s_type != type && s_type != MORTAR_FP32) return mortar_fail(MORTAR_ERR_ARG, "%s: scales in the type of x or fp32", what);
+    CHECK(check_group(what, group));
+    if (M == 0) return MORTAR_OK;
+    CHECK(check_codes(what, c, K, ldc));
+    if (!x || K % 8 || ldx % 8 || (M > 1 && ldx < K) || (reinterpret_cast<uintptr_t>(x) & 15)) return mortar_fail(MORTAR_ERR_ARG, "%s: x needs rows of a multiple of 8 values on 16-byte addresses", what);
+    if (!s || !y || ldy < N || (reinterpret_cast<uintptr_t>(y) & 1)) return mortar_fail(MORTAR_ERR_ARG, "%s: s or y is null, or rows of y overlap", what);
+    if (s_n < 0 || s_g < 0 || z_n < 0 || z_g < 0) return mortar_fail(MORTAR_ERR_ARG, "%s: negative strides", what);
+    if (128 * ldx * 2 >= (int64_t)DENSE_OUTSIDE || K >= 1 << 28) return mortar_fail(MORTAR_ERR_LIMIT, "%s: the rows of x are too far apart", what);
+    if (M >= INT32_MAX / 2 || N >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many rows or columns", what);
+    if (mortar_int4_workspace_bytes(M, N, K, group) && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return mortar_fail(MORTAR_ERR_ARG, "%s: this shape needs a workspace", what);
+    Int4Args a{};
+    a.x = x; a.ldx = ldx * 2; a.c = c; a.ldc = ldc * 4;
+    a.s = s; a.s_n = s_n; a.s_g = s_g; a.z = z; a.z_n = z_n; a.z_g = z_g;
+    a.y = static_cast<uint16_t *>(y); a.ldy = ldy;
+    a.M = (int32_t)M; a.N = N; a.K = K; a.groups = (K + group - 1) / group;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    float *ws = static_cast<float *>(workspace);
+    return type == MORTAR_BF16 ? launch_group<DENSE_BF16>(a, group, s_type == MORTAR_FP32, ws, st, what) : launch_group<DENSE_F16>(a, group, s_type == MORTAR_FP32, ws, st, what);
+}

@@ -1,96 +1,9 @@
-// Native calls of the dense operators: LayerNorm and the dense SwiGLU MLP with their autograd nodes, and the 8-bit dense layer.
+// Native calls of the dense operators: LayerNorm and the dense SwiGLU MLP with their autograd nodes, and the dense layers in 8 and 4 bits.
 // One Python call each: checks, allocation, stream, launches.  Unlike the calls of mortar_torch.cpp these have no general path behind
 // them: what they do not take they refuse, with the error worded here.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
-
-#include <algorithm>
-
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/GradMode.h>
-#include <c10/core/impl/LocalDispatchKeySet.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/python_variable.h>
-
-#include "../../include/mortar_hip.h"
+#include "mortar_torch_args.h"
 
 namespace {
-
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-void *stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-void check_rc(int rc, const char *what) {
-    if (rc == MORTAR_OK) return;
-    TORCH_CHECK(rc != MORTAR_ERR_HIP, what, " failed (", rc, "): ", mortar_last_error());
-    TORCH_CHECK_VALUE(false, what, " failed (", rc, "): ", mortar_last_error());
-}
-
-// Kinds of tensors whose values a kernel launched on their address would miss.
-c10::DispatchKeySet riders() {
-    using K = c10::DispatchKey;
-    return c10::DispatchKeySet({K::Python, K::PythonTLSSnapshot, K::FuncTorchGradWrapper, K::FuncTorchBatched, K::FuncTorchDynamicLayerFrontMode,
-                                K::FuncTorchDynamicLayerBackMode, K::Batched, K::Functionalize, K::Conjugate, K::Negative, K::ZeroTensor, K::Tracer});
-}
-
-bool plain_values(const at::Tensor &t) { return !t.key_set().has_any(riders()) && t.layout() == at::kStrided; }
-bool plain(const at::Tensor &t) { return !c10::impl::tls_local_dispatch_key_set().included_.has_any(riders()) && plain_values(t); }
-
-// Argument `name` as a plain tensor on the GPU.
-const at::Tensor &tensor_arg(PyObject *o, const char *what, const char *name) {
-    TORCH_CHECK_TYPE(THPVariable_CheckExact(o) || THPVariable_Check(o), what, ": ", name, " must be a tensor");
-    const at::Tensor &t = THPVariable_Unpack(o);
-    TORCH_CHECK(plain(t), what, ": ", name, " must be a plain strided tensor, outside functional transforms and tracing");
-    TORCH_CHECK(t.is_cuda(), what, ": tensor must live on a ROCm device (the MORTAR runtime has no CPU path)");
-    TORCH_CHECK(!t._fw_grad(0).defined(), what, ": no forward-mode gradients");
-    return t;
-}
-at::Tensor optional_arg(PyObject *o, const char *what, const char *name) { return o == Py_None ? at::Tensor() : tensor_arg(o, what, name); }
-
-void same_device(const at::Tensor &a, const at::Tensor &b, const char *what, const char *name) {
-    TORCH_CHECK_VALUE(a.device() == b.device(), what, ": ", name, " is on ", b.device(), ", x on ", a.device());
-}
-
-int type_code(at::ScalarType t) { return t == at::kBFloat16 ? MORTAR_BF16 : t == at::kHalf ? MORTAR_FP16 : t == at::kFloat ? MORTAR_FP32 : -1; }
-
-// t [..., d] as rows [M, d] that the kernels can read: `unit` values per 16 bytes, tiles: 256 rows within 2 GiB; copied where strides or
-// address do not allow it.
-at::Tensor rows_of(const at::Tensor &t, int64_t d, int64_t unit, bool tiles = true) {
-    at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, d});
-    const bool one = r.size(0) <= 1;
-    if ((d > 1 && r.stride(1) != 1) || (!one && (r.stride(0) % unit || r.stride(0) < d || (tiles && r.stride(0) * 256 * r.element_size() >= INT64_C(1) << 31))) ||
-        !aligned16(r.const_data_ptr()))
-        r = r.clone(at::MemoryFormat::Contiguous);
-    return r;
-}
-int64_t ld_of(const at::Tensor &r) { return r.size(0) <= 1 ? r.size(1) : r.stride(0); }
-
-at::Tensor empty_like_rows(const at::Tensor &like, at::IntArrayRef shape) { return at::empty(shape, like.options().requires_grad(false)); }
-at::Tensor empty_bytes(const at::Tensor &like, int64_t n) { return at::empty({n}, like.options().dtype(at::kByte).requires_grad(false)); }
-float *floats(const at::Tensor &t) { return t.defined() ? static_cast<float *>(t.data_ptr()) : nullptr; }
-const void *data(const at::Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
-void *mut(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-// The gradient of a result as the backward reads it: values as they lie in memory, once.
-at::Tensor plain_gradient(const at::Tensor &dy, const char *what) {
-    TORCH_CHECK(!c10::GradMode::is_enabled(), what, ": its gradients cannot be differentiated again (create_graph=True)");
-    if (!dy.defined()) return dy;
-    const at::Tensor g = dy.resolve_neg();                 // (the imaginary part of a conjugate is negated lazily)
-    TORCH_CHECK(plain_values(g), what, ": its gradient must be a plain strided tensor");
-    return g;
-}
-
-// A tensor kept from the forward, as it comes back: saved-tensor hooks may have brought it to another place and other strides, and no further.
-const at::Tensor &kept(const at::Tensor &t, const at::Tensor &dy, at::IntArrayRef sizes, at::ScalarType type, const char *what) {
-    TORCH_CHECK(t.defined() && plain_values(t) && t.device() == dy.device() && t.scalar_type() == type && t.sizes() == sizes, what,
-                ": a tensor that was saved for the backward came back with another shape, type or device");
-    return t;
-}
 
 // ---- LayerNorm -------------------------------------------------------------------------------------------------------
 
@@ -337,8 +250,8 @@ PyObject *py_dense_mlp_covers(PyObject *, PyObject *const *a, Py_ssize_t na) {
 
 // ---- 8 bits ----------------------------------------------------------------------------------------------------------
 
-void no_gradients(const at::Tensor &t, const char *what) {
-    TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), what, ": no gradients flow through 8-bit values (detach the input or call under no_grad)");
+void no_gradients(const at::Tensor &t, const char *what, const char *values = "8-bit") {
+    TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), what, ": no gradients flow through ", values, " values (detach the input or call under no_grad)");
 }
 void check_k(int64_t K, const char *what) { TORCH_CHECK_VALUE(K > 0 && K % 16 == 0 && K < (1 << 28), what, ": in_features must be a positive multiple of 16, got ", K); }
 
@@ -455,20 +368,94 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *a, Py_ssize_t na) {
     return THPVariable_Wrap(std::move(y));
 }
 
-template <PyObject *(*F)(PyObject *, PyObject *const *, Py_ssize_t)>
-PyObject *guarded(PyObject *self, PyObject *const *a, Py_ssize_t na) {
-    HANDLE_TH_ERRORS
-    return F(self, a, na);
-    END_HANDLE_TH_ERRORS
+// ---- 4 bits ----------------------------------------------------------------------------------------------------------
+
+int group_arg(PyObject *o, const char *what) {
+    const long g = PyLong_AsLong(o);
+    if (g == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK_VALUE(g == 32 || g == 64 || g == 128, what, ": group_size must be 32, 64 or 128, got ", g);
+    return (int)g;
+}
+int64_t groups_of(int64_t K, int group) { return (K + group - 1) / group; }
+
+// quantize_int4_weight(w, group_size, zero_points) -> (codes int32 [N, 4 ceil(K / 32)], scales [N, groups], zeros uint8 [N, groups] or None); scales
+// in the type of w, consecutive along the rows
+PyObject *py_quantize_int4_weight(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    const char *what = "quantize_int4_weight";
+    TORCH_CHECK_TYPE(na == 3, "quantize_int4_weight: 3 arguments");
+    const at::Tensor w = tensor_arg(a[0], what, "w");
+    const int group = group_arg(a[1], what), with_zeros = PyObject_IsTrue(a[2]);
+    if (with_zeros < 0) throw python_error();
+    TORCH_CHECK_TYPE(type_code(w.scalar_type()) >= 0, what, ": expected bfloat16, float16 or float32, got ", w.scalar_type());
+    TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) > 0 && w.size(1) > 0, what, ": expected a matrix [out_features, in_features]");
+    no_gradients(w, what, "quantised");
+    const int64_t N = w.size(0), K = w.size(1), groups = groups_of(K, group), words = (K + 31) / 32 * 4;
+    TORCH_CHECK_VALUE(N < (1 << 24) && K < (1 << 28), what, ": too many rows or columns");
+    const c10::DeviceGuard guard(w.device());
+    const at::Tensor r = (K > 1 && w.stride(1) != 1) || (N > 1 && w.stride(0) < K) ? w.clone(at::MemoryFormat::Contiguous) : w;
+    const auto options = w.options().requires_grad(false);
+    at::Tensor c = at::empty({N, words}, options.dtype(at::kInt)), s = at::empty({groups, N}, options).t();
+    at::Tensor z = with_zeros ? at::empty({groups, N}, options.dtype(at::kByte)).t() : at::Tensor();
+    const int type = type_code(w.scalar_type());
+    check_rc(mortar_int4_quantize(data(r), (int32_t)N, (int32_t)K, N > 1 ? r.stride(0) : K, type, group, static_cast<uint32_t *>(mut(c)), words, mut(s), type, s.stride(0),
+                                  s.stride(1), static_cast<uint8_t *>(mut(z)), 1, N, stream_of(w)),
+             "mortar_int4_quantize");
+    PyObject *pz = Py_None;
+    if (with_zeros) pz = THPVariable_Wrap(std::move(z));
+    else Py_INCREF(pz);
+    PyObject *pc = THPVariable_Wrap(std::move(c)), *ps = THPVariable_Wrap(std::move(s));
+    return Py_BuildValue("(NNN)", pc, ps, pz);
 }
 
-#define MORTAR_METHOD(name, f, doc) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<f>)), METH_FASTCALL, doc}
+// linear_int4(x, codes, scales, zeros, group_size) -> y [..., N] in the type of x
+PyObject *py_linear_int4(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    const char *what = "linear_int4";
+    TORCH_CHECK_TYPE(na == 5, "linear_int4: 5 arguments");
+    const at::Tensor x = tensor_arg(a[0], what, "x"), c = tensor_arg(a[1], what, "codes"), s = tensor_arg(a[2], what, "scales"), z = optional_arg(a[3], what, "zeros");
+    const int group = group_arg(a[4], what);
+    TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, what, ": expected bfloat16 or float16, got ", x.scalar_type());
+    TORCH_CHECK_TYPE(c.scalar_type() == at::kInt, what, ": codes must be int32");
+    TORCH_CHECK_TYPE(s.scalar_type() == x.scalar_type() || s.scalar_type() == at::kFloat, what, ": scales must have the type of x or float32");
+    TORCH_CHECK_TYPE(!z.defined() || z.scalar_type() == at::kByte, what, ": zeros must be uint8");
+    no_gradients(x, what, "4-bit");
+    no_gradients(s, what, "4-bit");
+    same_device(x, c, what, "codes");
+    same_device(x, s, what, "scales");
+    if (z.defined()) same_device(x, z, what, "zeros");
+    TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) < (1 << 28), what, ": expected a tensor [..., K] with K > 0");
+    const int64_t K = x.size(-1), words = (K + 31) / 32 * 4, groups = groups_of(K, group), M = x.numel() / K;
+    TORCH_CHECK_VALUE(c.dim() == 2 && c.size(0) > 0 && c.size(1) == words, what, ": codes must be [out_features, ", words, "] for ", K, " features, got ", c.sizes());
+    const int64_t N = c.size(0);
+    TORCH_CHECK_VALUE(N < (1 << 24), what, ": too many rows of codes");
+    TORCH_CHECK_VALUE(s.dim() == 2 && s.size(0) == N && s.size(1) == groups, what, ": scales must be [", N, ", ", groups, "], got ", s.sizes());
+    TORCH_CHECK_VALUE(!z.defined() || z.sizes() == s.sizes(), what, ": zeros must be [", N, ", ", groups, "], got ", z.sizes());
+    TORCH_CHECK_VALUE(c.stride(1) == 1 && (N == 1 || (c.stride(0) % 4 == 0 && c.stride(0) >= words)) && aligned16(c.const_data_ptr()), what,
+                      ": the rows of codes must be contiguous and 16-byte aligned");
+    TORCH_CHECK_VALUE(M < (1 << 30), what, ": too many rows");
+    const c10::DeviceGuard guard(x.device());
+    at::DimVector shape(x.sizes());
+    shape.back() = N;
+    at::Tensor y = at::empty(shape, x.options().requires_grad(false));
+    if (M) {
+        const at::Tensor r = K % 8 ? at::constant_pad_nd(x.reshape({M, K}), {0, 8 - K % 8}) : rows_of(x, K, 8);
+        const int64_t n = mortar_int4_workspace_bytes(M, N, r.size(1), group);
+        const at::Tensor ws = n ? empty_bytes(x, n) : at::Tensor();
+        check_rc(mortar_int4_linear(data(r), M, (int32_t)r.size(1), ld_of(r), type_code(x.scalar_type()), static_cast<const uint32_t *>(data(c)), N > 1 ? c.stride(0) : words,
+                                    (int32_t)N, group, data(s), type_code(s.scalar_type()), s.stride(0), s.stride(1), static_cast<const uint8_t *>(data(z)),
+                                    z.defined() ? z.stride(0) : 0, z.defined() ? z.stride(1) : 0, mut(y), N, mut(ws), stream_of(x)),
+                 "mortar_int4_linear");
+    }
+    return THPVariable_Wrap(std::move(y));
+}
+
 PyMethodDef methods[] = {MORTAR_METHOD("layernorm", py_layernorm, "LayerNorm of the rows of x, with its autograd node."),
                          MORTAR_METHOD("dense_mlp", py_dense_mlp, "The dense SwiGLU MLP of the rows of x, with its autograd node."),
                          MORTAR_METHOD("dense_mlp_covers", py_dense_mlp_covers, "Whether dense_mlp takes these tensors."),
                          MORTAR_METHOD("quantize_fp8", py_quantize_fp8, "e4m3 codes and scales of activations."),
                          MORTAR_METHOD("quantize_fp8_weight", py_quantize_fp8_weight, "e4m3 codes and block scales of a weight."),
                          MORTAR_METHOD("linear_fp8", py_linear_fp8, "x W^T in e4m3."),
+                         MORTAR_METHOD("quantize_int4_weight", py_quantize_int4_weight, "4-bit codes, scales and zero points of a weight."),
+                         MORTAR_METHOD("linear_int4", py_linear_int4, "x W^T from 4-bit codes."),
                          {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

@@ -1,0 +1,327 @@
+// Native calls around the products of a training step: the norm of many gradients and their clipping, tokens to their experts' rows and back with
+// the autograd nodes.  As in mortar_torch_dense.cpp one Python call each, and what they do not take they refuse.
+#include "mortar_torch_args.h"
+
+#include <vector>
+
+#include <ATen/MemoryOverlap.h>
+#include <torch/csrc/utils/object_ptr.h>
+
+namespace {
+
+// ---- gradients -------------------------------------------------------------------------------------------------------
+
+std::vector<at::Tensor> tensor_list(PyObject *o, const char *what, const char *name) {
+    if (THPVariable_Check(o)) return {tensor_arg(o, what, name)};
+    THPObjectPtr owned(PySequence_Fast(o, "expected a sequence of tensors"));
+    PyObject *fast = owned.get();
+    if (!fast) throw python_error();
+    std::vector<at::Tensor> v;
+    v.reserve(PySequence_Fast_GET_SIZE(fast));
+    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(fast); ++i) v.push_back(tensor_arg(PySequence_Fast_GET_ITEM(fast, i), what, name));
+    return v;
+}
+
+void check_grads(const std::vector<at::Tensor> &v, const char *what) {
+    for (const at::Tensor &t : v) {
+        TORCH_CHECK_TYPE(type_code(t.scalar_type()) >= 0, what, ": expected bfloat16, float16 or float32 gradients, got ", t.scalar_type());
+        TORCH_CHECK_VALUE(t.device() == v[0].device(), what, ": gradients on ", t.device(), " and on ", v[0].device());
+        TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), what, ": no gradients flow through this call (detach the tensors or call under no_grad)");
+    }
+}
+
+// Memory of a tensor, from its first value to behind its last, and what happens to it while the kernels run.
+struct Span {
+    uintptr_t begin, end;
+    size_t i;
+    bool written;
+};
+
+// Nothing that is written is written twice, or read for another tensor.  drop: a gradient that is there twice is counted once (in place).
+void check_overlap(std::vector<mortar_grad_t> &list, std::vector<Span> spans, bool drop, const char *what) {
+    const auto size = [](int type) { return type == MORTAR_FP32 ? 4 : 2; };
+    for (size_t i = 0; i < list.size(); ++i) {
+        const mortar_grad_t &g = list[i];
+        if (!g.n) continue;
+        const uintptr_t s = reinterpret_cast<uintptr_t>(g.src), d = reinterpret_cast<uintptr_t>(g.dst);
+        spans.push_back({d, d + g.n * size(g.out_type), i, true});
+        if (s != d || g.type != g.out_type) spans.push_back({s, s + g.n * size(g.type), i, false});
+    }
+    const auto less = [](const Span &a, const Span &b) { return a.begin < b.begin; };
+    if (!std::is_sorted(spans.begin(), spans.end(), less)) std::stable_sort(spans.begin(), spans.end(), less);
+    uintptr_t any = 0, written = 0;
+    const Span *last = nullptr;                      // written
+    for (const Span &s : spans) {
+        if (drop && last && s.written && s.begin == last->begin && s.end == last->end && list[s.i].type == list[last->i].type) {
+            list[s.i].n = 0;
+            continue;
+        }
+        TORCH_CHECK_VALUE(s.begin >= (s.written ? any : written), what, ": results overlap each other or another gradient");
+        any = std::max(any, s.end);
+        if (s.written) written = std::max(written, s.end), last = &s;
+    }
+}
+
+PyObject *empty_norm() {
+    at::Tensor zero = at::zeros({}, at::TensorOptions().dtype(at::kFloat));
+    return THPVariable_Wrap(std::move(zero));
+}
+
+// grad_norm(grads, largest) -> fp32 []
+PyObject *py_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    const char *what = "grad_norm";
+    TORCH_CHECK_TYPE(na == 2, "grad_norm: 2 arguments");
+    const std::vector<at::Tensor> grads = tensor_list(a[0], what, "each gradient");
+    check_grads(grads, what);
+    if (grads.empty()) return empty_norm();
+    const c10::DeviceGuard guard(grads[0].device());
+    std::vector<at::Tensor> held;
+    std::vector<mortar_grad_t> list;
+    list.reserve(grads.size());
+    for (const at::Tensor &g : grads) {
+        if (!g.is_non_overlapping_and_dense()) held.push_back(g.contiguous());
+        list.push_back({data(g.is_non_overlapping_and_dense() ? g : held.back()), nullptr, g.numel(), type_code(g.scalar_type()), 0});
+    }
+    at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+    const at::Tensor ws = empty_bytes(norm, std::max<int64_t>(8, mortar_grad_workspace_bytes(list.data(), (int64_t)list.size())));
+    check_rc(mortar_grad_norm(list.data(), (int64_t)list.size(), a[1] == Py_True, floats(norm), mut(ws), stream_of(norm)), "mortar_grad_norm");
+    return THPVariable_Wrap(std::move(norm));
+}
+
+// grad_clip(grads, out, max_norm, largest) -> (results, norm fp32 []); out: a sequence of tensors, None (new ones) or True (in place, a gradient that is
+// there twice counts once)
+PyObject *py_grad_clip(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    const char *what = "clip_grads";
+    TORCH_CHECK_TYPE(na == 4, "grad_clip: 4 arguments");
+    const std::vector<at::Tensor> grads = tensor_list(a[0], what, "each gradient");
+    const bool in_place = a[1] == Py_True, fresh = a[1] == Py_None;
+    std::vector<at::Tensor> out = in_place ? grads : fresh ? std::vector<at::Tensor>() : tensor_list(a[1], what, "each result");
+    const double max_norm = PyFloat_AsDouble(a[2]);
+    if (PyErr_Occurred()) throw python_error();
+    check_grads(grads, what);
+    TORCH_CHECK_VALUE(max_norm >= 0, what, ": max_norm is negative or NaN");
+    TORCH_CHECK_VALUE(fresh || out.size() == grads.size(), what, ": ", out.size(), " results for ", grads.size(), " gradients");
+    if (!fresh) check_grads(out, what);
+    for (size_t i = 0; i < out.size(); ++i) {
+        TORCH_CHECK_VALUE(out[i].sizes() == grads[i].sizes() && out[i].device() == grads[i].device(), what, ": result ", i, " has another shape or device than its gradient");
+        TORCH_CHECK_TYPE(out[i].scalar_type() == grads[i].scalar_type() || out[i].scalar_type() == at::kFloat, what, ": result ", i, " must have the type of its gradient or float32");
+        TORCH_CHECK_VALUE(at::has_internal_overlap(out[i]) != at::MemOverlap::Yes, what, ": result ", i, " refers to one place several times");
+    }
+    at::Tensor norm;
+    if (!grads.empty()) {
+        const c10::DeviceGuard guard(grads[0].device());
+        if (fresh)
+            for (const at::Tensor &g : grads) out.push_back(at::empty_like(g, g.options().requires_grad(false)));
+        std::vector<at::Tensor> held;                                // copies of gradients that do not fill their memory, and
+        std::vector<std::pair<size_t, at::Tensor>> back;             // results that go to where they belong behind the launches
+        std::vector<mortar_grad_t> list;
+        std::vector<Span> spans;
+        list.reserve(grads.size());
+        for (size_t i = 0; i < grads.size(); ++i) {
+            const at::Tensor &g = grads[i], &o = out[i];
+            at::Tensor s = g, d = o;
+            if (!g.is_non_overlapping_and_dense() || (o.strides() != g.strides() && !(g.is_contiguous() && o.is_contiguous()))) {
+                const auto same = [&](const std::pair<size_t, at::Tensor> &b) {
+                    const at::Tensor &t = grads[b.first];
+                    return t.const_data_ptr() == g.const_data_ptr() && t.sizes() == g.sizes() && t.strides() == g.strides() && t.scalar_type() == g.scalar_type();
+                };
+                if (!g.numel() || (in_place && std::any_of(back.begin(), back.end(), same))) continue;
+                s = g.clone(at::MemoryFormat::Contiguous);
+                d = at::empty(o.sizes(), o.options().requires_grad(false));
+                held.push_back(s);
+                back.emplace_back(i, d);
+                int64_t last = 0;
+                for (int64_t k = 0; k < o.dim(); ++k) last += (o.size(k) - 1) * o.stride(k);
+                const uintptr_t at = reinterpret_cast<uintptr_t>(o.const_data_ptr());
+                spans.push_back({at, at + (last + 1) * o.element_size(), i, false});
+            }
+            list.push_back({data(s), mut(d), g.numel(), type_code(g.scalar_type()), type_code(o.scalar_type())});
+        }
+        check_overlap(list, std::move(spans), in_place, what);
+        norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+        const at::Tensor ws = empty_bytes(norm, std::max<int64_t>(8, mortar_grad_workspace_bytes(list.data(), (int64_t)list.size())));
+        check_rc(mortar_grad_clip(list.data(), (int64_t)list.size(), a[3] == Py_True, max_norm, floats(norm), mut(ws), stream_of(norm)), "mortar_grad_clip");
+        const at::NoGradGuard no_grad;
+        for (const auto &b : back) out[b.first].copy_(b.second);
+        if (!fresh)
+            for (const at::Tensor &o : out) torch::autograd::impl::bump_version(o);
+    }
+    PyObject *results = PyList_New((Py_ssize_t)out.size());
+    if (!results) throw python_error();
+    for (size_t i = 0; i < out.size(); ++i) PyList_SET_ITEM(results, (Py_ssize_t)i, THPVariable_Wrap(out[i]));
+    PyObject *n = norm.defined() ? THPVariable_Wrap(std::move(norm)) : empty_norm();
+    return Py_BuildValue("(NN)", results, n);
+}
+
+// ---- experts ---------------------------------------------------------------------------------------------------------
+
+// expert_sort(ids, n_experts) -> (position int32 [N, k], token int32 [N k], offsets int32 [n_experts + 1])
+PyObject *py_expert_sort(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    const char *what = "expert_sort";
+    TORCH_CHECK_TYPE(na == 2, "expert_sort: 2 arguments");
+    const at::Tensor ids = tensor_arg(a[0], what, "ids");
+    const long experts = PyLong_AsLong(a[1]);
+    if (experts == -1 && PyErr_Occurred()) throw python_error();
+    TORCH_CHECK_TYPE(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, what, ": ids must be int32 or int64, got ", ids.scalar_type());
+    TORCH_CHECK_VALUE(ids.dim() == 2 && ids.size(1) > 0, what, ": expected ids [tokens, slots], got ", ids.sizes());
+    TORCH_CHECK_VALUE(experts > 0 && experts <= 1024, what, ": 1 to 1024 experts, got ", experts);
+    TORCH_CHECK_VALUE(ids.numel() < (1 << 26), what, ": too many slots");
+    const c10::DeviceGuard guard(ids.device());
+    const at::Tensor c = ids.contiguous();
+    const auto options = ids.options().dtype(at::kInt);
+    at::Tensor position = at::empty(ids.sizes(), options), token = at::empty({ids.numel()}, options), offsets = at::empty({experts + 1}, options);
+    const int64_t n = mortar_expert_sort_workspace_bytes(ids.numel(), (int32_t)experts);
+    const at::Tensor ws = n ? empty_bytes(ids, n) : at::Tensor();
+    check_rc(mortar_expert_sort(data(c), ids.scalar_type() == at::kLong, ids.size(0), (int32_t)ids.size(1), (int32_t)experts, static_cast<int32_t *>(mut(position)),
+                                static_cast<int32_t *>(mut(token)), static_cast<int32_t *>(mut(offsets)), mut(ws), stream_of(ids)),
+             "mortar_expert_sort");
+    PyObject *p = THPVariable_Wrap(std::move(position)), *t = THPVariable_Wrap(std::move(token)), *o = THPVariable_Wrap(std::move(offsets));
+    return Py_BuildValue("(NNN)", p, t, o);
+}
+
+// Positions [N, k] and offsets [E + 1] of an order, as a launch reads them.
+struct Order {
+    at::Tensor position, offsets;
+    int64_t N, k;
+    const int32_t *pos() const { return static_cast<const int32_t *>(position.const_data_ptr()); }
+    const int32_t *full() const { return static_cast<const int32_t *>(offsets.const_data_ptr()) + offsets.size(0) - 1; }
+};
+
+Order order_of(const at::Tensor &position, const at::Tensor &offsets) { return {position.contiguous(), offsets.contiguous(), position.size(0), position.size(1)}; }
+
+Order order_arg(PyObject *p, PyObject *o, const at::Tensor &x, const char *what) {
+    const at::Tensor position = tensor_arg(p, what, "position"), offsets = tensor_arg(o, what, "offsets");
+    same_device(x, position, what, "position");
+    same_device(x, offsets, what, "offsets");
+    TORCH_CHECK_TYPE(position.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt, what, ": position and offsets must be int32");
+    TORCH_CHECK_VALUE(position.dim() == 2 && position.size(1) > 0 && offsets.dim() == 1 && offsets.size(0) > 1, what, ": expected position [tokens, slots] and offsets [experts + 1]");
+    TORCH_CHECK_VALUE(position.numel() < (1 << 26), what, ": too many slots");
+    return order_of(position, offsets);
+}
+
+void check_rows(const at::Tensor &x, int64_t rows, const char *what, const char *name) {
+    TORCH_CHECK_TYPE(type_code(x.scalar_type()) >= 0, what, ": expected bfloat16, float16 or float32, got ", x.scalar_type());
+    TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) == rows && x.size(1) > 0, what, ": expected ", name, " [", rows, ", d], got ", x.sizes());
+    TORCH_CHECK_VALUE(x.size(1) < (1 << 28), what, ": rows of ", x.size(1), " values are too long");
+}
+
+// x [N, d] with consecutive values in its rows.
+at::Tensor lines(const at::Tensor &x) { return x.size(1) > 1 && x.stride(1) != 1 ? x.contiguous() : x; }
+
+at::Tensor dispatch(const at::Tensor &x, const Order &o) {
+    const c10::DeviceGuard guard(x.device());
+    const at::Tensor r = lines(x);
+    at::Tensor xs = empty_like_rows(x, {o.N * o.k, x.size(1)});
+    check_rc(mortar_expert_dispatch(data(r), o.N, (int32_t)x.size(1), r.stride(0), type_code(x.scalar_type()), (int32_t)o.k, o.pos(), o.full(), mut(xs), stream_of(x)),
+             "mortar_expert_dispatch");
+    return xs;
+}
+
+at::Tensor combine(const at::Tensor &ys, const at::Tensor &w, const Order &o) {
+    const c10::DeviceGuard guard(ys.device());
+    const at::Tensor r = ys.contiguous(), wc = w.defined() ? w.contiguous() : w;
+    at::Tensor y = empty_like_rows(ys, {o.N, ys.size(1)});
+    check_rc(mortar_expert_combine(data(r), o.N, (int32_t)ys.size(1), type_code(ys.scalar_type()), (int32_t)o.k, o.pos(), o.full(), data(wc),
+                                   w.defined() ? type_code(w.scalar_type()) : 0, mut(y), stream_of(ys)),
+             "mortar_expert_combine");
+    return y;
+}
+
+struct DispatchFn : public torch::autograd::Function<DispatchFn> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &position, const at::Tensor &offsets) {
+        ctx->save_for_backward({position, offsets});
+        ctx->saved_data["offsets"] = offsets.size(0);
+        ctx->saved_data["shape"] = position.sizes();
+        return dispatch(x, order_of(position, offsets));
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(3);
+        const char *what = "expert_dispatch";
+        const at::Tensor g = plain_gradient(grads[0], what);
+        if (!g.defined()) return out;
+        const auto v = ctx->get_saved_variables();
+        out[0] = combine(g, at::Tensor(), order_of(kept(v[0], g, ctx->saved_data["shape"].toIntVector(), at::kInt, what),
+                                                   kept(v[1], g, {ctx->saved_data["offsets"].toInt()}, at::kInt, what)));
+        return out;
+    }
+};
+
+struct CombineFn : public torch::autograd::Function<CombineFn> {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &ys, const std::optional<at::Tensor> &weights, const at::Tensor &position, const at::Tensor &offsets) {
+        const at::Tensor w = weights ? *weights : at::Tensor();
+        const bool need_w = w.defined() && ctx->needs_input_grad(1);
+        ctx->save_for_backward({need_w ? ys : at::Tensor(), w, position, offsets});
+        ctx->saved_data["offsets"] = offsets.size(0);
+        ctx->saved_data["shape"] = position.sizes();
+        ctx->saved_data["type"] = w.defined() ? c10::IValue(w.scalar_type()) : c10::IValue();
+        return combine(ys, w, order_of(position, offsets));
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(4);
+        const char *what = "expert_combine";
+        const at::Tensor g = plain_gradient(grads[0], what);
+        if (!g.defined()) return out;
+        const auto v = ctx->get_saved_variables();
+        const auto shape = ctx->saved_data["shape"].toIntVector();
+        const int64_t d = g.size(1), slots = shape[0] * shape[1];
+        const bool weighted = !ctx->saved_data["type"].isNone();
+        // (edges are counted over the tensors that are there)
+        const bool need_y = ctx->needs_input_grad(0), need_w = weighted && ctx->needs_input_grad(1);
+        const Order o = order_of(kept(v[2], g, shape, at::kInt, what), kept(v[3], g, {ctx->saved_data["offsets"].toInt()}, at::kInt, what));
+        const c10::DeviceGuard guard(g.device());
+        at::Tensor w, ys, dys, dw;
+        if (weighted) w = kept(v[1], g, shape, ctx->saved_data["type"].toScalarType(), what).contiguous();
+        if (need_w) ys = kept(v[0], g, {slots, d}, g.scalar_type(), what).contiguous();
+        if (need_y) dys = empty_like_rows(g, {slots, d});
+        if (need_w) dw = at::empty(shape, w.options().requires_grad(false));
+        const at::Tensor r = lines(g);
+        check_rc(mortar_expert_combine_bwd(data(r), r.stride(0), data(ys), o.N, (int32_t)d, type_code(g.scalar_type()), (int32_t)o.k, o.pos(), o.full(), data(w),
+                                           weighted ? type_code(w.scalar_type()) : 0, mut(dys), mut(dw), stream_of(g)),
+                 "mortar_expert_combine_bwd");
+        out[0] = dys;
+        out[1] = dw;
+        return out;
+    }
+};
+
+// expert_dispatch(x, position, offsets) -> xs [N k, d]
+PyObject *py_expert_dispatch(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    const char *what = "expert_dispatch";
+    TORCH_CHECK_TYPE(na == 3, "expert_dispatch: 3 arguments");
+    const at::Tensor x = tensor_arg(a[0], what, "x");
+    const Order o = order_arg(a[1], a[2], x, what);
+    check_rows(x, o.N, what, "x");
+    at::Tensor xs = c10::GradMode::is_enabled() && x.requires_grad() ? DispatchFn::apply(x, o.position, o.offsets) : dispatch(x, o);
+    return THPVariable_Wrap(std::move(xs));
+}
+
+// expert_combine(ys, weights, position, offsets) -> y [N, d]
+PyObject *py_expert_combine(PyObject *, PyObject *const *a, Py_ssize_t na) {
+    const char *what = "expert_combine";
+    TORCH_CHECK_TYPE(na == 4, "expert_combine: 4 arguments");
+    const at::Tensor ys = tensor_arg(a[0], what, "ys"), w = optional_arg(a[1], what, "weights");
+    const Order o = order_arg(a[2], a[3], ys, what);
+    check_rows(ys, o.N * o.k, what, "ys");
+    if (w.defined()) {
+        same_device(ys, w, what, "weights");
+        TORCH_CHECK_TYPE(type_code(w.scalar_type()) >= 0, what, ": weights must be bfloat16, float16 or float32, got ", w.scalar_type());
+        TORCH_CHECK_VALUE(w.sizes() == o.position.sizes(), what, ": weights must be ", o.position.sizes(), " like the positions, got ", w.sizes());
+    }
+    at::Tensor y;
+    if (c10::GradMode::is_enabled() && (ys.requires_grad() || (w.defined() && w.requires_grad())))
+        y = CombineFn::apply(ys, w.defined() ? std::optional<at::Tensor>(w) : std::nullopt, o.position, o.offsets);
+    else
+        y = combine(ys, w, o);
+    return THPVariable_Wrap(std::move(y));
+}
+
+PyMethodDef methods[] = {MORTAR_METHOD("grad_norm", py_grad_norm, "The norm over the gradients of many tensors."),
+                         MORTAR_METHOD("grad_clip", py_grad_clip, "Gradients clipped to a norm over all of them."),
+                         MORTAR_METHOD("expert_sort", py_expert_sort, "Slots of tokens sorted by expert."),
+                         MORTAR_METHOD("expert_dispatch", py_expert_dispatch, "Tokens to the rows of their experts."),
+                         MORTAR_METHOD("expert_combine", py_expert_combine, "Rows of the experts back to their tokens."),
+                         {nullptr, nullptr, 0, nullptr}};
+
+}  // namespace
+
+int mortar_add_train_methods(PyObject *module) { return PyModule_AddFunctions(module, methods); }

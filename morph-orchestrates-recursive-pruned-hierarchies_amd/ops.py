@@ -3,6 +3,7 @@ the HIP library.  Every function requires tensors on a ROCm device; there is no 
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 from torch import Tensor
@@ -589,3 +590,82 @@ def linear_fp8(x: Tensor, wq: Tensor, ws: Tensor, x_scale: Tensor | None = None)
     """y = x W^T for a weight of quantize_fp8_weight: bf16 x [..., K] is quantised as quantize_fp8 does (a few rows inside the
     product's launch), float8_e4m3fn x is taken with its ``x_scale`` as it is.  fp32 sums, bf16 result [..., N]; no gradients."""
     return _lib.native().linear_fp8(x, wq, ws, x_scale)
+
+
+def quantize_int4_weight(w: Tensor, group_size: int = 128, zero_points: bool = False) -> tuple[Tensor, Tensor, Tensor | None]:
+    """(codes int32 [N, 4 * ceil(K / 32)], scales [N, groups] in the type of w, zeros uint8 [N, groups] or None) of a weight [N, K] in bf16, fp16 or fp32:
+    one scale per row and ``group_size`` (32, 64 or 128) consecutive values.  W = (code - 8) * scale with scale = max(max / 7, -min / 8), or with
+    ``zero_points`` W = (code - zero) * scale with scale = (max - min) / 15, zero = rne(-min / scale), both over the group and 0.  A word holds eight
+    values, value j of them in bits 4 p .. 4 p + 3, p = 0 4 1 5 2 6 3 7.  Scales and zeros are consecutive along the rows."""
+    return _lib.native().quantize_int4_weight(w, group_size, zero_points)
+
+
+def linear_int4(x: Tensor, codes: Tensor, scales: Tensor, zeros: Tensor | None = None, group_size: int = 128) -> Tensor:
+    """y = x W^T for a weight of quantize_int4_weight: x [..., K] in bf16 or fp16, result [..., N] in its type; scales in the type of x or fp32 and zeros
+    with any strides.  The codes are multiplied as they are and scaled per group in fp32, W itself is never rounded.  No gradients.  A row of
+    x that holds an infinity is NaN in the result."""
+    return _lib.native().linear_int4(x, codes, scales, zeros, group_size)
+
+
+# ----------------------------------------------------------------------------- gradients
+
+
+def _largest(norm_type, what: str) -> bool:
+    if norm_type not in (2, float("inf")):
+        raise ValueError(f"{what}: norm_type must be 2 or inf, got {norm_type}")
+    return norm_type != 2
+
+
+def grad_norm(grads, norm_type: float = 2.0) -> Tensor:
+    """The norm over all values of a sequence of gradients (bf16, fp16, fp32, mixed; any strides; one device) as an fp32 tensor []: the root of the
+    sum of squares, which is formed in 64 bits in a fixed order, or with inf the largest magnitude (NaN if there is one)."""
+    return _lib.native().grad_norm(grads, _largest(norm_type, "grad_norm"))
+
+
+def clip_grads(grads, max_norm: float, norm_type: float = 2.0, out=None) -> tuple[list[Tensor], Tensor]:
+    """(clipped, norm): every gradient times min(1, max_norm / (norm + 1e-6)), norm that of grad_norm.  ``out``: where the results go, tensors of the
+    gradients' shapes and types (or fp32), which may be the gradients themselves but may not overlap otherwise; None: new ones.  Nothing waits for
+    the GPU.  As in torch's clipping a norm that is infinite makes the finite gradients 0, one that is NaN all of them NaN."""
+    return _lib.native().grad_clip(grads, out, max_norm, _largest(norm_type, "clip_grads"))
+
+
+def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False) -> Tensor:
+    """clip_grads on the .grad of one or several parameters in place, those without one left out and one that several share counted once; returns the norm before it.
+    ``error_if_nonfinite`` waits for the norm and raises RuntimeError where it is not finite, with the gradients as they were."""
+    largest = _largest(norm_type, "clip_grad_norm_")
+    grads = [p.grad for p in ([parameters] if isinstance(parameters, Tensor) else parameters) if p.grad is not None]
+    with torch.no_grad():
+        if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
+            raise RuntimeError("clip_grad_norm_: the norm of the gradients is not finite, so they cannot be clipped")
+        return _lib.native().grad_clip(grads, True, max_norm, largest)[1]
+
+
+# ----------------------------------------------------------------------------- experts
+
+
+class ExpertOrder(NamedTuple):
+    """Slots [N, k] of tokens sorted by expert: ``position`` int32 [N, k], the row of each slot; ``token`` int32 [N * k], the token of each row; ``offsets`` int32
+    [n_experts + 1], the first row of each expert and behind them the number of rows that have one."""
+    position: Tensor
+    token: Tensor
+    offsets: Tensor
+
+
+def expert_sort(ids: Tensor, n_experts: int) -> ExpertOrder:
+    """The order of the slots of ``ids`` (int32 or int64 [N, k]) by expert, for expert_dispatch and expert_combine; within an expert as in ids.  Numbers outside
+    0 .. n_experts - 1 (at most 1024) are empty slots and lie behind all others: of TileRouter's gates, which leave fewer than k experts per token,
+    ``w, ids = gates.topk(k); ids = ids.masked_fill(w <= 0, -1)`` are weights and slots."""
+    return ExpertOrder(*_lib.native().expert_sort(ids, n_experts))
+
+
+def expert_dispatch(x: Tensor, order: ExpertOrder) -> Tensor:
+    """xs [N * k, d], differentiable: the rows of x [N, d] (bf16, fp16, fp32; any width and strides) at the positions of their slots, expert by expert, zeros in the
+    rows behind the last expert's.  The gradient of a token is the sum over its full slots, in order, in fp32.  First derivatives only."""
+    return _lib.native().expert_dispatch(x, order.position, order.offsets)
+
+
+def expert_combine(ys: Tensor, weights: Tensor | None, order: ExpertOrder) -> Tensor:
+    """y [N, d] = sum over a token's full slots of weights[n, j] * ys[position[n, j]], differentiable in ys [N * k, d] and weights [N, k] (None: 1).  Sums are fp32
+    in the order of the slots, the result is in the type of ys; rows and weights of empty slots are not looked at and have gradients of 0.
+    First derivatives only."""
+    return _lib.native().expert_combine(ys, weights, order.position, order.offsets)
