@@ -7,10 +7,15 @@
 // The codes of a word lie so that one shift brings a pair of neighbours into its two halves.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "mortar_dense_core.h"
 #include "mortar_internal.h"
 
 namespace {
+
+// Rows of x in LDS: whole chunks, and 16 bytes so that they start on different banks.
+__host__ __device__ constexpr int int4_pitch(int K) { return (K + 127) / 128 * 256 + 16; }
 
 struct Int4Args {
     const void *x;
@@ -28,17 +33,17 @@ struct Int4Args {
     int32_t Mp, Np, tiles_n, tiles_m;
 };
 
-// Eight weights 16 + c of a word, in the order of K.
+// Eight weights 16 + c of a word, in the order of K: one shift and one and-or for two.  (The constants are kept in registers: as literals, of which an instruction
+// takes one, the and and the or are two instructions.)
 template <DenseType T>
-__device__ __forceinline__ u32x4_t int4_unpack(uint32_t w) {
-    if constexpr (T == DENSE_F16) {
-        constexpr uint32_t mask = 0x03C003C0u, one = 0x4C004C00u;
-        return u32x4_t{(w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one, (w >> 6 & mask) | one};
-    } else {
-        constexpr uint32_t mask = 0x00780078u, one = 0x41804180u;
-        return u32x4_t{(w << 3 & mask) | one, (w >> 1 & mask) | one, (w >> 5 & mask) | one, (w >> 9 & mask) | one};
+struct Int4Unpack {
+    uint32_t mask = T == DENSE_F16 ? 0x03C003C0u : 0x00780078u, one = T == DENSE_F16 ? 0x4C004C00u : 0x41804180u;
+    __device__ __forceinline__ Int4Unpack() { asm("" : "+s"(mask), "+v"(one)); }
+    __device__ __forceinline__ u32x4_t operator()(uint32_t w) const {
+        if constexpr (T == DENSE_F16) return u32x4_t{(w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one, (w >> 6 & mask) | one};
+        else return u32x4_t{(w << 3 & mask) | one, (w >> 1 & mask) | one, (w >> 5 & mask) | one, (w >> 9 & mask) | one};
     }
-}
+};
 template <DenseType T, int S>
 __device__ __forceinline__ float int4_scale(const void *s, int64_t i) {
     if constexpr (S == 4) return static_cast<const float *>(s)[i];
@@ -47,96 +52,114 @@ __device__ __forceinline__ float int4_scale(const void *s, int64_t i) {
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// 16 rows of W per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what bounds
-// these calls.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per lane and
-// group.  The sums of x come from one more product, with ones.
+// 16 F rows of W and 16 of x per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what
+// bounds these calls.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
+// lane and group.  The sums of x come from one more product, with ones.
 // Groups of 128: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product:
 // the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7}.
-template <DenseType T, int G, int S, bool Z, int MT, int NW, int U>
+// XL: x goes through LDS, where the 16 rows of a fragment that are not there cost nothing; read as operands from memory, which takes as many load cycles
+// per chunk as four fragments of W, for more rows or K than fit.
+template <DenseType T, int G, int S, int F, int NW, bool XL>
 __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
     constexpr int GPC = 128 / G, PER = 4 / GPC;                 // groups of a chunk, products of a group
-    __shared__ f32x4_t part[NW][MT][64];
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    f32x4_t *part = reinterpret_cast<f32x4_t *>(smem);          // [wave][feature tile][lane]
+    unsigned char *xs = smem + NW * F * 1024;                   // XL: rows of x, whole chunks
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane >> 4, r = lane & 15;
-    const int n0 = blockIdx.x * 16, chunks = (a.K + 127) >> 7, words = (a.K + 31) >> 5 << 4;        // (bytes of a row of codes)
+    const int n0 = blockIdx.x * (16 * F), m0 = blockIdx.y * 16, rows = min(a.M - m0, 16);
+    const int chunks = (a.K + 127) >> 7, words = (a.K + 31) >> 5 << 4, pitch = int4_pitch(a.K);       // (words: bytes of a row of codes)
     const auto whole = [](const void *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, DENSE_OUTSIDE, 0x00020000); };
     const auto read = [](__amdgpu_buffer_rsrc_t b, uint32_t off) { return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0)); };
-    const __amdgpu_buffer_rsrc_t cb = whole(reinterpret_cast<const char *>(a.c) + (int64_t)n0 * a.ldc), xb = whole(a.x);
-    const uint32_t co = n0 + r < a.N ? (uint32_t)(r * a.ldc) + q * 16 : DENSE_OUTSIDE;
-    const int64_t n = min(n0 + r, a.N - 1);
-    uint32_t xo[MT];
+    const char *x0 = static_cast<const char *>(a.x) + (int64_t)m0 * a.ldx;
+    const __amdgpu_buffer_rsrc_t cb = whole(reinterpret_cast<const char *>(a.c) + (int64_t)n0 * a.ldc), xb = whole(x0);
+    uint32_t co[F];
+    int64_t n[F];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xo[t] = t * 16 + r < a.M ? (uint32_t)((t * 16 + r) * a.ldx) : DENSE_OUTSIDE;
+    for (int f = 0; f < F; ++f) {
+        co[f] = n0 + f * 16 + r < a.N ? (uint32_t)((f * 16 + r) * a.ldc) + q * 16 : DENSE_OUTSIDE;
+        n[f] = min(n0 + f * 16 + r, a.N - 1);
+    }
+    const uint32_t xo = (uint32_t)min(r, rows - 1) * (XL ? (uint32_t)pitch : (uint32_t)a.ldx);        // (results of rows behind the last one are not used)
     const uint32_t one2 = T == DENSE_F16 ? 0x3C003C00u : 0x3F803F80u;
     const u32x4_t ones = {one2, one2, one2, one2};
-    f32x4_t acc[MT];
+    const Int4Unpack<T> unpack;
+    f32x4_t acc[F];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int c0 = wave; c0 < chunks; c0 += NW * U) {
-        u32x4_t w[U], x[U][MT][4];
-        float s[U][GPC], z[U][GPC];
+    for (int f = 0; f < F; ++f) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c = wave; c < chunks || (XL && c == wave); c += NW) {
+        u32x4_t w[F], x[4];
+        float s[F][GPC], z[F][GPC];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = c0 + u * NW;
-            w[u] = read(cb, c * 64 + q * 16 < words ? co + c * 64 : DENSE_OUTSIDE);
+        for (int f = 0; f < F; ++f) w[f] = read(cb, c * 64 + q * 16 < words ? co[f] + c * 64 : DENSE_OUTSIDE);
+#pragma unroll
+        for (int f = 0; f < F; ++f)
 #pragma unroll
             for (int i = 0; i < GPC; ++i) {
                 const int g = min(c * GPC + i, a.groups - 1);
-                s[u][i] = int4_scale<T, S>(a.s, n * a.s_n + g * a.s_g);
-                z[u][i] = Z ? -16.0f - (float)a.z[n * a.z_n + g * a.z_g] : -24.0f;
+                s[f][i] = int4_scale<T, S>(a.s, n[f] * a.s_n + g * a.s_g);
+                z[f][i] = a.z ? -16.0f - (float)a.z[n[f] * a.z_n + g * a.z_g] : -24.0f;
             }
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    const int k = c * 128 + (G == 128 ? q * 32 + p * 8 : p * 32 + q * 8);
-                    x[u][t][p] = read(xb, k < a.K ? xo[t] + 2 * k : DENSE_OUTSIDE);
+        const auto x_at = [&](int p) { return c * 128 + (G == 128 ? q * 32 + p * 8 : p * 32 + q * 8); };
+        if constexpr (XL) {
+            if (c == wave) {                                     // every wave once
+                const int units = chunks * 16;
+                for (int i = threadIdx.x; i < rows * units; i += NW * 64) {
+                    const int m = i / units, u = i - m * units;
+                    u32x4_t v = {0, 0, 0, 0};
+                    if (u * 8 < a.K) v = *reinterpret_cast<const u32x4_t *>(x0 + m * a.ldx + u * 16);
+                    *reinterpret_cast<u32x4_t *>(xs + m * pitch + u * 16) = v;
                 }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = c0 + u * NW;
+                __syncthreads();
+            }
             if (c >= chunks) break;
-            if constexpr (G != 128) {                            // word p of lane q <-> word q of lane p
-                const auto l0 = __builtin_amdgcn_permlane16_swap(w[u][0], w[u][1], false, false), l1 = __builtin_amdgcn_permlane16_swap(w[u][2], w[u][3], false, false);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const u32x4_t *>(xs + xo + 2 * x_at(p));
+        } else {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) x[p] = read(xb, x_at(p) < a.K ? xo + 2 * x_at(p) : DENSE_OUTSIDE);
+        }
+        if constexpr (G != 128) {                                // word p of lane q <-> word q of lane p
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                const u32x4_t v = w[f];
+                const auto l0 = __builtin_amdgcn_permlane16_swap(v[0], v[1], false, false), l1 = __builtin_amdgcn_permlane16_swap(v[2], v[3], false, false);
                 const auto h0 = __builtin_amdgcn_permlane32_swap(l0[0], l1[0], false, false), h1 = __builtin_amdgcn_permlane32_swap(l0[1], l1[1], false, false);
-                w[u] = u32x4_t{h0[0], h1[0], h0[1], h1[1]};
+                w[f] = u32x4_t{h0[0], h1[0], h0[1], h1[1]};
             }
+        }
 #pragma unroll
-            for (int i = 0; i < GPC; ++i) {
-                if (c * GPC + i >= a.groups) break;
-                f32x4_t d[MT], e[MT];
+        for (int i = 0; i < GPC; ++i) {
+            if (c * GPC + i >= a.groups) break;
+            f32x4_t d[F], e = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int t = 0; t < MT; ++t) d[t] = e[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+            for (int f = 0; f < F; ++f) d[f] = e;
 #pragma unroll
-                for (int p = i * PER; p < (i + 1) * PER; ++p) {
-                    const uint32_t word = w[u][p];
-                    const u32x4_t f = int4_unpack<T>(word);
+            for (int p = i * PER; p < (i + 1) * PER; ++p) {
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        d[t] = dense_mfma<T>(x[u][t][p], f, d[t]);
-                        e[t] = dense_mfma<T>(x[u][t][p], ones, e[t]);
-                    }
+                for (int f = 0; f < F; ++f) {
+                    const uint32_t word = w[f][p];
+                    d[f] = dense_mfma<T>(x[p], unpack(word), d[f]);
                 }
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[t][v] = __builtin_fmaf(s[u][i], __builtin_fmaf(z[u][i], e[t][v], d[t][v]), acc[t][v]);
+                e = dense_mfma<T>(x[p], ones, e);
             }
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) acc[f][v] = __builtin_fmaf(s[f][i], __builtin_fmaf(z[f][i], e[v], d[f][v]), acc[f][v]);
         }
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) part[wave][t][lane] = acc[t];
+    for (int f = 0; f < F; ++f) part[(wave * F + f) * 64 + lane] = acc[f];
     __syncthreads();
-    if (wave >= MT) return;
-    f32x4_t sum = part[0][wave][lane];
+    if (wave >= F) return;
+    f32x4_t sum = part[wave * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) sum += part[w][wave][lane];
-    if (n0 + r >= a.N) return;
+    for (int w = 1; w < NW; ++w) sum += part[(w * F + wave) * 64 + lane];
+    const int at = n0 + wave * 16 + r;
+    if (at >= a.N) return;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        const int m = wave * 16 + 4 * q + v;
-        if (m < a.M) a.y[m * a.ldy + n0 + r] = (uint16_t)dense_pack2<T>(sum[v], 0.f);
-    }
+    for (int v = 0; v < 4; ++v)
+        if (4 * q + v < rows) a.y[(int64_t)(m0 + 4 * q + v) * a.ldy + at] = (uint16_t)dense_pack2<T>(sum[v], 0.f);
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------
@@ -226,6 +249,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
     };
     const uint32_t ax = l0 + dense_row_addr(wm * FM * 16, lane), ac = l0 + X + (wn * FN * 16 + r) * 32 + q * 4, ag = l0 + X + C;
 
+    const Int4Unpack<T> unpack;
     f32x4_t acc[FN][FM], part[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
@@ -244,7 +268,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             const uint32_t gt = ga + (GPS == 2 ? t * GC * 1024 : 0);
             u32x4_t xf[FM], wf[FN];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) wf[i] = int4_unpack<T>(*(const MORTAR_LDS uint32_t *)(uintptr_t)(ac + slot + i * 512 + t * 16));
+            for (int i = 0; i < FN; ++i) wf[i] = unpack(*(const MORTAR_LDS uint32_t *)(uintptr_t)(ac + slot + i * 512 + t * 16));
 #pragma unroll
             for (int j = 0; j < FM; ++j) xf[j] = dense_read(((ax + slot) ^ (t * 64)) + j * 2048);
             const bool begin = GPS == 2 || (first.value && t == 0), end = GPS == 2 || (last.value && t == 1);
@@ -381,17 +405,66 @@ int launch_error(const char *what) {
     return e == hipSuccess ? MORTAR_OK : mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
-constexpr int FEW_ROWS = 32;
-bool few_rows(int64_t M) { return M <= FEW_ROWS; }
+// Which kernel: the smallest estimate, in us, from products of 1 to 4096 rows of 2048 -> 11264, 5632 -> 2048 and 1040 -> 2736.
+// Few rows: workgroups of 16 x 16 F results; as many rows of W in each as leave 170 of them (16 rows of 2048 -> 11264 6.9 with F = 4 and 8.3 with 2, 64 of 5632
+// -> 2048 10.3 with 2, 256 of them, and 13.9 with 4), and 16 waves instead of 8 where they are one round of the chip.  Tiles are bound by the instructions of
+// a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second launch for the sums of x.
+struct Int4Plan {
+    int f, waves, tile;          // few rows: f > 0; else index into INT4_TILES
+    bool xl;
+};
+struct Int4Tile {
+    int bn, bm;
+    double alone, more;          // us of a step of 64 K: of the only workgroup of a CU, and of each of many
+};
+constexpr Int4Tile INT4_TILES[] = {{128, 128, 0.62, 0.48}, {64, 64, 0.375, 0.2}};
+constexpr int MOST_FEW_ROWS = 4096, FEW_LDS = 64 * 1024;
+
+Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
+    const int64_t chunks = (K + 127) / 128, steps = (K + 63) / 64, n16 = (N + 15) / 16, m16 = (M + 15) / 16;
+    Int4Plan p{1, 8, 0, false};
+    if (M <= 8 && M * int4_pitch((int)K) <= FEW_LDS) {
+        p.xl = true;
+        p.f = n16 >= 512 && chunks >= 32 ? 2 : 1;
+        p.waves = chunks > 16 ? 16 : 8;
+        return p;
+    }
+    for (int f = 4; f > 1 && p.f == 1; f /= 2)
+        if ((n16 + f - 1) / f * m16 >= 170) p.f = f;
+    const int64_t wgs = (n16 + p.f - 1) / p.f * m16;
+    p.waves = wgs <= 256 && chunks > 8 ? 16 : 8;
+    if (M <= 16) return p;
+    double best = M <= MOST_FEW_ROWS ? 4.5 + 2.3e-4 * (double)(n16 * m16 * chunks) : 1e300;
+    for (int t = 0; t < 2; ++t) {
+        const Int4Tile &d = INT4_TILES[t];
+        const int64_t per_cu = (((N + d.bn - 1) / d.bn) * ((M + d.bm - 1) / d.bm) + 255) / 256;
+        const double us = 8.0 + (double)steps * (group == 32 ? 1.3 : 1.0) * std::max(d.alone, d.more * (double)per_cu);
+        if (us < best) best = us, p = Int4Plan{0, 0, t, false};
+    }
+    return p;
+}
 int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 int64_t groups_padded(int64_t K, int group) { return group == 32 ? (K + 63) / 64 * 2 : (K + group - 1) / group; }
 
-template <DenseType T, int G, int S, bool Z>
-int launch_few(const Int4Args &a, hipStream_t st, const char *what) {
-    const dim3 grid((unsigned)((a.N + 15) / 16));
-    if (a.M <= 16) hipLaunchKernelGGL((int4_few_kernel<T, G, S, Z, 1, 16, 2>), grid, dim3(1024), 0, st, a);
-    else hipLaunchKernelGGL((int4_few_kernel<T, G, S, Z, 2, 16, 1>), grid, dim3(1024), 0, st, a);
+template <DenseType T, int G, int S, int F, int NW, bool XL>
+int launch_few_form(const Int4Args &a, hipStream_t st, const char *what) {
+    const auto kern = int4_few_kernel<T, G, S, F, NW, XL>;
+    constexpr int sums = NW * F * 1024;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, sums + (XL ? FEW_LDS : 0));
+    if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    const dim3 grid((unsigned)((a.N + 16 * F - 1) / (16 * F)), (unsigned)((a.M + 15) / 16));
+    hipLaunchKernelGGL(kern, grid, dim3(NW * 64), sums + (XL ? a.M * int4_pitch(a.K) : 0), st, a);
     return launch_error(what);
+}
+template <DenseType T, int G, int S>
+int launch_few(const Int4Args &a, const Int4Plan &p, hipStream_t st, const char *what) {
+    if (p.xl) {
+        if (p.f == 2) return launch_few_form<T, G, S, 2, 16, true>(a, st, what);
+        return p.waves == 16 ? launch_few_form<T, G, S, 1, 16, true>(a, st, what) : launch_few_form<T, G, S, 1, 8, true>(a, st, what);
+    }
+    if (p.waves == 16)
+        return p.f == 4 ? launch_few_form<T, G, S, 4, 16, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 16, false>(a, st, what) : launch_few_form<T, G, S, 1, 16, false>(a, st, what);
+    return p.f == 4 ? launch_few_form<T, G, S, 4, 8, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 8, false>(a, st, what) : launch_few_form<T, G, S, 1, 8, false>(a, st, what);
 }
 
 template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS>
@@ -410,7 +483,7 @@ int launch_tile_form(Int4Args a, hipStream_t st, const char *what) {
 }
 
 template <DenseType T, int G, int S, bool Z>
-int launch_many(Int4Args a, float *ws, hipStream_t st, const char *what) {
+int launch_many(Int4Args a, int tile, float *ws, hipStream_t st, const char *what) {
     const int64_t groups = groups_padded(a.K, G);
     a.Mp = (int32_t)up128(a.M);
     a.Np = (int32_t)up128(a.N);
@@ -420,16 +493,14 @@ int launch_many(Int4Args a, float *ws, hipStream_t st, const char *what) {
     if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
     hipLaunchKernelGGL((int4_prepare_kernel<T, S>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, G, (int)groups, xs, s, zt, (unsigned)x_blocks);
     if (const int rc = launch_error(what)) return rc;
-    return launch_tile_form<T, G, Z, 128, 128, 2, 2, 3>(a, st, what);
+    return tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 2, 3>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 4, 4>(a, st, what);
 }
 
-template <DenseType T, int G, int S, bool Z>
-int launch_last(const Int4Args &a, float *ws, hipStream_t st, const char *what) {
-    return few_rows(a.M) ? launch_few<T, G, S, Z>(a, st, what) : launch_many<T, G, S, Z>(a, ws, st, what);
-}
 template <DenseType T, int G, int S>
 int launch_zeros(const Int4Args &a, float *ws, hipStream_t st, const char *what) {
-    return a.z ? launch_last<T, G, S, true>(a, ws, st, what) : launch_last<T, G, S, false>(a, ws, st, what);
+    const Int4Plan p = plan(a.M, a.N, a.K, G);
+    if (p.f) return launch_few<T, G, S>(a, p, st, what);
+    return a.z ? launch_many<T, G, S, true>(a, p.tile, ws, st, what) : launch_many<T, G, S, false>(a, p.tile, ws, st, what);
 }
 template <DenseType T, int G>
 int launch_scales(const Int4Args &a, bool s32, float *ws, hipStream_t st, const char *what) {
@@ -475,8 +546,19 @@ extern "C" int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t
     return type == MORTAR_FP32 ? scales(Const<MORTAR_FP32>{}) : type == MORTAR_FP16 ? scales(Const<MORTAR_FP16>{}) : scales(Const<MORTAR_BF16>{});
 }
 
+extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t group, int32_t *tile_n, int32_t *tile_m, int32_t *waves) {
+    const char *what = "int4_form";
+    CHECK(check_group(what, group));
+    if (M <= 0 || N <= 0 || K <= 0 || !tile_n || !tile_m || !waves) return mortar_fail(MORTAR_ERR_ARG, "%s: bad argument", what);
+    const Int4Plan p = plan(M, N, K, group);
+    *tile_n = p.f ? 16 * p.f : INT4_TILES[p.tile].bn;
+    *tile_m = p.f ? 16 : INT4_TILES[p.tile].bm;
+    *waves = p.xl ? -p.waves : p.f ? p.waves : 8;
+    return MORTAR_OK;
+}
+
 extern "C" int64_t mortar_int4_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t group) {
-    if (M <= 0 || N <= 0 || K <= 0 || group < 32 || few_rows(M)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || group < 32 || plan(M, N, K, group).f) return 0;
     return 4 * groups_padded(K, group) * (up128(M) + 2 * up128(N));
 }
 

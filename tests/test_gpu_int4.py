@@ -4,7 +4,7 @@ import torch
 
 from dense_util import assert_within, ints, normals
 from mortar_amd import ops
-from operators_util import int4_bound, int4_weight, pack_codes, quantize_reference, unpack_codes
+from operators_util import INT4_SIZES, int4_bound, int4_weight, pack_codes, quantize_reference, unpack_codes
 
 pytestmark = pytest.mark.gpu
 
@@ -38,15 +38,10 @@ def test_weights_that_are_not_finite(dev):
     assert torch.equal(torch.isnan(y).any(0).cpu(), torch.tensor([i in (3, 5) for i in range(9)]))
 
 
-#: rows, outputs, inputs: one to many rows on both sides of every switch, odd widths, ends inside a word, a group, a chunk, a tile
-SIZES = [(1, 1, 1), (1, 16, 32), (1, 17, 40), (2, 24, 128), (3, 130, 257), (13, 264, 1040), (16, 2048, 5632), (17, 136, 400), (31, 33, 264), (32, 256, 1999), (33, 256, 144),
-         (64, 520, 1040), (65, 9, 72), (129, 264, 400), (130, 127, 2736), (300, 135, 272), (520, 1031, 264), (2100, 2056, 392)]
-
-
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("t", TYPES, ids=str)
-@pytest.mark.parametrize("M,N,K", SIZES)
+@pytest.mark.parametrize("M,N,K", INT4_SIZES)
 def test_products_of_integers_are_exact(dev, M, N, K, t, group, zeros):
     """Small integers in x and powers of two as scales: every sum is exact in fp32 (K 31 3 4 below 2^24), the result its rounding."""
     x = ints((M, K), 2, M + K, t, dev)
@@ -64,7 +59,7 @@ def test_products_of_integers_are_exact(dev, M, N, K, t, group, zeros):
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("t", TYPES, ids=str)
-@pytest.mark.parametrize("M,N,K", [(1, 264, 2048), (16, 2048, 5632), (20, 520, 1999), (77, 1031, 1040), (1000, 1040, 2056)])
+@pytest.mark.parametrize("M,N,K", [(1, 264, 2048), (16, 2048, 5632), (20, 520, 1999), (77, 1031, 1040), (1000, 1040, 2056), (2100, 2056, 392)])
 def test_products(dev, M, N, K, t, group, zeros):
     """Within the bound, and in all as near as the rounding of the result: fp32 sums add less than 1e-5 of it."""
     x = normals((M, K), M, t, dev)
@@ -102,7 +97,7 @@ def test_strides_shapes_and_padding(dev):
 
 def test_rows_do_not_touch_each_other(dev):
     """An infinity or NaN stays in its row."""
-    for M in (5, 40):
+    for M in (5, 40, 5000):
         x = normals((M, 256), M, torch.float16, dev)
         c, s, _ = ops.quantize_int4_weight(normals((48, 256), 1, torch.float16, dev))
         clean = ops.linear_int4(x, c, s)
@@ -132,7 +127,7 @@ def test_refusals(dev):
         ops.linear_int4(x, c, s, group_size=32)
 
 
-@pytest.mark.parametrize("M", [3, 100])
+@pytest.mark.parametrize("M", [3, 100, 5000])
 def test_captured_and_on_another_stream(dev, M):
     x = normals((M, 400), 0, torch.bfloat16, dev)
     c, s, z = ops.quantize_int4_weight(normals((136, 400), 1, torch.bfloat16, dev), 64, True)

@@ -1,11 +1,12 @@
 """CPU tests of the 4-bit layer, clipping and the expert order: what is refused before anything is launched, and the 64-bit forms that the GPU tests compare with."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 from mortar_amd import _lib, ops
-from operators_util import draw_ids, expert_order, int4_weight, pack_codes, quantize_reference, unpack_codes
+from operators_util import INT4_SIZES, draw_ids, expert_order, int4_weight, pack_codes, quantize_reference, unpack_codes
 
 A = 1 << 20                                   # an aligned address that is never read: every call here is refused
 
@@ -20,14 +21,31 @@ def test_int4_linear_refuses():
     call = lambda **k: f(*{**base, **k}.values())
     for bad in (dict(M=-1), dict(K=0), dict(N=0), dict(type=2), dict(s_type=1), dict(s_type=3), dict(group=16), dict(group=0), dict(group=256), dict(x=None), dict(x=A + 2),
                 dict(K=60), dict(ldx=60), dict(M=2, ldx=56), dict(c=None), dict(c=A + 4), dict(ldc=4), dict(ldc=9), dict(s=None), dict(y=None), dict(y=A + 1), dict(ldy=15),
-                dict(s_n=-1), dict(s_g=-1), dict(z_n=-1), dict(z_g=-1), dict(M=33, ldy=16)):
+                dict(s_n=-1), dict(s_g=-1), dict(z_n=-1), dict(z_g=-1), dict(M=5000, ldy=16)):
         _refused(call(**bad))
     _refused(call(ldc=1 << 22), -4)
     _refused(call(ldx=1 << 23), -4)
     _refused(call(N=1 << 24, ldy=1 << 24), -4)
     assert call(M=0, x=None, c=None, s=None, y=None) == 0
     ws = _lib.lib().mortar_int4_workspace_bytes
-    assert ws(1, 16, 64, 32) == 0 and ws(0, 16, 64, 32) == 0 and ws(4096, 16, 64, 32) == 4 * 2 * (4096 + 2 * 128)
+    assert ws(1, 16, 64, 32) == 0 and ws(0, 16, 64, 32) == 0 and ws(5000, 16, 64, 32) == 4 * 2 * (5120 + 2 * 128)
+
+
+def _form(M, N, K, group):
+    v = [C.c_int32() for _ in range(3)]
+    assert _lib.lib().mortar_int4_form_host(M, N, K, group, *[C.byref(i) for i in v]) == 0
+    return tuple(i.value for i in v)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_sizes_reach_every_form(group):
+    """Rows of x through LDS, straight from memory, and tiles."""
+    few = [(16, 16, -8), (16, 16, -16), (32, 16, -16)] + [(16 * f, 16, w) for f in (1, 2, 4) for w in (8, 16)]
+    assert {_form(*s, group) for s in INT4_SIZES} == {*few, (64, 64, 8), (128, 128, 8)}
+    f = _lib.lib().mortar_int4_form_host
+    _refused(f(0, 16, 64, group, A, A, A))
+    _refused(f(1, 16, 64, 16, A, A, A))
+    _refused(f(1, 16, 64, group, None, A, A))
 
 
 def test_int4_quantize_refuses():
