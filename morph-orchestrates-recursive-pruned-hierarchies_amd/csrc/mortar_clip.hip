@@ -6,11 +6,13 @@
 //
 // A launch takes the table of up to 128 tensors as its argument, so nothing is copied to the device and a captured launch keeps what it needs.  Tensors
 // are cut into chunks of 16 KB that no two tensors share, a workgroup takes a run of chunks and leaves one partial sum in a slot of its own; the
-// slots are added in a fixed order, so that a call gives the same bits every time.
+// slots are added in a fixed order, so that a call gives the same bits every time.  Neighbouring workgroups take neighbouring chunks (a run of chunks for each
+// instead: 51 -> 55 us for the 82 MB above).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <cmath>
+#include <memory>
+#include <new>
 
 #include "mortar_device.h"
 #include "mortar_internal.h"
@@ -19,17 +21,19 @@ namespace {
 
 constexpr int TENSORS = 128;             // of a launch: the table fits a kernel's 4 KB of arguments
 constexpr int CHUNK_BYTES = 16384;       // of gradients
-constexpr int MOST_WORKGROUPS = 2048;    // 8 per CU
+constexpr int MOST_WORKGROUPS = 1024;    // 4 per CU: 380 MB in 194 us, with 8 in 194, with 32 in 209
+constexpr int MOST_SLOTS = 2048;         // that every workgroup of the clipping adds for itself
 
 struct Table {
     const void *src[TENSORS];
     void *dst[TENSORS];
-    int64_t n[TENSORS];
-    int32_t first[TENSORS + 1];          // chunks in front of each tensor's
-    uint8_t type[TENSORS];               // of the gradients, and of the results << 4
+    int64_t size[TENSORS];               // values, and << 48 the type of the gradients, and << 52 of the results (a table of bytes would be read by scalar
+                                         // loads from addresses whose parts are no multiples of 4, and those lose their lower bits)
+    int32_t first[TENSORS + 1];          // chunks in front of each tensor's; all of them behind the last
     int32_t count;
 };
 static_assert(sizeof(Table) <= 4000, "a kernel's arguments");
+constexpr int64_t SIZE_MASK = (INT64_C(1) << 48) - 1;
 
 // Gradients are parts of flat buffers: their addresses need not be multiples of 16.
 typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
@@ -80,21 +84,20 @@ struct Values {
     }
 };
 
-// The run of chunks of a workgroup, tensor by tensor: f(tensor, first value, values).  All of it is the same for all lanes.
+// The chunks of a workgroup, every gridDim.x-th one, from the last to the first with `back`: f(tensor, its types, first value, values).  All of it is the same for all
+// lanes.  A lane keeps two of the table's counts, and a chunk's tensor is found with two ballots (reading the table from its front took the
+// 500 odd tensors of a call 3 us a launch).
 template <typename F>
-__device__ __forceinline__ void each_chunk(const Table &t, F f) {
-    const int64_t all = t.first[t.count];
-    const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
-    int i = 0;
-    for (int lo = 0, hi = t.count; lo < hi;) {          // the last tensor that starts at or in front of `begin` and has chunks
-        const int mid = (lo + hi) >> 1;
-        if (t.first[mid + 1] > begin) hi = i = mid;
-        else lo = mid + 1;
-    }
-    for (int c = begin; c < end; ++c) {
-        while (t.first[i + 1] <= c) ++i;
-        const int64_t per = CHUNK_BYTES / ((t.type[i] & 15) == MORTAR_FP32 ? 4 : 2), at = (c - t.first[i]) * per, left = t.n[i] - at;
-        f(i, at, (int)(left < per ? left : per));
+__device__ __forceinline__ void each_chunk(const Table &t, bool back, F f) {
+    const int all = t.first[TENSORS], lane = threadIdx.x & 63;
+    const int f0 = t.first[lane + 1], f1 = t.first[lane + 65];
+    for (int k = blockIdx.x; k < all; k += gridDim.x) {
+        const int c = back ? all - 1 - k : k;
+        const int i = __popcll(__ballot(f0 <= c)) + __popcll(__ballot(f1 <= c));
+        const int64_t size = t.size[i];
+        const int types = (int)(size >> 48);
+        const int64_t per = CHUNK_BYTES / ((types & 15) == MORTAR_FP32 ? 4 : 2), at = (c - t.first[i]) * per, left = (size & SIZE_MASK) - at;
+        f(i, types, at, (int)(left < per ? left : per));
     }
 }
 
@@ -162,8 +165,8 @@ __device__ __forceinline__ void take_chunk(R (&r)[2], const void *base, int64_t 
 template <typename R>
 __global__ __launch_bounds__(256) void grad_norm_kernel(const Table t, uint64_t *slots) {
     R r[2];
-    each_chunk(t, [&](int i, int64_t at, int n) {
-        const int type = t.type[i] & 15;
+    each_chunk(t, false, [&](int i, int types, int64_t at, int n) {
+        const int type = types & 15;
         if (type == MORTAR_BF16) take_chunk<R, MORTAR_BF16>(r, t.src[i], at, n);
         else if (type == MORTAR_FP16) take_chunk<R, MORTAR_FP16>(r, t.src[i], at, n);
         else take_chunk<R, MORTAR_FP32>(r, t.src[i], at, n);
@@ -184,15 +187,20 @@ __device__ __forceinline__ double join_slots(const uint64_t *slots, int count) {
     __syncthreads();
     return norm;
 }
+// The norm, and (not null) the slot that all of them make.
 template <typename R>
-__global__ __launch_bounds__(256) void grad_join_kernel(const uint64_t *slots, int count, float *norm_out) {
-    const double n = join_slots<R>(slots, count);
-    if (threadIdx.x == 0) *norm_out = (float)n;
+__global__ __launch_bounds__(256) void grad_join_kernel(const uint64_t *slots, int count, float *norm_out, uint64_t *joined) {
+    R r;
+    for (int i = threadIdx.x; i < count; i += 256) r.join(slots[i]);
+    join_workgroup(r);
+    if (threadIdx.x) return;
+    if (norm_out) *norm_out = (float)r.norm();
+    if (joined) *joined = r.bits();
 }
 
 // ---- clipping --------------------------------------------------------------------------------------------------------
 
-template <int TYPE, int OUT>
+template <int TYPE, int OUT, bool STREAM>
 __device__ __forceinline__ void scale_chunk(const void *base, void *out, int64_t at, int n, float c) {
     using V = Values<TYPE>;
     using O = Values<OUT>;
@@ -207,7 +215,9 @@ __device__ __forceinline__ void scale_chunk(const void *base, void *out, int64_t
             float f[O::UNIT];
 #pragma unroll
             for (int j = 0; j < O::UNIT; ++j) f[j] = v[k * O::UNIT + j] * c;
-            reinterpret_cast<u32x4_any_t *>(q)[u * (V::UNIT / O::UNIT) + k] = O::pack(f);
+            u32x4_any_t *to = reinterpret_cast<u32x4_any_t *>(q) + u * (V::UNIT / O::UNIT) + k;
+            if constexpr (STREAM) __builtin_nontemporal_store((u32x4_any_t)O::pack(f), to);
+            else *to = O::pack(f);
         }
     };
     if (n == CHUNK_BYTES / V::SIZE) {
@@ -223,22 +233,24 @@ __device__ __forceinline__ void scale_chunk(const void *base, void *out, int64_t
     }
 }
 
-// Every workgroup adds the slots for itself: a launch less than with a kernel that does it once.
-template <typename R>
+// Every workgroup adds the slots for itself: a launch less than with a kernel that does it once.  The chunks are taken in the opposite order, those
+// first that the norm read last and the caches still hold.  STREAM: results that the L2s cannot hold go past the caches, which keep the gradients then
+// (a block of 39 M values, 82 MB, 51 -> 40 us with its norm; 380 MB 227 -> 194, of that 33 by the order).
+template <typename R, bool STREAM>
 __global__ __launch_bounds__(256) void grad_clip_kernel(const Table t, const uint64_t *slots, int count, double max_norm, float *norm_out) {
     const double n = join_slots<R>(slots, count);
     if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)n;
     double ratio = max_norm / (n + 1e-6);
     if (ratio > 1.0) ratio = 1.0;                        // (NaN stays)
     const float c = (float)ratio;
-    each_chunk(t, [&](int i, int64_t at, int n) {
+    each_chunk(t, true, [&](int i, int types, int64_t at, int n) {
         if (c == 1.0f && t.dst[i] == t.src[i]) return;   // in place, and nothing changes
-        switch (t.type[i]) {
-            case MORTAR_BF16 | MORTAR_BF16 << 4: scale_chunk<MORTAR_BF16, MORTAR_BF16>(t.src[i], t.dst[i], at, n, c); break;
-            case MORTAR_FP16 | MORTAR_FP16 << 4: scale_chunk<MORTAR_FP16, MORTAR_FP16>(t.src[i], t.dst[i], at, n, c); break;
-            case MORTAR_BF16 | MORTAR_FP32 << 4: scale_chunk<MORTAR_BF16, MORTAR_FP32>(t.src[i], t.dst[i], at, n, c); break;
-            case MORTAR_FP16 | MORTAR_FP32 << 4: scale_chunk<MORTAR_FP16, MORTAR_FP32>(t.src[i], t.dst[i], at, n, c); break;
-            default: scale_chunk<MORTAR_FP32, MORTAR_FP32>(t.src[i], t.dst[i], at, n, c);
+        switch (types) {
+            case MORTAR_BF16 | MORTAR_BF16 << 4: scale_chunk<MORTAR_BF16, MORTAR_BF16, STREAM>(t.src[i], t.dst[i], at, n, c); break;
+            case MORTAR_FP16 | MORTAR_FP16 << 4: scale_chunk<MORTAR_FP16, MORTAR_FP16, STREAM>(t.src[i], t.dst[i], at, n, c); break;
+            case MORTAR_BF16 | MORTAR_FP32 << 4: scale_chunk<MORTAR_BF16, MORTAR_FP32, STREAM>(t.src[i], t.dst[i], at, n, c); break;
+            case MORTAR_FP16 | MORTAR_FP32 << 4: scale_chunk<MORTAR_FP16, MORTAR_FP32, STREAM>(t.src[i], t.dst[i], at, n, c); break;
+            default: scale_chunk<MORTAR_FP32, MORTAR_FP32, STREAM>(t.src[i], t.dst[i], at, n, c);
         }
     });
 }
@@ -280,45 +292,54 @@ int64_t fill(Table &t, const mortar_grad_t *g, int64_t count, int64_t at) {
         const int i = t.count++;
         t.src[i] = g[at].src;
         t.dst[i] = g[at].dst;
-        t.n[i] = g[at].n;
-        t.type[i] = (uint8_t)(g[at].type | (g[at].out_type & 15) << 4);
+        t.size[i] = g[at].n | (int64_t)(g[at].type | (g[at].out_type & 15) << 4) << 48;
         t.first[i + 1] = t.first[i] + (int32_t)chunks;
     }
+    std::fill(t.first + t.count + 1, t.first + TENSORS + 1, t.first[t.count]);
     return at;
 }
 int workgroups(const Table &t) { return std::min(t.first[t.count], MOST_WORKGROUPS); }
 
-// Slots of all launches of the norm.
-int64_t slots_of(const mortar_grad_t *g, int64_t count) {
+// Slots of all launches of the norm, and (not null) how many launches.
+int64_t slots_of(const mortar_grad_t *g, int64_t count, int64_t *launches = nullptr) {
     Table t;
-    int64_t all = 0;
-    for (int64_t at = 0; at < count;) {
+    int64_t all = 0, n = 0;
+    for (int64_t at = 0; at < count; ++n) {
         at = fill(t, g, count, at);
         all += workgroups(t);
     }
+    if (launches) *launches = n;
     return all;
 }
 
 template <typename R>
 int run(const mortar_grad_t *g, int64_t count, bool clip, double max_norm, float *norm, uint64_t *slots, hipStream_t st, const char *what) {
     Table t;
-    int64_t used = 0;
-    for (int64_t at = 0; at < count;) {
+    int64_t used = 0, bytes = 0, launches = 0;
+    if (slots_of(g, count, &launches) >= INT32_MAX) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tensors", what);
+    const std::unique_ptr<int64_t[]> starts(new (std::nothrow) int64_t[launches + 1]);        // first tensor of each launch
+    if (!starts) return mortar_fail(MORTAR_ERR_LIMIT, "%s: no memory for the list of launches", what);
+    for (int64_t at = 0, k = 0; at < count;) {
+        starts[k++] = at;
         at = fill(t, g, count, at);
         if (!t.count) continue;
         hipLaunchKernelGGL(grad_norm_kernel<R>, dim3(workgroups(t)), dim3(256), 0, st, t, slots + used);
         used += workgroups(t);
         if (const int rc = launch_error(what)) return rc;
     }
-    if (used > INT32_MAX) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tensors", what);
-    if (!clip || !used) {
-        hipLaunchKernelGGL(grad_join_kernel<R>, dim3(1), dim3(256), 0, st, slots, (int)used, norm);
-        return launch_error(what);
+    if (!clip || !used || used > MOST_SLOTS) {
+        uint64_t *joined = clip && used ? slots + used : nullptr;
+        hipLaunchKernelGGL(grad_join_kernel<R>, dim3(1), dim3(256), 0, st, slots, (int)used, norm, joined);
+        if (const int rc = launch_error(what)) return rc;
+        if (!joined) return MORTAR_OK;
+        slots = joined, used = 1, norm = nullptr;
     }
-    for (int64_t at = 0; at < count;) {
-        at = fill(t, g, count, at);
+    for (int64_t i = 0; i < count; ++i) bytes += g[i].n * size_of(g[i].out_type);
+    const auto kern = bytes > 32 << 20 ? grad_clip_kernel<R, true> : grad_clip_kernel<R, false>;
+    for (int64_t k = launches; k-- > 0;) {
+        fill(t, g, count, starts[k]);
         if (!t.count) continue;
-        hipLaunchKernelGGL(grad_clip_kernel<R>, dim3(workgroups(t)), dim3(256), 0, st, t, slots, (int)used, max_norm, norm);
+        hipLaunchKernelGGL(kern, dim3(workgroups(t)), dim3(256), 0, st, t, slots, (int)used, max_norm, norm);
         norm = nullptr;
         if (const int rc = launch_error(what)) return rc;
     }
@@ -338,7 +359,7 @@ int grad(const mortar_grad_t *g, int64_t count, bool clip, int32_t largest, doub
 
 extern "C" int64_t mortar_grad_workspace_bytes(const mortar_grad_t *grads, int64_t count) {
     if (const int rc = check("grad_workspace", grads, count, false)) return rc;
-    return 8 * slots_of(grads, count);
+    return 8 * (slots_of(grads, count) + 1);
 }
 extern "C" int mortar_grad_norm(const mortar_grad_t *grads, int64_t count, int32_t largest, float *norm, void *workspace, void *stream) {
     return grad(grads, count, false, largest, 0.0, norm, workspace, stream, "grad_norm");

@@ -23,44 +23,47 @@ int launch_error(const char *what) {
 }
 
 // ---- sort ------------------------------------------------------------------------------------------------------------
-// Up to SORT_BLOCKS workgroups of 16 waves, each with a run of slots: first they count the slots per expert, then each of them adds up what lies in
-// front of its own (the experts in front, the runs in front) and places its slots.  The counts of a run are kept per wave; within a wave's 64 slots
-// the order is found with one ballot per bit of the expert's number.  Few slots are one workgroup's, in one launch.
-constexpr int SORT_WAVES = 16, SORT_BLOCKS = 64, SORT_ALONE = 4096;
+// Workgroups of 16 waves, each with a run of slots: first they count the slots per expert, then each of them adds up what lies in front of its own (the
+// experts in front, the runs in front) and places its slots.  A wave owns 64 HELD consecutive slots and keeps their experts in registers; the counts of a
+// run are kept per wave, so that the order within a run needs nothing of other waves but their counts, and within 64 slots it is found with one
+// ballot per bit of the expert's number.  Few slots are one workgroup's, in one launch.  Both launches are chains of latencies: ids, counts, sums.
+constexpr int SORT_WAVES = 16, SORT_THREADS = SORT_WAVES * 64, SORT_ALONE = 4096, SORT_BLOCKS = 64;
 
 template <typename ID>
 struct Slots {
     const ID *ids;
     int64_t n;
     int experts;
-    __device__ __forceinline__ int key(int64_t i) const {
-        const ID v = ids[i];
-        return v >= 0 && v < experts ? (int)v : experts;
-    }
 };
 
-// counts[e] of the slots [first, last) of each wave: one row of `counts` per wave, in LDS and zeroed here.
-template <typename ID>
-__device__ __forceinline__ void count_run(const Slots<ID> &s, int64_t first, int64_t last, int *counts) {
+// The experts of this wave's slots, from `at` on (-1: no slot), and counts[e] of them: one row of `counts` per wave, in LDS and zeroed here.
+template <typename ID, int HELD>
+__device__ __forceinline__ void count_run(const Slots<ID> &s, int64_t at, int (&key)[HELD], int *counts) {
     const int keys = s.experts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < keys * SORT_WAVES; i += SORT_WAVES * 64) counts[i] = 0;
-    __syncthreads();
-    const int64_t per = (last - first + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) * 64, begin = first + wave * per;
-    for (int64_t i = begin + lane; i < min(begin + per, last); i += 64) atomicAdd(&counts[wave * keys + s.key(i)], 1);
+    ID id[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) id[h] = at + h * 64 + lane < s.n ? s.ids[at + h * 64 + lane] : 0;
+    for (int i = lane; i < keys; i += 64) counts[wave * keys + i] = 0;          // (a wave's row is its own)
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        key[h] = at + h * 64 + lane < s.n ? (id[h] >= 0 && id[h] < s.experts ? (int)id[h] : s.experts) : -1;
+        if (key[h] >= 0) atomicAdd(&counts[wave * keys + key[h]], 1);
+    }
     __syncthreads();
 }
 
-template <typename ID>
-__global__ __launch_bounds__(SORT_WAVES * 64) void expert_count_kernel(const Slots<ID> s, int64_t run, int32_t *totals) {
+// totals [expert][run]: those of one expert lie together, where a thread reads them.
+template <typename ID, int HELD>
+__global__ __launch_bounds__(SORT_THREADS) void expert_count_kernel(const Slots<ID> s, int32_t *totals) {
     extern __shared__ int counts[];
     const int keys = s.experts + 1;
-    const int64_t first = blockIdx.x * run, last = min(first + run, s.n);
-    count_run(s, first, last, counts);
-    for (int e = threadIdx.x; e < keys; e += SORT_WAVES * 64) {
+    int key[HELD];
+    count_run(s, ((int64_t)blockIdx.x * SORT_WAVES + (threadIdx.x >> 6)) * 64 * HELD, key, counts);
+    for (int e = threadIdx.x; e < keys; e += SORT_THREADS) {
         int sum = 0;
 #pragma unroll
         for (int w = 0; w < SORT_WAVES; ++w) sum += counts[w * keys + e];
-        totals[(int64_t)blockIdx.x * keys + e] = sum;
+        totals[(int64_t)e * gridDim.x + blockIdx.x] = sum;
     }
 }
 
@@ -76,99 +79,127 @@ __device__ __forceinline__ int scan_workgroup(int v, int *part) {
     if (lane == 63) part[wave] = sum;
     __syncthreads();
     int base = 0;
-    for (int w = 0; w < wave; ++w) base += part[w];
-    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; ++w) base += w < wave ? part[w] : 0;
     return base + sum - v;
 }
 
 // ALONE: one workgroup has all slots and no totals of others.
-template <typename ID, bool ALONE>
-__global__ __launch_bounds__(SORT_WAVES * 64) void expert_place_kernel(const Slots<ID> s, int64_t run, int slots_per_token, const int32_t *totals, int32_t *position,
-                                                                       int32_t *token, int32_t *offsets) {
+template <typename ID, int HELD, bool ALONE>
+__global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const Slots<ID> s, uint32_t slots_per_token, const int32_t *totals, int32_t *position, int32_t *token,
+                                                                    int32_t *offsets) {
     extern __shared__ int counts[];
-    __shared__ int part[SORT_WAVES];
+    __shared__ int part[2][SORT_WAVES];
     const int keys = s.experts + 1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t first = blockIdx.x * run, last = min(first + run, s.n);
-    count_run(s, first, last, counts);
-    // Rows in front of this workgroup's slots of an expert, and from them those of each wave: in place of the counts.
-    for (int e0 = 0, before = 0; e0 < keys; e0 += SORT_WAVES * 64) {
-        const int e = e0 + threadIdx.x;
-        int all = 0, mine = 0;
-        if (e < keys) {
-            if constexpr (ALONE) {
-                for (int w = 0; w < SORT_WAVES; ++w) all += counts[w * keys + e];
-            } else {
-                for (int b = 0; b < (int)gridDim.x; ++b) {
-                    const int c = totals[(int64_t)b * keys + e];
-                    if (b < (int)blockIdx.x) mine += c;
-                    all += c;
-                }
+    const int64_t at = ((int64_t)blockIdx.x * SORT_WAVES + wave) * 64 * HELD;
+    int all[2] = {0, 0}, mine[2] = {0, 0};               // of experts threadIdx.x and (the one key beyond 1024) threadIdx.x + 1024
+    if constexpr (!ALONE) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int e = threadIdx.x + k * SORT_THREADS;
+            if (e >= keys) continue;
+            const int32_t *t = totals + (int64_t)e * gridDim.x;
+            for (int b = 0; b < (int)gridDim.x; ++b) {
+                const int c = t[b];
+                if (b < (int)blockIdx.x) mine[k] += c;
+                all[k] += c;
             }
         }
-        const int front = before + scan_workgroup(all, part);
+    }
+    int key[HELD];
+    count_run(s, at, key, counts);
+    // Rows in front of this workgroup's slots of an expert, and from them those of each wave: in place of the counts.
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int e = threadIdx.x + k * SORT_THREADS;
+        if (k * SORT_THREADS >= keys) break;
+        int c[SORT_WAVES];
         if (e < keys) {
-            int at = front + mine;
 #pragma unroll
             for (int w = 0; w < SORT_WAVES; ++w) {
-                const int c = counts[w * keys + e];
-                counts[w * keys + e] = at;
-                at += c;
+                c[w] = counts[w * keys + e];
+                if (ALONE) all[k] += c[w];
+            }
+        }
+        const int front = before + scan_workgroup(all[k], part[k]);
+        if (e < keys) {
+            int row = front + mine[k];
+#pragma unroll
+            for (int w = 0; w < SORT_WAVES; ++w) {
+                counts[w * keys + e] = row;
+                row += c[w];
             }
             if (blockIdx.x == 0) offsets[e] = front;
         }
-        if (e0 + SORT_WAVES * 64 < keys) {               // (more keys than threads: 1025)
-            if (threadIdx.x == SORT_WAVES * 64 - 1) part[0] = front + all;
-            __syncthreads();
-            before = part[0];
-            __syncthreads();
+        if (k == 0) {
+#pragma unroll
+            for (int w = 0; w < SORT_WAVES; ++w) before += part[0][w];
         }
     }
     __syncthreads();
     const int bits = 32 - __builtin_clz(s.experts);
     int *next = counts + wave * keys;
-    const int64_t per = (last - first + SORT_WAVES * 64 - 1) / (SORT_WAVES * 64) * 64, begin = first + wave * per, end = min(begin + per, last);
-    for (int64_t i0 = begin; i0 < end; i0 += 64) {
-        const int64_t i = i0 + lane;
-        const bool on = i < end;
-        const int key = on ? s.key(i) : 0;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int64_t i = at + h * 64 + lane;
+        const bool on = key[h] >= 0;
         uint64_t same = __ballot(on);
         for (int b = 0; b < bits; ++b) {
-            const uint64_t set = __ballot(key >> b & 1);
-            same &= key >> b & 1 ? set : ~set;
+            const uint64_t set = __ballot(key[h] >> b & 1);
+            same &= key[h] >> b & 1 ? set : ~set;
         }
         const int rank = __popcll(same & ((UINT64_C(1) << lane) - 1));
-        int at = 0;
-        if (on) at = __hip_atomic_load(next + key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) + rank;
+        int row = 0;
+        if (on) row = __hip_atomic_load(next + key[h], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) + rank;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (on && (same >> lane) == 1) __hip_atomic_store(next + key, at + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);      // the last lane of its expert
+        if (on && same >> lane == 1) __hip_atomic_store(next + key[h], row + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);      // the last lane of its expert
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (on) {
-            position[i] = at;
-            token[at] = (int32_t)(i / slots_per_token);
+            position[i] = row;
+            token[row] = (int32_t)((uint32_t)i / slots_per_token);
         }
     }
 }
 
-template <typename ID>
-int sort(const Slots<ID> &s, int slots_per_token, int32_t *position, int32_t *token, int32_t *offsets, int32_t *totals, hipStream_t st, const char *what) {
+// Slots that a lane holds: a power of two, so that there are at most SORT_BLOCKS runs up to 2^20 slots.
+int held_of(int64_t n) {
+    for (const int held : {2, 4, 8})
+        if (n <= (int64_t)SORT_BLOCKS * SORT_THREADS * held) return held;
+    return 16;
+}
+
+template <typename ID, int HELD>
+int sort_held(const Slots<ID> &s, int slots_per_token, int32_t *position, int32_t *token, int32_t *offsets, int32_t *totals, hipStream_t st, const char *what) {
     const int smem = (s.experts + 1) * SORT_WAVES * 4;
-    const auto room = [&](const void *kern) { return hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (MOST_EXPERTS + 1) * SORT_WAVES * 4); };
+    const auto room = [&](const void *kern) {
+        return smem <= 64 * 1024 ? hipSuccess : hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (MOST_EXPERTS + 1) * SORT_WAVES * 4);
+    };
     if (s.n <= SORT_ALONE) {
-        const auto kern = expert_place_kernel<ID, true>;
+        const auto kern = expert_place_kernel<ID, HELD, true>;
         if (const hipError_t e = room(reinterpret_cast<const void *>(kern)); e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-        hipLaunchKernelGGL(kern, dim3(1), dim3(SORT_WAVES * 64), smem, st, s, s.n, slots_per_token, nullptr, position, token, offsets);
+        hipLaunchKernelGGL(kern, dim3(1), dim3(SORT_THREADS), smem, st, s, (uint32_t)slots_per_token, nullptr, position, token, offsets);
         return launch_error(what);
     }
-    const int64_t run = std::max<int64_t>(2048, ((s.n + SORT_BLOCKS - 1) / SORT_BLOCKS + 63) / 64 * 64);
-    const unsigned blocks = (unsigned)((s.n + run - 1) / run);
-    const auto count = expert_count_kernel<ID>;
-    const auto place = expert_place_kernel<ID, false>;
+    const unsigned blocks = (unsigned)((s.n + SORT_THREADS * HELD - 1) / (SORT_THREADS * HELD));
+    const auto count = expert_count_kernel<ID, HELD>;
+    const auto place = expert_place_kernel<ID, HELD, false>;
     for (const void *kern : {reinterpret_cast<const void *>(count), reinterpret_cast<const void *>(place)})
         if (const hipError_t e = room(kern); e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-    hipLaunchKernelGGL(count, dim3(blocks), dim3(SORT_WAVES * 64), smem, st, s, run, totals);
+    hipLaunchKernelGGL(count, dim3(blocks), dim3(SORT_THREADS), smem, st, s, totals);
     if (const int rc = launch_error(what)) return rc;
-    hipLaunchKernelGGL(place, dim3(blocks), dim3(SORT_WAVES * 64), smem, st, s, run, slots_per_token, totals, position, token, offsets);
+    hipLaunchKernelGGL(place, dim3(blocks), dim3(SORT_THREADS), smem, st, s, (uint32_t)slots_per_token, totals, position, token, offsets);
     return launch_error(what);
+}
+template <typename ID>
+int sort(const Slots<ID> &s, int slots_per_token, int32_t *position, int32_t *token, int32_t *offsets, int32_t *totals, hipStream_t st, const char *what) {
+    if (s.n <= SORT_ALONE) return s.n <= 1024 ? sort_held<ID, 1>(s, slots_per_token, position, token, offsets, totals, st, what) : sort_held<ID, 4>(s, slots_per_token, position, token, offsets, totals, st, what);
+    switch (held_of(s.n)) {
+        case 2: return sort_held<ID, 2>(s, slots_per_token, position, token, offsets, totals, st, what);
+        case 4: return sort_held<ID, 4>(s, slots_per_token, position, token, offsets, totals, st, what);
+        case 8: return sort_held<ID, 8>(s, slots_per_token, position, token, offsets, totals, st, what);
+        default: return sort_held<ID, 16>(s, slots_per_token, position, token, offsets, totals, st, what);
+    }
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
@@ -378,7 +409,9 @@ int check_pointer(const char *what, const char *name, const void *p, int32_t typ
 }  // namespace
 
 extern "C" int64_t mortar_expert_sort_workspace_bytes(int64_t slots, int32_t n_experts) {
-    return slots <= SORT_ALONE || n_experts <= 0 ? 0 : INT64_C(4) * SORT_BLOCKS * (n_experts + 1);
+    if (slots <= SORT_ALONE || n_experts <= 0) return 0;
+    const int64_t run = SORT_THREADS * held_of(slots);
+    return 4 * ((slots + run - 1) / run) * (n_experts + 1);
 }
 
 extern "C" int mortar_expert_sort(const void *ids, int32_t ids_64, int64_t N, int32_t k, int32_t n_experts, int32_t *position, int32_t *token, int32_t *offsets,

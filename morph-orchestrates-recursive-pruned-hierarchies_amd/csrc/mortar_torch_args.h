@@ -34,10 +34,11 @@ void check_rc(int rc, const char *what) {
 }
 
 // Kinds of tensors whose values a kernel launched on their address would miss.
-c10::DispatchKeySet riders() {
+const c10::DispatchKeySet &riders() {
     using K = c10::DispatchKey;
-    return c10::DispatchKeySet({K::Python, K::PythonTLSSnapshot, K::FuncTorchGradWrapper, K::FuncTorchBatched, K::FuncTorchDynamicLayerFrontMode,
+    static const c10::DispatchKeySet keys({K::Python, K::PythonTLSSnapshot, K::FuncTorchGradWrapper, K::FuncTorchBatched, K::FuncTorchDynamicLayerFrontMode,
                                 K::FuncTorchDynamicLayerBackMode, K::Batched, K::Functionalize, K::Conjugate, K::Negative, K::ZeroTensor, K::Tracer});
+    return keys;
 }
 
 bool plain_values(const at::Tensor &t) { return !t.key_set().has_any(riders()) && t.layout() == at::kStrided; }

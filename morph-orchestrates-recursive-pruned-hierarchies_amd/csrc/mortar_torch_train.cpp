@@ -11,54 +11,68 @@ namespace {
 
 // ---- gradients -------------------------------------------------------------------------------------------------------
 
-std::vector<at::Tensor> tensor_list(PyObject *o, const char *what, const char *name) {
-    if (THPVariable_Check(o)) return {tensor_arg(o, what, name)};
-    THPObjectPtr owned(PySequence_Fast(o, "expected a sequence of tensors"));
-    PyObject *fast = owned.get();
-    if (!fast) throw python_error();
-    std::vector<at::Tensor> v;
-    v.reserve(PySequence_Fast_GET_SIZE(fast));
-    for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(fast); ++i) v.push_back(tensor_arg(PySequence_Fast_GET_ITEM(fast, i), what, name));
+// The tensors of a Python sequence (or a single one), which keeps them.
+struct TensorList {
+    THPObjectPtr sequence;
+    std::vector<const at::Tensor *> all;
+    size_t size() const { return all.size(); }
+    const at::Tensor &operator[](size_t i) const { return *all[i]; }
+};
+
+TensorList tensor_list(PyObject *o, const char *what, const char *name) {
+    TensorList v;
+    v.sequence = THPVariable_Check(o) ? PyTuple_Pack(1, o) : PySequence_Fast(o, "expected a sequence of tensors");
+    if (!v.sequence) throw python_error();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(v.sequence.get());
+    v.all.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) v.all.push_back(&tensor_arg(PySequence_Fast_GET_ITEM(v.sequence.get(), i), what, name));
     return v;
 }
 
-void check_grads(const std::vector<at::Tensor> &v, const char *what) {
-    for (const at::Tensor &t : v) {
-        TORCH_CHECK_TYPE(type_code(t.scalar_type()) >= 0, what, ": expected bfloat16, float16 or float32 gradients, got ", t.scalar_type());
-        TORCH_CHECK_VALUE(t.device() == v[0].device(), what, ": gradients on ", t.device(), " and on ", v[0].device());
-        TORCH_CHECK(!(c10::GradMode::is_enabled() && t.requires_grad()), what, ": no gradients flow through this call (detach the tensors or call under no_grad)");
+void check_grads(const TensorList &v, const char *what) {
+    const bool record = c10::GradMode::is_enabled();
+    for (const at::Tensor *t : v.all) {
+        TORCH_CHECK_TYPE(type_code(t->scalar_type()) >= 0, what, ": expected bfloat16, float16 or float32 gradients, got ", t->scalar_type());
+        TORCH_CHECK_VALUE(t->device() == v[0].device(), what, ": gradients on ", t->device(), " and on ", v[0].device());
+        TORCH_CHECK(!(record && t->requires_grad()), what, ": no gradients flow through this call (detach the tensors or call under no_grad)");
     }
 }
 
-// Memory of a tensor, from its first value to behind its last, and what happens to it while the kernels run.
+// Memory of a tensor, from its first value to behind its last.
 struct Span {
     uintptr_t begin, end;
     size_t i;
-    bool written;
 };
 
-// Nothing that is written is written twice, or read for another tensor.  drop: a gradient that is there twice is counted once (in place).
-void check_overlap(std::vector<mortar_grad_t> &list, std::vector<Span> spans, bool drop, const char *what) {
+// Nothing that is written is written twice, or read for another tensor.  drop: a gradient that is there twice is counted once (in place).  Tensors mostly
+// come in the order of their addresses, results and gradients each: two lists that are merged.
+void check_overlap(std::vector<mortar_grad_t> &list, std::vector<Span> read, bool drop, const char *what) {
+    std::vector<Span> written;
+    written.reserve(list.size());
+    read.reserve(read.size() + list.size());
     const auto size = [](int type) { return type == MORTAR_FP32 ? 4 : 2; };
     for (size_t i = 0; i < list.size(); ++i) {
         const mortar_grad_t &g = list[i];
         if (!g.n) continue;
         const uintptr_t s = reinterpret_cast<uintptr_t>(g.src), d = reinterpret_cast<uintptr_t>(g.dst);
-        spans.push_back({d, d + g.n * size(g.out_type), i, true});
-        if (s != d || g.type != g.out_type) spans.push_back({s, s + g.n * size(g.type), i, false});
+        written.push_back({d, d + g.n * size(g.out_type), i});
+        if (s != d || g.type != g.out_type) read.push_back({s, s + g.n * size(g.type), i});
     }
     const auto less = [](const Span &a, const Span &b) { return a.begin < b.begin; };
-    if (!std::is_sorted(spans.begin(), spans.end(), less)) std::stable_sort(spans.begin(), spans.end(), less);
-    uintptr_t any = 0, written = 0;
-    const Span *last = nullptr;                      // written
-    for (const Span &s : spans) {
-        if (drop && last && s.written && s.begin == last->begin && s.end == last->end && list[s.i].type == list[last->i].type) {
+    for (std::vector<Span> *v : {&written, &read})
+        if (!std::is_sorted(v->begin(), v->end(), less)) std::stable_sort(v->begin(), v->end(), less);
+    uintptr_t end_written = 0, end_read = 0;
+    const Span *last = nullptr;
+    for (auto w = written.begin(), r = read.begin(); w != written.end() || r != read.end();) {
+        const bool is_read = w == written.end() || (r != read.end() && r->begin < w->begin);
+        const Span &s = is_read ? *r++ : *w++;
+        if (!is_read && drop && last && s.begin == last->begin && s.end == last->end && list[s.i].type == list[last->i].type) {
             list[s.i].n = 0;
             continue;
         }
-        TORCH_CHECK_VALUE(s.begin >= (s.written ? any : written), what, ": results overlap each other or another gradient");
-        any = std::max(any, s.end);
-        if (s.written) written = std::max(written, s.end), last = &s;
+        TORCH_CHECK_VALUE(s.begin >= end_written && (is_read || s.begin >= end_read), what, ": results overlap each other or another gradient");
+        if (is_read) end_read = std::max(end_read, s.end);
+        else end_written = std::max(end_written, s.end), last = &s;
     }
 }
 
@@ -71,16 +85,17 @@ PyObject *empty_norm() {
 PyObject *py_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t na) {
     const char *what = "grad_norm";
     TORCH_CHECK_TYPE(na == 2, "grad_norm: 2 arguments");
-    const std::vector<at::Tensor> grads = tensor_list(a[0], what, "each gradient");
+    const TensorList grads = tensor_list(a[0], what, "each gradient");
     check_grads(grads, what);
-    if (grads.empty()) return empty_norm();
+    if (!grads.size()) return empty_norm();
     const c10::DeviceGuard guard(grads[0].device());
     std::vector<at::Tensor> held;
     std::vector<mortar_grad_t> list;
     list.reserve(grads.size());
-    for (const at::Tensor &g : grads) {
-        if (!g.is_non_overlapping_and_dense()) held.push_back(g.contiguous());
-        list.push_back({data(g.is_non_overlapping_and_dense() ? g : held.back()), nullptr, g.numel(), type_code(g.scalar_type()), 0});
+    for (const at::Tensor *g : grads.all) {
+        const bool flat = g->is_non_overlapping_and_dense();
+        if (!flat) held.push_back(g->contiguous());
+        list.push_back({data(flat ? *g : held.back()), nullptr, g->numel(), type_code(g->scalar_type()), 0});
     }
     at::Tensor norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
     const at::Tensor ws = empty_bytes(norm, std::max<int64_t>(8, mortar_grad_workspace_bytes(list.data(), (int64_t)list.size())));
@@ -93,25 +108,34 @@ PyObject *py_grad_norm(PyObject *, PyObject *const *a, Py_ssize_t na) {
 PyObject *py_grad_clip(PyObject *, PyObject *const *a, Py_ssize_t na) {
     const char *what = "clip_grads";
     TORCH_CHECK_TYPE(na == 4, "grad_clip: 4 arguments");
-    const std::vector<at::Tensor> grads = tensor_list(a[0], what, "each gradient");
+    const TensorList grads = tensor_list(a[0], what, "each gradient");
     const bool in_place = a[1] == Py_True, fresh = a[1] == Py_None;
-    std::vector<at::Tensor> out = in_place ? grads : fresh ? std::vector<at::Tensor>() : tensor_list(a[1], what, "each result");
     const double max_norm = PyFloat_AsDouble(a[2]);
     if (PyErr_Occurred()) throw python_error();
     check_grads(grads, what);
     TORCH_CHECK_VALUE(max_norm >= 0, what, ": max_norm is negative or NaN");
-    TORCH_CHECK_VALUE(fresh || out.size() == grads.size(), what, ": ", out.size(), " results for ", grads.size(), " gradients");
-    if (!fresh) check_grads(out, what);
+    TensorList out;
+    std::vector<at::Tensor> made;                        // results of its own
+    if (fresh) {
+        made.reserve(grads.size());
+        for (const at::Tensor *g : grads.all) {
+            const c10::DeviceGuard guard(g->device());
+            made.push_back(at::empty_like(*g, g->options().requires_grad(false)));
+            out.all.push_back(&made.back());
+        }
+    } else {
+        out = tensor_list(in_place ? a[0] : a[1], what, "each result");
+        TORCH_CHECK_VALUE(out.size() == grads.size(), what, ": ", out.size(), " results for ", grads.size(), " gradients");
+        check_grads(out, what);
+    }
     for (size_t i = 0; i < out.size(); ++i) {
         TORCH_CHECK_VALUE(out[i].sizes() == grads[i].sizes() && out[i].device() == grads[i].device(), what, ": result ", i, " has another shape or device than its gradient");
         TORCH_CHECK_TYPE(out[i].scalar_type() == grads[i].scalar_type() || out[i].scalar_type() == at::kFloat, what, ": result ", i, " must have the type of its gradient or float32");
-        TORCH_CHECK_VALUE(at::has_internal_overlap(out[i]) != at::MemOverlap::Yes, what, ": result ", i, " refers to one place several times");
+        TORCH_CHECK_VALUE(out[i].is_non_overlapping_and_dense() || at::has_internal_overlap(out[i]) != at::MemOverlap::Yes, what, ": result ", i, " refers to one place several times");
     }
     at::Tensor norm;
-    if (!grads.empty()) {
+    if (grads.size()) {
         const c10::DeviceGuard guard(grads[0].device());
-        if (fresh)
-            for (const at::Tensor &g : grads) out.push_back(at::empty_like(g, g.options().requires_grad(false)));
         std::vector<at::Tensor> held;                                // copies of gradients that do not fill their memory, and
         std::vector<std::pair<size_t, at::Tensor>> back;             // results that go to where they belong behind the launches
         std::vector<mortar_grad_t> list;
@@ -133,7 +157,7 @@ PyObject *py_grad_clip(PyObject *, PyObject *const *a, Py_ssize_t na) {
                 int64_t last = 0;
                 for (int64_t k = 0; k < o.dim(); ++k) last += (o.size(k) - 1) * o.stride(k);
                 const uintptr_t at = reinterpret_cast<uintptr_t>(o.const_data_ptr());
-                spans.push_back({at, at + (last + 1) * o.element_size(), i, false});
+                spans.push_back({at, at + (last + 1) * o.element_size(), i});
             }
             list.push_back({data(s), mut(d), g.numel(), type_code(g.scalar_type()), type_code(o.scalar_type())});
         }
@@ -144,11 +168,11 @@ PyObject *py_grad_clip(PyObject *, PyObject *const *a, Py_ssize_t na) {
         const at::NoGradGuard no_grad;
         for (const auto &b : back) out[b.first].copy_(b.second);
         if (!fresh)
-            for (const at::Tensor &o : out) torch::autograd::impl::bump_version(o);
+            for (const at::Tensor *o : out.all) torch::autograd::impl::bump_version(*o);
     }
-    PyObject *results = PyList_New((Py_ssize_t)out.size());
+    PyObject *results = fresh ? PyList_New((Py_ssize_t)out.size()) : PySequence_List(out.sequence.get());
     if (!results) throw python_error();
-    for (size_t i = 0; i < out.size(); ++i) PyList_SET_ITEM(results, (Py_ssize_t)i, THPVariable_Wrap(out[i]));
+    for (size_t i = 0; i < made.size(); ++i) PyList_SET_ITEM(results, (Py_ssize_t)i, THPVariable_Wrap(std::move(made[i])));
     PyObject *n = norm.defined() ? THPVariable_Wrap(std::move(norm)) : empty_norm();
     return Py_BuildValue("(NN)", results, n);
 }
