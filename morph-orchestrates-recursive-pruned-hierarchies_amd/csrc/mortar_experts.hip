@@ -99,10 +99,16 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const Slots<
             const int e = threadIdx.x + k * SORT_THREADS;
             if (e >= keys) continue;
             const int32_t *t = totals + (int64_t)e * gridDim.x;
-            for (int b = 0; b < (int)gridDim.x; ++b) {
-                const int c = t[b];
-                if (b < (int)blockIdx.x) mine[k] += c;
-                all[k] += c;
+            const int runs = gridDim.x, own = blockIdx.x;
+            for (int b = 0; b < runs; b += 16) {         // (sixteen loads on their way)
+                int c[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) c[i] = t[min(b + i, runs - 1)];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    mine[k] += b + i < own ? c[i] : 0;
+                    all[k] += b + i < runs ? c[i] : 0;
+                }
             }
         }
     }
@@ -206,6 +212,11 @@ int sort(const Slots<ID> &s, int slots_per_token, int32_t *position, int32_t *to
 // Rows are read and written in 16-byte units on whatever addresses they lie (odd widths: multiples of 2 bytes), what is left behind the last whole one
 // value by value.
 typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+template <bool STREAM>
+__device__ __forceinline__ void put16(char *p, u32x4_any_t w) {
+    if constexpr (STREAM) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any_t *>(p));
+    else *reinterpret_cast<u32x4_any_t *>(p) = w;
+}
 
 template <int TYPE>
 struct Row {
@@ -266,7 +277,7 @@ __device__ __forceinline__ float read_weight(const RowArgs &a, int64_t i) {
 }
 
 // A wave per slot; the rows of a token are read by neighbouring waves and come out of the caches but once.
-template <int SIZE>
+template <int SIZE, bool STREAM>
 __global__ __launch_bounds__(256) void expert_dispatch_kernel(const RowArgs a) {
     const int lane = threadIdx.x & 63;
     const uint32_t i = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -283,9 +294,9 @@ __global__ __launch_bounds__(256) void expert_dispatch_kernel(const RowArgs a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) v[q] = live ? *reinterpret_cast<const u32x4_any_t *>(src + (u + q * 64) * 16) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<u32x4_any_t *>(dst + (u + q * 64) * 16) = v[q];
+        for (int q = 0; q < 4; ++q) put16<STREAM>(dst + (u + q * 64) * 16, v[q]);
     }
-    for (; u < units; u += 64) *reinterpret_cast<u32x4_any_t *>(dst + u * 16) = live ? *reinterpret_cast<const u32x4_any_t *>(src + u * 16) : u32x4_t{0, 0, 0, 0};
+    for (; u < units; u += 64) put16<STREAM>(dst + u * 16, live ? *reinterpret_cast<const u32x4_any_t *>(src + u * 16) : u32x4_any_t{0, 0, 0, 0});
     const int at = units * 16 + lane * SIZE;
     if (at < bytes) {
         if constexpr (SIZE == 4) *reinterpret_cast<uint32_t *>(dst + at) = live ? *reinterpret_cast<const uint32_t *>(src + at) : 0u;
@@ -293,62 +304,105 @@ __global__ __launch_bounds__(256) void expert_dispatch_kernel(const RowArgs a) {
     }
 }
 
-// A wave per token and 64 units of the row; the rows of eight slots are on their way at a time.
-template <int TYPE>
+// A wave per TOKENS consecutive tokens and 64 units of their rows, the rows of eight slots on their way at a time: with few slots per token one token alone
+// leaves too little on the way (two slots of 768 values: 16384 tokens in 20 us, 14 with four tokens).  The wave's lanes hold the positions and weights of its slots.
+constexpr int NO_WEIGHT = 3;
+template <int TYPE, int WTYPE, int TOKENS>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const RowArgs a, int parts) {
     using R = Row<TYPE>;
+    constexpr int J = 8 / TOKENS;                        // slots of a token at a time
     const int lane = threadIdx.x & 63;
-    const uint32_t task = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int64_t n = task / (uint32_t)parts;
-    if (n * a.k >= a.slots) return;
-    const int unit = (int)(task - (uint32_t)n * parts) * 64 + lane, left = a.d - unit * R::UNIT;
+    const uint32_t task = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), group = task / (uint32_t)parts;
+    const int64_t first = (int64_t)group * TOKENS * a.k;  // slot
+    if (first >= a.slots) return;
+    const int unit = (int)(task - group * parts) * 64 + lane, left = a.d - unit * R::UNIT;
     const int64_t pitch = (int64_t)a.d * R::SIZE, in = (int64_t)unit * 16;
     const uint32_t full = min((uint32_t)*a.full, (uint32_t)a.slots);
-    float sum[R::UNIT];
+    const int mine = (int)min((int64_t)(TOKENS * a.k), a.slots - first);
+    float sum[TOKENS][R::UNIT];
 #pragma unroll
-    for (int v = 0; v < R::UNIT; ++v) sum[v] = 0.f;
-    for (int j0 = 0; j0 < a.k; j0 += 8) {
-        u32x4_t v[8];
-        float w[8];
-        uint32_t row[8];
+    for (int t = 0; t < TOKENS; ++t)
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            row[q] = j0 + q < a.k ? (uint32_t)a.position[n * a.k + j0 + q] : UINT32_MAX;
-            w[q] = row[q] < full ? read_weight(a, n * a.k + j0 + q) : 0.f;
+        for (int v = 0; v < R::UNIT; ++v) sum[t][v] = 0.f;
+    for (int s0 = 0; s0 < (TOKENS > 1 ? 1 : a.k); s0 += 64) {        // (several tokens: 8 slots in all)
+        int position = -1;
+        float weight = 1.0f;
+        if (s0 + lane < mine) {
+            position = a.position[first + s0 + lane];
+            if constexpr (WTYPE != NO_WEIGHT) weight = Row<WTYPE>::one(a.w + (first + s0 + lane) * (16 / Row<WTYPE>::UNIT));
         }
-        if (left >= R::UNIT) {
+        const int slots = TOKENS > 1 ? a.k : min(64, a.k - s0);
+        for (int j0 = 0; j0 < slots; j0 += J) {
+            u32x4_t v[TOKENS][J];
+            uint32_t row[TOKENS][J];
+            float w[TOKENS][J];
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (row[q] < full) v[q] = R::load(a.ys + row[q] * pitch + in);
+            for (int t = 0; t < TOKENS; ++t)
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (row[q] < full) {
-                    float f[R::UNIT];
-                    R::unpack(v[q], f);
-#pragma unroll
-                    for (int t = 0; t < R::UNIT; ++t) sum[t] = __builtin_fmaf(w[q], f[t], sum[t]);
+                for (int q = 0; q < J; ++q) {
+                    const int from = t * a.k + j0 + q;
+                    row[t][q] = j0 + q < slots ? (uint32_t)__builtin_amdgcn_readlane(position, from) : UINT32_MAX;
+                    w[t][q] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), from & 63));
                 }
-        } else {
-            for (int q = 0; q < 8; ++q)
-                if (row[q] < full) {
+            if (left >= R::UNIT) {
 #pragma unroll
-                    for (int t = 0; t < R::UNIT; ++t)
-                        if (t < left) sum[t] = __builtin_fmaf(w[q], R::one(a.ys + row[q] * pitch + in + t * R::SIZE), sum[t]);
-                }
+                for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+                    for (int q = 0; q < J; ++q)
+                        if (row[t][q] < full) v[t][q] = R::load(a.ys + row[t][q] * pitch + in);
+#pragma unroll
+                for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+                    for (int q = 0; q < J; ++q)
+                        if (row[t][q] < full) {
+                            float f[R::UNIT];
+                            R::unpack(v[t][q], f);
+#pragma unroll
+                            for (int u = 0; u < R::UNIT; ++u) sum[t][u] = __builtin_fmaf(w[t][q], f[u], sum[t][u]);
+                        }
+            } else {
+#pragma unroll
+                for (int t = 0; t < TOKENS; ++t)
+                    for (int q = 0; q < J; ++q)
+                        if (row[t][q] < full) {
+#pragma unroll
+                            for (int u = 0; u < R::UNIT; ++u)
+                                if (u < left) sum[t][u] = __builtin_fmaf(w[t][q], R::one(a.ys + row[t][q] * pitch + in + u * R::SIZE), sum[t][u]);
+                        }
+            }
         }
     }
-    char *dst = a.out + n * pitch + in;
-    if (left >= R::UNIT) {
-        R::store(dst, R::pack(sum));
-    } else {
 #pragma unroll
-        for (int t = 0; t < R::UNIT; ++t)
-            if (t < left) R::put(dst + t * R::SIZE, sum[t]);
+    for (int t = 0; t < TOKENS; ++t) {
+        if (t * a.k >= mine) break;
+        char *dst = a.out + ((int64_t)group * TOKENS + t) * pitch + in;
+        if (left >= R::UNIT) {
+            R::store(dst, R::pack(sum[t]));
+        } else {
+#pragma unroll
+            for (int u = 0; u < R::UNIT; ++u)
+                if (u < left) R::put(dst + u * R::SIZE, sum[t][u]);
+        }
     }
 }
 
-// A wave per slot: its row of dys, and the dot product over the row.
+template <int TYPE, int WTYPE>
+int launch_combine(const RowArgs &a, hipStream_t st, const char *what) {
+    const int per = 64 * Row<TYPE>::UNIT, parts = (a.d + per - 1) / per, tokens = a.k <= 2 ? 4 : a.k <= 4 ? 2 : 1;
+    const int64_t N = a.slots / a.k, groups = ((N + tokens - 1) / tokens * parts + 3) / 4;
+    if (groups >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
+    const auto kern = tokens == 4 ? expert_combine_kernel<TYPE, WTYPE, 4> : tokens == 2 ? expert_combine_kernel<TYPE, WTYPE, 2> : expert_combine_kernel<TYPE, WTYPE, 1>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, st, a, parts);
+    return launch_error(what);
+}
 template <int TYPE>
+int launch_combine_weights(const RowArgs &a, hipStream_t st, const char *what) {
+    if (!a.w) return launch_combine<TYPE, NO_WEIGHT>(a, st, what);
+    return a.w_type == MORTAR_FP32 ? launch_combine<TYPE, MORTAR_FP32>(a, st, what) : a.w_type == MORTAR_FP16 ? launch_combine<TYPE, MORTAR_FP16>(a, st, what) : launch_combine<TYPE, MORTAR_BF16>(a, st, what);
+}
+
+// A wave per slot: its row of dys, and the dot product over the row.
+template <int TYPE, bool STREAM>
 __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a) {
     using R = Row<TYPE>;
     const int lane = threadIdx.x & 63;
@@ -376,7 +430,7 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a
         if (a.out) {
 #pragma unroll
             for (int t = 0; t < R::UNIT; ++t) g[t] = live ? g[t] * w : 0.f;
-            R::store(a.out + at_row + (int64_t)u * 16, R::pack(g));
+            put16<STREAM>(a.out + at_row + (int64_t)u * 16, R::pack(g));
         }
     }
     const int last = units * R::UNIT + lane;
@@ -391,6 +445,15 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a
     if (a.w_type == MORTAR_FP32) Row<MORTAR_FP32>::put(a.dw + i * 4, dot);
     else if (a.w_type == MORTAR_FP16) Row<MORTAR_FP16>::put(a.dw + i * 2, dot);
     else Row<MORTAR_BF16>::put(a.dw + i * 2, dot);
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Rows by slot that the memory-side cache (256 MB) cannot hold for whoever reads them next are stored past it: 268 MB of fp32 dispatched in 63 -> 51 us.
+// Smaller ones gain little (134 MB 26.4 -> 25.7) and are read from there; rows on odd addresses lose (35 -> 43).
+bool past_caches(const RowArgs &a, int32_t type) {
+    const int64_t row = (int64_t)a.d * (type == MORTAR_FP32 ? 4 : 2);
+    return a.slots * row > 256 << 20 && row % 16 == 0 && aligned16(a.out);
 }
 
 bool known(int32_t type) { return type == MORTAR_BF16 || type == MORTAR_FP16 || type == MORTAR_FP32; }
@@ -444,8 +507,9 @@ extern "C" int mortar_expert_dispatch(const void *x, int64_t N, int32_t d, int64
     a.slots = N * k; a.k = k; a.d = d;
     const dim3 grid((unsigned)((a.slots + 3) / 4));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (type == MORTAR_FP32) hipLaunchKernelGGL(expert_dispatch_kernel<4>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(expert_dispatch_kernel<2>, grid, dim3(256), 0, st, a);
+    const bool past = past_caches(a, type);
+    const auto kern = type == MORTAR_FP32 ? (past ? expert_dispatch_kernel<4, true> : expert_dispatch_kernel<4, false>) : (past ? expert_dispatch_kernel<2, true> : expert_dispatch_kernel<2, false>);
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a);
     return launch_error(what);
 }
 
@@ -463,13 +527,8 @@ extern "C" int mortar_expert_combine(const void *ys, int64_t N, int32_t d, int32
     RowArgs a{};
     a.ys = static_cast<const char *>(ys); a.out = static_cast<char *>(y); a.w = static_cast<const char *>(weights); a.w_type = w_type;
     a.position = position; a.full = full; a.slots = N * k; a.k = k; a.d = d;
-    const int per = 64 * (type == MORTAR_FP32 ? 4 : 8), parts = (d + per - 1) / per;
-    const int64_t groups = (N * parts + 3) / 4;
-    if (groups >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const auto kern = type == MORTAR_FP32 ? expert_combine_kernel<MORTAR_FP32> : type == MORTAR_FP16 ? expert_combine_kernel<MORTAR_FP16> : expert_combine_kernel<MORTAR_BF16>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)groups), dim3(256), 0, st, a, parts);
-    return launch_error(what);
+    return type == MORTAR_FP32 ? launch_combine_weights<MORTAR_FP32>(a, st, what) : type == MORTAR_FP16 ? launch_combine_weights<MORTAR_FP16>(a, st, what) : launch_combine_weights<MORTAR_BF16>(a, st, what);
 }
 
 extern "C" int mortar_expert_combine_bwd(const void *dy, int64_t lddy, const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position,
@@ -492,7 +551,11 @@ extern "C" int mortar_expert_combine_bwd(const void *dy, int64_t lddy, const voi
     a.position = position; a.full = full; a.slots = N * k; a.k = k; a.d = d;
     const dim3 grid((unsigned)((a.slots + 3) / 4));
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const auto kern = type == MORTAR_FP32 ? expert_combine_bwd_kernel<MORTAR_FP32> : type == MORTAR_FP16 ? expert_combine_bwd_kernel<MORTAR_FP16> : expert_combine_bwd_kernel<MORTAR_BF16>;
+    const bool past = past_caches(a, type);
+    const auto pick = [&](auto plain, auto streaming) { return past ? streaming : plain; };
+    const auto kern = type == MORTAR_FP32   ? pick(expert_combine_bwd_kernel<MORTAR_FP32, false>, expert_combine_bwd_kernel<MORTAR_FP32, true>)
+                      : type == MORTAR_FP16 ? pick(expert_combine_bwd_kernel<MORTAR_FP16, false>, expert_combine_bwd_kernel<MORTAR_FP16, true>)
+                                            : pick(expert_combine_bwd_kernel<MORTAR_BF16, false>, expert_combine_bwd_kernel<MORTAR_BF16, true>);
     hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a);
     return launch_error(what);
 }

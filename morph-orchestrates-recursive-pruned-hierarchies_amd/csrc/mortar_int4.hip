@@ -51,6 +51,28 @@ __device__ __forceinline__ float int4_scale(const void *s, int64_t i) {
     else return bf16_to_f32(static_cast<const uint16_t *>(s)[i]);
 }
 
+// The values of a row's groups from those that its four lanes hold, one each (two groups: one for two lanes).
+template <int GPC>
+__device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    if constexpr (GPC == 1) {
+        all[0] = v;
+    } else {
+        const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);            // lanes of q 0, 1 and of q 2, 3, twice each
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t w = h[i];
+            if constexpr (GPC == 2) {
+                all[i] = __builtin_bit_cast(float, w);
+            } else {
+                const auto l = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+                all[2 * i] = __builtin_bit_cast(float, (uint32_t)l[0]);
+                all[2 * i + 1] = __builtin_bit_cast(float, (uint32_t)l[1]);
+            }
+        }
+    }
+}
+
 // ---- few rows --------------------------------------------------------------------------------------------------------
 // 16 F rows of W and 16 of x per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what
 // bounds these calls.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
@@ -88,17 +110,15 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
     for (int f = 0; f < F; ++f) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     for (int c = wave; c < chunks || (XL && c == wave); c += NW) {
         u32x4_t w[F], x[4];
-        float s[F][GPC], z[F][GPC];
+        float s1[F], z1[F];                                     // of the lane's own group of the chunk: K 32 q on
 #pragma unroll
         for (int f = 0; f < F; ++f) w[f] = read(cb, c * 64 + q * 16 < words ? co[f] + c * 64 : DENSE_OUTSIDE);
+        const int own = min(c * GPC + q * GPC / 4, a.groups - 1);
 #pragma unroll
-        for (int f = 0; f < F; ++f)
-#pragma unroll
-            for (int i = 0; i < GPC; ++i) {
-                const int g = min(c * GPC + i, a.groups - 1);
-                s[f][i] = int4_scale<T, S>(a.s, n[f] * a.s_n + g * a.s_g);
-                z[f][i] = a.z ? -16.0f - (float)a.z[n[f] * a.z_n + g * a.z_g] : -24.0f;
-            }
+        for (int f = 0; f < F; ++f) {
+            s1[f] = int4_scale<T, S>(a.s, n[f] * a.s_n + own * a.s_g);
+            z1[f] = a.z ? -16.0f - (float)a.z[n[f] * a.z_n + own * a.z_g] : -24.0f;
+        }
         const auto x_at = [&](int p) { return c * 128 + (G == 128 ? q * 32 + p * 8 : p * 32 + q * 8); };
         if constexpr (XL) {
             if (c == wave) {                                     // every wave once
@@ -117,6 +137,12 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
         } else {
 #pragma unroll
             for (int p = 0; p < 4; ++p) x[p] = read(xb, x_at(p) < a.K ? xo + 2 * x_at(p) : DENSE_OUTSIDE);
+        }
+        float s[F][GPC], z[F][GPC];
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+            int4_share<GPC>(s1[f], s[f]);
+            int4_share<GPC>(z1[f], z[f]);
         }
         if constexpr (G != 128) {                                // word p of lane q <-> word q of lane p
 #pragma unroll
