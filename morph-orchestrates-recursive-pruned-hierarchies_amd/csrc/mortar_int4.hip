@@ -189,7 +189,7 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------
-// What a tile needs of the groups, laid out so that its pieces are whole 16-byte units: sums of x [groups][Mp], scales and 16 + z [groups][Np], zeros beyond M,
+// What a tile needs of the groups, laid out so that its pieces are whole 16-byte units: sums of x times -1 or, without zero points, -24 [groups][Mp], scales and 16 + z [groups][Np], zeros beyond M,
 // N and the last group.
 template <DenseType T, int S>
 __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int group, int groups, float *xs, float *st, float *zt, unsigned x_blocks) {
@@ -205,7 +205,7 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
         if (per > 4) add(mortar_row_xor<4>(__builtin_bit_cast(uint32_t, sum)));
         add(mortar_row_xor<2>(__builtin_bit_cast(uint32_t, sum)));
         add(mortar_row_xor<1>(__builtin_bit_cast(uint32_t, sum)));
-        if (lane == 0 && m < a.Mp) xs[(int64_t)g * a.Mp + m] = sum;
+        if (lane == 0 && m < a.Mp) xs[(int64_t)g * a.Mp + m] = a.z ? -sum : -24.0f * sum;
         return;
     }
     const int64_t i = (int64_t)(blockIdx.x - x_blocks) * 256 + threadIdx.x;
@@ -241,6 +241,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
     const u32x4_t xbuf = dense_buffer(static_cast<const char *>(a.x) + (int64_t)m0 * a.ldx), cbuf = dense_buffer(reinterpret_cast<const char *>(a.c) + (int64_t)n0 * a.ldc);
     uint32_t xoff[LX], coff[LE];
     int kx;
+    const int kc = (lane & 1) ^ ((lane >> 4) & 1);               // unit of a row of codes (rows 8 apart, which share banks, have theirs in opposite order)
     {
         const int u = lane & 7;
 #pragma unroll
@@ -253,18 +254,19 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
         for (int i = 0; i < LE; ++i) {
             const int e = i * NW + wave;                         // copies of codes, then those of the groups
             const int row = e * 32 + (lane >> 1);
-            coff[i] = e < CC && n0 + row < a.N ? (uint32_t)(row * a.ldc) + (lane & 1) * 16 : DENSE_OUTSIDE;
+            coff[i] = e < CC && n0 + row < a.N ? (uint32_t)(row * a.ldc) + kc * 16 : DENSE_OUTSIDE;
         }
     }
-    const auto copy_step = [&](int k, uint32_t slot) {           // k: the step; beyond the last one it copies zeros
+    const auto copy_to = [&](auto whole, int k, uint32_t slot) {  // k: the step; beyond the last one it copies zeros; whole: all of it is inside K
+        constexpr bool inside = whole.value;
         const uint32_t base = l0 + slot;
 #pragma unroll
-        for (int i = 0; i < LX; ++i) dense_copy(xbuf, kx + k * 128 < a.K * 2 ? xoff[i] + k * 128 : DENSE_OUTSIDE, base + (i * NW + wave) * 1024);
+        for (int i = 0; i < LX; ++i) dense_copy(xbuf, inside || kx + k * 128 < a.K * 2 ? xoff[i] + k * 128 : DENSE_OUTSIDE, base + (i * NW + wave) * 1024);
 #pragma unroll
         for (int i = 0; i < LE; ++i) {
             const int e = i * NW + wave;
             if (e < CC) {
-                dense_copy(cbuf, (lane & 1) * 16 + k * 32 < row_bytes ? coff[i] + k * 32 : DENSE_OUTSIDE, base + X + e * 1024);
+                dense_copy(cbuf, inside || kc * 16 + k * 32 < row_bytes ? coff[i] + k * 32 : DENSE_OUTSIDE, base + X + e * 1024);
             } else if (e < EXTRA) {
                 const int gc = e - CC, gi = gc / GC, at = (gc - gi * GC) * 256 + lane * 4;      // float of the group's piece: scales, sums, zero points
                 const int64_t g = k < steps ? (G == 128 ? k >> 1 : G == 64 ? k : 2 * k + gi) : 0;
@@ -273,7 +275,11 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             }
         }
     };
-    const uint32_t ax = l0 + dense_row_addr(wm * FM * 16, lane), ac = l0 + X + (wn * FN * 16 + r) * 32 + q * 4, ag = l0 + X + C;
+    const auto copy_step = [&](int k, uint32_t slot) {
+        if (k * 64 + 64 <= a.K) copy_to(Const<1>{}, k, slot);
+        else copy_to(Const<0>{}, k, slot);
+    };
+    const uint32_t ax = l0 + dense_row_addr(wm * FM * 16, lane), ac = l0 + X + (wn * FN * 16 + r) * 32 + (r >> 3) * 16 + q * 4, ag = l0 + X + C;
 
     const Int4Unpack<T> unpack;
     f32x4_t acc[FN][FM], part[FN][FM];
@@ -294,7 +300,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             const uint32_t gt = ga + (GPS == 2 ? t * GC * 1024 : 0);
             u32x4_t xf[FM], wf[FN];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) wf[i] = unpack(*(const MORTAR_LDS uint32_t *)(uintptr_t)(ac + slot + i * 512 + t * 16));
+            for (int i = 0; i < FN; ++i) wf[i] = unpack(*(const MORTAR_LDS uint32_t *)(uintptr_t)(((ac + slot) ^ (t * 16)) + i * 512));
 #pragma unroll
             for (int j = 0; j < FM; ++j) xf[j] = dense_read(((ax + slot) ^ (t * 64)) + j * 2048);
             const bool begin = GPS == 2 || (first.value && t == 0), end = GPS == 2 || (last.value && t == 1);
@@ -304,13 +310,13 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
                 for (int j = 0; j < FM; ++j) sx[j] = *(const MORTAR_LDS float *)(uintptr_t)(gt + (BN + (wm * FM + j) * 16 + r) * 4);
 #pragma unroll
                 for (int i = 0; i < FN; ++i) {
-                    f32x4_t zv = {24.f, 24.f, 24.f, 24.f};
+                    f32x4_t zv = {1.f, 1.f, 1.f, 1.f};
                     if constexpr (Z) zv = *(const MORTAR_LDS f32x4_t *)(uintptr_t)(gt + (BN + BM + (wn * FN + i) * 16 + 4 * q) * 4);
 #pragma unroll
                     for (int j = 0; j < FM; ++j) {
                         f32x4_t c;
 #pragma unroll
-                        for (int v = 0; v < 4; ++v) c[v] = -zv[v] * sx[j];
+                        for (int v = 0; v < 4; ++v) c[v] = Z ? zv[v] * sx[j] : sx[j];
                         part[i][j] = dense_mfma<T>(wf[i], xf[j], c);
                     }
                 }
@@ -443,7 +449,7 @@ struct Int4Tile {
     int bn, bm;
     double alone, more;          // us of a step of 64 K: of the only workgroup of a CU, and of each of many
 };
-constexpr Int4Tile INT4_TILES[] = {{128, 128, 0.62, 0.48}, {64, 64, 0.375, 0.2}};
+constexpr Int4Tile INT4_TILES[] = {{128, 128, 0.63, 0.53}, {64, 64, 0.39, 0.24}};
 constexpr int MOST_FEW_ROWS = 4096, FEW_LDS = 64 * 1024;
 
 Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
@@ -519,7 +525,7 @@ int launch_many(Int4Args a, int tile, float *ws, hipStream_t st, const char *wha
     if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
     hipLaunchKernelGGL((int4_prepare_kernel<T, S>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, G, (int)groups, xs, s, zt, (unsigned)x_blocks);
     if (const int rc = launch_error(what)) return rc;
-    return tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 2, 3>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 4, 4>(a, st, what);
+    return tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 1, 2>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 4, 4>(a, st, what);
 }
 
 template <DenseType T, int G, int S>
@@ -579,7 +585,7 @@ extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t gr
     const Int4Plan p = plan(M, N, K, group);
     *tile_n = p.f ? 16 * p.f : INT4_TILES[p.tile].bn;
     *tile_m = p.f ? 16 : INT4_TILES[p.tile].bm;
-    *waves = p.xl ? -p.waves : p.f ? p.waves : 8;
+    *waves = p.xl ? -p.waves : p.f ? p.waves : p.tile == 0 ? 4 : 8;
     return MORTAR_OK;
 }
 

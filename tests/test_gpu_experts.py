@@ -192,6 +192,20 @@ def test_refusals(dev):
             bad()
 
 
+def test_rows_that_no_cache_holds(dev):
+    """Rows by slot of 268 MB and more, which are stored past the caches."""
+    N, k, E, d = 8200, 8, 16, 1024
+    ids, x, ys, dxs, dy, w = _case(dev, N, k, E, d, torch.float32, torch.float32, 2)
+    assert N * k * d * 4 > 256 << 20
+    order = ops.expert_sort(ids, E)
+    full = int(order.offsets[-1])
+    xs = ops.expert_dispatch(x, order)
+    assert torch.equal(xs[:full], x[order.token[:full].long()]) and bool((xs[full:] == 0).all())
+    (dys,) = torch.autograd.grad(ops.expert_combine(ys.requires_grad_(), w, order), ys, dy)
+    want = torch.zeros_like(ys.detach()).index_copy_(0, order.position.view(-1).long(), torch.where(ids < 0, 0.0, w).unsqueeze(2).mul(dy.unsqueeze(1)).view(-1, d))
+    assert torch.equal(dys, want)
+
+
 def test_positions_outside_are_left_out(dev):
     """An order whose positions are none of its rows writes and reads nothing there."""
     ids, x, ys, dxs, dy, w = _case(dev, 20, 3, 4, 72, torch.float32, torch.float32, 5)

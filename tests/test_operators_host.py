@@ -41,7 +41,7 @@ def _form(M, N, K, group):
 def test_sizes_reach_every_form(group):
     """Rows of x through LDS, straight from memory, and tiles."""
     few = [(16, 16, -8), (16, 16, -16), (32, 16, -16)] + [(16 * f, 16, w) for f in (1, 2, 4) for w in (8, 16)]
-    assert {_form(*s, group) for s in INT4_SIZES} == {*few, (64, 64, 8), (128, 128, 8)}
+    assert {_form(*s, group) for s in INT4_SIZES} == {*few, (64, 64, 8), (128, 128, 4)}
     f = _lib.lib().mortar_int4_form_host
     _refused(f(0, 16, 64, group, A, A, A))
     _refused(f(1, 16, 64, 16, A, A, A))
