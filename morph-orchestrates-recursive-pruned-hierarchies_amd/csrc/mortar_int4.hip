@@ -30,7 +30,8 @@ struct Int4Args {
     int64_t ldy;
     int32_t M, N, K, groups;
     const float *xs, *st, *zt;           // tiles: sums of x [groups][Mp], scales and 16 + z [groups][Np]
-    int32_t Mp, Np, tiles_n, tiles_m;
+    int32_t Mp, Np, tiles_n, tiles_m, splits;
+    float *slabs;                        // more than one K range: their fp32 sums [splits][M][Np]
 };
 
 // Eight weights 16 + c of a word, in the order of K: one shift and one and-or for two.  (The constants are kept in registers: as literals, of which an instruction
@@ -231,11 +232,14 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
     const int wn = wave % WN, wm = wave / WN;
     const uint32_t l0 = mortar_lds_addr(lds);
     // As in the 16-bit products: workgroups of one XCD take a contiguous run of tiles, in bands of 8 along m.
-    const int total = a.tiles_n * a.tiles_m, per_xcd = (total + 7) >> 3, id = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if (id >= min(total, (int)((blockIdx.x & 7) + 1) * per_xcd)) return;
+    const int tiles = a.tiles_n * a.tiles_m, total = tiles * a.splits, per_xcd = (total + 7) >> 3, place = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (place >= min(total, (int)((blockIdx.x & 7) + 1) * per_xcd)) return;
+    const int split = place / tiles, id = place - split * tiles;
     const int band = id / (8 * a.tiles_n), rest = id - band * 8 * a.tiles_n, bh = min(8, a.tiles_m - band * 8), tn = rest / bh;
     const int n0 = tn * BN, m0 = (band * 8 + rest - tn * bh) * BM;
     const int steps = (a.K + 63) >> 6, row_bytes = (a.K + 31) >> 5 << 4;
+    constexpr int WHOLE = G == 128 ? 2 : 1;                      // a range begins with a group
+    const int units = (steps + WHOLE - 1) / WHOLE, begin_step = WHOLE * (int)((int64_t)units * split / a.splits), end_step = min(steps, WHOLE * (int)((int64_t)units * (split + 1) / a.splits));
 
     // Sources of this lane's copies: offsets that move on with the steps, and where K ends for them.
     const u32x4_t xbuf = dense_buffer(static_cast<const char *>(a.x) + (int64_t)m0 * a.ldx), cbuf = dense_buffer(reinterpret_cast<const char *>(a.c) + (int64_t)n0 * a.ldc);
@@ -288,7 +292,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = part[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i) copy_step(i, i * SLOT);
+    for (int i = 0; i < NS - 1; ++i) copy_step(begin_step + i, i * SLOT);
     uint32_t slot = 0, free_slot = (NS - 1) * SLOT;
     // first / last: the step begins / ends a group (groups of 128: two steps)
     const auto step = [&](int k, auto first, auto last) {
@@ -341,14 +345,14 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
         slot = slot + SLOT == NS * SLOT ? 0u : slot + SLOT;
     };
     if constexpr (G == 128) {
-        int k = 0;
-        for (; k + 1 < steps; k += 2) {
+        int k = begin_step;
+        for (; k + 1 < end_step; k += 2) {
             step(k, Const<1>{}, Const<0>{});
             step(k + 1, Const<0>{}, Const<1>{});
         }
-        if (k < steps) step(k, Const<1>{}, Const<1>{});
+        if (k < end_step) step(k, Const<1>{}, Const<1>{});
     } else {
-        for (int k = 0; k < steps; ++k) step(k, Const<1>{}, Const<1>{});
+        for (int k = begin_step; k < end_step; ++k) step(k, Const<1>{}, Const<1>{});
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (the copies of the steps behind the last)
 
@@ -363,6 +367,12 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             dense_join8(acc[i][j], acc[i + 1][j], d);
             const int n = n0 + (wn * FN + i) * 16 + dense_lane_n(lane);
             if (n >= a.N) continue;
+            if (a.splits > 1) {
+                float *p = a.slabs + ((int64_t)split * a.M + m) * a.Np + n;
+                *reinterpret_cast<f32x4_t *>(p) = f32x4_t{d[0], d[1], d[2], d[3]};
+                *reinterpret_cast<f32x4_t *>(p + 4) = f32x4_t{d[4], d[5], d[6], d[7]};
+                continue;
+            }
             uint16_t *o = a.y + m * a.ldy + n;
             if (vector) {
                 *reinterpret_cast<u32x4_t *>(o) = dense_pack8<T>(d);
@@ -373,6 +383,25 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             }
         }
     }
+}
+
+// The slabs of the K ranges added in their order.
+template <DenseType T>
+__global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (a.N + 3) >> 2;
+    if (i >= a.M * per) return;
+    const int64_t m = i / per, n = (i - m * per) * 4, slab = (int64_t)a.M * a.Np;
+    const float *p = a.slabs + m * a.Np + n;
+    f32x4_t v[8], sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = *reinterpret_cast<const f32x4_t *>(p + (k < a.splits ? k : 0) * slab);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+        if (k < a.splits) sum += v[k];
+    uint16_t *o = a.y + m * a.ldy + n;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (n + k < a.N) o[k] = (uint16_t)dense_pack2<T>(sum[k], 0.f);
 }
 
 // ---- quantising ------------------------------------------------------------------------------------------------------
@@ -437,12 +466,14 @@ int launch_error(const char *what) {
     return e == hipSuccess ? MORTAR_OK : mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
+
 // Which kernel: the smallest estimate, in us, from products of 1 to 4096 rows of 2048 -> 11264, 5632 -> 2048 and 1040 -> 2736.
 // Few rows: workgroups of 16 x 16 F results; as many rows of W in each as leave 170 of them (16 rows of 2048 -> 11264 6.9 with F = 4 and 8.3 with 2, 64 of 5632
 // -> 2048 10.3 with 2, 256 of them, and 13.9 with 4), and 16 waves instead of 8 where they are one round of the chip.  Tiles are bound by the instructions of
 // a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second launch for the sums of x.
 struct Int4Plan {
-    int f, waves, tile;          // few rows: f > 0; else index into INT4_TILES
+    int f, waves, tile, splits;  // few rows: f > 0; else index into INT4_TILES and ranges of K
     bool xl;
 };
 struct Int4Tile {
@@ -454,7 +485,7 @@ constexpr int MOST_FEW_ROWS = 4096, FEW_LDS = 64 * 1024;
 
 Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
     const int64_t chunks = (K + 127) / 128, steps = (K + 63) / 64, n16 = (N + 15) / 16, m16 = (M + 15) / 16;
-    Int4Plan p{1, 8, 0, false};
+    Int4Plan p{1, 8, 0, 1, false};
     if (M <= 8 && M * int4_pitch((int)K) <= FEW_LDS) {
         p.xl = true;
         p.f = n16 >= 512 && chunks >= 32 ? 2 : 1;
@@ -467,15 +498,20 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
     p.waves = wgs <= 256 && chunks > 8 ? 16 : 8;
     if (M <= 16) return p;
     double best = M <= MOST_FEW_ROWS ? 4.5 + 2.3e-4 * (double)(n16 * m16 * chunks) : 1e300;
+    const int64_t whole = group == 128 ? 2 : 1, units = (steps + whole - 1) / whole;
     for (int t = 0; t < 2; ++t) {
         const Int4Tile &d = INT4_TILES[t];
-        const int64_t per_cu = (((N + d.bn - 1) / d.bn) * ((M + d.bm - 1) / d.bm) + 255) / 256;
-        const double us = 8.0 + (double)steps * (group == 32 ? 1.3 : 1.0) * std::max(d.alone, d.more * (double)per_cu);
-        if (us < best) best = us, p = Int4Plan{0, 0, t, false};
+        const int64_t tiles = ((N + d.bn - 1) / d.bn) * ((M + d.bm - 1) / d.bm);
+        for (const int splits : {1, 2, 3, 4, 6, 8}) {
+            if (splits > 1 && (units * whole < 4 * splits || tiles * splits > 1024)) break;
+            const int64_t per_cu = (tiles * splits + 255) / 256, each = (units + splits - 1) / splits * whole;
+            double us = 8.0 + (double)each * (group == 32 ? 1.3 : 1.0) * std::max(d.alone, d.more * (double)per_cu);
+            if (splits > 1) us += 2.5 + 1.2e-6 * (double)splits * (double)M * (double)up128(N);
+            if (us < best) best = us, p = Int4Plan{0, 0, t, splits, false};
+        }
     }
     return p;
 }
-int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 int64_t groups_padded(int64_t K, int group) { return group == 32 ? (K + 63) / 64 * 2 : (K + group - 1) / group; }
 
 template <DenseType T, int G, int S, int F, int NW, bool XL>
@@ -507,32 +543,37 @@ int launch_tile_form(Int4Args a, hipStream_t st, const char *what) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
     const int64_t tn = ((int64_t)a.N + BN - 1) / BN, tm = ((int64_t)a.M + BM - 1) / BM;
-    if (tn * tm > 1 << 22) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tiles", what);
+    if (tn * tm * a.splits > 1 << 22) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many tiles", what);
     a.tiles_n = (int)tn;
     a.tiles_m = (int)tm;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(8 * ((tn * tm + 7) / 8))), dim3(WN * WM * 64), smem, st, a);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(8 * ((tn * tm * a.splits + 7) / 8))), dim3(WN * WM * 64), smem, st, a);
     return launch_error(what);
 }
 
 template <DenseType T, int G, int S, bool Z>
-int launch_many(Int4Args a, int tile, float *ws, hipStream_t st, const char *what) {
+int launch_many(Int4Args a, const Int4Plan &p, float *ws, hipStream_t st, const char *what) {
     const int64_t groups = groups_padded(a.K, G);
     a.Mp = (int32_t)up128(a.M);
     a.Np = (int32_t)up128(a.N);
     float *xs = ws, *s = xs + groups * a.Mp, *zt = Z ? s + groups * a.Np : nullptr;
     a.xs = xs; a.st = s; a.zt = zt;
+    a.splits = p.splits;
+    a.slabs = s + 2 * groups * a.Np;
     const int64_t x_blocks = (groups * a.Mp * (G / 8) + 255) / 256, n_blocks = (groups * a.Np + 255) / 256;
     if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
     hipLaunchKernelGGL((int4_prepare_kernel<T, S>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, G, (int)groups, xs, s, zt, (unsigned)x_blocks);
     if (const int rc = launch_error(what)) return rc;
-    return tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 1, 2>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 4, 4>(a, st, what);
+    const int rc = p.tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 1, 2>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 4, 4>(a, st, what);
+    if (rc || p.splits == 1) return rc;
+    hipLaunchKernelGGL(int4_join_kernel<T>, dim3((unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, st, a);
+    return launch_error(what);
 }
 
 template <DenseType T, int G, int S>
 int launch_zeros(const Int4Args &a, float *ws, hipStream_t st, const char *what) {
     const Int4Plan p = plan(a.M, a.N, a.K, G);
     if (p.f) return launch_few<T, G, S>(a, p, st, what);
-    return a.z ? launch_many<T, G, S, true>(a, p.tile, ws, st, what) : launch_many<T, G, S, false>(a, p.tile, ws, st, what);
+    return a.z ? launch_many<T, G, S, true>(a, p, ws, st, what) : launch_many<T, G, S, false>(a, p, ws, st, what);
 }
 template <DenseType T, int G>
 int launch_scales(const Int4Args &a, bool s32, float *ws, hipStream_t st, const char *what) {
@@ -578,20 +619,23 @@ extern "C" int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t
     return type == MORTAR_FP32 ? scales(Const<MORTAR_FP32>{}) : type == MORTAR_FP16 ? scales(Const<MORTAR_FP16>{}) : scales(Const<MORTAR_BF16>{});
 }
 
-extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t group, int32_t *tile_n, int32_t *tile_m, int32_t *waves) {
+extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t group, int32_t *tile_n, int32_t *tile_m, int32_t *waves, int32_t *ranges) {
     const char *what = "int4_form";
     CHECK(check_group(what, group));
-    if (M <= 0 || N <= 0 || K <= 0 || !tile_n || !tile_m || !waves) return mortar_fail(MORTAR_ERR_ARG, "%s: bad argument", what);
+    if (M <= 0 || N <= 0 || K <= 0 || !tile_n || !tile_m || !waves || !ranges) return mortar_fail(MORTAR_ERR_ARG, "%s: bad argument", what);
     const Int4Plan p = plan(M, N, K, group);
     *tile_n = p.f ? 16 * p.f : INT4_TILES[p.tile].bn;
     *tile_m = p.f ? 16 : INT4_TILES[p.tile].bm;
     *waves = p.xl ? -p.waves : p.f ? p.waves : p.tile == 0 ? 4 : 8;
+    *ranges = p.splits;
     return MORTAR_OK;
 }
 
 extern "C" int64_t mortar_int4_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t group) {
-    if (M <= 0 || N <= 0 || K <= 0 || group < 32 || plan(M, N, K, group).f) return 0;
-    return 4 * groups_padded(K, group) * (up128(M) + 2 * up128(N));
+    if (M <= 0 || N <= 0 || K <= 0 || group < 32) return 0;
+    const Int4Plan p = plan(M, N, K, group);
+    if (p.f) return 0;
+    return 4 * (groups_padded(K, group) * (up128(M) + 2 * up128(N)) + (p.splits > 1 ? p.splits * M * up128(N) : 0));
 }
 
 extern "C" int mortar_int4_linear(const void *x, int64_t M, int32_t K, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group, const void *s,

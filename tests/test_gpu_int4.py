@@ -59,7 +59,7 @@ def test_products_of_integers_are_exact(dev, M, N, K, t, group, zeros):
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("t", TYPES, ids=str)
-@pytest.mark.parametrize("M,N,K", [(1, 264, 2048), (16, 2048, 5632), (20, 520, 1999), (77, 1031, 1040), (1000, 1040, 2056), (2100, 2056, 392)])
+@pytest.mark.parametrize("M,N,K", [(1, 264, 2048), (16, 2048, 5632), (20, 520, 1999), (77, 1031, 1040), (1000, 1040, 2056), (2100, 2056, 392), (4200, 131, 4104)])
 def test_products(dev, M, N, K, t, group, zeros):
     """Within the bound, and in all as near as the rounding of the result: fp32 sums add less than 1e-5 of it."""
     x = normals((M, K), M, t, dev)

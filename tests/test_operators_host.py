@@ -32,20 +32,22 @@ def test_int4_linear_refuses():
 
 
 def _form(M, N, K, group):
-    v = [C.c_int32() for _ in range(3)]
+    v = [C.c_int32() for _ in range(4)]
     assert _lib.lib().mortar_int4_form_host(M, N, K, group, *[C.byref(i) for i in v]) == 0
     return tuple(i.value for i in v)
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_sizes_reach_every_form(group):
-    """Rows of x through LDS, straight from memory, and tiles."""
+    """Rows of x through LDS, straight from memory, and tiles of one and of several ranges of K."""
     few = [(16, 16, -8), (16, 16, -16), (32, 16, -16)] + [(16 * f, 16, w) for f in (1, 2, 4) for w in (8, 16)]
-    assert {_form(*s, group) for s in INT4_SIZES} == {*few, (64, 64, 8), (128, 128, 4)}
+    forms = {_form(*s, group) for s in INT4_SIZES}
+    assert {f[:3] for f in forms if f[3] == 1} == {*few, (64, 64, 8), (128, 128, 4)}
+    assert {f[:2] for f in forms if f[3] > 1} == {(64, 64), (128, 128)}
     f = _lib.lib().mortar_int4_form_host
-    _refused(f(0, 16, 64, group, A, A, A))
-    _refused(f(1, 16, 64, 16, A, A, A))
-    _refused(f(1, 16, 64, group, None, A, A))
+    _refused(f(0, 16, 64, group, A, A, A, A))
+    _refused(f(1, 16, 64, 16, A, A, A, A))
+    _refused(f(1, 16, 64, group, A, A, A, None))
 
 
 def test_int4_quantize_refuses():
