@@ -663,7 +663,10 @@ int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const fl
  *   mortar_int4_linear     y [M, N] = x W^T, x [M, K] and y in bf16 or fp16 (`type`), fp32 sums.  K a multiple of 8, rows of x on 16-byte addresses.
  *                          Sums are formed over x (16 + c) and x, both exact in the matrix cores, and joined per group in fp32: a row of x whose group
  *                          holds an infinity or NaN is NaN in every column.
+ *   mortar_int4_rows       out [M, 8 ceil(K / 8)] = rows of 16-bit values x(m, k) at x[m * s_m + k * s_k], zeros behind K: for x that mortar_int4_linear does
+ *                          not take as it is
  *   workspace              mortar_int4_workspace_bytes(M, N, K, group) bytes, 16-byte aligned, where that is not 0 */
+int mortar_int4_rows(const void *x, int64_t M, int32_t K, int64_t s_m, int64_t s_k, void *out, void *stream);
 int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t ldw, int32_t type, int32_t group, uint32_t *c, int64_t ldc, void *s, int32_t s_type,
                          int64_t s_n, int64_t s_g, uint8_t *z, int64_t z_n, int64_t z_g, void *stream);
 /* Form that a product takes (host only, nothing is launched): *tile_n x *tile_m of y per workgroup of *waves; 16 rows of x: the kernels of few rows,

@@ -118,6 +118,7 @@ _SIGS = {
     "mortar_fp8_quantizes_inside": (C.c_int, [c_i64, c_i64]),
     "mortar_fp8_linear": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i32, c_vp, c_i64, c_vp, c_vp]),
     "mortar_int4_quantize": (C.c_int, [c_vp, c_i32, c_i32, c_i64, c_i32, c_i32, c_vp, c_i64, c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp]),
+    "mortar_int4_rows": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_i64, c_vp, c_vp]),
     "mortar_int4_form_host": (C.c_int, [c_i64, c_i64, c_i64, c_i32, c_vp, c_vp, c_vp, c_vp]),
     "mortar_int4_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
     "mortar_int4_linear": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64,

@@ -404,6 +404,19 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
         if (n + k < a.N) o[k] = (uint16_t)dense_pack2<T>(sum[k], 0.f);
 }
 
+// Rows of x with any strides, on any address and of any length as rows of whole 16-byte units, zeros behind K.
+__global__ __launch_bounds__(256) void int4_rows_kernel(const uint16_t *x, int64_t M, int32_t K, int64_t s_m, int64_t s_k, uint16_t *o) {
+    const int units = (K + 7) >> 3;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / units;
+    if (m >= M) return;
+    const int k = (int)(i - m * units) * 8;
+    const uint16_t *p = x + m * s_m + k * s_k;
+    uint32_t v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < K ? p[j * s_k] : 0u;
+    *reinterpret_cast<u32x4_t *>(o + i * 8) = u32x4_t{v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16};
+}
+
 // ---- quantising ------------------------------------------------------------------------------------------------------
 template <int TYPE>
 __device__ __forceinline__ float int4_read(const void *p, int64_t i) {
@@ -617,6 +630,17 @@ extern "C" int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t
         return s_type == MORTAR_FP32 ? launch(t, Const<MORTAR_FP32>{}) : s_type == MORTAR_FP16 ? launch(t, Const<MORTAR_FP16>{}) : launch(t, Const<MORTAR_BF16>{});
     };
     return type == MORTAR_FP32 ? scales(Const<MORTAR_FP32>{}) : type == MORTAR_FP16 ? scales(Const<MORTAR_FP16>{}) : scales(Const<MORTAR_BF16>{});
+}
+
+extern "C" int mortar_int4_rows(const void *x, int64_t M, int32_t K, int64_t s_m, int64_t s_k, void *out, void *stream) {
+    const char *what = "int4_rows";
+    if (M < 0 || K <= 0) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
+    if (M == 0) return MORTAR_OK;
+    if (!x || !out || (reinterpret_cast<uintptr_t>(x) & 1) || (reinterpret_cast<uintptr_t>(out) & 15)) return mortar_fail(MORTAR_ERR_ARG, "%s: x or out is null or not on its address", what);
+    if (K >= 1 << 28 || M >= INT64_C(1) << 32 || M * ((K + 7) / 8) >= INT64_C(1) << 32) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
+    hipLaunchKernelGGL(int4_rows_kernel, dim3((unsigned)((M * ((K + 7) / 8) + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const uint16_t *>(x), M, K,
+                       s_m, s_k, static_cast<uint16_t *>(out));
+    return launch_error(what);
 }
 
 extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t group, int32_t *tile_n, int32_t *tile_m, int32_t *waves, int32_t *ranges) {

@@ -437,10 +437,16 @@ PyObject *py_linear_int4(PyObject *, PyObject *const *a, Py_ssize_t na) {
     shape.back() = N;
     at::Tensor y = at::empty(shape, x.options().requires_grad(false));
     if (M) {
-        const at::Tensor r = K % 8 ? at::constant_pad_nd(x.reshape({M, K}), {0, 8 - K % 8}) : rows_of(x, K, 8);
-        const int64_t n = mortar_int4_workspace_bytes(M, N, r.size(1), group);
+        at::Tensor r = x.dim() == 2 ? x : x.reshape({M, K});
+        const int64_t Kp = (K + 7) / 8 * 8;
+        if (K % 8 || r.stride(1) != 1 || (M > 1 && (r.stride(0) % 8 || r.stride(0) < K || r.stride(0) * 256 >= INT64_C(1) << 31)) || !aligned16(r.const_data_ptr())) {
+            const at::Tensor whole = empty_like_rows(x, {M, Kp});
+            check_rc(mortar_int4_rows(data(r), M, (int32_t)K, r.stride(0), r.stride(1), mut(whole), stream_of(x)), "mortar_int4_rows");
+            r = whole;
+        }
+        const int64_t n = mortar_int4_workspace_bytes(M, N, Kp, group);
         const at::Tensor ws = n ? empty_bytes(x, n) : at::Tensor();
-        check_rc(mortar_int4_linear(data(r), M, (int32_t)r.size(1), ld_of(r), type_code(x.scalar_type()), static_cast<const uint32_t *>(data(c)), N > 1 ? c.stride(0) : words,
+        check_rc(mortar_int4_linear(data(r), M, (int32_t)Kp, M > 1 ? r.stride(0) : Kp, type_code(x.scalar_type()), static_cast<const uint32_t *>(data(c)), N > 1 ? c.stride(0) : words,
                                     (int32_t)N, group, data(s), type_code(s.scalar_type()), s.stride(0), s.stride(1), static_cast<const uint8_t *>(data(z)),
                                     z.defined() ? z.stride(0) : 0, z.defined() ? z.stride(1) : 0, mut(y), N, mut(ws), stream_of(x)),
                  "mortar_int4_linear");

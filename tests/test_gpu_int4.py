@@ -83,6 +83,9 @@ def test_strides_shapes_and_padding(dev):
         wide[:, at:at + K] = x
         assert torch.equal(ops.linear_int4(wide[:, at:at + K], c, s), want)
     assert torch.equal(ops.linear_int4(x.view(2, 3, K), c, s), want.view(2, 3, N))
+    assert torch.equal(ops.linear_int4(x.t().contiguous().t(), c, s), want) and torch.equal(ops.linear_int4(x.repeat_interleave(2, 1)[:, ::2], c, s), want)
+    part = c.clone()[:, :4 * -(-67 // 32)]
+    assert torch.equal(ops.linear_int4(x[:, :67], part, s), (x[:, :67].double() @ (q[:, :67].double() - 8).t()).to(t))
     assert torch.equal(ops.linear_int4(x[0], c, s), want[0])
     assert torch.equal(ops.linear_int4(x[:1].expand(50, K), c, s), want[:1].expand(50, N))
     assert ops.linear_int4(x[:0], c, s).shape == (0, N)

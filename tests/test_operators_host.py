@@ -50,6 +50,14 @@ def test_sizes_reach_every_form(group):
     _refused(f(1, 16, 64, group, A, A, A, None))
 
 
+def test_int4_rows_refuses():
+    f = _lib.lib().mortar_int4_rows
+    for bad in ((A, -1, 8, 8, 1, A), (A, 1, 0, 8, 1, A), (None, 1, 8, 8, 1, A), (A, 1, 8, 8, 1, None), (A + 1, 1, 8, 8, 1, A), (A, 1, 8, 8, 1, A + 8)):
+        _refused(f(*bad, None))
+    _refused(f(A, 1 << 32, 8, 8, 1, A, None), -4)
+    assert f(None, 0, 8, 8, 1, None, None) == 0
+
+
 def test_int4_quantize_refuses():
     f = _lib.lib().mortar_int4_quantize
     base = dict(w=A, N=16, K=64, ldw=64, type=0, group=32, c=A, ldc=8, s=A, s_type=0, s_n=1, s_g=16, z=None, z_n=0, z_g=0, st=None)
