@@ -217,14 +217,17 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
     if (a.z) zt[i] = on ? 16.0f + (float)a.z[n * a.z_n + g * a.z_g] : 0.f;
 }
 
-// BN features x BM tokens by WN x WM waves, steps of 64 K through a ring of NS slots in LDS filled by asynchronous copies: x in rows of 128 bytes with their
-// units permuted, codes in rows of 32 bytes, and the step's groups: scales, sums of x, 16 + z.  One barrier per step.  A wave makes its weights from
-// the codes in registers.  The first product of a group starts at -(16 + z) sum x instead of 0.
-template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS>
+// BN features x BM tokens by WN x WM waves, SPS steps of 64 K per turn through a ring of NS turns in LDS filled by asynchronous copies: x in rows of 128 bytes
+// with their units permuted, codes in rows of 32 bytes, and each step's groups: scales, sums of x, 16 + z.  One barrier per turn.  A wave makes its
+// weights from the codes in registers.  The first product of a group starts at -(16 + z) sum x instead of 0.
+// What bounds it is the instructions that a wave issues beside the products: 128 x 128 with 32 x 128 per wave has 3 per product (4096 rows of 2048 -> 11264
+// in 189 us, 64 x 64 per wave 194, eight waves of 32 x 64 201; the library's bf16 product 183).  A third turn in the ring costs more than it hides (197).
+// The ranges of a product over several of them leave fp32 sums.
+template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS, int SPS>
 __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Args a) {
     constexpr int NW = WN * WM, FN = BN / WN / 16, FM = BM / WM / 16, GPS = G == 32 ? 2 : 1;
     constexpr int X = BM * 128, C = BN * 32, GB = (BN + BM + (Z ? BN : 0)) * 4, GC = (GB + 1023) / 1024, SLOT = X + C + GPS * GC * 1024;
-    constexpr int LX = X / 1024 / NW, CC = C / 1024, EXTRA = CC + GPS * GC, LE = (EXTRA + NW - 1) / NW, LEAST = LX + EXTRA / NW;
+    constexpr int LX = X / 1024 / NW, CC = C / 1024, EXTRA = CC + GPS * GC, LE = (EXTRA + NW - 1) / NW, LEAST = (LX + EXTRA / NW) * SPS;
     static_assert(X % (1024 * NW) == 0 && C % 1024 == 0, "whole copies");
     static_assert(FN % 2 == 0, "fragments are joined in pairs");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
@@ -236,10 +239,11 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
     if (place >= min(total, (int)((blockIdx.x & 7) + 1) * per_xcd)) return;
     const int split = place / tiles, id = place - split * tiles;
     const int band = id / (8 * a.tiles_n), rest = id - band * 8 * a.tiles_n, bh = min(8, a.tiles_m - band * 8), tn = rest / bh;
-    const int n0 = tn * BN, m0 = (band * 8 + rest - tn * bh) * BM;
+    const int n0 = __builtin_amdgcn_readfirstlane(tn * BN), m0 = __builtin_amdgcn_readfirstlane((band * 8 + rest - tn * bh) * BM);
     const int steps = (a.K + 63) >> 6, row_bytes = (a.K + 31) >> 5 << 4;
-    constexpr int WHOLE = G == 128 ? 2 : 1;                      // a range begins with a group
-    const int units = (steps + WHOLE - 1) / WHOLE, begin_step = WHOLE * (int)((int64_t)units * split / a.splits), end_step = min(steps, WHOLE * (int)((int64_t)units * (split + 1) / a.splits));
+    constexpr int WHOLE = G == 128 || SPS == 2 ? 2 : 1;          // a range begins with a group and whole turns
+    const int units = (steps + WHOLE - 1) / WHOLE, begin_step = WHOLE * __builtin_amdgcn_readfirstlane(units * split / a.splits),
+              end_step = min(steps, WHOLE * __builtin_amdgcn_readfirstlane(units * (split + 1) / a.splits));
 
     // Sources of this lane's copies: offsets that move on with the steps, and where K ends for them.
     const u32x4_t xbuf = dense_buffer(static_cast<const char *>(a.x) + (int64_t)m0 * a.ldx), cbuf = dense_buffer(reinterpret_cast<const char *>(a.c) + (int64_t)n0 * a.ldc);
@@ -261,7 +265,16 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             coff[i] = e < CC && n0 + row < a.N ? (uint32_t)(row * a.ldc) + kc * 16 : DENSE_OUTSIDE;
         }
     }
-    const auto copy_to = [&](auto whole, int k, uint32_t slot) {  // k: the step; beyond the last one it copies zeros; whole: all of it is inside K
+    const char *gsrc[LE];                                        // the lane's part of a group's piece (scales, sums, zero points): of group 0, and the
+    uint32_t gpitch[LE];                                         // bytes to the next
+#pragma unroll
+    for (int i = 0; i < LE; ++i) {
+        const int gc = i * NW + wave - CC, at = (gc < 0 ? 0 : gc % GC) * 256 + lane * 4;
+        const bool sums = at >= BN && (at < BN + BM || !Z);
+        gsrc[i] = reinterpret_cast<const char *>(at < BN ? a.st + n0 + at : sums ? a.xs + m0 + min(at - BN, BM - 4) : a.zt + n0 + min(at - BN - BM, BN - 4));
+        gpitch[i] = (uint32_t)(sums ? a.Mp : a.Np) * 4u;
+    }
+    const auto copy_to = [&](auto whole, int k, uint32_t slot) __attribute__((always_inline)) {  // k: the step; beyond the last one it copies zeros; whole: all of it is inside K
         constexpr bool inside = whole.value;
         const uint32_t base = l0 + slot;
 #pragma unroll
@@ -272,16 +285,19 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             if (e < CC) {
                 dense_copy(cbuf, inside || kc * 16 + k * 32 < row_bytes ? coff[i] + k * 32 : DENSE_OUTSIDE, base + X + e * 1024);
             } else if (e < EXTRA) {
-                const int gc = e - CC, gi = gc / GC, at = (gc - gi * GC) * 256 + lane * 4;      // float of the group's piece: scales, sums, zero points
-                const int64_t g = k < steps ? (G == 128 ? k >> 1 : G == 64 ? k : 2 * k + gi) : 0;
-                const float *src = at < BN ? a.st + g * a.Np + n0 + at : at < BN + BM || !Z ? a.xs + g * a.Mp + m0 + min(at - BN, BM - 4) : a.zt + g * a.Np + n0 + min(at - BN - BM, BN - 4);
+                const int gc = e - CC;
+                const uint32_t g = k < steps ? (G == 128 ? k >> 1 : G == 64 ? k : 2 * k + gc / GC) : 0;
+                const char *src = gsrc[i] + (uint64_t)g * gpitch[i];
                 mortar_load_to_lds(reinterpret_cast<const MORTAR_GLOBAL char *>(reinterpret_cast<uintptr_t>(src)), base + X + C + gc * 1024);
             }
         }
     };
-    const auto copy_step = [&](int k, uint32_t slot) {
-        if (k * 64 + 64 <= a.K) copy_to(Const<1>{}, k, slot);
-        else copy_to(Const<0>{}, k, slot);
+    const auto copy_step = [&](int k, uint32_t slot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < SPS; ++u) {
+            if ((k + SPS) * 64 <= a.K) copy_to(Const<1>{}, k + u, slot + u * SLOT);
+            else copy_to(Const<0>{}, k + u, slot + u * SLOT);
+        }
     };
     const uint32_t ax = l0 + dense_row_addr(wm * FM * 16, lane), ac = l0 + X + (wn * FN * 16 + r) * 32 + (r >> 3) * 16 + q * 4, ag = l0 + X + C;
 
@@ -292,21 +308,19 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
 #pragma unroll
         for (int j = 0; j < FM; ++j) acc[i][j] = part[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NS - 1; ++i) copy_step(begin_step + i, i * SLOT);
-    uint32_t slot = 0, free_slot = (NS - 1) * SLOT;
-    // first / last: the step begins / ends a group (groups of 128: two steps)
-    const auto step = [&](int k, auto first, auto last) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * LEAST) : "memory");
-        copy_step(k + NS - 1, free_slot);
-        const uint32_t ga = ag + slot;
+    for (int i = 0; i < NS - 1; ++i) copy_step(begin_step + i * SPS, i * SPS * SLOT);
+    uint32_t slot = 0, free_slot = (NS - 1) * SPS * SLOT;
+    // first / last: the step, in slot `at`, begins / ends a group (groups of 128: two steps)
+    const auto multiply = [&](uint32_t at, auto first, auto last) __attribute__((always_inline)) {
+        const uint32_t ga = ag + at;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const uint32_t gt = ga + (GPS == 2 ? t * GC * 1024 : 0);
             u32x4_t xf[FM], wf[FN];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) wf[i] = unpack(*(const MORTAR_LDS uint32_t *)(uintptr_t)(((ac + slot) ^ (t * 16)) + i * 512));
+            for (int i = 0; i < FN; ++i) wf[i] = unpack(*(const MORTAR_LDS uint32_t *)(uintptr_t)(((ac + at) ^ (t * 16)) + i * 512));
 #pragma unroll
-            for (int j = 0; j < FM; ++j) xf[j] = dense_read(((ax + slot) ^ (t * 64)) + j * 2048);
+            for (int j = 0; j < FM; ++j) xf[j] = dense_read(((ax + at) ^ (t * 64)) + j * 2048);
             const bool begin = GPS == 2 || (first.value && t == 0), end = GPS == 2 || (last.value && t == 1);
             if (begin) {
                 float sx[FM];
@@ -341,18 +355,36 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
                 }
             }
         }
-        free_slot = slot;
-        slot = slot + SLOT == NS * SLOT ? 0u : slot + SLOT;
     };
-    if constexpr (G == 128) {
+    // A turn: all waves meet, SPS steps are multiplied and as many copied to where the last turn's were.
+    const auto meet = [&](int k) __attribute__((always_inline)) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * LEAST) : "memory");
+        copy_step(k + (NS - 1) * SPS, free_slot);
+    };
+    const auto turned = [&] {
+        free_slot = slot;
+        slot = slot + SPS * SLOT == NS * SPS * SLOT ? 0u : slot + SPS * SLOT;
+    };
+    if constexpr (G == 128 || SPS == 2) {
+        constexpr int C1 = G == 128 ? 0 : 1;
         int k = begin_step;
         for (; k + 1 < end_step; k += 2) {
-            step(k, Const<1>{}, Const<0>{});
-            step(k + 1, Const<0>{}, Const<1>{});
+            meet(k);
+            multiply(slot, Const<1>{}, Const<C1>{});
+            if constexpr (SPS == 1) turned(), meet(k + 1);
+            multiply(slot + (SPS - 1) * SLOT, Const<C1>{}, Const<1>{});
+            turned();
         }
-        if (k < end_step) step(k, Const<1>{}, Const<1>{});
+        if (k < end_step) {
+            meet(k);
+            multiply(slot, Const<1>{}, Const<1>{});
+        }
     } else {
-        for (int k = begin_step; k < end_step; ++k) step(k, Const<1>{}, Const<1>{});
+        for (int k = begin_step; k < end_step; ++k) {
+            meet(k);
+            multiply(slot, Const<1>{}, Const<1>{});
+            turned();
+        }
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");             // (the copies of the steps behind the last)
 
@@ -493,7 +525,7 @@ struct Int4Tile {
     int bn, bm;
     double alone, more;          // us of a step of 64 K: of the only workgroup of a CU, and of each of many
 };
-constexpr Int4Tile INT4_TILES[] = {{128, 128, 0.63, 0.53}, {64, 64, 0.39, 0.24}};
+constexpr Int4Tile INT4_TILES[] = {{128, 128, 0.63, 0.53}, {64, 64, 0.365, 0.19}};
 constexpr int MOST_FEW_ROWS = 4096, FEW_LDS = 64 * 1024;
 
 Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
@@ -511,7 +543,7 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
     p.waves = wgs <= 256 && chunks > 8 ? 16 : 8;
     if (M <= 16) return p;
     double best = M <= MOST_FEW_ROWS ? 4.5 + 2.3e-4 * (double)(n16 * m16 * chunks) : 1e300;
-    const int64_t whole = group == 128 ? 2 : 1, units = (steps + whole - 1) / whole;
+    const int64_t whole = 2, units = (steps + whole - 1) / whole;
     for (int t = 0; t < 2; ++t) {
         const Int4Tile &d = INT4_TILES[t];
         const int64_t tiles = ((N + d.bn - 1) / d.bn) * ((M + d.bm - 1) / d.bm);
@@ -548,10 +580,10 @@ int launch_few(const Int4Args &a, const Int4Plan &p, hipStream_t st, const char 
     return p.f == 4 ? launch_few_form<T, G, S, 4, 8, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 8, false>(a, st, what) : launch_few_form<T, G, S, 1, 8, false>(a, st, what);
 }
 
-template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS>
+template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS, int SPS>
 int launch_tile_form(Int4Args a, hipStream_t st, const char *what) {
-    const auto kern = int4_tile_kernel<T, G, Z, BN, BM, WN, WM, NS>;
-    constexpr int smem = NS * (BM * 128 + BN * 32 + (G == 32 ? 2 : 1) * (((BN + BM + (Z ? BN : 0)) * 4 + 1023) / 1024) * 1024);
+    const auto kern = int4_tile_kernel<T, G, Z, BN, BM, WN, WM, NS, SPS>;
+    constexpr int smem = NS * SPS * (BM * 128 + BN * 32 + (G == 32 ? 2 : 1) * (((BN + BM + (Z ? BN : 0)) * 4 + 1023) / 1024) * 1024);
     static_assert(smem * 2 <= 160 * 1024, "two workgroups per CU");
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
@@ -576,7 +608,7 @@ int launch_many(Int4Args a, const Int4Plan &p, float *ws, hipStream_t st, const 
     if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
     hipLaunchKernelGGL((int4_prepare_kernel<T, S>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, G, (int)groups, xs, s, zt, (unsigned)x_blocks);
     if (const int rc = launch_error(what)) return rc;
-    const int rc = p.tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 1, 2>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 4, 4>(a, st, what);
+    const int rc = p.tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 1, 2, 1>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 2, 2, 2>(a, st, what);
     if (rc || p.splits == 1) return rc;
     hipLaunchKernelGGL(int4_join_kernel<T>, dim3((unsigned)(((int64_t)a.M * ((a.N + 3) / 4) + 255) / 256)), dim3(256), 0, st, a);
     return launch_error(what);
@@ -650,7 +682,7 @@ extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t gr
     const Int4Plan p = plan(M, N, K, group);
     *tile_n = p.f ? 16 * p.f : INT4_TILES[p.tile].bn;
     *tile_m = p.f ? 16 : INT4_TILES[p.tile].bm;
-    *waves = p.xl ? -p.waves : p.f ? p.waves : p.tile == 0 ? 4 : 8;
+    *waves = p.xl ? -p.waves : p.f ? p.waves : 4;
     *ranges = p.splits;
     return MORTAR_OK;
 }

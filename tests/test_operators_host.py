@@ -42,7 +42,7 @@ def test_sizes_reach_every_form(group):
     """Rows of x through LDS, straight from memory, and tiles of one and of several ranges of K."""
     few = [(16, 16, -8), (16, 16, -16), (32, 16, -16)] + [(16 * f, 16, w) for f in (1, 2, 4) for w in (8, 16)]
     forms = {_form(*s, group) for s in INT4_SIZES}
-    assert {f[:3] for f in forms if f[3] == 1} == {*few, (64, 64, 8), (128, 128, 4)}
+    assert {f[:3] for f in forms if f[3] == 1} == {*few, (64, 64, 4), (128, 128, 4)}
     assert {f[:2] for f in forms if f[3] > 1} == {(64, 64), (128, 128)}
     f = _lib.lib().mortar_int4_form_host
     _refused(f(0, 16, 64, group, A, A, A, A))
