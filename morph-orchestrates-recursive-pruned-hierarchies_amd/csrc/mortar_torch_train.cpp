@@ -5,6 +5,7 @@
 #include <vector>
 
 #include <ATen/MemoryOverlap.h>
+#include <c10/core/InferenceMode.h>
 #include <torch/csrc/utils/object_ptr.h>
 
 namespace {
@@ -131,6 +132,7 @@ PyObject *py_grad_clip(PyObject *, PyObject *const *a, Py_ssize_t na) {
     for (size_t i = 0; i < out.size(); ++i) {
         TORCH_CHECK_VALUE(out[i].sizes() == grads[i].sizes() && out[i].device() == grads[i].device(), what, ": result ", i, " has another shape or device than its gradient");
         TORCH_CHECK_TYPE(out[i].scalar_type() == grads[i].scalar_type() || out[i].scalar_type() == at::kFloat, what, ": result ", i, " must have the type of its gradient or float32");
+        TORCH_CHECK(fresh || !out[i].is_inference() || c10::InferenceMode::is_enabled(), what, ": result ", i, " is an inference tensor, which nothing may write outside of inference mode");
         TORCH_CHECK_VALUE(out[i].is_non_overlapping_and_dense() || at::has_internal_overlap(out[i]) != at::MemOverlap::Yes, what, ": result ", i, " refers to one place several times");
     }
     at::Tensor norm;

@@ -190,3 +190,28 @@ def test_captured(dev):
         eager, n = ops.clip_grads(grads, 1.0)
         torch.cuda.synchronize()
         assert torch.equal(n, norm) and all(torch.equal(a, b) for a, b in zip(eager, out))
+
+
+@pytest.mark.parametrize("norm_type", [2.0, math.inf])
+def test_many_launches(dev, norm_type):
+    """More partial sums than the clipping adds in every workgroup, and results that go past the caches."""
+    grads = _many([70000] * 300, 4, dev, [torch.bfloat16, torch.float32])
+    before = [g.clone() for g in grads]
+    top = _norm(grads, norm_type)
+    got, n = ops.clip_grads(grads, 0.4 * top, norm_type)
+    _check(grads, got, n, 0.4 * top, norm_type)
+    got, again = ops.clip_grads(grads, 0.4 * top, norm_type, out=grads)
+    assert torch.equal(n, again) and torch.equal(n, ops.grad_norm(before, norm_type))
+    _check(before, grads, n, 0.4 * top, norm_type)
+
+
+def test_tensors_of_inference_mode(dev):
+    """Writing them is refused outside of it, as torch's own calls do, with nothing written."""
+    with torch.inference_mode():
+        g = normals((100,), 0, torch.float32, dev)
+        ops.clip_grads([g], 1.0, out=[g])
+        keep = g.clone()
+    with pytest.raises(RuntimeError, match="inference"):
+        ops.clip_grads([g], 0.1, out=[g])
+    assert torch.equal(g, keep)
+    assert torch.allclose(ops.clip_grads([g], 0.1)[0][0], keep * 0.1, rtol=1e-5)

@@ -250,3 +250,38 @@ def test_captured(dev, N):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("N,k,E", [(150000, 2, 40), (600000, 1, 7), (150001, 4, 1024), (1200, 1000, 64)])
+def test_order_of_many_slots(dev, N, k, E):
+    """Runs of more slots per lane, and of more workgroups than one batch of their counts."""
+    ids = draw_ids(N, k, E, N, repeat=True).to(dev)
+    order = ops.expert_sort(ids, E)
+    key = torch.where((ids >= 0) & (ids < E), ids, E).view(-1)
+    key, rows = torch.sort(key, stable=True)
+    assert torch.equal(order.token, (rows // k).int())
+    assert torch.equal(order.position.view(-1)[rows], torch.arange(N * k, dtype=torch.int32, device=dev))
+    assert torch.equal(order.offsets, torch.searchsorted(key, torch.arange(E + 1, dtype=key.dtype, device=dev)).int())
+
+
+@pytest.mark.parametrize("N,k,E,d", [(9, 70, 80, 264), (5, 130, 200, 77), (2, 64, 64, 520)])
+@pytest.mark.parametrize("t,wt", [(torch.bfloat16, torch.float32), (torch.float32, torch.float16)], ids=str)
+def test_more_slots_than_lanes(dev, N, k, E, d, t, wt):
+    ids, x, ys, dxs, dy, w = _case(dev, N, k, E, d, t, wt)
+    r = _reference(ids, E, x, ys, dxs, dy, w)
+    order = ops.expert_sort(ids, E)
+    for v in (x, ys, w):
+        v.requires_grad_(True)
+    xs, y = ops.expert_dispatch(x, order), ops.expert_combine(ys, w, order)
+    dx, dys, dw = torch.autograd.grad((xs, y), (x, ys, w), (dxs, dy))
+    _compare((xs.detach(), y.detach(), dx, dys, dw), r, k, d, t, wt)
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 4])
+@pytest.mark.parametrize("N", [1, 2, 3, 5, 6, 7])
+def test_tokens_that_share_a_wave(dev, N, k):
+    """Few slots per token: waves of several tokens, the last of them with fewer."""
+    ids, x, ys, dxs, dy, w = _case(dev, N, k, 6, 100, torch.bfloat16, torch.float32, 40 + k)
+    r = _reference(ids, 6, x, ys, dxs, dy, w)
+    y = ops.expert_combine(ys, w, ops.expert_sort(ids, 6))
+    assert_within(y, r["y"], (k + 1) * U32 * r["y_size"] + rounding(torch.bfloat16, r["y"]), "y")
