@@ -5,9 +5,11 @@
 // below 1e-23), and the two conversions and multiply-adds per value are still less than the memory takes.  The product is fp32, rounded once.
 //
 // A launch takes the table of up to 128 tensors as its argument, so nothing is copied to the device and a captured launch keeps what it needs.  Tensors
-// are cut into chunks of 16 KB that no two tensors share, a workgroup takes a run of chunks and leaves one partial sum in a slot of its own; the
+// are cut into chunks of 16 KB that no two tensors share, a workgroup takes every n-th chunk and leaves one partial sum in a slot of its own; the
 // slots are added in a fixed order, so that a call gives the same bits every time.  Neighbouring workgroups take neighbouring chunks (a run of chunks for each
-// instead: 51 -> 55 us for the 82 MB above).
+// instead: 51 -> 55 us for 86 MB).
+// Measured, norm and product: 86 MB of gradients 15 + 25 us (the norm 5.7 TB/s, the product 6.9 of which the caches hold a part), 400 MB 194 (6.2 TB/s),
+// 2.4 MB two launches of 4; 500 tensors of 10 MB in all 8 launches of 4, which the host takes 90 us to prepare.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -21,8 +23,8 @@ namespace {
 
 constexpr int TENSORS = 128;             // of a launch: the table fits a kernel's 4 KB of arguments
 constexpr int CHUNK_BYTES = 16384;       // of gradients
-constexpr int MOST_WORKGROUPS = 1024;    // 4 per CU: 380 MB in 194 us, with 8 in 194, with 32 in 209
-constexpr int MOST_SLOTS = 2048;         // that every workgroup of the clipping adds for itself
+constexpr int MOST_WORKGROUPS = 1024;    // 4 per CU: 400 MB in 194 us, with 8 in 194, with 32 in 209
+constexpr int MOST_SLOTS = 2048;         // that every workgroup of the clipping adds for itself: of 2200, 284 MB, 149 us that way and 148 with one launch for it
 
 struct Table {
     const void *src[TENSORS];
@@ -235,7 +237,7 @@ __device__ __forceinline__ void scale_chunk(const void *base, void *out, int64_t
 
 // Every workgroup adds the slots for itself: a launch less than with a kernel that does it once.  The chunks are taken in the opposite order, those
 // first that the norm read last and the caches still hold.  STREAM: results that the L2s cannot hold go past the caches, which keep the gradients then
-// (a block of 39 M values, 82 MB, 51 -> 40 us with its norm; 380 MB 227 -> 194, of that 33 by the order).
+// (86 MB 51 -> 40 us with the norm; 400 MB 227 -> 194, all of that by the order).
 template <typename R, bool STREAM>
 __global__ __launch_bounds__(256) void grad_clip_kernel(const Table t, const uint64_t *slots, int count, double max_norm, float *norm_out) {
     const double n = join_slots<R>(slots, count);

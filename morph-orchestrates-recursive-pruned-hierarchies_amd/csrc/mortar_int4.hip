@@ -76,7 +76,8 @@ __device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
 // 16 F rows of W and 16 of x per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what
-// bounds these calls.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
+// bounds these calls, from about 20 MB on: one row of 8192 -> 8192 8.5 us (34 MB, 4.0 TB/s; the library's bf16 product 21.6), of 2048 -> 11264 4.7 (12 MB;
+// 10.2), the rest of which is the launch and one load behind the other.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
 // lane and group.  The sums of x come from one more product, with ones.
 // Groups of 128: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product:
 // the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7}.
@@ -221,7 +222,9 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
 // with their units permuted, codes in rows of 32 bytes, and each step's groups: scales, sums of x, 16 + z.  One barrier per turn.  A wave makes its
 // weights from the codes in registers.  The first product of a group starts at -(16 + z) sum x instead of 0.
 // What bounds it is the instructions that a wave issues beside the products: 128 x 128 with 32 x 128 per wave has 3 per product (4096 rows of 2048 -> 11264
-// in 189 us, 64 x 64 per wave 194, eight waves of 32 x 64 201; the library's bf16 product 183).  A third turn in the ring costs more than it hides (197).
+// in 189 us, 64 x 64 per wave 194, eight waves of 32 x 64 201; the library's bf16 product 183), and the power that the chip may draw: the same on zeros takes
+// 164.  A third turn in the ring costs more than it hides (197), and so do 32 x 32 products (204), operands read a half step ahead of them (196) and
+// copies issued behind the reads.
 // The ranges of a product over several of them leave fp32 sums.
 template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS, int SPS>
 __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Args a) {
@@ -282,7 +285,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
 #pragma unroll
         for (int i = 0; i < LE; ++i) {
             const int e = i * NW + wave;
-            if (e < CC) {
+            if ((i + 1) * NW <= CC || e < CC) {                  // (the first half known to the compiler)
                 dense_copy(cbuf, inside || kc * 16 + k * 32 < row_bytes ? coff[i] + k * 32 : DENSE_OUTSIDE, base + X + e * 1024);
             } else if (e < EXTRA) {
                 const int gc = e - CC;
@@ -417,7 +420,8 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
     }
 }
 
-// The slabs of the K ranges added in their order.
+// The slabs of the K ranges added in their order: 2.5 us and their reading, which plan() weighs against rounds of idle CUs (1738 rows of 5728 -> 869: 67 us in
+// one range, 52 in several).
 template <DenseType T>
 __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (a.N + 3) >> 2;
@@ -436,7 +440,8 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
         if (n + k < a.N) o[k] = (uint16_t)dense_pack2<T>(sum[k], 0.f);
 }
 
-// Rows of x with any strides, on any address and of any length as rows of whole 16-byte units, zeros behind K.
+// Rows of x with any strides, on any address and of any length as rows of whole 16-byte units, zeros behind K: bound by the memory, a launch in front of the
+// product (680 rows of 410 -> 749 9.7 us with both, with torch's padding 16).
 __global__ __launch_bounds__(256) void int4_rows_kernel(const uint16_t *x, int64_t M, int32_t K, int64_t s_m, int64_t s_k, uint16_t *o) {
     const int units = (K + 7) >> 3;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / units;
@@ -456,7 +461,7 @@ __device__ __forceinline__ float int4_read(const void *p, int64_t i) {
     else if constexpr (TYPE == MORTAR_FP16) return (float)static_cast<const _Float16 *>(p)[i];
     else return bf16_to_f32(static_cast<const uint16_t *>(p)[i]);
 }
-// 8 values per thread, the lanes of a group side by side (16 of them at most: within a row of lanes).
+// 8 values per thread, the lanes of a group side by side (16 of them at most: within a row of lanes).  One pass, once per weight: bound by its reading.
 template <int TYPE, int STYPE>
 __global__ __launch_bounds__(256) void int4_quantize_kernel(const void *w, int32_t N, int32_t K, int64_t ldw, int group, uint32_t *c, int64_t ldc, void *s, int64_t s_n,
                                                             int64_t s_g, uint8_t *z, int64_t z_n, int64_t z_g) {

@@ -192,10 +192,11 @@ def test_captured(dev):
         assert torch.equal(n, norm) and all(torch.equal(a, b) for a, b in zip(eager, out))
 
 
+@pytest.mark.parametrize("tensors", [300, 620])
 @pytest.mark.parametrize("norm_type", [2.0, math.inf])
-def test_many_launches(dev, norm_type):
-    """More partial sums than the clipping adds in every workgroup, and results that go past the caches."""
-    grads = _many([70000] * 300, 4, dev, [torch.bfloat16, torch.float32])
+def test_many_launches(dev, norm_type, tensors):
+    """More partial sums than the clipping adds in every workgroup; results that go past the caches."""
+    grads = _many([70000] * tensors, 4, dev, [torch.bfloat16, torch.float32])
     before = [g.clone() for g in grads]
     top = _norm(grads, norm_type)
     got, n = ops.clip_grads(grads, 0.4 * top, norm_type)
