@@ -518,19 +518,21 @@ int launch_error(const char *what) {
 
 int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 
-// Which kernel: the smallest estimate, in us, from products of 1 to 4096 rows of 2048 -> 11264, 5632 -> 2048 and 1040 -> 2736.
-// Few rows: workgroups of 16 x 16 F results; as many rows of W in each as leave 170 of them (16 rows of 2048 -> 11264 6.9 with F = 4 and 8.3 with 2, 64 of 5632
-// -> 2048 10.3 with 2, 256 of them, and 13.9 with 4), and 16 waves instead of 8 where they are one round of the chip.  Tiles are bound by the instructions of
-// a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second launch for the sums of x.
+// Which kernel: the smallest estimate, in us, from products of 9 to 4096 rows with 16 weights of 300 to 16384 rows and 512 to 8192 columns in every form (what is
+// chosen takes 1.1 % longer than the best one on average).
+// Few rows: workgroups of 16 x 16 F results, one round of the chip if F = 4 still gives one, with the smallest such F (16 rows of 2048 -> 11264 7.6 with F = 4 and 10.1 in
+// two rounds with 2; 64 of 5632 -> 2048 10.9 with 2, 13.3 with 4 on half of the CUs; 77 of them 13.4 with 4, 17.2 in two rounds with 2), and 16 waves instead of 8 if there
+// is work for them.  Tiles are bound by the instructions of a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second
+// launch for the sums of x; 32 x 128 per wave pays for the sums of smaller groups, the small tile less so.
 struct Int4Plan {
     int f, waves, tile, splits;  // few rows: f > 0; else index into INT4_TILES and ranges of K
     bool xl;
 };
 struct Int4Tile {
     int bn, bm;
-    double alone, more;          // us of a step of 64 K: of the only workgroup of a CU, and of each of many
+    double alone[3], more[3];    // us of a step of 64 K with groups of 128, 64, 32: of the only workgroup of a CU, and of each of many
 };
-constexpr Int4Tile INT4_TILES[] = {{128, 128, 0.63, 0.53}, {64, 64, 0.365, 0.19}};
+constexpr Int4Tile INT4_TILES[] = {{128, 128, {0.60, 0.78, 1.09}, {0.53, 0.58, 0.80}}, {64, 64, {0.335, 0.335, 0.43}, {0.19, 0.215, 0.285}}};
 constexpr int MOST_FEW_ROWS = 4096, FEW_LDS = 64 * 1024;
 
 Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
@@ -542,21 +544,24 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
         p.waves = chunks > 16 ? 16 : 8;
         return p;
     }
-    for (int f = 4; f > 1 && p.f == 1; f /= 2)
-        if ((n16 + f - 1) / f * m16 >= 170) p.f = f;
+    p.f = 4;
+    for (const int f : {2, 1})
+        if ((n16 + f - 1) / f * m16 <= 256) p.f = f;
     const int64_t wgs = (n16 + p.f - 1) / p.f * m16;
     p.waves = wgs <= 256 && chunks > 8 ? 16 : 8;
     if (M <= 16) return p;
-    double best = M <= MOST_FEW_ROWS ? 4.5 + 2.3e-4 * (double)(n16 * m16 * chunks) : 1e300;
+    const double chunk = p.f == 1 ? 0.12 : p.f == 2 ? 0.155 : 0.206;
+    double best = M <= MOST_FEW_ROWS ? 3.3 + (double)((wgs + 255) / 256) * (0.5 + chunk * (double)chunks) : 1e300;
     const int64_t whole = 2, units = (steps + whole - 1) / whole;
+    const int g = group == 128 ? 0 : group == 64 ? 1 : 2;
     for (int t = 0; t < 2; ++t) {
         const Int4Tile &d = INT4_TILES[t];
         const int64_t tiles = ((N + d.bn - 1) / d.bn) * ((M + d.bm - 1) / d.bm);
         for (const int splits : {1, 2, 3, 4, 6, 8}) {
             if (splits > 1 && (units * whole < 4 * splits || tiles * splits > 1024)) break;
             const int64_t per_cu = (tiles * splits + 255) / 256, each = (units + splits - 1) / splits * whole;
-            double us = 8.0 + (double)each * (group == 32 ? 1.3 : 1.0) * std::max(d.alone, d.more * (double)per_cu);
-            if (splits > 1) us += 2.5 + 1.2e-6 * (double)splits * (double)M * (double)up128(N);
+            double us = 7.0 + (double)each * std::max(d.alone[g], d.more[g] * (double)per_cu);
+            if (splits > 1) us += 3.0 + 1.2e-6 * (double)splits * (double)M * (double)up128(N);
             if (us < best) best = us, p = Int4Plan{0, 0, t, splits, false};
         }
     }
