@@ -660,7 +660,8 @@ def expert_sort(ids: Tensor, n_experts: int) -> ExpertOrder:
 
 def expert_dispatch(x: Tensor, order: ExpertOrder) -> Tensor:
     """xs [N * k, d], differentiable: the rows of x [N, d] (bf16, fp16, fp32; any width and strides) at the positions of their slots, expert by expert, zeros in the
-    rows behind the last expert's.  The gradient of a token is the sum over its full slots, in order, in fp32.  First derivatives only."""
+    rows behind the last expert's.  The gradient of a token is the sum over its full slots, in order, in fp32.  First derivatives only.  As with torch's own
+    operators a backward pass is captured into a graph only once no graph of the same leaves that was recorded on the default stream is left."""
     return _lib.native().expert_dispatch(x, order.position, order.offsets)
 
 
