@@ -75,7 +75,7 @@ __device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
 }
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
-// 16 F rows of W and 16 of x per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what
+// 16 F rows of W and 16 MX of x per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what
 // bounds these calls, from about 20 MB on: one row of 8192 -> 8192 8.5 us (34 MB, 4.0 TB/s; the library's bf16 product 21.6), of 2048 -> 11264 4.7 (12 MB;
 // 10.2), the rest of which is the launch and one load behind the other.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
 // lane and group.  The sums of x come from one more product, with ones.
@@ -83,14 +83,14 @@ __device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
 // the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7}.
 // XL: x goes through LDS, where the 16 rows of a fragment that are not there cost nothing; read as operands from memory, which takes as many load cycles
 // per chunk as four fragments of W, for more rows or K than fit.
-template <DenseType T, int G, int S, int F, int NW, bool XL>
+template <DenseType T, int G, int S, int F, int MX, int NW, bool XL>
 __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
     constexpr int GPC = 128 / G, PER = 4 / GPC;                 // groups of a chunk, products of a group
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    f32x4_t *part = reinterpret_cast<f32x4_t *>(smem);          // [wave][feature tile][lane]
-    unsigned char *xs = smem + NW * F * 1024;                   // XL: rows of x, whole chunks
+    f32x4_t *part = reinterpret_cast<f32x4_t *>(smem);          // [wave][tile][lane]
+    unsigned char *xs = smem + NW * F * MX * 1024;                   // XL: rows of x, whole chunks
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane >> 4, r = lane & 15;
-    const int n0 = blockIdx.x * (16 * F), m0 = blockIdx.y * 16, rows = min(a.M - m0, 16);
+    const int n0 = blockIdx.x * (16 * F), m0 = blockIdx.y * (16 * MX), rows = min(a.M - m0, 16 * MX);
     const int chunks = (a.K + 127) >> 7, words = (a.K + 31) >> 5 << 4, pitch = int4_pitch(a.K);       // (words: bytes of a row of codes)
     const auto whole = [](const void *p) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, DENSE_OUTSIDE, 0x00020000); };
     const auto read = [](__amdgpu_buffer_rsrc_t b, uint32_t off) { return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, 0)); };
@@ -103,15 +103,19 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
         co[f] = n0 + f * 16 + r < a.N ? (uint32_t)((f * 16 + r) * a.ldc) + q * 16 : DENSE_OUTSIDE;
         n[f] = min(n0 + f * 16 + r, a.N - 1);
     }
-    const uint32_t xo = (uint32_t)min(r, rows - 1) * (XL ? (uint32_t)pitch : (uint32_t)a.ldx);        // (results of rows behind the last one are not used)
+    uint32_t xo[MX];                                            // (results of rows behind the last one are not used)
+#pragma unroll
+    for (int j = 0; j < MX; ++j) xo[j] = (uint32_t)min(j * 16 + r, rows - 1) * (XL ? (uint32_t)pitch : (uint32_t)a.ldx);
     const uint32_t one2 = T == DENSE_F16 ? 0x3C003C00u : 0x3F803F80u;
     const u32x4_t ones = {one2, one2, one2, one2};
     const Int4Unpack<T> unpack;
-    f32x4_t acc[F];
+    f32x4_t acc[F][MX];
 #pragma unroll
-    for (int f = 0; f < F; ++f) acc[f] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int j = 0; j < MX; ++j) acc[f][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     for (int c = wave; c < chunks || (XL && c == wave); c += NW) {
-        u32x4_t w[F], x[4];
+        u32x4_t w[F], x[MX][4];
         float s1[F], z1[F];                                     // of the lane's own group of the chunk: K 32 q on
 #pragma unroll
         for (int f = 0; f < F; ++f) w[f] = read(cb, c * 64 + q * 16 < words ? co[f] + c * 64 : DENSE_OUTSIDE);
@@ -135,10 +139,12 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
             }
             if (c >= chunks) break;
 #pragma unroll
-            for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const u32x4_t *>(xs + xo + 2 * x_at(p));
+            for (int p = 0; p < 4; ++p) x[0][p] = *reinterpret_cast<const u32x4_t *>(xs + xo[0] + 2 * x_at(p));
         } else {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) x[p] = read(xb, x_at(p) < a.K ? xo + 2 * x_at(p) : DENSE_OUTSIDE);
+            for (int j = 0; j < MX; ++j)
+#pragma unroll
+                for (int p = 0; p < 4; ++p) x[j][p] = read(xb, x_at(p) < a.K ? xo[j] + 2 * x_at(p) : DENSE_OUTSIDE);
         }
         float s[F][GPC], z[F][GPC];
 #pragma unroll
@@ -158,36 +164,47 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
 #pragma unroll
         for (int i = 0; i < GPC; ++i) {
             if (c * GPC + i >= a.groups) break;
-            f32x4_t d[F], e = {0.f, 0.f, 0.f, 0.f};
+            f32x4_t d[F][MX], e[MX];
 #pragma unroll
-            for (int f = 0; f < F; ++f) d[f] = e;
+            for (int j = 0; j < MX; ++j) {
+                e[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int f = 0; f < F; ++f) d[f][j] = e[j];
+            }
 #pragma unroll
             for (int p = i * PER; p < (i + 1) * PER; ++p) {
 #pragma unroll
                 for (int f = 0; f < F; ++f) {
                     const uint32_t word = w[f][p];
-                    d[f] = dense_mfma<T>(x[p], unpack(word), d[f]);
+                    const u32x4_t u = unpack(word);
+#pragma unroll
+                    for (int j = 0; j < MX; ++j) d[f][j] = dense_mfma<T>(x[j][p], u, d[f][j]);
                 }
-                e = dense_mfma<T>(x[p], ones, e);
+#pragma unroll
+                for (int j = 0; j < MX; ++j) e[j] = dense_mfma<T>(x[j][p], ones, e[j]);
             }
 #pragma unroll
             for (int f = 0; f < F; ++f)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) acc[f][v] = __builtin_fmaf(s[f][i], __builtin_fmaf(z[f][i], e[v], d[f][v]), acc[f][v]);
+                for (int j = 0; j < MX; ++j)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) acc[f][j][v] = __builtin_fmaf(s[f][i], __builtin_fmaf(z[f][i], e[j][v], d[f][j][v]), acc[f][j][v]);
         }
     }
 #pragma unroll
-    for (int f = 0; f < F; ++f) part[(wave * F + f) * 64 + lane] = acc[f];
+    for (int f = 0; f < F; ++f)
+#pragma unroll
+        for (int j = 0; j < MX; ++j) part[(wave * F * MX + f * MX + j) * 64 + lane] = acc[f][j];
     __syncthreads();
-    if (wave >= F) return;
+    if (wave >= F * MX) return;
     f32x4_t sum = part[wave * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) sum += part[(w * F + wave) * 64 + lane];
-    const int at = n0 + wave * 16 + r;
+    for (int w = 1; w < NW; ++w) sum += part[(w * F * MX + wave) * 64 + lane];
+    const int at = n0 + wave / MX * 16 + r, row = wave % MX * 16 + 4 * q;
     if (at >= a.N) return;
 #pragma unroll
     for (int v = 0; v < 4; ++v)
-        if (4 * q + v < rows) a.y[(int64_t)(m0 + 4 * q + v) * a.ldy + at] = (uint16_t)dense_pack2<T>(sum[v], 0.f);
+        if (row + v < rows) a.y[(int64_t)(m0 + row + v) * a.ldy + at] = (uint16_t)dense_pack2<T>(sum[v], 0.f);
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------
@@ -522,11 +539,13 @@ int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 // chosen takes 1.1 % longer than the best one on average).
 // Few rows: workgroups of 16 x 16 F results, one round of the chip if F = 4 still gives one, with the smallest such F (16 rows of 2048 -> 11264 7.6 with F = 4 and 10.1 in
 // two rounds with 2; 64 of 5632 -> 2048 10.9 with 2, 13.3 with 4 on half of the CUs; 77 of them 13.4 with 4, 17.2 in two rounds with 2), and 16 waves instead of 8 if there
-// is work for them.  Tiles are bound by the instructions of a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second
+// is work for them.  Where that takes several rounds, 32 rows of x share what is unpacked of W (32 rows of 2048 -> 11264 11.1 -> 9.4, 17 of 5120 -> 12288 20.1 -> 15.2,
+// 256 of 5632 -> 2048 24.1 -> 19.1).  Tiles are bound by the instructions of a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second
 // launch for the sums of x; 32 x 128 per wave pays for the sums of smaller groups, the small tile less so.
 struct Int4Plan {
     int f, waves, tile, splits;  // few rows: f > 0; else index into INT4_TILES and ranges of K
     bool xl;
+    int mx = 1;                  // few rows: 16 of x each
 };
 struct Int4Tile {
     int bn, bm;
@@ -551,7 +570,10 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
     p.waves = wgs <= 256 && chunks > 8 ? 16 : 8;
     if (M <= 16) return p;
     const double chunk = p.f == 1 ? 0.12 : p.f == 2 ? 0.155 : 0.206;
-    double best = M <= MOST_FEW_ROWS ? 3.3 + (double)((wgs + 255) / 256) * (0.5 + chunk * (double)chunks) : 1e300;
+    const auto few = [&](int64_t workgroups, double us) { return 3.3 + (double)((workgroups + 255) / 256) * (0.5 + us * (double)chunks); };
+    double best = M <= MOST_FEW_ROWS ? few(wgs, chunk) : 1e300;
+    const int64_t wgs32 = (n16 + 3) / 4 * ((m16 + 1) / 2);
+    if (const double us = few(wgs32, wgs32 <= 256 ? 0.33 : 0.40); M <= MOST_FEW_ROWS && us < best) best = us, p = Int4Plan{4, 8, 0, 1, false, 2};
     const int64_t whole = 2, units = (steps + whole - 1) / whole;
     const int g = group == 128 ? 0 : group == 64 ? 1 : 2;
     for (int t = 0; t < 2; ++t) {
@@ -569,25 +591,26 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
 }
 int64_t groups_padded(int64_t K, int group) { return group == 32 ? (K + 63) / 64 * 2 : (K + group - 1) / group; }
 
-template <DenseType T, int G, int S, int F, int NW, bool XL>
+template <DenseType T, int G, int S, int F, int MX, int NW, bool XL>
 int launch_few_form(const Int4Args &a, hipStream_t st, const char *what) {
-    const auto kern = int4_few_kernel<T, G, S, F, NW, XL>;
-    constexpr int sums = NW * F * 1024;
+    const auto kern = int4_few_kernel<T, G, S, F, MX, NW, XL>;
+    constexpr int sums = NW * F * MX * 1024;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, sums + (XL ? FEW_LDS : 0));
     if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
-    const dim3 grid((unsigned)((a.N + 16 * F - 1) / (16 * F)), (unsigned)((a.M + 15) / 16));
+    const dim3 grid((unsigned)((a.N + 16 * F - 1) / (16 * F)), (unsigned)((a.M + 16 * MX - 1) / (16 * MX)));
     hipLaunchKernelGGL(kern, grid, dim3(NW * 64), sums + (XL ? a.M * int4_pitch(a.K) : 0), st, a);
     return launch_error(what);
 }
 template <DenseType T, int G, int S>
 int launch_few(const Int4Args &a, const Int4Plan &p, hipStream_t st, const char *what) {
     if (p.xl) {
-        if (p.f == 2) return launch_few_form<T, G, S, 2, 16, true>(a, st, what);
-        return p.waves == 16 ? launch_few_form<T, G, S, 1, 16, true>(a, st, what) : launch_few_form<T, G, S, 1, 8, true>(a, st, what);
+        if (p.f == 2) return launch_few_form<T, G, S, 2, 1, 16, true>(a, st, what);
+        return p.waves == 16 ? launch_few_form<T, G, S, 1, 1, 16, true>(a, st, what) : launch_few_form<T, G, S, 1, 1, 8, true>(a, st, what);
     }
+    if (p.mx == 2) return launch_few_form<T, G, S, 4, 2, 8, false>(a, st, what);
     if (p.waves == 16)
-        return p.f == 4 ? launch_few_form<T, G, S, 4, 16, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 16, false>(a, st, what) : launch_few_form<T, G, S, 1, 16, false>(a, st, what);
-    return p.f == 4 ? launch_few_form<T, G, S, 4, 8, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 8, false>(a, st, what) : launch_few_form<T, G, S, 1, 8, false>(a, st, what);
+        return p.f == 4 ? launch_few_form<T, G, S, 4, 1, 16, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 1, 16, false>(a, st, what) : launch_few_form<T, G, S, 1, 1, 16, false>(a, st, what);
+    return p.f == 4 ? launch_few_form<T, G, S, 4, 1, 8, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 1, 8, false>(a, st, what) : launch_few_form<T, G, S, 1, 1, 8, false>(a, st, what);
 }
 
 template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS, int SPS>
@@ -691,7 +714,7 @@ extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t gr
     if (M <= 0 || N <= 0 || K <= 0 || !tile_n || !tile_m || !waves || !ranges) return mortar_fail(MORTAR_ERR_ARG, "%s: bad argument", what);
     const Int4Plan p = plan(M, N, K, group);
     *tile_n = p.f ? 16 * p.f : INT4_TILES[p.tile].bn;
-    *tile_m = p.f ? 16 : INT4_TILES[p.tile].bm;
+    *tile_m = p.f ? 16 * p.mx : INT4_TILES[p.tile].bm;
     *waves = p.xl ? -p.waves : p.f ? p.waves : 4;
     *ranges = p.splits;
     return MORTAR_OK;

@@ -40,7 +40,7 @@ def _form(M, N, K, group):
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_sizes_reach_every_form(group):
     """Rows of x through LDS, straight from memory, and tiles of one and of several ranges of K."""
-    few = [(16, 16, -8), (16, 16, -16), (32, 16, -16)] + [(16 * f, 16, w) for f in (1, 2, 4) for w in (8, 16)]
+    few = [(16, 16, -8), (16, 16, -16), (32, 16, -16), (64, 32, 8)] + [(16 * f, 16, w) for f in (1, 2, 4) for w in (8, 16)]
     forms = {_form(*s, group) for s in INT4_SIZES}
     assert {f[:3] for f in forms if f[3] == 1} == {*few, (64, 64, 4), (128, 128, 4)}
     assert {f[:2] for f in forms if f[3] > 1} == {(64, 64), (128, 128)}
