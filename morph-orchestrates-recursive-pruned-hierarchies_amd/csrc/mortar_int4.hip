@@ -81,8 +81,7 @@ __device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
 // lane and group.  The sums of x come from one more product, with ones.
 // Groups of 128: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product:
 // the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7}.
-// XL: x goes through LDS, where the 16 rows of a fragment that are not there cost nothing; read as operands from memory, which takes as many load cycles
-// per chunk as four fragments of W, for more rows or K than fit.
+// XL: x goes through LDS, where the rows of a fragment that are not there cost nothing and all loads are whole rows; otherwise it is read as operands from memory.
 template <DenseType T, int G, int S, int F, int MX, int NW, bool XL>
 __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
     constexpr int GPC = 128 / G, PER = 4 / GPC;                 // groups of a chunk, products of a group
@@ -552,16 +551,22 @@ struct Int4Tile {
     double alone[3], more[3];    // us of a step of 64 K with groups of 128, 64, 32: of the only workgroup of a CU, and of each of many
 };
 constexpr Int4Tile INT4_TILES[] = {{128, 128, {0.60, 0.78, 1.09}, {0.53, 0.58, 0.80}}, {64, 64, {0.335, 0.335, 0.43}, {0.19, 0.215, 0.285}}};
-constexpr int MOST_FEW_ROWS = 4096, FEW_LDS = 64 * 1024;
+constexpr int MOST_FEW_ROWS = 4096, MOST_LDS = 160 * 1024;
 
 Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
     const int64_t chunks = (K + 127) / 128, steps = (K + 63) / 64, n16 = (N + 15) / 16, m16 = (M + 15) / 16;
     Int4Plan p{1, 8, 0, 1, false};
-    if (M <= 8 && M * int4_pitch((int)K) <= FEW_LDS) {
-        p.xl = true;
+    if (M <= 16) {
+        // x through LDS: rows a multiple of 1 KB apart meet in the same channels when a fragment loads 16 of them at once (8 rows of 5632 -> 2048 7.2 -> 6.5 us, 5 of
+        // 11264 -> 2048 11.7 -> 8.2, long rows at the price of one workgroup per CU), groups of 128 load them in pieces of 16 bytes.  Others are better read as
+        // operands from 3 rows on (7 of 4104 -> 1500 5.4 -> 4.75), as short ones from 9 rows on (9 of 2048 -> 4096 4.6 -> 4.3).
+        const bool apart = K % 512 == 0;
+        const int64_t bytes = M * int4_pitch((int)K);
         p.f = n16 >= 512 && chunks >= 32 ? 2 : 1;
         p.waves = chunks > 16 ? 16 : 8;
-        return p;
+        p.xl = M <= 8 && (M <= 2 || apart || group == 128) && bytes <= 64 * 1024;
+        if (apart && chunks > 24 && (n16 + p.f - 1) / p.f <= 256) p.xl |= bytes <= MOST_LDS - p.waves * p.f * 1024;
+        if (p.xl) return p;
     }
     p.f = 4;
     for (const int f : {2, 1})
@@ -595,7 +600,7 @@ template <DenseType T, int G, int S, int F, int MX, int NW, bool XL>
 int launch_few_form(const Int4Args &a, hipStream_t st, const char *what) {
     const auto kern = int4_few_kernel<T, G, S, F, MX, NW, XL>;
     constexpr int sums = NW * F * MX * 1024;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, sums + (XL ? FEW_LDS : 0));
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, XL ? MOST_LDS : sums);
     if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
     const dim3 grid((unsigned)((a.N + 16 * F - 1) / (16 * F)), (unsigned)((a.M + 16 * MX - 1) / (16 * MX)));
     hipLaunchKernelGGL(kern, grid, dim3(NW * 64), sums + (XL ? a.M * int4_pitch(a.K) : 0), st, a);

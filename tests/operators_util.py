@@ -81,4 +81,5 @@ def draw_ids(n, k, n_experts, seed, empty=0.3, repeat=False):
 INT4_SIZES = [(1, 1, 1), (1, 16, 32), (1, 17, 40), (2, 24, 128), (3, 130, 257), (5, 264, 2120), (2, 8200, 4000), (13, 264, 1040), (16, 2048, 5632), (17, 136, 400), (31, 33, 264),
               (32, 256, 1999), (33, 256, 144), (64, 520, 1040), (65, 9, 72), (96, 1031, 264), (96, 1031, 1040), (129, 264, 400), (130, 127, 2736), (200, 1031, 1040), (300, 135, 272),
               (520, 1031, 264), (5000, 130, 72), (2100, 2056, 392), (4200, 264, 264), (6000, 517, 136), (300, 2055, 8200), (4200, 131, 4104),
-              (4200, 136, 2056), (1000, 1031, 4104), (200, 4103, 4104), (13, 8200, 264), (33, 8200, 136), (17, 8200, 1040), (70, 4103, 1999), (2000, 520, 6152)]
+              (4200, 136, 2056), (1000, 1031, 4104), (200, 4103, 4104), (13, 8200, 264), (33, 8200, 136), (17, 8200, 1040), (70, 4103, 1999), (2000, 520, 6152),
+              (5, 264, 2560), (13, 264, 5632), (9, 40, 7680), (7, 8200, 4096), (3, 130, 1024)]
