@@ -79,12 +79,13 @@ __device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
 // bounds these calls, from about 20 MB on: one row of 8192 -> 8192 8.5 us (34 MB, 4.0 TB/s; the library's bf16 product 21.6), of 2048 -> 11264 4.7 (12 MB;
 // 10.2), the rest of which is the launch and one load behind the other.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
 // lane and group.  The sums of x come from one more product, with ones.
-// Groups of 128: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product:
-// the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7}.
+// Groups of 128 with x in LDS: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product, and x from memory
+// comes in whole pieces of 64 bytes: the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7} (48 rows of 5640 -> 2048 9.1 -> 8.5 us).
 // XL: x goes through LDS, where the rows of a fragment that are not there cost nothing and all loads are whole rows; otherwise it is read as operands from memory.
 template <DenseType T, int G, int S, int F, int MX, int NW, bool XL>
 __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
     constexpr int GPC = 128 / G, PER = 4 / GPC;                 // groups of a chunk, products of a group
+    constexpr bool AS_LOADED = G == 128 && XL;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     f32x4_t *part = reinterpret_cast<f32x4_t *>(smem);          // [wave][tile][lane]
     unsigned char *xs = smem + NW * F * MX * 1024;                   // XL: rows of x, whole chunks
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
             s1[f] = int4_scale<T, S>(a.s, n[f] * a.s_n + own * a.s_g);
             z1[f] = a.z ? -16.0f - (float)a.z[n[f] * a.z_n + own * a.z_g] : -24.0f;
         }
-        const auto x_at = [&](int p) { return c * 128 + (G == 128 ? q * 32 + p * 8 : p * 32 + q * 8); };
+        const auto x_at = [&](int p) { return c * 128 + (AS_LOADED ? q * 32 + p * 8 : p * 32 + q * 8); };
         if constexpr (XL) {
             if (c == wave) {                                     // every wave once
                 const int units = chunks * 16;
@@ -151,7 +152,7 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
             int4_share<GPC>(s1[f], s[f]);
             int4_share<GPC>(z1[f], z[f]);
         }
-        if constexpr (G != 128) {                                // word p of lane q <-> word q of lane p
+        if constexpr (!AS_LOADED) {                              // word p of lane q <-> word q of lane p
 #pragma unroll
             for (int f = 0; f < F; ++f) {
                 const u32x4_t v = w[f];
@@ -558,13 +559,14 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
     Int4Plan p{1, 8, 0, 1, false};
     if (M <= 16) {
         // x through LDS: rows a multiple of 1 KB apart meet in the same channels when a fragment loads 16 of them at once (8 rows of 5632 -> 2048 7.2 -> 6.5 us, 5 of
-        // 11264 -> 2048 11.7 -> 8.2, long rows at the price of one workgroup per CU), groups of 128 load them in pieces of 16 bytes.  Others are better read as
-        // operands from 3 rows on (7 of 4104 -> 1500 5.4 -> 4.75), as short ones from 9 rows on (9 of 2048 -> 4096 4.6 -> 4.3).
+        // 11264 -> 2048 11.7 -> 8.2, long rows at the price of one workgroup per CU).  Others are better read as operands from 3 rows on (7 of 4104 -> 1500 5.4 ->
+        // 4.75), with groups of 128, whose words need no exchange there, from 6 on (4 of 5640 -> 2048 5.5, as operands 6.2), short ones all from 9 rows on (9 of
+        // 2048 -> 4096 4.6 -> 4.3).
         const bool apart = K % 512 == 0;
         const int64_t bytes = M * int4_pitch((int)K);
         p.f = n16 >= 512 && chunks >= 32 ? 2 : 1;
         p.waves = chunks > 16 ? 16 : 8;
-        p.xl = M <= 8 && (M <= 2 || apart || group == 128) && bytes <= 64 * 1024;
+        p.xl = M <= 8 && (M <= (group == 128 ? 5 : 2) || apart) && bytes <= 64 * 1024;
         if (apart && chunks > 24 && (n16 + p.f - 1) / p.f <= 256) p.xl |= bytes <= MOST_LDS - p.waves * p.f * 1024;
         if (p.xl) return p;
     }
