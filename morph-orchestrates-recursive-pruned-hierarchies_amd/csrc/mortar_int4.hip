@@ -536,7 +536,7 @@ int launch_error(const char *what) {
 int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 
 // Which kernel: the smallest estimate, in us, from products of 9 to 4096 rows with 16 weights of 300 to 16384 rows and 512 to 8192 columns in every form (what is
-// chosen takes 1.1 % longer than the best one on average).
+// chosen takes 1.7 % longer than the best one on average, over these and five others).
 // Few rows: workgroups of 16 x 16 F results, one round of the chip if F = 4 still gives one, with the smallest such F (16 rows of 2048 -> 11264 7.6 with F = 4 and 10.1 in
 // two rounds with 2; 64 of 5632 -> 2048 10.9 with 2, 13.3 with 4 on half of the CUs; 77 of them 13.4 with 4, 17.2 in two rounds with 2), and 16 waves instead of 8 if there
 // is work for them.  Where that takes several rounds, 32 rows of x share what is unpacked of W (32 rows of 2048 -> 11264 11.1 -> 9.4, 17 of 5120 -> 12288 20.1 -> 15.2,
