@@ -662,7 +662,9 @@ int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const fl
  *                          c = rne(w / s) + z, 0 at least and 15 at most, quotients in fp32.  What lies behind K gets the code 8.
  *   mortar_int4_linear     y [M, N] = x W^T, x [M, K] and y in bf16 or fp16 (`type`), fp32 sums.  K a multiple of 8, rows of x on 16-byte addresses.
  *                          Sums are formed over x (16 + c) and x, both exact in the matrix cores, and joined per group in fp32: a row of x whose group
- *                          holds an infinity or NaN is NaN in every column.
+ *                          holds an infinity or NaN is NaN in every column.  A group of weights that all are 0 (c = z) adds exactly 0 whatever s is.
+ *   mortar_int4_linear_part  the same for x whose last values, K_used .. K - 1 (fewer than 8), are zeros as mortar_int4_rows writes them: what c holds there is
+ *                          not looked at
  *   mortar_int4_rows       out [M, 8 ceil(K / 8)] = rows of 16-bit values x(m, k) at x[m * s_m + k * s_k], zeros behind K: for x that mortar_int4_linear does
  *                          not take as it is
  *   workspace              mortar_int4_workspace_bytes(M, N, K, group) bytes, 16-byte aligned, where that is not 0 */
@@ -672,6 +674,9 @@ int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t ldw, int32
 /* Form that a product takes (host only, nothing is launched): *tile_n x *tile_m of y per workgroup of *waves; 16 or 32 rows of x: the kernels of few rows,
  * negative: those that take x through LDS; *ranges that K is cut into. */
 int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t group, int32_t *tile_n, int32_t *tile_m, int32_t *waves, int32_t *ranges);
+int mortar_int4_linear_part(const void *x, int64_t M, int32_t K, int32_t K_used, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group,
+                            const void *s, int32_t s_type, int64_t s_n, int64_t s_g, const uint8_t *z, int64_t z_n, int64_t z_g, void *y, int64_t ldy,
+                            void *workspace, void *stream);
 int64_t mortar_int4_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t group);
 int mortar_int4_linear(const void *x, int64_t M, int32_t K, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group, const void *s,
                        int32_t s_type, int64_t s_n, int64_t s_g, const uint8_t *z, int64_t z_n, int64_t z_g, void *y, int64_t ldy, void *workspace,

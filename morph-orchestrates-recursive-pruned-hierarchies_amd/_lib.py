@@ -123,6 +123,8 @@ _SIGS = {
     "mortar_int4_workspace_bytes": (c_i64, [c_i64, c_i64, c_i64, c_i32]),
     "mortar_int4_linear": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_i32, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64,
                                      c_vp, c_vp]),
+    "mortar_int4_linear_part": (C.c_int, [c_vp, c_i64, c_i32, c_i32, c_i64, c_i32, c_vp, c_i64, c_i32, c_i32, c_vp, c_i32, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp,
+                                          c_i64, c_vp, c_vp]),
     "mortar_grad_workspace_bytes": (c_i64, [c_vp, c_i64]),
     "mortar_grad_norm": (C.c_int, [c_vp, c_i64, c_i32, c_vp, c_vp, c_vp]),
     "mortar_grad_clip": (C.c_int, [c_vp, c_i64, c_i32, C.c_double, c_vp, c_vp, c_vp]),

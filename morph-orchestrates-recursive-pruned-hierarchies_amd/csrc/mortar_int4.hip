@@ -3,7 +3,13 @@
 // 16 + c is exact in bf16 and in fp16: a code's four bits are the upper mantissa bits behind the exponent of 16, so that two weights are made
 // by one shift and one and-or, and go into the matrix cores beside x as it is.  The sums of a group come out of them unscaled and enter the fp32 result with one
 // multiply-add: W is never rounded.  (W in 16 bits instead would cost as much again as the rounding of y.)  What the 16 adds is a few times the
-// codes' own size in sums of 24 bits, and is taken off exactly.
+// codes' own size in sums of 24 bits.  It is taken off as a sum of its own, and what the two round differently is left: little beside what the group's weights
+// give, but not where they all are 0 (pruned ones, whose scale need not be small).  Such a group gives 0 exactly here:
+//   few rows   both sums run through the same instructions in the same order, with 24 in place of a weight of 0, which the code 8 is; with zero points the
+//              weights are 24 + (c - z) / 2: half a code, added to the bits of the row's 24 - z / 2 instead of set in those of 16.  Zero points beyond 15,
+//              which no code reaches, count as 15, and (z - 15) / 2 sums of x are taken off besides.
+//   many rows  a subtraction more per result and group takes 3 to 15 % longer, looking at the codes beside the products 3 to 17 %: the launch in front reads
+//              them instead (1.8 us for 23 million weights) and gives groups of zeros the scale 0.
 // The codes of a word lie so that one shift brings a pair of neighbours into its two halves.
 #include <hip/hip_runtime.h>
 
@@ -28,23 +34,37 @@ struct Int4Args {
     int64_t z_n, z_g;
     uint16_t *y;
     int64_t ldy;
-    int32_t M, N, K, groups;
+    int32_t M, N, K, groups, K_used;     // K_used: codes behind it are not looked at, x is 0 there
     const float *xs, *st, *zt;           // tiles: sums of x [groups][Mp], scales and 16 + z [groups][Np]
     int32_t Mp, Np, tiles_n, tiles_m, splits;
     float *slabs;                        // more than one K range: their fp32 sums [splits][M][Np]
 };
 
-// Eight weights 16 + c of a word, in the order of K: one shift and one and-or for two.  (The constants are kept in registers: as literals, of which an instruction
-// takes one, the and and the or are two instructions.)
-template <DenseType T>
+// Eight weights 16 + c, or with Z 24 + (c - z) / 2, of a word in the order of K: one shift and one and-or for two.  (The constants are kept in registers: as literals, of
+// which an instruction takes one, the and and the or are two instructions.)
+template <DenseType T, bool Z>
 struct Int4Unpack {
-    uint32_t mask = T == DENSE_F16 ? 0x03C003C0u : 0x00780078u, one = T == DENSE_F16 ? 0x4C004C00u : 0x41804180u;
+    static constexpr bool H = T == DENSE_F16;
+    static constexpr uint32_t BASE = H ? 0x4C004C00u : 0x41804180u, HALF = H ? 0x00200020u : 0x00040004u;       // 16, and what 1/2 adds to it
+    uint32_t mask = HALF * (Z ? 15 : 30), one = BASE;
     __device__ __forceinline__ Int4Unpack() { asm("" : "+s"(mask), "+v"(one)); }
-    __device__ __forceinline__ u32x4_t operator()(uint32_t w) const {
-        if constexpr (T == DENSE_F16) return u32x4_t{(w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one, (w >> 6 & mask) | one};
+    // Z: base is that of the row's zero point
+    __device__ __forceinline__ u32x4_t operator()(uint32_t w, uint32_t base) const {
+        if constexpr (Z && H) return u32x4_t{(w << 5 & mask) + base, (w << 1 & mask) + base, (w >> 3 & mask) + base, (w >> 7 & mask) + base};
+        else if constexpr (Z) return u32x4_t{(w << 2 & mask) + base, (w >> 2 & mask) + base, (w >> 6 & mask) + base, (w >> 10 & mask) + base};
+        else if constexpr (H) return u32x4_t{(w << 6 & mask) | one, (w << 2 & mask) | one, (w >> 2 & mask) | one, (w >> 6 & mask) | one};
         else return u32x4_t{(w << 3 & mask) | one, (w >> 1 & mask) | one, (w >> 5 & mask) | one, (w >> 9 & mask) | one};
     }
+    // 24 - z / 2 (zero points beyond 15 count as 15): what a code adds to, and never beyond 31.5.
+    static __device__ __forceinline__ uint32_t base(uint32_t z) { return (16 - min(z, 15u)) * HALF + BASE; }
+    // What a weight of 0 is among them: 24, eight times.
+    static __device__ __forceinline__ u32x4_t zeros() {
+        constexpr uint32_t v = H ? 0x4E004E00u : 0x41C041C0u;
+        return u32x4_t{v, v, v, v};
+    }
 };
+// What is taken off of 24 sum x: all of it, and (z - 15) / 2 sums of x for zero points beyond 15.
+__device__ __forceinline__ float int4_factor(uint32_t z) { return __builtin_fmaf((float)(max(z, 15u) - 15), -1.0f / 48.0f, -1.0f); }
 template <DenseType T, int S>
 __device__ __forceinline__ float int4_scale(const void *s, int64_t i) {
     if constexpr (S == 4) return static_cast<const float *>(s)[i];
@@ -53,8 +73,8 @@ __device__ __forceinline__ float int4_scale(const void *s, int64_t i) {
 }
 
 // The values of a row's groups from those that its four lanes hold, one each (two groups: one for two lanes).
-template <int GPC>
-__device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
+template <int GPC, typename V>
+__device__ __forceinline__ void int4_share(V v, V (&all)[GPC]) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
     if constexpr (GPC == 1) {
         all[0] = v;
@@ -64,11 +84,11 @@ __device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
         for (int i = 0; i < 2; ++i) {
             const uint32_t w = h[i];
             if constexpr (GPC == 2) {
-                all[i] = __builtin_bit_cast(float, w);
+                all[i] = __builtin_bit_cast(V, w);
             } else {
                 const auto l = __builtin_amdgcn_permlane16_swap(w, w, false, false);
-                all[2 * i] = __builtin_bit_cast(float, (uint32_t)l[0]);
-                all[2 * i + 1] = __builtin_bit_cast(float, (uint32_t)l[1]);
+                all[2 * i] = __builtin_bit_cast(V, (uint32_t)l[0]);
+                all[2 * i + 1] = __builtin_bit_cast(V, (uint32_t)l[1]);
             }
         }
     }
@@ -78,11 +98,11 @@ __device__ __forceinline__ void int4_share(float v, float (&all)[GPC]) {
 // 16 F rows of W and 16 MX of x per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what
 // bounds these calls, from about 20 MB on: one row of 8192 -> 8192 8.5 us (34 MB, 4.0 TB/s; the library's bf16 product 21.6), of 2048 -> 11264 4.7 (12 MB;
 // 10.2), the rest of which is the launch and one load behind the other.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
-// lane and group.  The sums of x come from one more product, with ones.
+// lane and group.  What is taken off comes from one more product, with 24.
 // Groups of 128 with x in LDS: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product, and x from memory
 // comes in whole pieces of 64 bytes: the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7} (48 rows of 5640 -> 2048 9.1 -> 8.5 us).
 // XL: x goes through LDS, where the rows of a fragment that are not there cost nothing and all loads are whole rows; otherwise it is read as operands from memory.
-template <DenseType T, int G, int S, int F, int MX, int NW, bool XL>
+template <DenseType T, int G, int S, bool Z, int F, int MX, int NW, bool XL>
 __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
     constexpr int GPC = 128 / G, PER = 4 / GPC;                 // groups of a chunk, products of a group
     constexpr bool AS_LOADED = G == 128 && XL;
@@ -106,9 +126,8 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
     uint32_t xo[MX];                                            // (results of rows behind the last one are not used)
 #pragma unroll
     for (int j = 0; j < MX; ++j) xo[j] = (uint32_t)min(j * 16 + r, rows - 1) * (XL ? (uint32_t)pitch : (uint32_t)a.ldx);
-    const uint32_t one2 = T == DENSE_F16 ? 0x3C003C00u : 0x3F803F80u;
-    const u32x4_t ones = {one2, one2, one2, one2};
-    const Int4Unpack<T> unpack;
+    const Int4Unpack<T, Z> unpack;
+    const u32x4_t zeros = unpack.zeros();
     f32x4_t acc[F][MX];
 #pragma unroll
     for (int f = 0; f < F; ++f)
@@ -116,15 +135,17 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
         for (int j = 0; j < MX; ++j) acc[f][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     for (int c = wave; c < chunks || (XL && c == wave); c += NW) {
         u32x4_t w[F], x[MX][4];
-        float s1[F], z1[F];                                     // of the lane's own group of the chunk: K 32 q on
+        float s1[F];                                            // of the lane's own group of the chunk: K 32 q on
+        uint32_t z1[F];
 #pragma unroll
         for (int f = 0; f < F; ++f) w[f] = read(cb, c * 64 + q * 16 < words ? co[f] + c * 64 : DENSE_OUTSIDE);
         const int own = min(c * GPC + q * GPC / 4, a.groups - 1);
 #pragma unroll
         for (int f = 0; f < F; ++f) {
-            s1[f] = int4_scale<T, S>(a.s, n[f] * a.s_n + own * a.s_g);
-            z1[f] = a.z ? -16.0f - (float)a.z[n[f] * a.z_n + own * a.z_g] : -24.0f;
+            s1[f] = int4_scale<T, S>(a.s, n[f] * a.s_n + own * a.s_g) * (Z ? 2.0f : 1.0f);
+            if constexpr (Z) z1[f] = a.z[n[f] * a.z_n + own * a.z_g];
         }
+        __builtin_amdgcn_sched_barrier(0);                       // (x behind the codes and scales: 13 rows of 8192 -> 8192 14.6 -> 13.2 us)
         const auto x_at = [&](int p) { return c * 128 + (AS_LOADED ? q * 32 + p * 8 : p * 32 + q * 8); };
         if constexpr (XL) {
             if (c == wave) {                                     // every wave once
@@ -146,11 +167,12 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
 #pragma unroll
                 for (int p = 0; p < 4; ++p) x[j][p] = read(xb, x_at(p) < a.K ? xo[j] + 2 * x_at(p) : DENSE_OUTSIDE);
         }
-        float s[F][GPC], z[F][GPC];
+        float s[F][GPC];
+        uint32_t z[F][GPC];
 #pragma unroll
         for (int f = 0; f < F; ++f) {
             int4_share<GPC>(s1[f], s[f]);
-            int4_share<GPC>(z1[f], z[f]);
+            if constexpr (Z) int4_share<GPC>(z1[f], z[f]);
         }
         if constexpr (!AS_LOADED) {                              // word p of lane q <-> word q of lane p
 #pragma unroll
@@ -165,6 +187,9 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
         for (int i = 0; i < GPC; ++i) {
             if (c * GPC + i >= a.groups) break;
             f32x4_t d[F][MX], e[MX];
+            uint32_t base[F];
+#pragma unroll
+            for (int f = 0; f < F; ++f) base[f] = Z ? unpack.base(z[f][i]) : 0u;
 #pragma unroll
             for (int j = 0; j < MX; ++j) {
                 e[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
@@ -176,19 +201,21 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
 #pragma unroll
                 for (int f = 0; f < F; ++f) {
                     const uint32_t word = w[f][p];
-                    const u32x4_t u = unpack(word);
+                    const u32x4_t u = unpack(word, base[f]);
 #pragma unroll
                     for (int j = 0; j < MX; ++j) d[f][j] = dense_mfma<T>(x[j][p], u, d[f][j]);
                 }
 #pragma unroll
-                for (int j = 0; j < MX; ++j) e[j] = dense_mfma<T>(x[j][p], ones, e[j]);
+                for (int j = 0; j < MX; ++j) e[j] = dense_mfma<T>(x[j][p], zeros, e[j]);
             }
 #pragma unroll
-            for (int f = 0; f < F; ++f)
+            for (int f = 0; f < F; ++f) {
+                const float factor = Z ? int4_factor(z[f][i]) : -1.0f;
 #pragma unroll
                 for (int j = 0; j < MX; ++j)
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) acc[f][j][v] = __builtin_fmaf(s[f][i], __builtin_fmaf(z[f][i], e[j][v], d[f][j][v]), acc[f][j][v]);
+                    for (int v = 0; v < 4; ++v) acc[f][j][v] = __builtin_fmaf(s[f][i], __builtin_fmaf(factor, e[j][v], d[f][j][v]), acc[f][j][v]);
+            }
         }
     }
 #pragma unroll
@@ -208,10 +235,33 @@ __global__ __launch_bounds__(NW * 64) void int4_few_kernel(const Int4Args a) {
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------
+// Which codes of a word count whose first value has `left` to the last one.
+__device__ __forceinline__ uint32_t int4_counted(int left) {
+    const int v = min(max(left, 0), 8);
+    return ((1u << 4 * ((v + 1) >> 1)) - 1) | ((1u << 4 * (v >> 1)) - 1) << 16;
+}
+// Whether all codes of group g of row n are z.
+__device__ __forceinline__ bool int4_all_zero(const Int4Args &a, int64_t n, int g, int group, uint32_t z) {
+    const u32x4_t *c = reinterpret_cast<const u32x4_t *>(reinterpret_cast<const char *>(a.c) + n * a.ldc + (int64_t)g * (group / 2));
+    const int units = min(group, a.K - g * group + 31) / 32;      // 16 bytes of codes
+    u32x4_t w[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) w[p] = c[min(p, units - 1)];
+    uint32_t other = z > 15;
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (p < units) other |= (w[p][j] ^ z * 0x11111111u) & int4_counted(a.K_used - (g * group + p * 32 + j * 8));
+    return !other;
+}
+
 // What a tile needs of the groups, laid out so that its pieces are whole 16-byte units: sums of x times -1 or, without zero points, -24 [groups][Mp], scales and 16 + z [groups][Np], zeros beyond M,
-// N and the last group.
-template <DenseType T, int S>
-__global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int group, int groups, float *xs, float *st, float *zt, unsigned x_blocks) {
+// N and the last group.  The scale is times 0 where all codes are the zero point.  A wave takes 16 rows of W and 64 units of 32 K, one per lane, of whose codes it reads whole
+// rows, all 16 at once; only where a group's codes are all the same they are compared with its zero point.
+template <DenseType T, int S, int G, bool Z>
+__global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int groups, float *xs, float *st, float *zt, unsigned x_blocks) {
+    constexpr int group = G;
     if (blockIdx.x < x_blocks) {                                 // 8 values per thread, the lanes of a group side by side
         const int per = group / 8;
         const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / per, m = i / groups;
@@ -224,15 +274,52 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
         if (per > 4) add(mortar_row_xor<4>(__builtin_bit_cast(uint32_t, sum)));
         add(mortar_row_xor<2>(__builtin_bit_cast(uint32_t, sum)));
         add(mortar_row_xor<1>(__builtin_bit_cast(uint32_t, sum)));
-        if (lane == 0 && m < a.Mp) xs[(int64_t)g * a.Mp + m] = a.z ? -sum : -24.0f * sum;
+        if (lane == 0 && m < a.Mp) xs[(int64_t)g * a.Mp + m] = Z ? -sum : -24.0f * sum;
         return;
     }
-    const int64_t i = (int64_t)(blockIdx.x - x_blocks) * 256 + threadIdx.x;
-    const int g = (int)(i / a.Np), n = (int)(i - (int64_t)g * a.Np);
-    if (g >= groups) return;
-    const bool on = g < a.groups && n < a.N;
-    st[i] = on ? int4_scale<T, S>(a.s, n * a.s_n + g * a.s_g) : 0.f;
-    if (a.z) zt[i] = on ? 16.0f + (float)a.z[n * a.z_n + g * a.z_g] : 0.f;
+    constexpr int PER = G / 32, GROUPS = 64 / PER, TURNS = GROUPS / 4;       // units of a group, groups of the wave; four of them are stored at a time, for 16 rows
+    const int lane = threadIdx.x & 63, chunks = (groups + GROUPS - 1) / GROUPS, units = (a.K + 31) >> 5;
+    const int64_t task = (int64_t)(blockIdx.x - x_blocks) * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), block = task / chunks, n = block * 16 + (lane & 15);
+    if (block * 16 >= a.Np) return;
+    const int g0 = (int)(task - block * chunks) * GROUPS, u = g0 * PER + lane, left = a.K_used - u * 32;
+    const char *c = reinterpret_cast<const char *>(a.c) + (int64_t)min(u, units - 1) * 16;
+    u32x4_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = *reinterpret_cast<const u32x4_t *>(c + min(block * 16 + i, (int64_t)a.N - 1) * a.ldc);
+    float s[TURNS];
+    uint32_t z[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        const int64_t row = min(n, (int64_t)a.N - 1), g = min(g0 + i * 4 + (lane >> 4), a.groups - 1);
+        s[i] = int4_scale<T, S>(a.s, row * a.s_n + g * a.s_g);
+        z[i] = 8;
+        if constexpr (Z) z[i] = a.z[row * a.z_n + g * a.z_g];
+    }
+    uint32_t same = 0;                                           // bit i: the lane's group has one code throughout in row i
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t first = (w[i][0] & 15) * 0x11111111u;
+        uint32_t other = 0;
+        if (left >= 32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) other |= w[i][j] ^ first;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) other |= (w[i][j] ^ first) & int4_counted(left - j * 8);
+        }
+        same |= (other == 0 ? 1u : 0u) << i;
+    }
+#pragma unroll
+    for (int d = 1; d < PER; d <<= 1) same &= __shfl_xor(same, d);
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        const int at = i * 4 + (lane >> 4), g = g0 + at;
+        const bool on = g < a.groups && n < a.N;
+        if ((__shfl(same, at * PER) >> (lane & 15) & 1) && on && int4_all_zero(a, n, g, G, z[i])) s[i] *= 0.f;       // (NaN stays)
+        if (g >= groups) continue;
+        st[(int64_t)g * a.Np + n] = on ? s[i] : 0.f;
+        if constexpr (Z) zt[(int64_t)g * a.Np + n] = on ? 16.0f + (float)z[i] : 0.f;
+    }
 }
 
 // BN features x BM tokens by WN x WM waves, SPS steps of 64 K per turn through a ring of NS turns in LDS filled by asynchronous copies: x in rows of 128 bytes
@@ -321,7 +408,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
     };
     const uint32_t ax = l0 + dense_row_addr(wm * FM * 16, lane), ac = l0 + X + (wn * FN * 16 + r) * 32 + (r >> 3) * 16 + q * 4, ag = l0 + X + C;
 
-    const Int4Unpack<T> unpack;
+    const Int4Unpack<T, false> unpack;
     f32x4_t acc[FN][FM], part[FN][FM];
 #pragma unroll
     for (int i = 0; i < FN; ++i)
@@ -338,7 +425,7 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
             const uint32_t gt = ga + (GPS == 2 ? t * GC * 1024 : 0);
             u32x4_t xf[FM], wf[FN];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) wf[i] = unpack(*(const MORTAR_LDS uint32_t *)(uintptr_t)(((ac + at) ^ (t * 16)) + i * 512));
+            for (int i = 0; i < FN; ++i) wf[i] = unpack(*(const MORTAR_LDS uint32_t *)(uintptr_t)(((ac + at) ^ (t * 16)) + i * 512), 0);
 #pragma unroll
             for (int j = 0; j < FM; ++j) xf[j] = dense_read(((ax + at) ^ (t * 64)) + j * 2048);
             const bool begin = GPS == 2 || (first.value && t == 0), end = GPS == 2 || (last.value && t == 1);
@@ -589,7 +676,7 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
         for (const int splits : {1, 2, 3, 4, 6, 8}) {
             if (splits > 1 && (units * whole < 4 * splits || tiles * splits > 1024)) break;
             const int64_t per_cu = (tiles * splits + 255) / 256, each = (units + splits - 1) / splits * whole;
-            double us = 7.0 + (double)each * std::max(d.alone[g], d.more[g] * (double)per_cu);
+            double us = 7.0 + 7.8e-8 * (double)N * (double)K + (double)each * std::max(d.alone[g], d.more[g] * (double)per_cu);
             if (splits > 1) us += 3.0 + 1.2e-6 * (double)splits * (double)M * (double)up128(N);
             if (us < best) best = us, p = Int4Plan{0, 0, t, splits, false};
         }
@@ -598,9 +685,9 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
 }
 int64_t groups_padded(int64_t K, int group) { return group == 32 ? (K + 63) / 64 * 2 : (K + group - 1) / group; }
 
-template <DenseType T, int G, int S, int F, int MX, int NW, bool XL>
+template <DenseType T, int G, int S, bool Z, int F, int MX, int NW, bool XL>
 int launch_few_form(const Int4Args &a, hipStream_t st, const char *what) {
-    const auto kern = int4_few_kernel<T, G, S, F, MX, NW, XL>;
+    const auto kern = int4_few_kernel<T, G, S, Z, F, MX, NW, XL>;
     constexpr int sums = NW * F * MX * 1024;
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, XL ? MOST_LDS : sums);
     if (e != hipSuccess) return mortar_fail(MORTAR_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
@@ -608,16 +695,16 @@ int launch_few_form(const Int4Args &a, hipStream_t st, const char *what) {
     hipLaunchKernelGGL(kern, grid, dim3(NW * 64), sums + (XL ? a.M * int4_pitch(a.K) : 0), st, a);
     return launch_error(what);
 }
-template <DenseType T, int G, int S>
+template <DenseType T, int G, int S, bool Z>
 int launch_few(const Int4Args &a, const Int4Plan &p, hipStream_t st, const char *what) {
     if (p.xl) {
-        if (p.f == 2) return launch_few_form<T, G, S, 2, 1, 16, true>(a, st, what);
-        return p.waves == 16 ? launch_few_form<T, G, S, 1, 1, 16, true>(a, st, what) : launch_few_form<T, G, S, 1, 1, 8, true>(a, st, what);
+        if (p.f == 2) return launch_few_form<T, G, S, Z, 2, 1, 16, true>(a, st, what);
+        return p.waves == 16 ? launch_few_form<T, G, S, Z, 1, 1, 16, true>(a, st, what) : launch_few_form<T, G, S, Z, 1, 1, 8, true>(a, st, what);
     }
-    if (p.mx == 2) return launch_few_form<T, G, S, 4, 2, 8, false>(a, st, what);
+    if (p.mx == 2) return launch_few_form<T, G, S, Z, 4, 2, 8, false>(a, st, what);
     if (p.waves == 16)
-        return p.f == 4 ? launch_few_form<T, G, S, 4, 1, 16, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 1, 16, false>(a, st, what) : launch_few_form<T, G, S, 1, 1, 16, false>(a, st, what);
-    return p.f == 4 ? launch_few_form<T, G, S, 4, 1, 8, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, 2, 1, 8, false>(a, st, what) : launch_few_form<T, G, S, 1, 1, 8, false>(a, st, what);
+        return p.f == 4 ? launch_few_form<T, G, S, Z, 4, 1, 16, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, Z, 2, 1, 16, false>(a, st, what) : launch_few_form<T, G, S, Z, 1, 1, 16, false>(a, st, what);
+    return p.f == 4 ? launch_few_form<T, G, S, Z, 4, 1, 8, false>(a, st, what) : p.f == 2 ? launch_few_form<T, G, S, Z, 2, 1, 8, false>(a, st, what) : launch_few_form<T, G, S, Z, 1, 1, 8, false>(a, st, what);
 }
 
 template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS, int SPS>
@@ -644,9 +731,9 @@ int launch_many(Int4Args a, const Int4Plan &p, float *ws, hipStream_t st, const 
     a.xs = xs; a.st = s; a.zt = zt;
     a.splits = p.splits;
     a.slabs = s + 2 * groups * a.Np;
-    const int64_t x_blocks = (groups * a.Mp * (G / 8) + 255) / 256, n_blocks = (groups * a.Np + 255) / 256;
+    const int64_t x_blocks = (groups * a.Mp * (G / 8) + 255) / 256, n_blocks = (a.Np / 16 * ((groups * (G / 32) + 63) / 64) + 3) / 4;       // (a wave each: 16 rows, 64 units)
     if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
-    hipLaunchKernelGGL((int4_prepare_kernel<T, S>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, G, (int)groups, xs, s, zt, (unsigned)x_blocks);
+    hipLaunchKernelGGL((int4_prepare_kernel<T, S, G, Z>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, (int)groups, xs, s, zt, (unsigned)x_blocks);
     if (const int rc = launch_error(what)) return rc;
     const int rc = p.tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 1, 2, 1>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 2, 2, 2>(a, st, what);
     if (rc || p.splits == 1) return rc;
@@ -657,7 +744,7 @@ int launch_many(Int4Args a, const Int4Plan &p, float *ws, hipStream_t st, const 
 template <DenseType T, int G, int S>
 int launch_zeros(const Int4Args &a, float *ws, hipStream_t st, const char *what) {
     const Int4Plan p = plan(a.M, a.N, a.K, G);
-    if (p.f) return launch_few<T, G, S>(a, p, st, what);
+    if (p.f) return a.z ? launch_few<T, G, S, true>(a, p, st, what) : launch_few<T, G, S, false>(a, p, st, what);
     return a.z ? launch_many<T, G, S, true>(a, p, ws, st, what) : launch_many<T, G, S, false>(a, p, ws, st, what);
 }
 template <DenseType T, int G>
@@ -737,8 +824,14 @@ extern "C" int64_t mortar_int4_workspace_bytes(int64_t M, int64_t N, int64_t K, 
 extern "C" int mortar_int4_linear(const void *x, int64_t M, int32_t K, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group, const void *s,
                                   int32_t s_type, int64_t s_n, int64_t s_g, const uint8_t *z, int64_t z_n, int64_t z_g, void *y, int64_t ldy, void *workspace,
                                   void *stream) {
+    return mortar_int4_linear_part(x, M, K, K, ldx, type, c, ldc, N, group, s, s_type, s_n, s_g, z, z_n, z_g, y, ldy, workspace, stream);
+}
+
+extern "C" int mortar_int4_linear_part(const void *x, int64_t M, int32_t K, int32_t K_used, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group,
+                                       const void *s, int32_t s_type, int64_t s_n, int64_t s_g, const uint8_t *z, int64_t z_n, int64_t z_g, void *y, int64_t ldy,
+                                       void *workspace, void *stream) {
     const char *what = "int4_linear";
-    if (M < 0 || K <= 0 || N <= 0) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
+    if (M < 0 || K <= 0 || N <= 0 || K_used > K || K_used <= K - 8) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape", what);
     if (type != MORTAR_BF16 && type != MORTAR_FP16) return mortar_fail(MORTAR_ERR_ARG, "%s: bf16 or fp16", what);
     if (s_type != type && s_type != MORTAR_FP32) return mortar_fail(MORTAR_ERR_ARG, "%s: scales in the type of x or fp32", what);
     CHECK(check_group(what, group));
@@ -755,7 +848,7 @@ extern "C" int mortar_int4_linear(const void *x, int64_t M, int32_t K, int64_t l
     a.x = x; a.ldx = ldx * 2; a.c = c; a.ldc = ldc * 4;
     a.s = s; a.s_n = s_n; a.s_g = s_g; a.z = z; a.z_n = z_n; a.z_g = z_g;
     a.y = static_cast<uint16_t *>(y); a.ldy = ldy;
-    a.M = (int32_t)M; a.N = N; a.K = K; a.groups = (K + group - 1) / group;
+    a.M = (int32_t)M; a.N = N; a.K = K; a.groups = (K + group - 1) / group; a.K_used = K_used;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     float *ws = static_cast<float *>(workspace);
     return type == MORTAR_BF16 ? launch_group<DENSE_BF16>(a, group, s_type == MORTAR_FP32, ws, st, what) : launch_group<DENSE_F16>(a, group, s_type == MORTAR_FP32, ws, st, what);

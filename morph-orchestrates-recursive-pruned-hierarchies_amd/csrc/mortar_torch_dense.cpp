@@ -446,10 +446,11 @@ PyObject *py_linear_int4(PyObject *, PyObject *const *a, Py_ssize_t na) {
         }
         const int64_t n = mortar_int4_workspace_bytes(M, N, Kp, group);
         const at::Tensor ws = n ? empty_bytes(x, n) : at::Tensor();
-        check_rc(mortar_int4_linear(data(r), M, (int32_t)Kp, M > 1 ? r.stride(0) : Kp, type_code(x.scalar_type()), static_cast<const uint32_t *>(data(c)), N > 1 ? c.stride(0) : words,
-                                    (int32_t)N, group, data(s), type_code(s.scalar_type()), s.stride(0), s.stride(1), static_cast<const uint8_t *>(data(z)),
-                                    z.defined() ? z.stride(0) : 0, z.defined() ? z.stride(1) : 0, mut(y), N, mut(ws), stream_of(x)),
-                 "mortar_int4_linear");
+        check_rc(mortar_int4_linear_part(data(r), M, (int32_t)Kp, (int32_t)K, M > 1 ? r.stride(0) : Kp, type_code(x.scalar_type()), static_cast<const uint32_t *>(data(c)),
+                                         N > 1 ? c.stride(0) : words, (int32_t)N, group, data(s), type_code(s.scalar_type()), s.stride(0), s.stride(1),
+                                         static_cast<const uint8_t *>(data(z)), z.defined() ? z.stride(0) : 0, z.defined() ? z.stride(1) : 0, mut(y), N, mut(ws),
+                                         stream_of(x)),
+                 "mortar_int4_linear_part");
     }
     return THPVariable_Wrap(std::move(y));
 }

@@ -1,0 +1,76 @@
+"""Calls at the edges of the 4-bit layer, clipping and the expert rows: weights that are zeros."""
+import pytest
+import torch
+
+from dense_util import assert_within, normals
+from mortar_amd import ops
+from operators_util import int4_bound, int4_weight, pack_codes
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- 4-bit layers
+
+
+#: rows, outputs, inputs, group: products of few rows (x through LDS, as operands, 32 rows of x) and tiles of both sizes, in one and several ranges of K
+ZERO_FORMS = [(1, 40, 2048, 128), (3, 40, 1024, 64), (13, 264, 5632, 32), (7, 520, 1999, 128), (40, 264, 1040, 64), (17, 8200, 1040, 32), (300, 2055, 8200, 128), (4200, 264, 264, 32),
+              (4200, 131, 4104, 64), (4200, 131, 4099, 128), (6000, 517, 131, 32), (6000, 517, 136, 128), (2000, 520, 6152, 32)]
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M,N,K,group", ZERO_FORMS)
+def test_weights_of_zero_add_nothing(dev, M, N, K, group, t, zeros):
+    """Rows of zeros give exactly 0, and what x holds where a group of weights is zeros does not change a bit."""
+    w = normals((N, K), N, torch.float32, dev, 1e-4).to(t)
+    first, last = slice(0, group), slice((K - 1) // group * group, K)
+    w[1], w[N - 2] = 0, 0
+    w[2:20, first], w[20:36, last] = 0, 0
+    c, s, z = ops.quantize_int4_weight(w, group, zeros)
+    x = normals((M, K), M, t, dev, 8.0)
+    y = ops.linear_int4(x, c, s, z, group)
+    assert bool((y[:, [1, N - 2]] == 0).all()) and bool((y[:, 0] != 0).any())
+    for rows, part in ((slice(2, 20), first), (slice(20, 36), last)):
+        other = x.clone()
+        other[:, part] = normals(tuple(other[:, part].shape), 3, t, dev, 100.0)
+        assert torch.equal(ops.linear_int4(other, c, s, z, group)[:, rows], y[:, rows])
+    other = x.clone()
+    other[:, first] = 0
+    ref = other[:, :].double() @ int4_weight(c, s, z, group, K).t()
+    got = ops.linear_int4(other, c, s, z, group)
+    assert_within(got[:, 2:20], ref[:, 2:20], int4_bound(other, s[2:20], None if z is None else z[2:20], group, t, ref[:, 2:20]), "y")
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("M,N,K,group", ZERO_FORMS)
+def test_codes_at_their_zero_points_add_nothing(dev, M, N, K, group, t):
+    """The same for codes of a caller's own, whatever the zero point and the scale."""
+    g = torch.Generator().manual_seed(K)
+    groups = -(-K // group)
+    z = torch.randint(0, 16, (N, groups), generator=g, dtype=torch.uint8).to(dev)
+    s = (torch.rand((N, groups), generator=g) + 0.5).to(dev)
+    at = z.long().repeat_interleave(group, 1)[:, :K]
+    q = torch.randint(0, 16, (N, K), generator=g).to(dev)
+    zero = torch.rand((N, groups), generator=g).to(dev).round().bool().repeat_interleave(group, 1)[:, :K]
+    q[::3] = torch.where(zero, at, q)[::3]
+    q[::4] = at[::4]
+    x = normals((M, K), M, t, dev, 8.0)
+    y = ops.linear_int4(x, pack_codes(q), s, z, group)
+    assert bool((y[:, ::4] == 0).all())
+    ref = x.double() @ int4_weight(pack_codes(q), s, z, group, K).t()
+    assert_within(y, ref, int4_bound(x, s, z, group, t, ref), "y")
+
+
+@pytest.mark.parametrize("M,N,K,group", [(1, 40, 2048, 128), (7, 520, 1999, 64), (40, 264, 1040, 32), (4200, 264, 264, 128), (6000, 517, 136, 32), (4200, 131, 4104, 64)])
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=str)
+def test_zero_points_beyond_the_codes(dev, M, N, K, group, t):
+    """Zero points take 8 bits: W = (c - z) s also where z is more than any code."""
+    groups = -(-K // group)
+    g = torch.Generator().manual_seed(N)
+    z = torch.randint(0, 256, (N, groups), generator=g, dtype=torch.uint8).to(dev)
+    z[0], z[1], z[2], z[3] = 255, 16, 15, 241
+    q = torch.randint(0, 16, (N, K), generator=g).to(dev)
+    s = torch.full((N, groups), 2.0 ** -6, dtype=t, device=dev)
+    x = normals((M, K), M, t, dev)
+    ref = x.double() @ int4_weight(pack_codes(q), s, z, group, K).t()
+    assert_within(ops.linear_int4(x, pack_codes(q), s, z, group), ref, int4_bound(x, s, z, group, t, ref), "y")
