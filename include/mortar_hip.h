@@ -710,6 +710,7 @@ int mortar_grad_clip(const mortar_grad_t *grads, int64_t count, int32_t largest,
  *                              NULL for 1; rows of empty slots are not read
  *   mortar_expert_combine_bwd  dys [N k, d]: row position[n, j] = weights[n, j] dy[n], zeros for empty slots; dw [N, k] in w_type = <dy[n], ys[position[n, j]]>,
  *                              0 for empty slots; either may be NULL
+ * Positions that are none of the rows 0 .. N k - 1 are empty slots, too.
  * full: device, the number of full rows (offsets + n_experts).  x, ys, xs, y, dy, dys in `type` (bf16, fp16 or fp32) of any width and on any address of the type.
  * N k below 2^26. */
 int64_t mortar_expert_sort_workspace_bytes(int64_t slots, int32_t n_experts);

@@ -412,7 +412,15 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a
     const uint32_t i = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (i >= a.slots) return;
     const int row = a.position[i];
-    if ((uint32_t)row >= (uint32_t)a.slots) return;
+    const auto put_dw = [&](float v) {
+        if (a.w_type == MORTAR_FP32) Row<MORTAR_FP32>::put(a.dw + i * 4, v);
+        else if (a.w_type == MORTAR_FP16) Row<MORTAR_FP16>::put(a.dw + i * 2, v);
+        else Row<MORTAR_BF16>::put(a.dw + i * 2, v);
+    };
+    if ((uint32_t)row >= (uint32_t)a.slots) {              // (as an empty slot)
+        if (a.dw && lane == 0) put_dw(0.f);
+        return;
+    }
     const bool live = row < *a.full;
     const float w = live ? read_weight(a, i) : 0.f;
     const char *dy = a.x + i / (uint32_t)a.k * a.ldx;
@@ -444,10 +452,7 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a
     }
     if (!a.dw) return;
     dot = mortar_wave_sum(dot);
-    if (lane) return;
-    if (a.w_type == MORTAR_FP32) Row<MORTAR_FP32>::put(a.dw + i * 4, dot);
-    else if (a.w_type == MORTAR_FP16) Row<MORTAR_FP16>::put(a.dw + i * 2, dot);
-    else Row<MORTAR_BF16>::put(a.dw + i * 2, dot);
+    if (lane == 0) put_dw(dot);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

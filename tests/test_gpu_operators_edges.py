@@ -1,10 +1,11 @@
-"""Calls at the edges of the 4-bit layer, clipping and the expert rows: weights that are zeros."""
+"""Calls at the edges of the 4-bit layer, clipping and the expert rows: weights that are zeros, orders with slots taken
+out."""
 import pytest
 import torch
 
 from dense_util import assert_within, normals
 from mortar_amd import ops
-from operators_util import int4_bound, int4_weight, pack_codes
+from operators_util import draw_ids, int4_bound, int4_weight, pack_codes
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +75,43 @@ def test_zero_points_beyond_the_codes(dev, M, N, K, group, t):
     x = normals((M, K), M, t, dev)
     ref = x.double() @ int4_weight(pack_codes(q), s, z, group, K).t()
     assert_within(ops.linear_int4(x, pack_codes(q), s, z, group), ref, int4_bound(x, s, z, group, t, ref), "y")
+
+
+# ---- expert rows
+
+
+def _soil(*shapes, dtype, dev):
+    """Memory that the next allocations of these shapes take holds NaN."""
+    held = [torch.full(s, float("nan"), dtype=dtype, device=dev) for s in shapes for _ in range(3)]
+    torch.cuda.synchronize()
+    del held
+
+
+def _taken_out(N, k, dev):
+    """(order, the same with some positions that are none of its rows, which slots those are)"""
+    ids = draw_ids(N, k, 9, N, repeat=True).to(dev)
+    good = ops.expert_sort(ids, 9)
+    out = torch.rand((N, k), generator=torch.Generator().manual_seed(6)).to(dev) < 0.3
+    out[0, 0], out[N - 1] = True, True
+    bad = torch.tensor([-1, N * k, 1 << 30, -(1 << 31)], dtype=torch.int32, device=dev)[torch.arange(N * k, device=dev).view(N, k) % 4]
+    return good, ops.ExpertOrder(torch.where(out, bad, good.position), good.token, good.offsets), out
+
+
+TAKEN_OUT = [(20, 3, 72), (300, 8, 520), (9, 70, 77), (700, 1, 1999)]
+
+
+@pytest.mark.parametrize("t,wt", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.float16, torch.float16)], ids=str)
+@pytest.mark.parametrize("N,k,d", TAKEN_OUT)
+def test_slots_taken_out_have_no_gradient(dev, N, k, d, t, wt):
+    """Positions that are none of the rows (slots dropped behind the sort) are empty slots: their weights have a gradient of 0, the others theirs."""
+    good, order, out = _taken_out(N, k, dev)
+    dy, w, ys = normals((N, d), 2, t, dev), normals((N, k), 3, wt, dev), normals((N * k, d), 4, t, dev)
+    ys.requires_grad_(), w.requires_grad_()
+    _soil((N, k), dtype=wt, dev=dev)
+    (dw,) = torch.autograd.grad(ops.expert_combine(ys.detach(), w, order), w, dy)
+    (want,) = torch.autograd.grad(ops.expert_combine(ys.detach(), w, good), w, dy)
+    assert torch.equal(dw, torch.where(out, 0, want))
+    dys, dw = torch.autograd.grad(ops.expert_combine(ys, w, order), (ys, w), dy)
+    hole = torch.where(out, 0, w.detach())
+    rows = good.position[~out].long()
+    assert torch.equal(dw, torch.where(out, 0, want)) and torch.equal(dys[rows], torch.autograd.grad(ops.expert_combine(ys, hole, good), ys, dy)[0][rows])
