@@ -710,6 +710,7 @@ int mortar_grad_clip(const mortar_grad_t *grads, int64_t count, int32_t largest,
  *                              NULL for 1; rows of empty slots are not read
  *   mortar_expert_combine_bwd  dys [N k, d]: row position[n, j] = weights[n, j] dy[n], zeros for empty slots; dw [N, k] in w_type = <dy[n], ys[position[n, j]]>,
  *                              0 for empty slots; either may be NULL
+ *   mortar_expert_dispatch_rows, mortar_expert_combine_bwd_rows  the same with the token of each row: rows that no slot of their token names are zeros as well
  * Positions that are none of the rows 0 .. N k - 1 are empty slots, too.
  * full: device, the number of full rows (offsets + n_experts).  x, ys, xs, y, dy, dys in `type` (bf16, fp16 or fp32) of any width and on any address of the type.
  * N k below 2^26. */
@@ -718,10 +719,14 @@ int mortar_expert_sort(const void *ids, int32_t ids_64, int64_t N, int32_t k, in
                        void *workspace, void *stream);
 int mortar_expert_dispatch(const void *x, int64_t N, int32_t d, int64_t ldx, int32_t type, int32_t k, const int32_t *position, const int32_t *full, void *xs,
                            void *stream);
+int mortar_expert_dispatch_rows(const void *x, int64_t N, int32_t d, int64_t ldx, int32_t type, int32_t k, const int32_t *position, const int32_t *full,
+                                const int32_t *token, void *xs, void *stream);
 int mortar_expert_combine(const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position, const int32_t *full, const void *weights,
                           int32_t w_type, void *y, void *stream);
 int mortar_expert_combine_bwd(const void *dy, int64_t lddy, const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position,
                               const int32_t *full, const void *weights, int32_t w_type, void *dys, void *dw, void *stream);
+int mortar_expert_combine_bwd_rows(const void *dy, int64_t lddy, const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position,
+                                   const int32_t *full, const int32_t *token, const void *weights, int32_t w_type, void *dys, void *dw, void *stream);
 
 #ifdef __cplusplus
 }

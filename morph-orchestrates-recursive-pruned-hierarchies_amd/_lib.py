@@ -131,7 +131,9 @@ _SIGS = {
     "mortar_expert_sort_workspace_bytes": (c_i64, [c_i64, c_i32]),
     "mortar_expert_sort": (C.c_int, [c_vp, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "mortar_expert_dispatch": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp]),
+    "mortar_expert_dispatch_rows": (C.c_int, [c_vp, c_i64, c_i32, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "mortar_expert_combine": (C.c_int, [c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp]),
+    "mortar_expert_combine_bwd_rows": (C.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
     "mortar_expert_combine_bwd": (C.c_int, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
 }
 

@@ -6,6 +6,8 @@
 //              backward: dys[position[n, j]] = w[n, j] dy[n] (zeros for empty slots),  dw[n, j] = <dy[n], ys[position[n, j]]> (0 for empty ones)
 // Positions are a permutation of the rows, so every row is written by exactly one wave and no atomics are needed: sums run over a token's slots in
 // their order, in fp32, and are rounded once.  Rows of empty slots are not read.  What bounds all but the sort is the memory.
+// A position that is none of the rows takes its slot out of the order; the row that it had is then named by no slot.  With the tokens of the rows at hand a wave
+// looks whether its row is, and makes it zeros otherwise.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -267,7 +269,7 @@ struct RowArgs {
     char *out;                   // dispatch: xs, combine: y, combine backward: dys or null
     char *dw;                    // combine backward: gradients of the weights or null
     const char *w;               // weights [N, k], or null for 1
-    const int32_t *position, *full;
+    const int32_t *position, *full, *token;      // token: of each row, or null
     int64_t ldx, slots;          // slots: N k
     int32_t k, d, w_type;
 };
@@ -275,6 +277,33 @@ struct RowArgs {
 __device__ __forceinline__ float read_weight(const RowArgs &a, int64_t i) {
     if (!a.w) return 1.0f;
     return a.w_type == MORTAR_FP32 ? Row<MORTAR_FP32>::one(a.w + i * 4) : a.w_type == MORTAR_FP16 ? Row<MORTAR_FP16>::one(a.w + i * 2) : Row<MORTAR_BF16>::one(a.w + i * 2);
+}
+
+// Whether one of its token's slots names row i.  The loads are on their way while the wave does something else: begin, then named.
+struct Named {
+    int64_t first;               // slot of the token, below a.slots if there is one
+    int32_t position;
+    __device__ __forceinline__ void begin(const RowArgs &a, uint32_t i, int lane) {
+        first = a.token ? (int64_t)(uint32_t)a.token[i] * a.k : a.slots;
+        position = -1;
+        if (first < a.slots && lane < a.k) position = a.position[first + lane];
+    }
+    __device__ __forceinline__ bool named(const RowArgs &a, uint32_t i, int lane) const {
+        bool is = __ballot(position == (int)i) != 0;
+        if (first < a.slots)
+            for (int j = 64; j < a.k; j += 64) is |= __ballot(j + lane < a.k && a.position[first + min(j + lane, a.k - 1)] == (int)i) != 0;
+        return is;
+    }
+};
+// Row i as zeros.
+template <int SIZE>
+__device__ __forceinline__ void clear_row(const RowArgs &a, uint32_t i, int lane) {
+    const int bytes = a.d * SIZE, units = bytes / 16, at = units * 16 + lane * SIZE;
+    char *dst = a.out + (int64_t)i * bytes;
+    for (int u = lane; u < units; u += 64) *reinterpret_cast<u32x4_any_t *>(dst + u * 16) = u32x4_any_t{0, 0, 0, 0};
+    if (at >= bytes) return;
+    if constexpr (SIZE == 4) *reinterpret_cast<uint32_t *>(dst + at) = 0u;
+    else *reinterpret_cast<uint16_t *>(dst + at) = 0;
 }
 
 // A wave per slot; the rows of a token are read by neighbouring waves and come out of the caches but once.  Bound by the rows written: 4096 tokens, 8 slots
@@ -285,25 +314,29 @@ __global__ __launch_bounds__(256) void expert_dispatch_kernel(const RowArgs a) {
     const uint32_t i = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (i >= a.slots) return;
     const int row = a.position[i];
-    if ((uint32_t)row >= (uint32_t)a.slots) return;        // (no order of this many slots)
-    const char *src = a.x + i / (uint32_t)a.k * a.ldx;
-    char *dst = a.out + (int64_t)row * a.d * SIZE;
-    const int bytes = a.d * SIZE, units = bytes / 16;
     const bool live = row < *a.full;
-    int u = lane;
-    for (; u + 192 < units; u += 256) {
-        u32x4_t v[4];
+    Named own;
+    own.begin(a, i, lane);
+    if ((uint32_t)row < (uint32_t)a.slots) {
+        const char *src = a.x + i / (uint32_t)a.k * a.ldx;
+        char *dst = a.out + (int64_t)row * a.d * SIZE;
+        const int bytes = a.d * SIZE, units = bytes / 16;
+        int u = lane;
+        for (; u + 192 < units; u += 256) {
+            u32x4_t v[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = live ? *reinterpret_cast<const u32x4_any_t *>(src + (u + q * 64) * 16) : u32x4_t{0, 0, 0, 0};
+            for (int q = 0; q < 4; ++q) v[q] = live ? *reinterpret_cast<const u32x4_any_t *>(src + (u + q * 64) * 16) : u32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int q = 0; q < 4; ++q) put16<STREAM>(dst + (u + q * 64) * 16, v[q]);
+            for (int q = 0; q < 4; ++q) put16<STREAM>(dst + (u + q * 64) * 16, v[q]);
+        }
+        for (; u < units; u += 64) put16<STREAM>(dst + u * 16, live ? *reinterpret_cast<const u32x4_any_t *>(src + u * 16) : u32x4_any_t{0, 0, 0, 0});
+        const int at = units * 16 + lane * SIZE;
+        if (at < bytes) {
+            if constexpr (SIZE == 4) *reinterpret_cast<uint32_t *>(dst + at) = live ? *reinterpret_cast<const uint32_t *>(src + at) : 0u;
+            else *reinterpret_cast<uint16_t *>(dst + at) = live ? *reinterpret_cast<const uint16_t *>(src + at) : (uint16_t)0;
+        }
     }
-    for (; u < units; u += 64) put16<STREAM>(dst + u * 16, live ? *reinterpret_cast<const u32x4_any_t *>(src + u * 16) : u32x4_any_t{0, 0, 0, 0});
-    const int at = units * 16 + lane * SIZE;
-    if (at < bytes) {
-        if constexpr (SIZE == 4) *reinterpret_cast<uint32_t *>(dst + at) = live ? *reinterpret_cast<const uint32_t *>(src + at) : 0u;
-        else *reinterpret_cast<uint16_t *>(dst + at) = live ? *reinterpret_cast<const uint16_t *>(src + at) : (uint16_t)0;
-    }
+    if (a.token && !own.named(a, i, lane)) clear_row<SIZE>(a, i, lane);
 }
 
 // A wave per TOKENS consecutive tokens and 64 units of their rows, the rows of eight slots on their way at a time: with few slots per token one token alone
@@ -412,47 +445,47 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a
     const uint32_t i = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     if (i >= a.slots) return;
     const int row = a.position[i];
-    const auto put_dw = [&](float v) {
-        if (a.w_type == MORTAR_FP32) Row<MORTAR_FP32>::put(a.dw + i * 4, v);
-        else if (a.w_type == MORTAR_FP16) Row<MORTAR_FP16>::put(a.dw + i * 2, v);
-        else Row<MORTAR_BF16>::put(a.dw + i * 2, v);
-    };
-    if ((uint32_t)row >= (uint32_t)a.slots) {              // (as an empty slot)
-        if (a.dw && lane == 0) put_dw(0.f);
-        return;
-    }
-    const bool live = row < *a.full;
-    const float w = live ? read_weight(a, i) : 0.f;
-    const char *dy = a.x + i / (uint32_t)a.k * a.ldx;
-    const int64_t at_row = (int64_t)row * a.d * R::SIZE;
-    const int units = a.d / R::UNIT;
-    float dot = 0.f;
-    for (int u = lane; u < units; u += 64) {
-        float g[R::UNIT], f[R::UNIT];
+    const int32_t full = *a.full;
+    Named own;
+    own.begin(a, i, lane);
+    float dot = 0.f;                                       // (a slot whose position is none of the rows: as an empty one)
+    if ((uint32_t)row < (uint32_t)a.slots) {
+        const bool live = row < full;
+        const float w = live ? read_weight(a, i) : 0.f;
+        const char *dy = a.x + i / (uint32_t)a.k * a.ldx;
+        const int64_t at_row = (int64_t)row * a.d * R::SIZE;
+        const int units = a.d / R::UNIT;
+        for (int u = lane; u < units; u += 64) {
+            float g[R::UNIT], f[R::UNIT];
 #pragma unroll
-        for (int t = 0; t < R::UNIT; ++t) g[t] = f[t] = 0.f;
-        if (live) {
-            const u32x4_t gw = R::load(dy + (int64_t)u * 16);
-            if (a.dw) R::unpack(R::load(a.ys + at_row + (int64_t)u * 16), f);
-            R::unpack(gw, g);
+            for (int t = 0; t < R::UNIT; ++t) g[t] = f[t] = 0.f;
+            if (live) {
+                const u32x4_t gw = R::load(dy + (int64_t)u * 16);
+                if (a.dw) R::unpack(R::load(a.ys + at_row + (int64_t)u * 16), f);
+                R::unpack(gw, g);
 #pragma unroll
-            for (int t = 0; t < R::UNIT; ++t) dot = __builtin_fmaf(g[t], f[t], dot);
+                for (int t = 0; t < R::UNIT; ++t) dot = __builtin_fmaf(g[t], f[t], dot);
+            }
+            if (a.out) {
+#pragma unroll
+                for (int t = 0; t < R::UNIT; ++t) g[t] = live ? g[t] * w : 0.f;
+                put16<STREAM>(a.out + at_row + (int64_t)u * 16, R::pack(g));
+            }
         }
-        if (a.out) {
-#pragma unroll
-            for (int t = 0; t < R::UNIT; ++t) g[t] = live ? g[t] * w : 0.f;
-            put16<STREAM>(a.out + at_row + (int64_t)u * 16, R::pack(g));
+        const int last = units * R::UNIT + lane;
+        if (last < a.d) {
+            const float g = live ? R::one(dy + (int64_t)last * R::SIZE) : 0.f;
+            if (live && a.dw) dot = __builtin_fmaf(g, R::one(a.ys + at_row + (int64_t)last * R::SIZE), dot);
+            if (a.out) R::put(a.out + at_row + (int64_t)last * R::SIZE, live ? g * w : 0.f);
         }
     }
-    const int last = units * R::UNIT + lane;
-    if (last < a.d) {
-        const float g = live ? R::one(dy + (int64_t)last * R::SIZE) : 0.f;
-        if (live && a.dw) dot = __builtin_fmaf(g, R::one(a.ys + at_row + (int64_t)last * R::SIZE), dot);
-        if (a.out) R::put(a.out + at_row + (int64_t)last * R::SIZE, live ? g * w : 0.f);
-    }
+    if (a.out && a.token && !own.named(a, i, lane)) clear_row<R::SIZE>(a, i, lane);
     if (!a.dw) return;
     dot = mortar_wave_sum(dot);
-    if (lane == 0) put_dw(dot);
+    if (lane) return;
+    if (a.w_type == MORTAR_FP32) Row<MORTAR_FP32>::put(a.dw + i * 4, dot);
+    else if (a.w_type == MORTAR_FP16) Row<MORTAR_FP16>::put(a.dw + i * 2, dot);
+    else Row<MORTAR_BF16>::put(a.dw + i * 2, dot);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -502,6 +535,11 @@ extern "C" int mortar_expert_sort(const void *ids, int32_t ids_64, int64_t N, in
 
 extern "C" int mortar_expert_dispatch(const void *x, int64_t N, int32_t d, int64_t ldx, int32_t type, int32_t k, const int32_t *position, const int32_t *full, void *xs,
                                       void *stream) {
+    return mortar_expert_dispatch_rows(x, N, d, ldx, type, k, position, full, nullptr, xs, stream);
+}
+
+extern "C" int mortar_expert_dispatch_rows(const void *x, int64_t N, int32_t d, int64_t ldx, int32_t type, int32_t k, const int32_t *position, const int32_t *full,
+                                           const int32_t *token, void *xs, void *stream) {
     const char *what = "expert_dispatch";
     CHECK(check_rows(what, N, k, d, type));
     if (N == 0) return MORTAR_OK;
@@ -509,9 +547,10 @@ extern "C" int mortar_expert_dispatch(const void *x, int64_t N, int32_t d, int64
     CHECK(check_pointer(what, "xs", xs, type));
     CHECK(check_pointer(what, "position", position, MORTAR_FP32));
     CHECK(check_pointer(what, "full", full, MORTAR_FP32));
+    if (token) CHECK(check_pointer(what, "token", token, MORTAR_FP32));
     RowArgs a{};
     a.x = static_cast<const char *>(x); a.ldx = ldx * (type == MORTAR_FP32 ? 4 : 2);
-    a.out = static_cast<char *>(xs); a.position = position; a.full = full;
+    a.out = static_cast<char *>(xs); a.position = position; a.full = full; a.token = token;
     a.slots = N * k; a.k = k; a.d = d;
     const dim3 grid((unsigned)((a.slots + 3) / 4));
     const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -541,12 +580,18 @@ extern "C" int mortar_expert_combine(const void *ys, int64_t N, int32_t d, int32
 
 extern "C" int mortar_expert_combine_bwd(const void *dy, int64_t lddy, const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position,
                                          const int32_t *full, const void *weights, int32_t w_type, void *dys, void *dw, void *stream) {
+    return mortar_expert_combine_bwd_rows(dy, lddy, ys, N, d, type, k, position, full, nullptr, weights, w_type, dys, dw, stream);
+}
+
+extern "C" int mortar_expert_combine_bwd_rows(const void *dy, int64_t lddy, const void *ys, int64_t N, int32_t d, int32_t type, int32_t k, const int32_t *position,
+                                              const int32_t *full, const int32_t *token, const void *weights, int32_t w_type, void *dys, void *dw, void *stream) {
     const char *what = "expert_combine_bwd";
     CHECK(check_rows(what, N, k, d, type));
     if (N == 0 || (!dys && !dw)) return MORTAR_OK;
     CHECK(check_pointer(what, "dy", dy, type));
     CHECK(check_pointer(what, "position", position, MORTAR_FP32));
     CHECK(check_pointer(what, "full", full, MORTAR_FP32));
+    if (token) CHECK(check_pointer(what, "token", token, MORTAR_FP32));
     if (dys) CHECK(check_pointer(what, "dys", dys, type));
     if ((weights || dw) && !known(w_type)) return mortar_fail(MORTAR_ERR_ARG, "%s: bad type of the weights", what);
     if (weights) CHECK(check_pointer(what, "weights", weights, w_type));
@@ -556,7 +601,7 @@ extern "C" int mortar_expert_combine_bwd(const void *dy, int64_t lddy, const voi
     a.x = static_cast<const char *>(dy); a.ldx = lddy * (type == MORTAR_FP32 ? 4 : 2);
     a.ys = static_cast<const char *>(ys); a.out = static_cast<char *>(dys); a.dw = static_cast<char *>(dw);
     a.w = static_cast<const char *>(weights); a.w_type = w_type;
-    a.position = position; a.full = full; a.slots = N * k; a.k = k; a.d = d;
+    a.position = position; a.full = full; a.token = token; a.slots = N * k; a.k = k; a.d = d;
     const dim3 grid((unsigned)((a.slots + 3) / 4));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const bool past = past_caches(a, type);

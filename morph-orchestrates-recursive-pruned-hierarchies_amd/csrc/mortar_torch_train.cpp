@@ -205,24 +205,37 @@ PyObject *py_expert_sort(PyObject *, PyObject *const *a, Py_ssize_t na) {
     return Py_BuildValue("(NNN)", p, t, o);
 }
 
-// Positions [N, k] and offsets [E + 1] of an order, as a launch reads them.
+// Positions [N, k], offsets [E + 1] and (where there are any) the rows' tokens [N k] of an order, as a launch reads them.
 struct Order {
-    at::Tensor position, offsets;
+    at::Tensor position, offsets, token;
     int64_t N, k;
     const int32_t *pos() const { return static_cast<const int32_t *>(position.const_data_ptr()); }
     const int32_t *full() const { return static_cast<const int32_t *>(offsets.const_data_ptr()) + offsets.size(0) - 1; }
+    const int32_t *tokens() const { return static_cast<const int32_t *>(data(token)); }
 };
 
-Order order_of(const at::Tensor &position, const at::Tensor &offsets) { return {position.contiguous(), offsets.contiguous(), position.size(0), position.size(1)}; }
+Order order_of(const at::Tensor &position, const at::Tensor &offsets, const at::Tensor &token) {
+    return {position.contiguous(), offsets.contiguous(), token.defined() ? token.contiguous() : token, position.size(0), position.size(1)};
+}
 
-Order order_arg(PyObject *p, PyObject *o, const at::Tensor &x, const char *what) {
-    const at::Tensor position = tensor_arg(p, what, "position"), offsets = tensor_arg(o, what, "offsets");
+Order order_arg(PyObject *p, PyObject *t, PyObject *o, const at::Tensor &x, const char *what) {
+    const at::Tensor position = tensor_arg(p, what, "position"), offsets = tensor_arg(o, what, "offsets"), token = optional_arg(t, what, "token");
     same_device(x, position, what, "position");
     same_device(x, offsets, what, "offsets");
     TORCH_CHECK_TYPE(position.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt, what, ": position and offsets must be int32");
     TORCH_CHECK_VALUE(position.dim() == 2 && position.size(1) > 0 && offsets.dim() == 1 && offsets.size(0) > 1, what, ": expected position [tokens, slots] and offsets [experts + 1]");
     TORCH_CHECK_VALUE(position.numel() < (1 << 26), what, ": too many slots");
-    return order_of(position, offsets);
+    if (token.defined()) {
+        same_device(x, token, what, "token");
+        TORCH_CHECK_TYPE(token.scalar_type() == at::kInt, what, ": token must be int32");
+        TORCH_CHECK_VALUE(token.dim() == 1 && token.size(0) == position.numel(), what, ": expected token [", position.numel(), "], got ", token.sizes());
+    }
+    return order_of(position, offsets, token);
+}
+
+// Memory of rows [N k, d] by slot: without the rows' tokens a launch leaves what no position names as it was.
+at::Tensor empty_slots(const at::Tensor &like, const Order &o, int64_t d) {
+    return o.token.defined() ? empty_like_rows(like, {o.N * o.k, d}) : at::zeros({o.N * o.k, d}, like.options().requires_grad(false));
 }
 
 void check_rows(const at::Tensor &x, int64_t rows, const char *what, const char *name) {
@@ -237,9 +250,10 @@ at::Tensor lines(const at::Tensor &x) { return x.size(1) > 1 && x.stride(1) != 1
 at::Tensor dispatch(const at::Tensor &x, const Order &o) {
     const c10::DeviceGuard guard(x.device());
     const at::Tensor r = lines(x);
-    at::Tensor xs = empty_like_rows(x, {o.N * o.k, x.size(1)});
-    check_rc(mortar_expert_dispatch(data(r), o.N, (int32_t)x.size(1), r.stride(0), type_code(x.scalar_type()), (int32_t)o.k, o.pos(), o.full(), mut(xs), stream_of(x)),
-             "mortar_expert_dispatch");
+    at::Tensor xs = empty_slots(x, o, x.size(1));
+    check_rc(mortar_expert_dispatch_rows(data(r), o.N, (int32_t)x.size(1), r.stride(0), type_code(x.scalar_type()), (int32_t)o.k, o.pos(), o.full(), o.tokens(), mut(xs),
+                                         stream_of(x)),
+             "mortar_expert_dispatch_rows");
     return xs;
 }
 
@@ -253,37 +267,49 @@ at::Tensor combine(const at::Tensor &ys, const at::Tensor &w, const Order &o) {
     return y;
 }
 
+// What a node keeps of an order, behind `first` saved tensors: positions, offsets, tokens.
+void keep_order(AutogradContext *ctx, const Order &o) {
+    ctx->saved_data["offsets"] = o.offsets.size(0);
+    ctx->saved_data["shape"] = o.position.sizes();
+    ctx->saved_data["tokens"] = o.token.defined();
+}
+Order kept_order(AutogradContext *ctx, const variable_list &v, size_t first, const at::Tensor &g, const char *what) {
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    return order_of(kept(v[first], g, shape, at::kInt, what), kept(v[first + 1], g, {ctx->saved_data["offsets"].toInt()}, at::kInt, what),
+                    ctx->saved_data["tokens"].toBool() ? kept(v[first + 2], g, {shape[0] * shape[1]}, at::kInt, what) : at::Tensor());
+}
+
 struct DispatchFn : public torch::autograd::Function<DispatchFn> {
-    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &position, const at::Tensor &offsets) {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &position, const at::Tensor &offsets, const std::optional<at::Tensor> &token) {
+        const Order o = order_of(position, offsets, token ? *token : at::Tensor());
         ctx->save_for_backward({position, offsets});
-        ctx->saved_data["offsets"] = offsets.size(0);
-        ctx->saved_data["shape"] = position.sizes();
-        return dispatch(x, order_of(position, offsets));
+        keep_order(ctx, o);
+        ctx->saved_data["tokens"] = false;               // (rows by slot are read only)
+        return dispatch(x, o);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        variable_list out(3);
+        variable_list out(4);
         const char *what = "expert_dispatch";
         const at::Tensor g = plain_gradient(grads[0], what);
         if (!g.defined()) return out;
-        const auto v = ctx->get_saved_variables();
-        out[0] = combine(g, at::Tensor(), order_of(kept(v[0], g, ctx->saved_data["shape"].toIntVector(), at::kInt, what),
-                                                   kept(v[1], g, {ctx->saved_data["offsets"].toInt()}, at::kInt, what)));
+        out[0] = combine(g, at::Tensor(), kept_order(ctx, ctx->get_saved_variables(), 0, g, what));
         return out;
     }
 };
 
 struct CombineFn : public torch::autograd::Function<CombineFn> {
-    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &ys, const std::optional<at::Tensor> &weights, const at::Tensor &position, const at::Tensor &offsets) {
+    static at::Tensor forward(AutogradContext *ctx, const at::Tensor &ys, const std::optional<at::Tensor> &weights, const at::Tensor &position, const at::Tensor &offsets,
+                              const std::optional<at::Tensor> &token) {
         const at::Tensor w = weights ? *weights : at::Tensor();
         const bool need_w = w.defined() && ctx->needs_input_grad(1);
-        ctx->save_for_backward({need_w ? ys : at::Tensor(), w, position, offsets});
-        ctx->saved_data["offsets"] = offsets.size(0);
-        ctx->saved_data["shape"] = position.sizes();
+        const Order o = order_of(position, offsets, token ? *token : at::Tensor());
+        ctx->save_for_backward({need_w ? ys : at::Tensor(), w, position, offsets, o.token});
+        keep_order(ctx, o);
         ctx->saved_data["type"] = w.defined() ? c10::IValue(w.scalar_type()) : c10::IValue();
-        return combine(ys, w, order_of(position, offsets));
+        return combine(ys, w, o);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        variable_list out(4);
+        variable_list out(5);
         const char *what = "expert_combine";
         const at::Tensor g = plain_gradient(grads[0], what);
         if (!g.defined()) return out;
@@ -293,40 +319,42 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
         const bool weighted = !ctx->saved_data["type"].isNone();
         // (edges are counted over the tensors that are there)
         const bool need_y = ctx->needs_input_grad(0), need_w = weighted && ctx->needs_input_grad(1);
-        const Order o = order_of(kept(v[2], g, shape, at::kInt, what), kept(v[3], g, {ctx->saved_data["offsets"].toInt()}, at::kInt, what));
+        const Order o = kept_order(ctx, v, 2, g, what);
         const c10::DeviceGuard guard(g.device());
         at::Tensor w, ys, dys, dw;
         if (weighted) w = kept(v[1], g, shape, ctx->saved_data["type"].toScalarType(), what).contiguous();
         if (need_w) ys = kept(v[0], g, {slots, d}, g.scalar_type(), what).contiguous();
-        if (need_y) dys = empty_like_rows(g, {slots, d});
+        if (need_y) dys = empty_slots(g, o, d);
         if (need_w) dw = at::empty(shape, w.options().requires_grad(false));
         const at::Tensor r = lines(g);
-        check_rc(mortar_expert_combine_bwd(data(r), r.stride(0), data(ys), o.N, (int32_t)d, type_code(g.scalar_type()), (int32_t)o.k, o.pos(), o.full(), data(w),
-                                           weighted ? type_code(w.scalar_type()) : 0, mut(dys), mut(dw), stream_of(g)),
-                 "mortar_expert_combine_bwd");
+        check_rc(mortar_expert_combine_bwd_rows(data(r), r.stride(0), data(ys), o.N, (int32_t)d, type_code(g.scalar_type()), (int32_t)o.k, o.pos(), o.full(), o.tokens(),
+                                                data(w), weighted ? type_code(w.scalar_type()) : 0, mut(dys), mut(dw), stream_of(g)),
+                 "mortar_expert_combine_bwd_rows");
         out[0] = dys;
         out[1] = dw;
         return out;
     }
 };
 
-// expert_dispatch(x, position, offsets) -> xs [N k, d]
+std::optional<at::Tensor> maybe(const at::Tensor &t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+
+// expert_dispatch(x, position, token, offsets) -> xs [N k, d]
 PyObject *py_expert_dispatch(PyObject *, PyObject *const *a, Py_ssize_t na) {
     const char *what = "expert_dispatch";
-    TORCH_CHECK_TYPE(na == 3, "expert_dispatch: 3 arguments");
+    TORCH_CHECK_TYPE(na == 4, "expert_dispatch: 4 arguments");
     const at::Tensor x = tensor_arg(a[0], what, "x");
-    const Order o = order_arg(a[1], a[2], x, what);
+    const Order o = order_arg(a[1], a[2], a[3], x, what);
     check_rows(x, o.N, what, "x");
-    at::Tensor xs = c10::GradMode::is_enabled() && x.requires_grad() ? DispatchFn::apply(x, o.position, o.offsets) : dispatch(x, o);
+    at::Tensor xs = c10::GradMode::is_enabled() && x.requires_grad() ? DispatchFn::apply(x, o.position, o.offsets, maybe(o.token)) : dispatch(x, o);
     return THPVariable_Wrap(std::move(xs));
 }
 
-// expert_combine(ys, weights, position, offsets) -> y [N, d]
+// expert_combine(ys, weights, position, token, offsets) -> y [N, d]
 PyObject *py_expert_combine(PyObject *, PyObject *const *a, Py_ssize_t na) {
     const char *what = "expert_combine";
-    TORCH_CHECK_TYPE(na == 4, "expert_combine: 4 arguments");
+    TORCH_CHECK_TYPE(na == 5, "expert_combine: 5 arguments");
     const at::Tensor ys = tensor_arg(a[0], what, "ys"), w = optional_arg(a[1], what, "weights");
-    const Order o = order_arg(a[2], a[3], ys, what);
+    const Order o = order_arg(a[2], a[3], a[4], ys, what);
     check_rows(ys, o.N * o.k, what, "ys");
     if (w.defined()) {
         same_device(ys, w, what, "weights");
@@ -335,7 +363,7 @@ PyObject *py_expert_combine(PyObject *, PyObject *const *a, Py_ssize_t na) {
     }
     at::Tensor y;
     if (c10::GradMode::is_enabled() && (ys.requires_grad() || (w.defined() && w.requires_grad())))
-        y = CombineFn::apply(ys, w.defined() ? std::optional<at::Tensor>(w) : std::nullopt, o.position, o.offsets);
+        y = CombineFn::apply(ys, maybe(w), o.position, o.offsets, maybe(o.token));
     else
         y = combine(ys, w, o);
     return THPVariable_Wrap(std::move(y));

@@ -645,9 +645,10 @@ def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, error_i
 
 class ExpertOrder(NamedTuple):
     """Slots [N, k] of tokens sorted by expert: ``position`` int32 [N, k], the row of each slot; ``token`` int32 [N * k], the token of each row; ``offsets`` int32
-    [n_experts + 1], the first row of each expert and behind them the number of rows that have one."""
+    [n_experts + 1], the first row of each expert and behind them the number of rows that have one.  A position that is none of the rows (-1, say) takes
+    its slot out: it counts as empty, and the row that it had as one of zeros.  An order of one's own may do without the tokens (None)."""
     position: Tensor
-    token: Tensor
+    token: Tensor | None
     offsets: Tensor
 
 
@@ -662,11 +663,11 @@ def expert_dispatch(x: Tensor, order: ExpertOrder) -> Tensor:
     """xs [N * k, d], differentiable: the rows of x [N, d] (bf16, fp16, fp32; any width and strides) at the positions of their slots, expert by expert, zeros in the
     rows behind the last expert's.  The gradient of a token is the sum over its full slots, in order, in fp32.  First derivatives only.  As with torch's own
     operators a backward pass is captured into a graph only once no graph of the same leaves that was recorded on the default stream is left."""
-    return _lib.native().expert_dispatch(x, order.position, order.offsets)
+    return _lib.native().expert_dispatch(x, order.position, order.token, order.offsets)
 
 
 def expert_combine(ys: Tensor, weights: Tensor | None, order: ExpertOrder) -> Tensor:
     """y [N, d] = sum over a token's full slots of weights[n, j] * ys[position[n, j]], differentiable in ys [N * k, d] and weights [N, k] (None: 1).  Sums are fp32
     in the order of the slots, the result is in the type of ys; rows and weights of empty slots are not looked at and have gradients of 0.
     First derivatives only."""
-    return _lib.native().expert_combine(ys, weights, order.position, order.offsets)
+    return _lib.native().expert_combine(ys, weights, order.position, order.token, order.offsets)

@@ -115,3 +115,41 @@ def test_slots_taken_out_have_no_gradient(dev, N, k, d, t, wt):
     hole = torch.where(out, 0, w.detach())
     rows = good.position[~out].long()
     assert torch.equal(dw, torch.where(out, 0, want)) and torch.equal(dys[rows], torch.autograd.grad(ops.expert_combine(ys, hole, good), ys, dy)[0][rows])
+
+
+@pytest.mark.parametrize("t,wt", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.float16, torch.float16)], ids=str)
+@pytest.mark.parametrize("named", [True, False])
+@pytest.mark.parametrize("N,k,d", TAKEN_OUT)
+def test_rows_without_a_slot_are_zeros(dev, N, k, d, t, wt, named):
+    """Rows whose slots were taken out, in what is dispatched and in the gradient of the combined rows; an order of a caller's own may have no tokens."""
+    good, order, out = _taken_out(N, k, dev)
+    order = order if named else order._replace(token=None)
+    x, dy, w, ys = (normals(s, i, v, dev) for i, (s, v) in enumerate((((N, d), t), ((N, d), t), ((N, k), wt), ((N * k, d), t))))
+    gone = torch.zeros((N * k, 1), dtype=torch.bool, device=dev)
+    gone[good.position[out].long()] = True
+    x.requires_grad_(), ys.requires_grad_(), w.requires_grad_()
+    _soil((N * k, d), dtype=t, dev=dev)
+    xs = ops.expert_dispatch(x, order)
+    assert torch.equal(xs.detach(), torch.where(gone, 0, ops.expert_dispatch(x.detach(), good)))
+    (dx,) = torch.autograd.grad(xs, x, ys.detach())
+    assert torch.equal(dx, torch.autograd.grad(ops.expert_dispatch(x, good), x, torch.where(gone, 0, ys.detach()))[0])
+    y = ops.expert_combine(ys, w, order)
+    hole = torch.where(out, 0, w.detach())
+    want = ops.expert_combine(ys, hole, good)
+    _soil((N * k, d), dtype=t, dev=dev)
+    dys, dw = torch.autograd.grad(y, (ys, w), dy)
+    assert torch.equal(y, want) and torch.equal(dys, torch.autograd.grad(want, ys, dy)[0])
+    plain = ops.expert_combine(ys, None, order)
+    _soil((N * k, d), dtype=t, dev=dev)
+    one = ops.expert_combine(ys, torch.where(out, 0, torch.ones_like(w)).detach(), good)
+    assert torch.equal(plain, one) and torch.equal(torch.autograd.grad(plain, ys, dy)[0], torch.autograd.grad(one, ys, dy)[0])
+
+
+def test_tokens_of_an_order_are_checked(dev):
+    order = ops.expert_sort(draw_ids(20, 3, 4, 0).to(dev), 4)
+    x = normals((20, 16), 0, torch.float32, dev)
+    for token, error in ((order.token[:-1], ValueError), (order.token.view(20, 3), ValueError), (order.token.long(), TypeError), (order.token.cpu(), RuntimeError)):
+        with pytest.raises(error, match="token|ROCm"):
+            ops.expert_dispatch(x, order._replace(token=token))
+        with pytest.raises(error, match="token|ROCm"):
+            ops.expert_combine(x.repeat(3, 1), None, order._replace(token=token))
