@@ -301,7 +301,8 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
     static at::Tensor forward(AutogradContext *ctx, const at::Tensor &ys, const std::optional<at::Tensor> &weights, const at::Tensor &position, const at::Tensor &offsets,
                               const std::optional<at::Tensor> &token) {
         const at::Tensor w = weights ? *weights : at::Tensor();
-        const bool need_w = w.defined() && ctx->needs_input_grad(1);
+        // (not needs_input_grad: that asks the backward pass that is running, if a forward is run again within one)
+        const bool need_w = w.defined() && w.requires_grad();
         const Order o = order_of(position, offsets, token ? *token : at::Tensor());
         ctx->save_for_backward({need_w ? ys : at::Tensor(), w, position, offsets, o.token});
         keep_order(ctx, o);

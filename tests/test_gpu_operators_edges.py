@@ -1,7 +1,8 @@
 """Calls at the edges of the 4-bit layer, clipping and the expert rows: weights that are zeros, orders with slots taken
-out."""
+out, recomputed forwards."""
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 from dense_util import assert_within, normals
 from mortar_amd import ops
@@ -153,3 +154,25 @@ def test_tokens_of_an_order_are_checked(dev):
             ops.expert_dispatch(x, order._replace(token=token))
         with pytest.raises(error, match="token|ROCm"):
             ops.expert_combine(x.repeat(3, 1), None, order._replace(token=token))
+
+
+@pytest.mark.parametrize("named", [False, True])
+def test_recomputed_forward(dev, named):
+    """The forward run again inside a backward that names its inputs saves what the first one did."""
+    ids = draw_ids(40, 3, 5, 0).to(dev)
+    order = ops.expert_sort(ids, 5)
+    x, dy, scores = (normals(s, i, torch.float32, dev) for i, s in enumerate(((40, 64), (40, 64), (40, 3))))
+    x.requires_grad_(), scores.requires_grad_()
+
+    def block(x, scores):
+        xs = ops.expert_dispatch(x, order)
+        return ops.expert_combine(xs * xs, torch.softmax(scores, dim=1), order)
+
+    want = torch.autograd.grad(block(x, scores), (x, scores), dy)
+    y = checkpoint(block, x, scores, use_reentrant=False)
+    if named:
+        got = torch.autograd.grad(y, (x, scores), dy)
+    else:
+        y.backward(dy)
+        got = x.grad, scores.grad
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
