@@ -45,12 +45,12 @@ struct Span {
     size_t i;
 };
 
-// Nothing that is written is written twice, or read for another tensor.  drop: a gradient that is there twice is counted once (in place).  Tensors mostly
+// Nothing that a launch writes is written twice, or read for another tensor.  drop: a gradient that is there twice is counted once (in place).  Tensors mostly
 // come in the order of their addresses, results and gradients each: two lists that are merged.
-void check_overlap(std::vector<mortar_grad_t> &list, std::vector<Span> read, bool drop, const char *what) {
-    std::vector<Span> written;
+void check_overlap(std::vector<mortar_grad_t> &list, bool drop, const char *what) {
+    std::vector<Span> written, read;
     written.reserve(list.size());
-    read.reserve(read.size() + list.size());
+    read.reserve(list.size());
     const auto size = [](int type) { return type == MORTAR_FP32 ? 4 : 2; };
     for (size_t i = 0; i < list.size(); ++i) {
         const mortar_grad_t &g = list[i];
@@ -74,6 +74,61 @@ void check_overlap(std::vector<mortar_grad_t> &list, std::vector<Span> read, boo
         TORCH_CHECK_VALUE(s.begin >= end_written && (is_read || s.begin >= end_read), what, ": results overlap each other or another gradient");
         if (is_read) end_read = std::max(end_read, s.end);
         else end_written = std::max(end_written, s.end), last = &s;
+    }
+}
+
+// Where a tensor's values lie: runs of `run` bytes at `at` plus any sum of multiples of the strides, the largest one first.
+struct Places {
+    uintptr_t at;
+    int64_t run;
+    std::vector<std::pair<int64_t, int64_t>> dims;           // stride in bytes, size
+    std::vector<int64_t> extent;                             // bytes from dimension d on, all of them in front
+    size_t i;                                                // of the gradient, or of the result that it has
+    bool result, copied;
+    uintptr_t end() const { return at + extent[0]; }
+    bool same(const Places &o) const { return at == o.at && run == o.run && dims == o.dims; }
+};
+
+Places places_of(const at::Tensor &t, size_t i, bool result, bool copied) {
+    Places p{reinterpret_cast<uintptr_t>(t.const_data_ptr()), (int64_t)t.element_size(), {}, {}, i, result, copied};
+    for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1 && t.stride(d)) p.dims.push_back({t.stride(d) * (int64_t)t.element_size(), t.size(d)});
+    std::sort(p.dims.begin(), p.dims.end(), std::greater<>());
+    for (; !p.dims.empty() && p.dims.back().first == p.run; p.dims.pop_back()) p.run *= p.dims.back().second;
+    p.extent.assign(p.dims.size() + 1, p.run);
+    for (size_t d = p.dims.size(); d-- > 0;) p.extent[d] = p.extent[d + 1] + (p.dims[d].second - 1) * p.dims[d].first;
+    return p;
+}
+
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+
+// Whether values of a from dimension da on and of b from db on, which begin `off` bytes behind a's, share a byte: exactly, by the dimension of the largest
+// stride, of which only the steps are tried that bring the rest of both together.
+bool meet(const Places &a, size_t da, const Places &b, size_t db, int64_t off) {
+    if (off >= a.extent[da] || off + b.extent[db] <= 0) return false;
+    const int64_t sa = da < a.dims.size() ? a.dims[da].first : 0, sb = db < b.dims.size() ? b.dims[db].first : 0;
+    if (!sa && !sb) return true;
+    const bool ia = sa >= sb, ib = sb >= sa;                 // which of them steps (both with one stride: what counts is the difference)
+    const int64_t s = std::max(sa, sb), ea = a.extent[da + ia], eb = b.extent[db + ib];
+    const int64_t least = ia ? 1 - a.dims[da].second : 0, most = ib ? b.dims[db].second - 1 : 0;
+    const int64_t from = std::max(least, floor_div(-eb - off, s) + 1), to = std::min(most, floor_div(ea - 1 - off, s));
+    for (int64_t t = from; t <= to; ++t)
+        if (meet(a, da + ia, b, db + ib, off + t * s)) return true;
+    return false;
+}
+
+// The same for results that are copied to where they belong, and for gradients that are copied from where they are, which may be in place all the same.  all: the
+// results and gradients.
+void check_copied(std::vector<Places> all, const char *what) {
+    std::sort(all.begin(), all.end(), [](const Places &a, const Places &b) { return a.at < b.at; });
+    std::vector<const Places *> open;                        // those that reach behind where the next one begins
+    for (const Places &p : all) {
+        open.erase(std::remove_if(open.begin(), open.end(), [&](const Places *o) { return o->end() <= p.at; }), open.end());
+        for (const Places *o : open) {
+            if (!(o->result || p.result) || !(o->copied || p.copied) || (o->i == p.i && o->same(p))) continue;
+            TORCH_CHECK_VALUE(!meet(*o, 0, p, 0, (int64_t)(p.at - o->at)), what, ": results overlap each other or another gradient");
+        }
+        open.push_back(&p);
     }
 }
 
@@ -141,12 +196,14 @@ PyObject *py_grad_clip(PyObject *, PyObject *const *a, Py_ssize_t na) {
         std::vector<at::Tensor> held;                                // copies of gradients that do not fill their memory, and
         std::vector<std::pair<size_t, at::Tensor>> back;             // results that go to where they belong behind the launches
         std::vector<mortar_grad_t> list;
-        std::vector<Span> spans;
+        std::vector<std::pair<size_t, bool>> entry;                  // of the list: which gradient it is, and whether it is one of those copies
         list.reserve(grads.size());
+        entry.reserve(grads.size());
         for (size_t i = 0; i < grads.size(); ++i) {
             const at::Tensor &g = grads[i], &o = out[i];
             at::Tensor s = g, d = o;
-            if (!g.is_non_overlapping_and_dense() || (o.strides() != g.strides() && !(g.is_contiguous() && o.is_contiguous()))) {
+            const bool copied = !g.is_non_overlapping_and_dense() || (o.strides() != g.strides() && !(g.is_contiguous() && o.is_contiguous()));
+            if (copied) {
                 const auto same = [&](const std::pair<size_t, at::Tensor> &b) {
                     const at::Tensor &t = grads[b.first];
                     return t.const_data_ptr() == g.const_data_ptr() && t.sizes() == g.sizes() && t.strides() == g.strides() && t.scalar_type() == g.scalar_type();
@@ -156,14 +213,22 @@ PyObject *py_grad_clip(PyObject *, PyObject *const *a, Py_ssize_t na) {
                 d = at::empty(o.sizes(), o.options().requires_grad(false));
                 held.push_back(s);
                 back.emplace_back(i, d);
-                int64_t last = 0;
-                for (int64_t k = 0; k < o.dim(); ++k) last += (o.size(k) - 1) * o.stride(k);
-                const uintptr_t at = reinterpret_cast<uintptr_t>(o.const_data_ptr());
-                spans.push_back({at, at + (last + 1) * o.element_size(), i});
             }
             list.push_back({data(s), mut(d), g.numel(), type_code(g.scalar_type()), type_code(o.scalar_type())});
+            entry.emplace_back(i, copied);
         }
-        check_overlap(list, std::move(spans), in_place, what);
+        check_overlap(list, in_place, what);
+        if (!back.empty() && !fresh) {
+            std::vector<Places> places;
+            places.reserve(2 * list.size());
+            for (size_t k = 0; k < list.size(); ++k) {
+                if (!list[k].n) continue;
+                const size_t i = entry[k].first;
+                for (const bool result : {true, false}) places.push_back(places_of(result ? out[i] : grads[i], i, result, entry[k].second));
+                if (places.back().same(places[places.size() - 2])) places.pop_back();
+            }
+            check_copied(std::move(places), what);
+        }
         norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
         const at::Tensor ws = empty_bytes(norm, std::max<int64_t>(8, mortar_grad_workspace_bytes(list.data(), (int64_t)list.size())));
         check_rc(mortar_grad_clip(list.data(), (int64_t)list.size(), a[3] == Py_True, max_norm, floats(norm), mut(ws), stream_of(norm)), "mortar_grad_clip");

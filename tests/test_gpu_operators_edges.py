@@ -1,5 +1,7 @@
 """Calls at the edges of the 4-bit layer, clipping and the expert rows: weights that are zeros, orders with slots taken
-out, recomputed forwards."""
+out, recomputed forwards, strided results that share memory."""
+import math
+
 import pytest
 import torch
 from torch.utils.checkpoint import checkpoint
@@ -176,3 +178,60 @@ def test_recomputed_forward(dev, named):
         y.backward(dy)
         got = x.grad, scores.grad
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- clipping
+
+
+def test_strided_results_that_share_memory_are_refused(dev):
+    """Results that do not lie as their gradients do, too, share memory neither with each other nor with another gradient."""
+    f = normals((20, 24), 0, torch.float32, dev)
+    a, b = normals((20, 3), 1, torch.float32, dev), normals((20, 3), 2, torch.float32, dev)
+    r, keep = torch.full((20, 24), 7.0, device=dev), f.clone()
+    square = [normals((8, 8), i, torch.float32, dev) for i in (3, 4)]
+    o = torch.zeros((8, 8), device=dev)
+    for grads, out in (([a, b], [r[:, :3], r[:, :3]]), ([a, b], [r[:, :3], r[:, 2:5]]), ([a, b], [r[:, 1:4], r[:, 0:6:2]]), ([square[0].t(), square[1].t()], [o, o]),
+                       ([square[0].t(), square[1]], [o, o]), ([a, f[:, :3]], [f[:, :3], r[:, :3]]), ([a, f], [f[:, 4:7], r]), ([a, b], [r[:, :3], r.view(-1)[480 - 62:480 - 2].view(20, 3)]),
+                       ([a, b[:10]], [r[:, :3], r[::2, 2:5]]), ([a, b], [r[:, :3], r.as_strided((20, 3), (23, 1))]),
+                       ([f[:, :3], a], [f[:, 1:4], r[:, :3]]), ([f[:, :3], a], [r[:, :3], f.view(-1)[24:84].view(20, 3)]), ([f[:, 0:6:2], a], [r[:, 5:8], f[:, 2:5]])):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.clip_grads(grads, 1.0, out=out)
+    assert bool((r == 7).all()) and torch.equal(f, keep)
+    with pytest.raises(ValueError, match="overlap"):                # in place: columns that two gradients share
+        ops.clip_grads([f[:, :3], f[:, 2:5]], 1.0, out=[f[:, :3], f[:, 2:5]])
+    ps = [torch.nn.Parameter(torch.zeros(20, 3, device=dev)) for _ in range(2)]
+    ps[0].grad, ps[1].grad = f[:, :3], f[:, 2:5]
+    with pytest.raises(ValueError, match="overlap"):
+        ops.clip_grad_norm_(ps, 1.0)
+    assert torch.equal(f, keep)
+
+
+def test_strided_results_side_by_side(dev):
+    """Slices of one matrix that share nothing are taken: columns, every other column, rows and columns of other distances, a row between the columns of another."""
+    a, b = normals((20, 3), 1, torch.float32, dev), normals((20, 3), 2, torch.float32, dev)
+    c = min(1.0, 1.0 / (math.sqrt(float((a.double() ** 2).sum() + (b.double() ** 2).sum())) + 1e-6))
+
+    def check(grads, out, views):
+        r = torch.full((20, 24), 7.0, device=dev)
+        keep = r.clone()
+        o = [v(r) for v in views]
+        ops.clip_grads(grads, 1.0, out=o)
+        for v, g in zip(o, grads):
+            torch.testing.assert_close(v.double(), g.double() * c, rtol=1e-6, atol=0)
+        mask = torch.zeros_like(r)
+        for v in views:
+            v(mask).fill_(1.0)
+        assert torch.equal(torch.where(mask.bool(), keep, r), keep)
+
+    check([a, b], None, [lambda r: r[:, :3], lambda r: r[:, 3:6]])
+    check([a, b], None, [lambda r: r[:, 0:6:2], lambda r: r[:, 1:6:2]])
+    check([a, b], None, [lambda r: r[:, 21:24], lambda r: r.as_strided((20, 3), (24, 8), 4)])
+    check([a, b], None, [lambda r: r.view(40, 12)[0::2, :3], lambda r: r.view(40, 12)[1::2, :3]])
+    one = normals((3,), 3, torch.float32, dev)
+    r = torch.zeros((20, 24), device=dev)
+    got, n = ops.clip_grads([a, one], 1e9, out=[r[:, :3], r[5, 8:11]])
+    assert torch.equal(r[:, :3], a) and torch.equal(r[5, 8:11], one)
+    halves = [r.copy_(normals((20, 24), 4, torch.float32, dev))[:, 0::2], r[:, 1::2]]
+    keep, n = r.clone(), ops.grad_norm([r])
+    ops.clip_grads(halves, 1.0, out=halves)
+    torch.testing.assert_close(r, keep * (1.0 / (n + 1e-6)), rtol=1e-6, atol=0)
