@@ -662,7 +662,8 @@ int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const fl
  *                          c = rne(w / s) + z, 0 at least and 15 at most, quotients in fp32.  What lies behind K gets the code 8.
  *   mortar_int4_linear     y [M, N] = x W^T, x [M, K] and y in bf16 or fp16 (`type`), fp32 sums.  K a multiple of 8, rows of x on 16-byte addresses.
  *                          Sums are formed over x (16 + c) and x, both exact in the matrix cores, and joined per group in fp32: a row of x whose group
- *                          holds an infinity or NaN is NaN in every column.  A group of weights that all are 0 (c = z) adds exactly 0 whatever s is.
+ *                          holds an infinity or NaN is NaN in every column, and one (bf16) where 32 sum |x|, or (16 + z) sum |x|, over a group is
+ *                          beyond fp32 may be NaN or infinite.  A group of weights that all are 0 (c = z) adds exactly 0 whatever s is.
  *   mortar_int4_linear_part  the same for x whose last values, K_used .. K - 1 (fewer than 8), are zeros as mortar_int4_rows writes them: what c holds there is
  *                          not looked at
  *   mortar_int4_rows       out [M, 8 ceil(K / 8)] = rows of 16-bit values x(m, k) at x[m * s_m + k * s_k], zeros behind K: for x that mortar_int4_linear does

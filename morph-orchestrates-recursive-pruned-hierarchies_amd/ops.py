@@ -602,8 +602,9 @@ def quantize_int4_weight(w: Tensor, group_size: int = 128, zero_points: bool = F
 
 def linear_int4(x: Tensor, codes: Tensor, scales: Tensor, zeros: Tensor | None = None, group_size: int = 128) -> Tensor:
     """y = x W^T for a weight of quantize_int4_weight: x [..., K] in bf16 or fp16, result [..., N] in its type; scales in the type of x or fp32 and zeros
-    with any strides.  The codes are multiplied as they are and scaled per group in fp32, W itself is never rounded.  No gradients.  A row of
-    x that holds an infinity is NaN in the result."""
+    with any strides.  The codes are multiplied as they are and scaled per group in fp32, W itself is never rounded.  No gradients.  A group's sums
+    are formed over x times up to 32 (16 + z where that is more): a row of x that holds an infinity is NaN in the result, and one in bf16 with a group whose sum of |x| is 1e37 and
+    more (32 times it no fp32 number) may be NaN or infinite where W x is not."""
     return _lib.native().linear_int4(x, codes, scales, zeros, group_size)
 
 

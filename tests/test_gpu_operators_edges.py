@@ -1,4 +1,4 @@
-"""Calls at the edges of the 4-bit layer, clipping and the expert rows: weights that are zeros, orders with slots taken
+"""Calls at the edges of the 4-bit layer, clipping and the expert rows: weights that are zeros, the end of the range of x, orders with slots taken
 out, recomputed forwards, strided results that share memory."""
 import math
 
@@ -78,6 +78,25 @@ def test_zero_points_beyond_the_codes(dev, M, N, K, group, t):
     x = normals((M, K), M, t, dev)
     ref = x.double() @ int4_weight(pack_codes(q), s, z, group, K).t()
     assert_within(ops.linear_int4(x, pack_codes(q), s, z, group), ref, int4_bound(x, s, z, group, t, ref), "y")
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M,N,K", [(1, 40, 2048), (7, 520, 1999), (40, 264, 1040), (4200, 264, 264), (6000, 517, 136)])
+def test_large_activations(dev, M, N, K, group, zeros):
+    """The end of the documented range: 32 times a group's sum of |x| just below the largest fp32 number."""
+    limit = torch.finfo(torch.float32).max / 32
+    w = normals((N, K), 5, torch.bfloat16, dev, 2.0 ** -6)
+    w[0] = 0
+    c, s, z = ops.quantize_int4_weight(w, group, zeros)
+    x = torch.zeros((M, K), dtype=torch.bfloat16, device=dev)
+    x[0, 3], x[0, K - 1] = 0.995 * limit, -0.995 * limit            # alone in their groups
+    if M > 1:
+        x[1] = 0.99 * limit / group                                  # all of one sign
+    y = ops.linear_int4(x, c, s, z, group)
+    ref = x.double() @ int4_weight(c, s, z, group, K).t()
+    assert bool((y[:, 0] == 0).all())
+    assert_within(y, ref, int4_bound(x, s, z, group, torch.bfloat16, ref), "y")
 
 
 # ---- expert rows
