@@ -714,7 +714,7 @@ int mortar_grad_clip(const mortar_grad_t *grads, int64_t count, int32_t largest,
  *   mortar_expert_dispatch_rows, mortar_expert_combine_bwd_rows  the same with the token of each row: rows that no slot of their token names are zeros as well
  * Positions that are none of the rows 0 .. N k - 1 are empty slots, too.
  * full: device, the number of full rows (offsets + n_experts).  x, ys, xs, y, dy, dys in `type` (bf16, fp16 or fp32) of any width and on any address of the type.
- * N k below 2^26. */
+ * N k at most 2^26 - 4. */
 int64_t mortar_expert_sort_workspace_bytes(int64_t slots, int32_t n_experts);
 int mortar_expert_sort(const void *ids, int32_t ids_64, int64_t N, int32_t k, int32_t n_experts, int32_t *position, int32_t *token, int32_t *offsets,
                        void *workspace, void *stream);

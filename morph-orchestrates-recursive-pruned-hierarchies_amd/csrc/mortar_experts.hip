@@ -17,7 +17,7 @@
 
 namespace {
 
-constexpr int MOST_EXPERTS = 1024, MOST_SLOTS = 1 << 26;        // (a wave per slot: a grid has 2^32 threads at most)
+constexpr int MOST_EXPERTS = 1024, MOST_SLOTS = (1 << 26) - 4;  // (a wave per slot, four per workgroup: a grid has fewer than 2^32 threads)
 
 int launch_error(const char *what) {
     const hipError_t e = hipGetLastError();
@@ -501,7 +501,7 @@ bool known(int32_t type) { return type == MORTAR_BF16 || type == MORTAR_FP16 || 
 
 int check_rows(const char *what, int64_t N, int32_t k, int32_t d, int32_t type) {
     if (N < 0 || k <= 0 || d <= 0 || !known(type)) return mortar_fail(MORTAR_ERR_ARG, "%s: bad shape or type", what);
-    if (d >= 1 << 28 || N >= MOST_SLOTS || N * k >= MOST_SLOTS) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many slots or values", what);
+    if (d >= 1 << 28 || N > MOST_SLOTS || N * k > MOST_SLOTS) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many slots or values", what);
     return MORTAR_OK;
 }
 int check_pointer(const char *what, const char *name, const void *p, int32_t type) {

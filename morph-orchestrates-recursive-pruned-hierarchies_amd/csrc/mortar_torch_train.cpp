@@ -256,7 +256,7 @@ PyObject *py_expert_sort(PyObject *, PyObject *const *a, Py_ssize_t na) {
     TORCH_CHECK_TYPE(ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong, what, ": ids must be int32 or int64, got ", ids.scalar_type());
     TORCH_CHECK_VALUE(ids.dim() == 2 && ids.size(1) > 0, what, ": expected ids [tokens, slots], got ", ids.sizes());
     TORCH_CHECK_VALUE(experts > 0 && experts <= 1024, what, ": 1 to 1024 experts, got ", experts);
-    TORCH_CHECK_VALUE(ids.numel() < (1 << 26), what, ": too many slots");
+    TORCH_CHECK_VALUE(ids.numel() <= (1 << 26) - 4, what, ": too many slots");
     const c10::DeviceGuard guard(ids.device());
     const at::Tensor c = ids.contiguous();
     const auto options = ids.options().dtype(at::kInt);
@@ -289,7 +289,7 @@ Order order_arg(PyObject *p, PyObject *t, PyObject *o, const at::Tensor &x, cons
     same_device(x, offsets, what, "offsets");
     TORCH_CHECK_TYPE(position.scalar_type() == at::kInt && offsets.scalar_type() == at::kInt, what, ": position and offsets must be int32");
     TORCH_CHECK_VALUE(position.dim() == 2 && position.size(1) > 0 && offsets.dim() == 1 && offsets.size(0) > 1, what, ": expected position [tokens, slots] and offsets [experts + 1]");
-    TORCH_CHECK_VALUE(position.numel() < (1 << 26), what, ": too many slots");
+    TORCH_CHECK_VALUE(position.numel() <= (1 << 26) - 4, what, ": too many slots");
     if (token.defined()) {
         same_device(x, token, what, "token");
         TORCH_CHECK_TYPE(token.scalar_type() == at::kInt, what, ": token must be int32");
