@@ -672,7 +672,7 @@ int mortar_fp8_linear(const void *x, int64_t M, int32_t K, int64_t ldx, const fl
 int mortar_int4_rows(const void *x, int64_t M, int32_t K, int64_t s_m, int64_t s_k, void *out, void *stream);
 int mortar_int4_quantize(const void *w, int32_t N, int32_t K, int64_t ldw, int32_t type, int32_t group, uint32_t *c, int64_t ldc, void *s, int32_t s_type,
                          int64_t s_n, int64_t s_g, uint8_t *z, int64_t z_n, int64_t z_g, void *stream);
-/* Form that a product takes (host only, nothing is launched): *tile_n x *tile_m of y per workgroup of *waves; 16 or 32 rows of x: the kernels of few rows,
+/* Form that a product takes (of rows of x without gaps; host only, nothing is launched): *tile_n x *tile_m of y per workgroup of *waves; 16 or 32 rows of x: the kernels of few rows,
  * negative: those that take x through LDS; *ranges that K is cut into. */
 int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t group, int32_t *tile_n, int32_t *tile_m, int32_t *waves, int32_t *ranges);
 int mortar_int4_linear_part(const void *x, int64_t M, int32_t K, int32_t K_used, int64_t ldx, int32_t type, const uint32_t *c, int64_t ldc, int32_t N, int32_t group,

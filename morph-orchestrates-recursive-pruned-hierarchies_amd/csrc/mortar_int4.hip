@@ -641,20 +641,21 @@ struct Int4Tile {
 constexpr Int4Tile INT4_TILES[] = {{128, 128, {0.60, 0.78, 1.09}, {0.53, 0.58, 0.80}}, {64, 64, {0.335, 0.335, 0.43}, {0.19, 0.215, 0.285}}};
 constexpr int MOST_FEW_ROWS = 4096, MOST_LDS = 160 * 1024;
 
-Int4Plan plan(int64_t M, int64_t N, int64_t K, int group) {
+// ldx: bytes between rows of x.
+Int4Plan plan(int64_t M, int64_t N, int64_t K, int group, int64_t ldx) {
     const int64_t chunks = (K + 127) / 128, steps = (K + 63) / 64, n16 = (N + 15) / 16, m16 = (M + 15) / 16;
     Int4Plan p{1, 8, 0, 1, false};
     if (M <= 16) {
-        // x through LDS: rows a multiple of 1 KB apart meet in the same channels when a fragment loads 16 of them at once (8 rows of 5632 -> 2048 7.2 -> 6.5 us, 5 of
-        // 11264 -> 2048 11.7 -> 8.2, long rows at the price of one workgroup per CU).  Others are better read as operands from 3 rows on (7 of 4104 -> 1500 5.4 ->
-        // 4.75), with groups of 128, whose words need no exchange there, from 6 on (4 of 5640 -> 2048 5.5, as operands 6.2), short ones all from 9 rows on (9 of
-        // 2048 -> 4096 4.6 -> 4.3).
-        const bool apart = K % 512 == 0;
+        // x through LDS: rows a multiple of 1 KB apart meet in the same channels when a fragment loads 16 of them at once (8 rows of 5632 -> 2048 7.2 -> 6.1 us, 8 of 5640
+        // in rows of 8192 6.6 -> 6.2, 5 of 11264 -> 2048 11.7 -> 8.2, long rows at the price of one workgroup per CU).  Others are better read as operands from 3 rows on
+        // (13 of 5632 in rows of 5640 7.1 -> 6.6), with groups of 128, whose words need no exchange there, from 6 on (5 of 5640 -> 2048 5.7, as operands 6.0), and of
+        // 9 rows and more all where 8 waves do (13 of 2048 -> 2048 4.8 -> 4.7, but 13 of 2560 5.3 as operands, 4.9 through LDS).
+        const bool apart = ldx % 1024 == 0;
         const int64_t bytes = M * int4_pitch((int)K);
         p.f = n16 >= 512 && chunks >= 32 ? 2 : 1;
         p.waves = chunks > 16 ? 16 : 8;
         p.xl = M <= 8 && (M <= (group == 128 ? 5 : 2) || apart) && bytes <= 64 * 1024;
-        if (apart && chunks > 24 && (n16 + p.f - 1) / p.f <= 256) p.xl |= bytes <= MOST_LDS - p.waves * p.f * 1024;
+        if (apart && chunks > 16 && (n16 + p.f - 1) / p.f <= 256) p.xl |= bytes <= MOST_LDS - p.waves * p.f * 1024;
         if (p.xl) return p;
     }
     p.f = 4;
@@ -743,7 +744,7 @@ int launch_many(Int4Args a, const Int4Plan &p, float *ws, hipStream_t st, const 
 
 template <DenseType T, int G, int S>
 int launch_zeros(const Int4Args &a, float *ws, hipStream_t st, const char *what) {
-    const Int4Plan p = plan(a.M, a.N, a.K, G);
+    const Int4Plan p = plan(a.M, a.N, a.K, G, a.ldx);
     if (p.f) return a.z ? launch_few<T, G, S, true>(a, p, st, what) : launch_few<T, G, S, false>(a, p, st, what);
     return a.z ? launch_many<T, G, S, true>(a, p, ws, st, what) : launch_many<T, G, S, false>(a, p, ws, st, what);
 }
@@ -806,7 +807,7 @@ extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t gr
     const char *what = "int4_form";
     CHECK(check_group(what, group));
     if (M <= 0 || N <= 0 || K <= 0 || !tile_n || !tile_m || !waves || !ranges) return mortar_fail(MORTAR_ERR_ARG, "%s: bad argument", what);
-    const Int4Plan p = plan(M, N, K, group);
+    const Int4Plan p = plan(M, N, K, group, 2 * K);
     *tile_n = p.f ? 16 * p.f : INT4_TILES[p.tile].bn;
     *tile_m = p.f ? 16 * p.mx : INT4_TILES[p.tile].bm;
     *waves = p.xl ? -p.waves : p.f ? p.waves : 4;
@@ -816,7 +817,7 @@ extern "C" int mortar_int4_form_host(int64_t M, int64_t N, int64_t K, int32_t gr
 
 extern "C" int64_t mortar_int4_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t group) {
     if (M <= 0 || N <= 0 || K <= 0 || group < 32) return 0;
-    const Int4Plan p = plan(M, N, K, group);
+    const Int4Plan p = plan(M, N, K, group, 2 * K);              // (the rows' distance chooses among forms of few rows only)
     if (p.f) return 0;
     return 4 * (groups_padded(K, group) * (up128(M) + 2 * up128(N)) + (p.splits > 1 ? p.splits * M * up128(N) : 0));
 }

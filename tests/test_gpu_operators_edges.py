@@ -99,6 +99,19 @@ def test_large_activations(dev, M, N, K, group, zeros):
     assert_within(y, ref, int4_bound(x, s, z, group, torch.bfloat16, ref), "y")
 
 
+@pytest.mark.parametrize("group", [64, 128])
+@pytest.mark.parametrize("K,wide", [(5640, 8192), (5632, 5640), (2560, 4096), (2048, 2056), (1040, 1536)])
+@pytest.mark.parametrize("M", [2, 5, 8, 13, 16])
+def test_rows_of_x_apart(dev, M, K, wide, group):
+    """Few rows of a wider buffer: the rows' distance chooses how x is read, and nothing else."""
+    buffer = torch.full((M, wide), float("nan"), dtype=torch.bfloat16, device=dev)
+    x = buffer[:, :K].copy_(normals((M, K), M, torch.bfloat16, dev))
+    c, s, _ = ops.quantize_int4_weight(normals((136, K), K, torch.bfloat16, dev, K ** -0.5), group)
+    ref = x.double() @ int4_weight(c, s, None, group, K).t()
+    for v in (x, x.contiguous()):
+        assert_within(ops.linear_int4(v, c, s, group_size=group), ref, int4_bound(x, s, None, group, torch.bfloat16, ref), "y")
+
+
 # ---- expert rows
 
 
