@@ -9,7 +9,7 @@
 //              weights are 24 + (c - z) / 2: half a code, added to the bits of the row's 24 - z / 2 instead of set in those of 16.  Zero points beyond 15,
 //              which no code reaches, count as 15, and (z - 15) / 2 sums of x are taken off besides.
 //   many rows  a subtraction more per result and group takes 3 to 15 % longer, looking at the codes beside the products 3 to 17 %: the launch in front reads
-//              them instead (1.8 us for 23 million weights) and gives groups of zeros the scale 0.
+//              them instead (1 to 2 us for 23 million weights) and gives groups of zeros the scale 0.
 // The codes of a word lie so that one shift brings a pair of neighbours into its two halves.
 #include <hip/hip_runtime.h>
 
@@ -260,11 +260,11 @@ __device__ __forceinline__ bool int4_all_zero(const Int4Args &a, int64_t n, int 
 // N and the last group.  The scale is times 0 where all codes are the zero point.  A wave takes 16 rows of W and 64 units of 32 K, one per lane, of whose codes it reads whole
 // rows, all 16 at once; only where a group's codes are all the same they are compared with its zero point.
 template <DenseType T, int S, int G, bool Z>
-__global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int groups, float *xs, float *st, float *zt, unsigned x_blocks) {
+__global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int groups, float *xs, float *st, float *zt, unsigned n_blocks) {
     constexpr int group = G;
-    if (blockIdx.x < x_blocks) {                                 // 8 values per thread, the lanes of a group side by side
+    if (blockIdx.x >= n_blocks) {                                // sums of x, behind the codes, which take longer: 8 values per thread, the lanes of a group side by side
         const int per = group / 8;
-        const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) / per, m = i / groups;
+        const int64_t i = ((int64_t)(blockIdx.x - n_blocks) * 256 + threadIdx.x) / per, m = i / groups;
         const int g = (int)(i - m * groups), lane = threadIdx.x & (per - 1), k = g * group + lane * 8;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (m < a.M && k < a.K) dense_unpack8<T>(*reinterpret_cast<const u32x4_t *>(static_cast<const char *>(a.x) + m * a.ldx + (int64_t)k * 2), v);
@@ -279,7 +279,7 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
     }
     constexpr int PER = G / 32, GROUPS = 64 / PER, TURNS = GROUPS / 4;       // units of a group, groups of the wave; four of them are stored at a time, for 16 rows
     const int lane = threadIdx.x & 63, chunks = (groups + GROUPS - 1) / GROUPS, units = (a.K + 31) >> 5;
-    const int64_t task = (int64_t)(blockIdx.x - x_blocks) * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), block = task / chunks, n = block * 16 + (lane & 15);
+    const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), block = task / chunks, n = block * 16 + (lane & 15);
     if (block * 16 >= a.Np) return;
     const int g0 = (int)(task - block * chunks) * GROUPS, u = g0 * PER + lane, left = a.K_used - u * 32;
     const char *c = reinterpret_cast<const char *>(a.c) + (int64_t)min(u, units - 1) * 16;
@@ -734,7 +734,7 @@ int launch_many(Int4Args a, const Int4Plan &p, float *ws, hipStream_t st, const 
     a.slabs = s + 2 * groups * a.Np;
     const int64_t x_blocks = (groups * a.Mp * (G / 8) + 255) / 256, n_blocks = (a.Np / 16 * ((groups * (G / 32) + 63) / 64) + 3) / 4;       // (a wave each: 16 rows, 64 units)
     if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
-    hipLaunchKernelGGL((int4_prepare_kernel<T, S, G, Z>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, (int)groups, xs, s, zt, (unsigned)x_blocks);
+    hipLaunchKernelGGL((int4_prepare_kernel<T, S, G, Z>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, (int)groups, xs, s, zt, (unsigned)n_blocks);
     if (const int rc = launch_error(what)) return rc;
     const int rc = p.tile == 0 ? launch_tile_form<T, G, Z, 128, 128, 4, 1, 2, 1>(a, st, what) : launch_tile_form<T, G, Z, 64, 64, 2, 2, 2, 2>(a, st, what);
     if (rc || p.splits == 1) return rc;
