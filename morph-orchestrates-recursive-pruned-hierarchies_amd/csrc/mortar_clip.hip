@@ -8,7 +8,7 @@
 // are cut into chunks of 16 KB that no two tensors share, a workgroup takes every n-th chunk and leaves one partial sum in a slot of its own; the
 // slots are added in a fixed order, so that a call gives the same bits every time.  Neighbouring workgroups take neighbouring chunks (a run of chunks for each
 // instead: 51 -> 55 us for 86 MB).
-// Measured, norm and product: 86 MB of gradients 15 + 25 us (the norm 5.7 TB/s, the product 6.9 of which the caches hold a part), 400 MB 194 (6.2 TB/s),
+// Measured, norm and product: 86 MB of gradients 14 + 28 us (6.1 TB/s, the product's reads partly from the caches), 400 MB 194 (6.2 TB/s),
 // 2.4 MB two launches of 4; 500 tensors of 10 MB in all 8 launches of 4, which the host takes 90 us to prepare.
 #include <hip/hip_runtime.h>
 

@@ -29,7 +29,7 @@ int launch_error(const char *what) {
 // experts in front, the runs in front) and places its slots.  A wave owns 64 HELD consecutive slots and keeps their experts in registers; the counts of a
 // run are kept per wave, so that the order within a run needs nothing of other waves but their counts, and within 64 slots it is found with one
 // ballot per bit of the expert's number.  Few slots are one workgroup's, in one launch.  Both launches are chains of latencies: ids, counts, sums.
-// Measured: up to 4096 slots 2.6 us, 32768 slots of 64 experts 2.9 + 4.4.
+// Measured: up to 4096 slots 2.7 us, 32768 slots of 64 experts 4.7 + 4.7 behind other work, 3.2 + 5.2 of 16.
 constexpr int SORT_WAVES = 16, SORT_THREADS = SORT_WAVES * 64, SORT_ALONE = 4096, SORT_BLOCKS = 64;
 
 template <typename ID>
@@ -307,7 +307,8 @@ __device__ __forceinline__ void clear_row(const RowArgs &a, uint32_t i, int lane
 }
 
 // A wave per slot; the rows of a token are read by neighbouring waves and come out of the caches but once.  Bound by the rows written: 4096 tokens, 8 slots
-// of 2048 bf16 values 26 us (134 MB, 5.7 TB/s with the reads), 16384 tokens, 2 of 768 13 (5.8); rows of 1999 values, on odd addresses, take 1.3 to 1.6 times as long.
+// of 2048 bf16 values 28 to 29 us (151 MB with the reads, 5.3 TB/s), 16384 tokens, 2 of 768 15 (75 MB, 5.0; 20 between the launches of a backward pass); rows of 1999
+// values, on odd addresses, take 1.7 times as long (50 us), small launches of them more (5105 of them 9.1, 2.7 TB/s).
 template <int SIZE, bool STREAM>
 __global__ __launch_bounds__(256) void expert_dispatch_kernel(const RowArgs a) {
     const int lane = threadIdx.x & 63;
@@ -341,7 +342,8 @@ __global__ __launch_bounds__(256) void expert_dispatch_kernel(const RowArgs a) {
 
 // A wave per TOKENS consecutive tokens and 64 units of their rows, the rows of eight slots on their way at a time: with few slots per token one token alone
 // leaves too little on the way (two slots of 768 values: 16384 tokens in 20 us, 14 with four tokens).  The wave's lanes hold the positions and weights of its slots.
-// Bound by the rows read: 4096 tokens, 8 slots of 2048 bf16 values 29 us (151 MB, 5.2 TB/s).
+// Bound by the rows read: 4096 tokens, 8 slots of 2048 bf16 values 34 us (151 MB, 4.5 TB/s), of 1999 45, without weights (the gradient of the dispatch) behind other
+// work 46 and 64.
 constexpr int NO_WEIGHT = 3;
 template <int TYPE, int WTYPE, int TOKENS>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const RowArgs a, int parts) {
@@ -437,7 +439,7 @@ int launch_combine_weights(const RowArgs &a, hipStream_t st, const char *what) {
     return a.w_type == MORTAR_FP32 ? launch_combine<TYPE, MORTAR_FP32>(a, st, what) : a.w_type == MORTAR_FP16 ? launch_combine<TYPE, MORTAR_FP16>(a, st, what) : launch_combine<TYPE, MORTAR_BF16>(a, st, what);
 }
 
-// A wave per slot: its row of dys, and the dot product over the row.  Bound by both: 4096 tokens, 8 slots of 2048 bf16 values 51 us (285 MB, 5.6 TB/s).
+// A wave per slot: its row of dys, and the dot product over the row.  Bound by both: 4096 tokens, 8 slots of 2048 bf16 values 54 us (285 MB, 5.3 TB/s), of 1999 66.
 template <int TYPE, bool STREAM>
 __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a) {
     using R = Row<TYPE>;
@@ -490,7 +492,8 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(const RowArgs a
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Rows by slot that the memory-side cache (256 MB) cannot hold for whoever reads them next are stored past it: 268 MB of fp32 dispatched in 63 -> 51 us.
+// Rows by slot that the memory-side cache (256 MB) cannot hold for whoever reads them next are stored past it: 268 MB of fp32 dispatched in 63 -> 51 us (54 with the look at the
+// rows' slots).
 // Smaller ones gain little (134 MB 26.4 -> 25.7) and are read from there; rows on odd addresses lose (35 -> 43).
 bool past_caches(const RowArgs &a, int32_t type) {
     const int64_t row = (int64_t)a.d * (type == MORTAR_FP32 ? 4 : 2);

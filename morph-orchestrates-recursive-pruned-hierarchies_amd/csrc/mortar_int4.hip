@@ -96,8 +96,8 @@ __device__ __forceinline__ void int4_share(V v, V (&all)[GPC]) {
 
 // ---- few rows --------------------------------------------------------------------------------------------------------
 // 16 F rows of W and 16 MX of x per workgroup, chunks of 128 K dealt to its waves, a lane's 16 bytes of codes straight into registers: their traffic is what
-// bounds these calls, from about 20 MB on: one row of 8192 -> 8192 8.5 us (34 MB, 4.0 TB/s; the library's bf16 product 21.6), of 2048 -> 11264 4.7 (12 MB;
-// 10.2), the rest of which is the launch and one load behind the other.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
+// bounds these calls, from about 20 MB on: one row of 8192 -> 8192 8.7 us (34 MB, 3.9 TB/s; the library's bf16 product 22.1), of 2048 -> 11264 4.8 (12 MB;
+// 10.6), the rest of which is the launch and one load behind the other.  The matrix cores take x as rows and W as columns, so that a lane's results belong to one row of W: one scale per
 // lane and group.  What is taken off comes from one more product, with 24.
 // Groups of 128 with x in LDS: lane (n, q) multiplies the words it loaded, K 32 q + 8 t + {0..7} in product t.  Smaller groups must not meet in a product, and x from memory
 // comes in whole pieces of 64 bytes: the four lanes of a row exchange their words first, so that product t is K 32 t + 8 q + {0..7} (48 rows of 5640 -> 2048 9.1 -> 8.5 us).
@@ -326,8 +326,8 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
 // with their units permuted, codes in rows of 32 bytes, and each step's groups: scales, sums of x, 16 + z.  One barrier per turn.  A wave makes its
 // weights from the codes in registers.  The first product of a group starts at -(16 + z) sum x instead of 0.
 // What bounds it is the instructions that a wave issues beside the products: 128 x 128 with 32 x 128 per wave has 3 per product (4096 rows of 2048 -> 11264
-// in 189 us, 64 x 64 per wave 194, eight waves of 32 x 64 201; the library's bf16 product 183), and the power that the chip may draw: the same on zeros takes
-// 164.  A third turn in the ring costs more than it hides (197), and so do 32 x 32 products (204), operands read a half step ahead of them (196) and
+// in 176 to 195 us with the launch in front; where it took 189, 64 x 64 per wave took 194, eight waves of 32 x 64 201; the library's bf16 product 149 to 160;
+// groups of 64 212 to 218, of 32 248 to 263, with zero points 192, 230 and 292 at least), and the power that the chip may draw: the same on zeros takes 164 of 189.  A third turn in the ring costs more than it hides (197), and so do 32 x 32 products (204), operands read a half step ahead of them (196) and
 // copies issued behind the reads.
 // The ranges of a product over several of them leave fp32 sums.
 template <DenseType T, int G, bool Z, int BN, int BM, int WN, int WM, int NS, int SPS>
@@ -524,8 +524,8 @@ __global__ __launch_bounds__(WN *WM * 64, 2) void int4_tile_kernel(const Int4Arg
     }
 }
 
-// The slabs of the K ranges added in their order: 2.5 us and their reading, which plan() weighs against rounds of idle CUs (1738 rows of 5728 -> 869: 67 us in
-// one range, 52 in several).
+// The slabs of the K ranges added in their order: 2.5 us and their reading, which plan() weighs against rounds of idle CUs (1738 rows of 5728 -> 869: 75 us in
+// one range, 51 in several).
 template <DenseType T>
 __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = (a.N + 3) >> 2;
@@ -545,7 +545,7 @@ __global__ __launch_bounds__(256) void int4_join_kernel(const Int4Args a) {
 }
 
 // Rows of x with any strides, on any address and of any length as rows of whole 16-byte units, zeros behind K: bound by the memory, a launch in front of the
-// product (680 rows of 410 -> 749 9.7 us with both, with torch's padding 16).
+// product (680 rows of 410 -> 749 9.0 us with both, with torch's padding 16).
 __global__ __launch_bounds__(256) void int4_rows_kernel(const uint16_t *x, int64_t M, int32_t K, int64_t s_m, int64_t s_k, uint16_t *o) {
     const int units = (K + 7) >> 3;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / units;
@@ -565,7 +565,8 @@ __device__ __forceinline__ float int4_read(const void *p, int64_t i) {
     else if constexpr (TYPE == MORTAR_FP16) return (float)static_cast<const _Float16 *>(p)[i];
     else return bf16_to_f32(static_cast<const uint16_t *>(p)[i]);
 }
-// 8 values per thread, the lanes of a group side by side (16 of them at most: within a row of lanes).  One pass, once per weight: bound by its reading.
+// 8 values per thread, the lanes of a group side by side (16 of them at most: within a row of lanes).  One pass, once per weight, bound by
+// its loads of one value each: 23 million bf16 weights 39 us (1.5 TB/s), with zero points 41, in fp32 43.
 template <int TYPE, int STYPE>
 __global__ __launch_bounds__(256) void int4_quantize_kernel(const void *w, int32_t N, int32_t K, int64_t ldw, int group, uint32_t *c, int64_t ldc, void *s, int64_t s_n,
                                                             int64_t s_g, uint8_t *z, int64_t z_n, int64_t z_g) {
@@ -622,12 +623,12 @@ int launch_error(const char *what) {
 
 int64_t up128(int64_t v) { return (v + 127) / 128 * 128; }
 
-// Which kernel: the smallest estimate, in us, from products of 9 to 4096 rows with 16 weights of 300 to 16384 rows and 512 to 8192 columns in every form (what is
-// chosen takes 1.7 % longer than the best one on average, over these and five others).
-// Few rows: workgroups of 16 x 16 F results, one round of the chip if F = 4 still gives one, with the smallest such F (16 rows of 2048 -> 11264 7.6 with F = 4 and 10.1 in
-// two rounds with 2; 64 of 5632 -> 2048 10.9 with 2, 13.3 with 4 on half of the CUs; 77 of them 13.4 with 4, 17.2 in two rounds with 2), and 16 waves instead of 8 if there
-// is work for them.  Where that takes several rounds, 32 rows of x share what is unpacked of W (32 rows of 2048 -> 11264 11.1 -> 9.4, 17 of 5120 -> 12288 20.1 -> 15.2,
-// 256 of 5632 -> 2048 24.1 -> 19.1).  Tiles are bound by the instructions of a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second
+// Which kernel: the smallest estimate, in us, from products of 9 to 4096 rows with 16 weights of 300 to 16384 rows and 512 to 8192 columns in every form (of 1334 random
+// products of 1 to 4096 rows what is chosen takes 2.6 % longer than the best form, of which timing itself makes about 1).
+// Few rows: workgroups of 16 x 16 F results, one round of the chip if F = 4 still gives one, with the smallest such F (16 rows of 2048 -> 11264 7.8 with F = 4 and 9.1 in
+// two rounds with 2; 64 of 5632 -> 2048 11.0 with 2, 13.3 with 4 on half of the CUs; 77 of them 13.5 with 4, 17.4 in two rounds with 2), and 16 waves instead of 8 if there
+// is work for them.  Where that takes several rounds, 32 rows of x share what is unpacked of W (32 rows of 2048 -> 11264 11.1 -> 9.5, 17 of 5120 -> 12288 20.3 -> 16.1,
+// 256 of 5632 -> 2048 24.3 -> 18.9).  Tiles are bound by the instructions of a step, which one workgroup of a CU alone cannot issue behind each other's latencies, and need a second
 // launch for the sums of x; 32 x 128 per wave pays for the sums of smaller groups, the small tile less so.
 struct Int4Plan {
     int f, waves, tile, splits;  // few rows: f > 0; else index into INT4_TILES and ranges of K
@@ -647,7 +648,7 @@ Int4Plan plan(int64_t M, int64_t N, int64_t K, int group, int64_t ldx) {
     Int4Plan p{1, 8, 0, 1, false};
     if (M <= 16) {
         // x through LDS: rows a multiple of 1 KB apart meet in the same channels when a fragment loads 16 of them at once (8 rows of 5632 -> 2048 7.2 -> 6.1 us, 8 of 5640
-        // in rows of 8192 6.6 -> 6.2, 5 of 11264 -> 2048 11.7 -> 8.2, long rows at the price of one workgroup per CU).  Others are better read as operands from 3 rows on
+        // in rows of 8192 6.6 -> 6.2, 5 of 11264 -> 2048 10.1 -> 8.5, long rows at the price of one workgroup per CU).  Others are better read as operands from 3 rows on
         // (13 of 5632 in rows of 5640 7.1 -> 6.6), with groups of 128, whose words need no exchange there, from 6 on (5 of 5640 -> 2048 5.7, as operands 6.0), and of
         // 9 rows and more all where 8 waves do (13 of 2048 -> 2048 4.8 -> 4.7, but 13 of 2560 5.3 as operands, 4.9 through LDS).
         const bool apart = ldx % 1024 == 0;
