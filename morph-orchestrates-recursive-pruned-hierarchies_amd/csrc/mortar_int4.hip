@@ -256,6 +256,7 @@ __device__ __forceinline__ bool int4_all_zero(const Int4Args &a, int64_t n, int 
     return !other;
 }
 
+constexpr int INT4_ROWS = 16;                                    // of W that a wave looks through (4: 8192 -> 8192 in groups of 32 85 -> 101 us)
 // What a tile needs of the groups, laid out so that its pieces are whole 16-byte units: sums of x times -1 or, without zero points, -24 [groups][Mp], scales and 16 + z [groups][Np], zeros beyond M,
 // N and the last group.  The scale is times 0 where all codes are the zero point.  A wave takes 16 rows of W and 64 units of 32 K, one per lane, of whose codes it reads whole
 // rows, all 16 at once; only where a group's codes are all the same they are compared with its zero point.
@@ -277,27 +278,27 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
         if (lane == 0 && m < a.Mp) xs[(int64_t)g * a.Mp + m] = Z ? -sum : -24.0f * sum;
         return;
     }
-    constexpr int PER = G / 32, GROUPS = 64 / PER, TURNS = GROUPS / 4;       // units of a group, groups of the wave; four of them are stored at a time, for 16 rows
+    constexpr int PER = G / 32, GROUPS = 64 / PER, ROWS = INT4_ROWS, SIDE = 64 / ROWS, TURNS = GROUPS / SIDE;   // units of a group, groups of the wave, SIDE at a time
     const int lane = threadIdx.x & 63, chunks = (groups + GROUPS - 1) / GROUPS, units = (a.K + 31) >> 5;
-    const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), block = task / chunks, n = block * 16 + (lane & 15);
-    if (block * 16 >= a.Np) return;
+    const int64_t task = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), block = task / chunks, n = block * ROWS + lane % ROWS;
+    if (block * ROWS >= a.Np) return;
     const int g0 = (int)(task - block * chunks) * GROUPS, u = g0 * PER + lane, left = a.K_used - u * 32;
     const char *c = reinterpret_cast<const char *>(a.c) + (int64_t)min(u, units - 1) * 16;
-    u32x4_t w[16];
+    u32x4_t w[ROWS];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = *reinterpret_cast<const u32x4_t *>(c + min(block * 16 + i, (int64_t)a.N - 1) * a.ldc);
+    for (int i = 0; i < ROWS; ++i) w[i] = *reinterpret_cast<const u32x4_t *>(c + min(block * ROWS + i, (int64_t)a.N - 1) * a.ldc);
+    const int64_t row = min(n, (int64_t)a.N - 1);
     float s[TURNS];
     uint32_t z[TURNS];
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-        const int64_t row = min(n, (int64_t)a.N - 1), g = min(g0 + i * 4 + (lane >> 4), a.groups - 1);
+        const int64_t g = min(g0 + i * SIDE + lane / ROWS, a.groups - 1);
         s[i] = int4_scale<T, S>(a.s, row * a.s_n + g * a.s_g);
-        z[i] = 8;
         if constexpr (Z) z[i] = a.z[row * a.z_n + g * a.z_g];
     }
     uint32_t same = 0;                                           // bit i: the lane's group has one code throughout in row i
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < ROWS; ++i) {
         const uint32_t first = (w[i][0] & 15) * 0x11111111u;
         uint32_t other = 0;
         if (left >= 32) {
@@ -311,13 +312,20 @@ __global__ __launch_bounds__(256) void int4_prepare_kernel(const Int4Args a, int
     }
 #pragma unroll
     for (int d = 1; d < PER; d <<= 1) same &= __shfl_xor(same, d);
+    uint32_t zeros = 0;                                          // bit i: of turn i
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) zeros |= (__shfl(same, (i * SIDE + lane / ROWS) * PER) >> lane % ROWS & 1) << i;
+    if (zeros)
+        for (int i = 0; i < TURNS; ++i) {
+            const int g = min(g0 + i * SIDE + lane / ROWS, a.groups - 1);
+            if ((zeros >> i & 1) && !int4_all_zero(a, row, g, G, Z ? a.z[row * a.z_n + g * a.z_g] : 8)) zeros &= ~(1u << i);
+        }
 #pragma unroll
     for (int i = 0; i < TURNS; ++i) {
-        const int at = i * 4 + (lane >> 4), g = g0 + at;
+        const int g = g0 + i * SIDE + lane / ROWS;
         const bool on = g < a.groups && n < a.N;
-        if ((__shfl(same, at * PER) >> (lane & 15) & 1) && on && int4_all_zero(a, n, g, G, z[i])) s[i] *= 0.f;       // (NaN stays)
         if (g >= groups) continue;
-        st[(int64_t)g * a.Np + n] = on ? s[i] : 0.f;
+        st[(int64_t)g * a.Np + n] = on ? (zeros >> i & 1 ? s[i] * 0.f : s[i]) : 0.f;          // (NaN stays)
         if constexpr (Z) zt[(int64_t)g * a.Np + n] = on ? 16.0f + (float)z[i] : 0.f;
     }
 }
@@ -733,7 +741,7 @@ int launch_many(Int4Args a, const Int4Plan &p, float *ws, hipStream_t st, const 
     a.xs = xs; a.st = s; a.zt = zt;
     a.splits = p.splits;
     a.slabs = s + 2 * groups * a.Np;
-    const int64_t x_blocks = (groups * a.Mp * (G / 8) + 255) / 256, n_blocks = (a.Np / 16 * ((groups * (G / 32) + 63) / 64) + 3) / 4;       // (a wave each: 16 rows, 64 units)
+    const int64_t x_blocks = (groups * a.Mp * (G / 8) + 255) / 256, n_blocks = (a.Np / INT4_ROWS * ((groups * (G / 32) + 63) / 64) + 3) / 4;     // (a wave each: rows, 64 units)
     if (x_blocks + n_blocks >= 1 << 24) return mortar_fail(MORTAR_ERR_LIMIT, "%s: too many values", what);
     hipLaunchKernelGGL((int4_prepare_kernel<T, S, G, Z>), dim3((unsigned)(x_blocks + n_blocks)), dim3(256), 0, st, a, (int)groups, xs, s, zt, (unsigned)n_blocks);
     if (const int rc = launch_error(what)) return rc;

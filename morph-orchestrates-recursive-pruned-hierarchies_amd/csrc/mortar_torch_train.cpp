@@ -2,6 +2,7 @@
 // the autograd nodes.  As in mortar_torch_dense.cpp one Python call each, and what they do not take they refuse.
 #include "mortar_torch_args.h"
 
+#include <array>
 #include <vector>
 
 #include <ATen/MemoryOverlap.h>
@@ -332,24 +333,19 @@ at::Tensor combine(const at::Tensor &ys, const at::Tensor &w, const Order &o) {
     return y;
 }
 
-// What a node keeps of an order, behind `first` saved tensors: positions, offsets, tokens.
-void keep_order(AutogradContext *ctx, const Order &o) {
-    ctx->saved_data["offsets"] = o.offsets.size(0);
-    ctx->saved_data["shape"] = o.position.sizes();
-    ctx->saved_data["tokens"] = o.token.defined();
-}
-Order kept_order(AutogradContext *ctx, const variable_list &v, size_t first, const at::Tensor &g, const char *what) {
-    const auto shape = ctx->saved_data["shape"].toIntVector();
-    return order_of(kept(v[first], g, shape, at::kInt, what), kept(v[first + 1], g, {ctx->saved_data["offsets"].toInt()}, at::kInt, what),
-                    ctx->saved_data["tokens"].toBool() ? kept(v[first + 2], g, {shape[0] * shape[1]}, at::kInt, what) : at::Tensor());
+// What a node keeps of an order besides the saved tensors: tokens, slots, length of the offsets, whether there are tokens.
+void keep_order(AutogradContext *ctx, const Order &o, bool tokens) { ctx->saved_data["order"] = std::vector<int64_t>{o.N, o.k, o.offsets.size(0), tokens}; }
+// The order in a backward pass: positions, offsets and tokens from the saved tensor `first` on.
+Order kept_order(const std::vector<int64_t> &n, const variable_list &v, size_t first, const at::Tensor &g, const char *what) {
+    return order_of(kept(v[first], g, {n[0], n[1]}, at::kInt, what), kept(v[first + 1], g, {n[2]}, at::kInt, what),
+                    n[3] ? kept(v[first + 2], g, {n[0] * n[1]}, at::kInt, what) : at::Tensor());
 }
 
 struct DispatchFn : public torch::autograd::Function<DispatchFn> {
     static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &position, const at::Tensor &offsets, const std::optional<at::Tensor> &token) {
         const Order o = order_of(position, offsets, token ? *token : at::Tensor());
         ctx->save_for_backward({position, offsets});
-        keep_order(ctx, o);
-        ctx->saved_data["tokens"] = false;               // (rows by slot are read only)
+        keep_order(ctx, o, false);                       // (rows by slot are read only)
         return dispatch(x, o);
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -357,7 +353,7 @@ struct DispatchFn : public torch::autograd::Function<DispatchFn> {
         const char *what = "expert_dispatch";
         const at::Tensor g = plain_gradient(grads[0], what);
         if (!g.defined()) return out;
-        out[0] = combine(g, at::Tensor(), kept_order(ctx, ctx->get_saved_variables(), 0, g, what));
+        out[0] = combine(g, at::Tensor(), kept_order(ctx->saved_data["order"].toIntVector(), ctx->get_saved_variables(), 0, g, what));
         return out;
     }
 };
@@ -370,7 +366,7 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
         const bool need_w = w.defined() && w.requires_grad();
         const Order o = order_of(position, offsets, token ? *token : at::Tensor());
         ctx->save_for_backward({need_w ? ys : at::Tensor(), w, position, offsets, o.token});
-        keep_order(ctx, o);
+        keep_order(ctx, o, o.token.defined());
         ctx->saved_data["type"] = w.defined() ? c10::IValue(w.scalar_type()) : c10::IValue();
         return combine(ys, w, o);
     }
@@ -380,12 +376,13 @@ struct CombineFn : public torch::autograd::Function<CombineFn> {
         const at::Tensor g = plain_gradient(grads[0], what);
         if (!g.defined()) return out;
         const auto v = ctx->get_saved_variables();
-        const auto shape = ctx->saved_data["shape"].toIntVector();
-        const int64_t d = g.size(1), slots = shape[0] * shape[1];
+        const auto n = ctx->saved_data["order"].toIntVector();
+        const std::array<int64_t, 2> shape{n[0], n[1]};
+        const int64_t d = g.size(1), slots = n[0] * n[1];
         const bool weighted = !ctx->saved_data["type"].isNone();
         // (edges are counted over the tensors that are there)
         const bool need_y = ctx->needs_input_grad(0), need_w = weighted && ctx->needs_input_grad(1);
-        const Order o = kept_order(ctx, v, 2, g, what);
+        const Order o = kept_order(n, v, 2, g, what);
         const c10::DeviceGuard guard(g.device());
         at::Tensor w, ys, dys, dw;
         if (weighted) w = kept(v[1], g, shape, ctx->saved_data["type"].toScalarType(), what).contiguous();
